@@ -233,6 +233,37 @@ int sbnet_reduce_mask_static(const float* mask, int N, int H, int W, float tol, 
                              int bCntH, int bCntW, int16_t* active_block_indices, int32_t* count_dev,
                              int32_t* count_host, void* stream);
 
+/*
+ * Per-position operators on a block stack (no counterpart in the reference, whose residual branches are
+ * built from the host framework's batch norm and convolutions, benchmark/sparse_conv_lib.py:677-824).  A
+ * stack [nB,bSzH,bSzW,C] is a list of nB*bSzH*bSzW rows of C channels; any other [..., C] tensor is one too.
+ * All tensors are contiguous; sums, products and statistics are fp32 whatever the element type.
+ *
+ * LayerNorm over the channels:  y = (x - mean) * rstd * weight + bias,  rstd = 1 / sqrt(var + eps).
+ *   dtype         element type of x and y (SBNET_F32, SBNET_F16, SBNET_BF16)
+ *   weight, bias  [C] of wdtype, which is dtype or SBNET_F32; either may be NULL (1 and 0)
+ *   mean, rstd    [rows] fp32 for the backward pass, both NULL when they are not wanted
+ *   y must not overlap x.  rows == 0 is a successful no-op.
+ * The _dyn form works on the first min(*num_blocks_dev, maxBlocks) blocks of rowsPerBlock rows each and
+ * leaves the rest of y (and of mean, rstd) as it was.
+ */
+int sbnet_layer_norm(const void* x, int dtype, int64_t rows, int C, const void* weight, const void* bias,
+                     int wdtype, float eps, void* y, float* mean, float* rstd, void* stream);
+int sbnet_layer_norm_dyn(const void* x, int dtype, int64_t maxBlocks, int rowsPerBlock,
+                         const int32_t* num_blocks_dev, int C, const void* weight, const void* bias, int wdtype,
+                         float eps, void* y, float* mean, float* rstd, void* stream);
+/*
+ * Backward pass: dx [rows,C] of dtype from dy, x and the forward pass' mean and rstd; dweight, dbias [C] of
+ * wdtype (either or both may be NULL).  workspace: 16-byte aligned device memory of at least
+ * sbnet_layer_norm_grad_workspace(rows, C) bytes, used by this call only until it is done on `stream`
+ * (not needed when dweight and dbias are both NULL).  The column sums are added in a fixed order: the same
+ * call on the same GPU model gives the same bits.  dx must not overlap x or dy.
+ */
+size_t sbnet_layer_norm_grad_workspace(int64_t rows, int C);
+int sbnet_layer_norm_grad(const void* dy, const void* x, int dtype, int64_t rows, int C, const void* weight,
+                          int wdtype, const float* mean, const float* rstd, void* dx, void* dweight, void* dbias,
+                          void* workspace, size_t workspace_bytes, void* stream);
+
 #ifdef __cplusplus
 }
 #endif

@@ -18,6 +18,7 @@ allocating the zero base.
 from __future__ import annotations
 
 import torch
+from torch.autograd.function import once_differentiable
 
 from . import ops
 
@@ -76,3 +77,24 @@ def sparse_scatter(x, bin_counts, active_block_indices, ybase, dynamic_bsize, dy
     """Differentiable ``SparseScatter`` (gradients flow to the block stack ``x`` and to ``ybase``)."""
     return _SparseScatter.apply(x, bin_counts, active_block_indices, ybase, dynamic_bsize,
                                 dynamic_bstride, dynamic_boffset, add, atomic, transpose)
+
+
+class _LayerNorm(torch.autograd.Function):
+    @staticmethod
+    def forward(ctx, x, weight, bias, eps):
+        y, mean, rstd = ops.layer_norm(x, weight, bias, eps, stats=True)
+        ctx.save_for_backward(x, weight, bias, mean, rstd)
+        return y
+
+    @staticmethod
+    @once_differentiable
+    def backward(ctx, grad):
+        x, weight, bias, mean, rstd = ctx.saved_tensors
+        gx, gw, gb = ops.layer_norm_grad(grad.contiguous(), x, mean, rstd, weight, bias,
+                                         sums=ctx.needs_input_grad[1] or ctx.needs_input_grad[2])
+        return gx, gw, gb, None
+
+
+def layer_norm(x, weight=None, bias=None, eps=1e-5):
+    """Differentiable :func:`sbnet_b200.ops.layer_norm` (gradients flow to ``x``, ``weight`` and ``bias``)."""
+    return _LayerNorm.apply(x, weight, bias, eps)

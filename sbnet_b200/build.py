@@ -19,7 +19,7 @@ LIB = os.path.join(PKG, "libsbnet_b200.so")
 
 NVCC_FLAGS = [
     "-gencode", "arch=compute_100a,code=sm_100a", "-lineinfo", "-O3", "-std=c++17",
-    "--cudart", "static", "-Xcompiler", "-fPIC,-fvisibility=hidden,-O3", "-shared",
+    "--cudart", "static", "-Xcompiler", "-fPIC,-fvisibility=hidden,-O3", "-shared", "--threads", "0",
 ]
 
 

@@ -370,3 +370,113 @@ SBNET_EXPORT int sbnet_wait_timeouts(unsigned int* count)
     *count = planes + mask + rows;
     return SBNET_OK;
 }
+
+namespace {
+bool known_dtype(int dtype) { return dtype == SBNET_F32 || dtype == SBNET_F16 || dtype == SBNET_BF16; }
+uintptr_t address(const void* p) { return reinterpret_cast<uintptr_t>(p); }
+uintptr_t elem_mask(int dtype) { return dtype == SBNET_F32 ? 3 : 1; }
+
+bool overlaps(const void* a, const void* b, size_t bytes)
+{
+    return address(a) < address(b) + bytes && address(b) < address(a) + bytes;
+}
+
+// Rules shared by the row operators: types, sizes (row counts and element counts are 64-bit).
+int check_rows(const char* op, int dtype, int64_t rows, int C)
+{
+    if (!known_dtype(dtype))
+        return reject(SBNET_ERR_INVALID_ARGUMENT, "%s: unknown dtype %d", op, dtype);
+    if (rows < 0 || C < 1)
+        return reject(SBNET_ERR_INVALID_ARGUMENT, "%s: needs rows >= 0 and at least one channel, got [%lld, %d]", op,
+                      (long long)rows, C);
+    if (C > (1 << 24) || rows > (1ll << 40) / C)
+        return reject(SBNET_ERR_UNSUPPORTED, "%s: more than 2^24 channels or 2^40 elements", op);
+    return SBNET_OK;
+}
+
+int norm_call(const void* x, int dtype, int64_t rows, int rowsPerBlock, const int32_t* num_blocks_dev, int C,
+              const void* weight, const void* bias, int wdtype, float eps, void* y, float* mean, float* rstd, void* stream)
+{
+    const char* op = "LayerNorm";
+    g_site = "";
+    if (int rc = check_rows(op, dtype, rows, C))
+        return rc;
+    if ((weight != nullptr || bias != nullptr) && wdtype != dtype && wdtype != SBNET_F32)
+        return reject(SBNET_ERR_INVALID_ARGUMENT, "%s: weight and bias must share the tensor's dtype or be fp32", op);
+    if (!(eps >= 0.f))
+        return reject(SBNET_ERR_INVALID_ARGUMENT, "%s: eps must not be negative", op);
+    if ((mean == nullptr) != (rstd == nullptr))
+        return reject(SBNET_ERR_INVALID_ARGUMENT, "%s: mean and rstd go together", op);
+    if (rows == 0)
+        return SBNET_OK;
+    if (x == nullptr || y == nullptr)
+        return reject(SBNET_ERR_INVALID_ARGUMENT, "%s: null tensor pointer", op);
+    if (((address(x) | address(y)) & elem_mask(dtype)) || ((address(weight) | address(bias)) & elem_mask(wdtype)) ||
+        ((address(mean) | address(rstd) | address(num_blocks_dev)) & 3))
+        return reject(SBNET_ERR_INVALID_ARGUMENT, "%s: tensor pointer not aligned to its element size", op);
+    if (overlaps(x, y, (size_t)rows * C * (elem_mask(dtype) + 1)))
+        return reject(SBNET_ERR_INVALID_ARGUMENT, "%s: the output must not overlap the input", op);
+    sbnet::NormArgs a = {};
+    a.x = x, a.y = y, a.weight = weight, a.bias = bias, a.mean = mean, a.rstd = rstd;
+    a.num_blocks_dev = num_blocks_dev, a.rows = rows, a.rowsPerBlock = rowsPerBlock, a.C = C, a.wdtype = wdtype, a.eps = eps;
+    return cuda_status(sbnet::launch_layer_norm(a, dtype, (cudaStream_t)stream));
+}
+} // namespace
+
+SBNET_EXPORT int sbnet_layer_norm(const void* x, int dtype, int64_t rows, int C, const void* weight, const void* bias,
+                                  int wdtype, float eps, void* y, float* mean, float* rstd, void* stream)
+{
+    return norm_call(x, dtype, rows, 1, nullptr, C, weight, bias, wdtype, eps, y, mean, rstd, stream);
+}
+
+SBNET_EXPORT int sbnet_layer_norm_dyn(const void* x, int dtype, int64_t maxBlocks, int rowsPerBlock,
+                                      const int32_t* num_blocks_dev, int C, const void* weight, const void* bias,
+                                      int wdtype, float eps, void* y, float* mean, float* rstd, void* stream)
+{
+    if (num_blocks_dev == nullptr)
+        return reject(SBNET_ERR_INVALID_ARGUMENT, "LayerNorm: num_blocks_dev is null");
+    if (maxBlocks < 0 || rowsPerBlock < 1 || maxBlocks > (1ll << 40) / rowsPerBlock)
+        return reject(SBNET_ERR_INVALID_ARGUMENT, "LayerNorm: bad stack of %lld blocks of %d rows", (long long)maxBlocks,
+                      rowsPerBlock);
+    return norm_call(x, dtype, maxBlocks * rowsPerBlock, rowsPerBlock, num_blocks_dev, C, weight, bias, wdtype, eps, y,
+                     mean, rstd, stream);
+}
+
+SBNET_EXPORT size_t sbnet_layer_norm_grad_workspace(int64_t rows, int C)
+{
+    if (rows < 1 || C < 1)
+        return 0;
+    return sizeof(float) * 2 * (size_t)C * sbnet::layer_norm_grad_parts(rows, C);
+}
+
+SBNET_EXPORT int sbnet_layer_norm_grad(const void* dy, const void* x, int dtype, int64_t rows, int C, const void* weight,
+                                       int wdtype, const float* mean, const float* rstd, void* dx, void* dweight,
+                                       void* dbias, void* workspace, size_t workspace_bytes, void* stream)
+{
+    const char* op = "LayerNormGrad";
+    g_site = "";
+    if (int rc = check_rows(op, dtype, rows, C))
+        return rc;
+    const bool sums = dweight != nullptr || dbias != nullptr;
+    if ((weight != nullptr || sums) && wdtype != dtype && wdtype != SBNET_F32)
+        return reject(SBNET_ERR_INVALID_ARGUMENT, "%s: weight and bias must share the tensor's dtype or be fp32", op);
+    if (rows == 0 && !sums)
+        return SBNET_OK;
+    if (rows > 0 && (dy == nullptr || x == nullptr || dx == nullptr || mean == nullptr || rstd == nullptr))
+        return reject(SBNET_ERR_INVALID_ARGUMENT, "%s: null tensor pointer", op);
+    if (((address(x) | address(dy) | address(dx)) & elem_mask(dtype)) ||
+        ((address(weight) | address(dweight) | address(dbias)) & elem_mask(wdtype)) || ((address(mean) | address(rstd)) & 3))
+        return reject(SBNET_ERR_INVALID_ARGUMENT, "%s: tensor pointer not aligned to its element size", op);
+    const size_t bytes = (size_t)rows * C * (elem_mask(dtype) + 1);
+    if (rows > 0 && (overlaps(dx, x, bytes) || overlaps(dx, dy, bytes)))
+        return reject(SBNET_ERR_INVALID_ARGUMENT, "%s: the output must not overlap an input", op);
+    if (sums && rows > 0 && (workspace == nullptr || (address(workspace) & 15) ||
+                 workspace_bytes < sbnet_layer_norm_grad_workspace(rows, C)))
+        return reject(SBNET_ERR_INVALID_ARGUMENT, "%s: needs %zu bytes of 16-byte aligned workspace", op,
+                      sbnet_layer_norm_grad_workspace(rows, C));
+    sbnet::NormArgs a = {};
+    a.x = x, a.g = dy, a.y = dx, a.weight = weight, a.mean = const_cast<float*>(mean), a.rstd = const_cast<float*>(rstd);
+    a.partials = sums ? static_cast<float*>(workspace) : nullptr, a.dweight = dweight, a.dbias = dbias;
+    a.rows = rows, a.rowsPerBlock = 1, a.C = C, a.wdtype = wdtype;
+    return cuda_status(sbnet::launch_layer_norm_grad(a, dtype, (cudaStream_t)stream));
+}

@@ -35,6 +35,24 @@ cudaError_t read_wait_timeouts(unsigned int* out);
 
 cudaError_t launch_copy(void* dst, const void* src, size_t bytes, cudaStream_t stream);
 
+// Layer norm over rows of C channels (layer_norm.cu).  dtype codes as in include/sbnet_b200.h.
+struct NormArgs {
+    const void* x;                 // [rows, C]
+    const void* g;                 // backward: gradient of y, [rows, C]
+    void* y;                       // forward: y; backward: dx
+    const void *weight, *bias;     // [C] of wdtype, or nullptr (1 and 0)
+    float *mean, *rstd;            // [rows]; forward: written unless nullptr, backward: read
+    float* partials;               // backward: [parts, 2, C] column sums, nullptr when no weight gradient is wanted
+    void *dweight, *dbias;         // backward: [C] of wdtype, or nullptr
+    const int32_t* num_blocks_dev; // forward: live blocks of rowsPerBlock rows, or nullptr (all rows)
+    long long rows;
+    int rowsPerBlock, C, wdtype;
+    float eps;
+};
+cudaError_t launch_layer_norm(const NormArgs& a, int dtype, cudaStream_t stream);
+cudaError_t launch_layer_norm_grad(const NormArgs& a, int dtype, cudaStream_t stream);
+int layer_norm_grad_parts(long long rows, int C);
+
 int sm_count();
 
 // Sets the calling thread's sbnet_last_error() text.

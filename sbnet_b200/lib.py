@@ -20,7 +20,7 @@ SBNET_COUNT_NOWAIT = 16
 SBNET_COUNT_PENDING = -(2 ** 31)
 SBNET_REDUCE_MASK_SCRATCH_INTS = 4
 
-_i, _f, _p, _sz = C.c_int, C.c_float, C.c_void_p, C.c_size_t
+_i, _f, _p, _sz, _l = C.c_int, C.c_float, C.c_void_p, C.c_size_t, C.c_int64
 _GEOM = [_i] * 6
 _TENSOR = [_p, _i, _i, _i, _i, _i, _p]  # x, dtype, N, H, W, C, y
 
@@ -40,6 +40,10 @@ SIGNATURES = {
     "sbnet_set_option": (_i, [C.c_char_p, _i]),
     "sbnet_get_option": (_i, [C.c_char_p, C.POINTER(_i)]),
     "sbnet_reduce_mask_static": (_i, [_p, _i, _i, _i, _f, _i] + _GEOM + [_i, _i, _p, _p, _p, _p]),
+    "sbnet_layer_norm": (_i, [_p, _i, _l, _i, _p, _p, _i, _f, _p, _p, _p, _p]),
+    "sbnet_layer_norm_dyn": (_i, [_p, _i, _l, _i, _p, _i, _p, _p, _i, _f, _p, _p, _p, _p]),
+    "sbnet_layer_norm_grad_workspace": (_sz, [_l, _i]),
+    "sbnet_layer_norm_grad": (_i, [_p, _p, _i, _l, _i, _p, _i, _p, _p, _p, _p, _p, _p, _sz, _p]),
 }
 
 _lib = None

@@ -368,6 +368,128 @@ def sparse_scatter_var_dyn(x, count_dev: torch.Tensor, max_blocks: int, active_b
     return ybase
 
 
+# ---- per-position operators on a block stack ---------------------------------------------------------
+# A stack ``[nB, bSzH, bSzW, C]`` in the rows layout (``transpose=False``) -- or any contiguous ``[..., C]``
+# tensor -- is a list of rows of C channels.
+
+def _check_rows(t: torch.Tensor, name: str):
+    """A contiguous ``[..., C]`` tensor of a supported type; returns ``(rows, C)``."""
+    if t.dim() < 1 or t.shape[-1] < 1:
+        raise ValueError(f"{name} must be [..., C] with at least one channel")
+    if t.dtype not in _DTYPES:
+        raise ValueError(f"unsupported dtype {t.dtype}")
+    if not t.is_contiguous():
+        raise ValueError(f"{name} must be contiguous")
+    channels = t.shape[-1]
+    return t.numel() // channels, channels
+
+
+def _check_like(t: torch.Tensor, name: str, like: torch.Tensor) -> None:
+    if t.shape != like.shape or t.dtype != like.dtype or t.device != like.device or not t.is_contiguous():
+        raise ValueError(f"{name} must be contiguous and of the shape, dtype and device of the input")
+
+
+def _check_norm_params(weight, bias, channels: int, x: torch.Tensor) -> int:
+    """weight / bias: None or contiguous ``[C]`` of the input's type or float32, both of one type."""
+    wdtype = None
+    for t, name in ((weight, "weight"), (bias, "bias")):
+        if t is None:
+            continue
+        if t.dim() != 1 or t.shape[0] != channels or not t.is_contiguous():
+            raise ValueError(f"{name} must be a contiguous [{channels}] tensor")
+        if t.dtype != x.dtype and t.dtype != torch.float32:
+            raise ValueError(f"{name} must be of the input's dtype or float32, got {t.dtype}")
+        if wdtype is not None and t.dtype != wdtype:
+            raise ValueError("weight and bias must share a dtype")
+        if t.device != x.device:
+            raise ValueError(f"{name} must live on the device of the input")
+        wdtype = t.dtype
+    return _DTYPES[x.dtype if wdtype is None else wdtype]
+
+
+def _ptr(t):
+    return None if t is None else t.data_ptr()
+
+
+def _blocks_of(x: torch.Tensor):
+    """``(maxBlocks, rows per block)`` of a stack ``[maxBlocks, ..., C]``."""
+    if x.dim() < 2:
+        raise ValueError("a block stack is [maxBlocks, ..., C]")
+    per = 1
+    for n in x.shape[1:-1]:
+        per *= n
+    if per < 1:
+        raise ValueError("a block must hold at least one row")
+    return x.shape[0], per
+
+
+def _layer_norm_call(x, weight, bias, eps, out, stats, count_dev):
+    rows, channels = _check_rows(x, "x")
+    wdtype = _check_norm_params(weight, bias, channels, x)
+    if count_dev is not None:
+        _check_count_dev(count_dev, x)
+        blocks, per = _blocks_of(x)
+    if out is not None:
+        _check_like(out, "out", x)
+    _require_cuda(x, "x")
+    with _on(x.device):
+        y = torch.empty_like(x) if out is None else out
+        mean = rstd = None
+        if stats:
+            both = torch.empty((2, rows), dtype=torch.float32, device=x.device)
+            mean, rstd = both[0], both[1]
+        tail = (channels, _ptr(weight), _ptr(bias), wdtype, eps, y.data_ptr(), _ptr(mean), _ptr(rstd), _stream(x.device))
+        if count_dev is None:
+            _lib.check(_lib.load().sbnet_layer_norm(x.data_ptr(), _DTYPES[x.dtype], rows, *tail))
+        else:
+            _lib.check(_lib.load().sbnet_layer_norm_dyn(x.data_ptr(), _DTYPES[x.dtype], blocks, per,
+                                                        count_dev.data_ptr(), *tail))
+    return (y, mean, rstd) if stats else y
+
+
+def layer_norm(x: torch.Tensor, weight=None, bias=None, eps: float = 1e-5, out=None, stats: bool = False):
+    """Layer norm over the channels of every row of ``x`` (``[..., C]``):
+    ``(x - mean) / sqrt(var + eps) * weight + bias``, statistics in fp32 over the biased variance.
+
+    ``weight`` / ``bias``: ``[C]`` of ``x``'s dtype or float32, or None.  ``stats=True`` also returns the
+    rows' fp32 ``mean`` and ``1 / sqrt(var + eps)`` for :func:`layer_norm_grad`.  ``out`` must not overlap ``x``."""
+    return _layer_norm_call(x, weight, bias, eps, out, stats, None)
+
+
+def layer_norm_dyn(x: torch.Tensor, count_dev: torch.Tensor, weight=None, bias=None, eps: float = 1e-5, out=None):
+    """:func:`layer_norm` of the first ``count_dev[0]`` blocks of a stack ``[maxBlocks, ..., C]``, the count read
+    on the device; the rest of the result (of ``out``) is left as it was."""
+    if count_dev is None:
+        raise ValueError("count_dev must be an int32 tensor with at least one element")
+    return _layer_norm_call(x, weight, bias, eps, out, False, count_dev)
+
+
+def layer_norm_grad(grad: torch.Tensor, x: torch.Tensor, mean: torch.Tensor, rstd: torch.Tensor, weight=None,
+                    bias=None, sums: bool = True):
+    """Backward pass of :func:`layer_norm`: ``(dx, dweight, dbias)``, the last two None where that parameter is
+    None or with ``sums=False``.  ``mean``, ``rstd``: what the forward call returned with ``stats=True``."""
+    rows, channels = _check_rows(x, "x")
+    _check_like(grad, "grad", x)
+    wdtype = _check_norm_params(weight, bias, channels, x)
+    for t, name in ((mean, "mean"), (rstd, "rstd")):
+        if t.dtype != torch.float32 or t.numel() != rows or not t.is_contiguous() or t.device != x.device:
+            raise ValueError(f"{name} must be contiguous float32 with one element per row")
+    _require_cuda(x, "x")
+    with _on(x.device):
+        dx = torch.empty_like(x)
+        dw = torch.empty_like(weight) if sums and weight is not None else None
+        db = torch.empty_like(bias) if sums and bias is not None else None
+        lib = _lib.load()
+        need, ws = 0, None
+        if dw is not None or db is not None:
+            need = lib.sbnet_layer_norm_grad_workspace(rows, channels)
+            ws = torch.empty(need, dtype=torch.uint8, device=x.device)
+        _lib.check(lib.sbnet_layer_norm_grad(
+            grad.data_ptr(), x.data_ptr(), _DTYPES[x.dtype], rows, channels, _ptr(weight), wdtype, mean.data_ptr(),
+            rstd.data_ptr(), dx.data_ptr(), _ptr(dw), _ptr(db), _ptr(ws), need, _stream(x.device)))
+    return dx, dw, db
+
+
 # ---- pre-validated calls for hot loops ---------------------------------------------------------------
 # The wrappers above re-check every argument on every call (about 7 us of interpreter time each, beside
 # the ~5 us of the foreign call itself).  A loop that calls the same op on the same buffers with the
