@@ -98,3 +98,27 @@ class _LayerNorm(torch.autograd.Function):
 def layer_norm(x, weight=None, bias=None, eps=1e-5):
     """Differentiable :func:`sbnet_b200.ops.layer_norm` (gradients flow to ``x``, ``weight`` and ``bias``)."""
     return _LayerNorm.apply(x, weight, bias, eps)
+
+
+class _GatedFfn(torch.autograd.Function):
+    @staticmethod
+    def forward(ctx, x, w_gate, w_up, w_down, activation):
+        if not any(ctx.needs_input_grad):
+            return ops.gated_ffn(x, w_gate, w_up, w_down, activation)
+        y, gate, up = ops.gated_ffn_train(x, w_gate, w_up, w_down, activation)
+        ctx.save_for_backward(x, w_gate, w_up, w_down, gate, up)
+        ctx.activation = activation
+        return y
+
+    @staticmethod
+    @once_differentiable
+    def backward(ctx, grad):
+        x, w_gate, w_up, w_down, gate, up = ctx.saved_tensors
+        need = ctx.needs_input_grad
+        return (*ops.gated_ffn_grad(grad.contiguous(), x, gate, up, w_gate, w_up, w_down, ctx.activation,
+                                    need[0], need[1] or need[2], need[3]), None)
+
+
+def gated_ffn(x, w_gate, w_up, w_down, activation="silu"):
+    """Differentiable :func:`sbnet_b200.ops.gated_ffn` (gradients flow to ``x`` and the three weights)."""
+    return _GatedFfn.apply(x, w_gate, w_up, w_down, activation)

@@ -360,14 +360,16 @@ SBNET_EXPORT int sbnet_wait_timeouts(unsigned int* count)
 {
     if (count == nullptr)
         return reject(SBNET_ERR_INVALID_ARGUMENT, "sbnet_wait_timeouts: null output");
-    unsigned int planes = 0, mask = 0, rows = 0;
+    unsigned int planes = 0, mask = 0, rows = 0, ffn = 0;
     if (cudaError_t e = sbnet::read_wait_timeouts(&planes))
         return cuda_status(e);
     if (cudaError_t e = sbnet::read_rm_wait_timeouts(&mask))
         return cuda_status(e);
     if (cudaError_t e = sbnet::read_rows_wait_timeouts(&rows))
         return cuda_status(e);
-    *count = planes + mask + rows;
+    if (cudaError_t e = sbnet::read_ffn_wait_timeouts(&ffn))
+        return cuda_status(e);
+    *count = planes + mask + rows + ffn;
     return SBNET_OK;
 }
 
@@ -479,4 +481,135 @@ SBNET_EXPORT int sbnet_layer_norm_grad(const void* dy, const void* x, int dtype,
     a.partials = sums ? static_cast<float*>(workspace) : nullptr, a.dweight = dweight, a.dbias = dbias;
     a.rows = rows, a.rowsPerBlock = 1, a.C = C, a.wdtype = wdtype;
     return cuda_status(sbnet::launch_layer_norm_grad(a, dtype, (cudaStream_t)stream));
+}
+
+namespace {
+int check_ffn(const char* op, int dtype, int64_t rows, int C, int F, int act)
+{
+    if (int rc = check_rows(op, dtype, rows, C))
+        return rc;
+    if (dtype == SBNET_F32)
+        return reject(SBNET_ERR_INVALID_ARGUMENT, "%s: fp16 and bf16 only (the tensor cores' operand types)", op);
+    if (F < 1)
+        return reject(SBNET_ERR_INVALID_ARGUMENT, "%s: needs at least one hidden channel, got %d", op, F);
+    if (act != SBNET_ACT_SILU && act != SBNET_ACT_GELU && act != SBNET_ACT_RELU)
+        return reject(SBNET_ERR_INVALID_ARGUMENT, "%s: unknown activation %d", op, act);
+    if (F > (1 << 24) || rows >= (1ll << 31) - 256 || (rows / 128 + 1) * ((C > F ? C : F) / 128 + 1) >= (1ll << 31) / 256)
+        return reject(SBNET_ERR_UNSUPPORTED, "%s: more than 2^31 work items", op);
+    return SBNET_OK;
+}
+
+int check_workspace(const char* op, const void* workspace, size_t bytes, size_t need)
+{
+    if (need != 0 && (workspace == nullptr || (address(workspace) & 255) || bytes < need))
+        return reject(SBNET_ERR_INVALID_ARGUMENT, "%s: needs %zu bytes of 256-byte aligned workspace, got %zu", op, need, bytes);
+    return SBNET_OK;
+}
+
+int ffn_call(const void* x, int dtype, int64_t rows, int rowsPerBlock, const int32_t* num_blocks_dev, int C, int F,
+             const void* w_gate, const void* w_up, const void* w_down, int act, void* y, void* gate, void* up,
+             void* workspace, size_t workspace_bytes, void* stream)
+{
+    const char* op = "GatedFfn";
+    g_site = "";
+    if (int rc = check_ffn(op, dtype, rows, C, F, act))
+        return rc;
+    if ((gate == nullptr) != (up == nullptr))
+        return reject(SBNET_ERR_INVALID_ARGUMENT, "%s: gate and up go together", op);
+    if (rows == 0)
+        return SBNET_OK;
+    if (x == nullptr || y == nullptr || w_gate == nullptr || w_up == nullptr || w_down == nullptr)
+        return reject(SBNET_ERR_INVALID_ARGUMENT, "%s: null tensor pointer", op);
+    const uintptr_t inputs = address(x) | address(w_gate) | address(w_up) | address(w_down);
+    if (((inputs | address(y)) & 1) || (address(num_blocks_dev) & 3) || ((address(gate) | address(up)) & 15))
+        return reject(SBNET_ERR_INVALID_ARGUMENT, "%s: tensor pointer not aligned to its element size (gate, up: 16 bytes)", op);
+    const size_t bytes = (size_t)rows * C * 2, wbytes = (size_t)F * C * 2;
+    if (overlaps(x, y, bytes) || (address(y) < address(w_gate) + wbytes && address(w_gate) < address(y) + bytes) ||
+        (address(y) < address(w_up) + wbytes && address(w_up) < address(y) + bytes) ||
+        (address(y) < address(w_down) + wbytes && address(w_down) < address(y) + bytes))
+        return reject(SBNET_ERR_INVALID_ARGUMENT, "%s: the output must not overlap an input", op);
+    if (int rc = check_workspace(op, workspace, workspace_bytes,
+                                 sbnet::gated_ffn_workspace(rows, C, F, false, (inputs & 15) == 0)))
+        return rc;
+    sbnet::FfnArgs f = {};
+    f.x = x, f.w_gate = w_gate, f.w_up = w_up, f.w_down = w_down, f.y = y, f.gate = gate, f.up = up;
+    f.num_blocks_dev = num_blocks_dev, f.workspace = workspace, f.rows = rows, f.rowsPerBlock = rowsPerBlock;
+    f.C = C, f.F = F, f.act = act;
+    return cuda_status(sbnet::launch_gated_ffn(f, dtype, (cudaStream_t)stream));
+}
+} // namespace
+
+SBNET_EXPORT size_t sbnet_gated_ffn_workspace(int64_t rows, int C, int F, int grad, int aligned)
+{
+    if (rows < 1 || C < 1 || F < 1)
+        return 0;
+    return sbnet::gated_ffn_workspace(rows, C, F, grad != 0, aligned != 0);
+}
+
+SBNET_EXPORT int sbnet_gated_ffn(const void* x, int dtype, int64_t rows, int C, int F, const void* w_gate,
+                                 const void* w_up, const void* w_down, int act, void* y, void* gate, void* up,
+                                 void* workspace, size_t workspace_bytes, void* stream)
+{
+    return ffn_call(x, dtype, rows, 1, nullptr, C, F, w_gate, w_up, w_down, act, y, gate, up, workspace, workspace_bytes,
+                    stream);
+}
+
+SBNET_EXPORT int sbnet_gated_ffn_dyn(const void* x, int dtype, int64_t maxBlocks, int rowsPerBlock,
+                                     const int32_t* num_blocks_dev, int C, int F, const void* w_gate, const void* w_up,
+                                     const void* w_down, int act, void* y, void* workspace, size_t workspace_bytes,
+                                     void* stream)
+{
+    if (num_blocks_dev == nullptr)
+        return reject(SBNET_ERR_INVALID_ARGUMENT, "GatedFfn: num_blocks_dev is null");
+    if (maxBlocks < 0 || rowsPerBlock < 1 || maxBlocks > (1ll << 40) / rowsPerBlock)
+        return reject(SBNET_ERR_INVALID_ARGUMENT, "GatedFfn: bad stack of %lld blocks of %d rows", (long long)maxBlocks,
+                      rowsPerBlock);
+    return ffn_call(x, dtype, maxBlocks * rowsPerBlock, rowsPerBlock, num_blocks_dev, C, F, w_gate, w_up, w_down, act, y,
+                    nullptr, nullptr, workspace, workspace_bytes, stream);
+}
+
+SBNET_EXPORT int sbnet_gated_ffn_grad(const void* dy, const void* x, const void* gate, const void* up, int dtype,
+                                      int64_t rows, int C, int F, const void* w_gate, const void* w_up,
+                                      const void* w_down, int act, void* dx, void* dw_gate, void* dw_up, void* dw_down,
+                                      void* workspace, size_t workspace_bytes, void* stream)
+{
+    const char* op = "GatedFfnGrad";
+    g_site = "";
+    if (int rc = check_ffn(op, dtype, rows, C, F, act))
+        return rc;
+    if ((dw_gate == nullptr) != (dw_up == nullptr))
+        return reject(SBNET_ERR_INVALID_ARGUMENT, "%s: dw_gate and dw_up go together", op);
+    if ((address(dx) | address(dw_gate) | address(dw_up) | address(dw_down)) & 1)
+        return reject(SBNET_ERR_INVALID_ARGUMENT, "%s: tensor pointer not aligned to its element size", op);
+    cudaStream_t s = (cudaStream_t)stream;
+    if (rows == 0) {     // sums over no rows
+        for (void* w : {dw_gate, dw_up, dw_down})
+            if (w != nullptr)
+                if (cudaError_t e = cudaMemsetAsync(w, 0, (size_t)F * C * 2, s))
+                    return cuda_status(e);
+        return SBNET_OK;
+    }
+    if (dy == nullptr || x == nullptr || gate == nullptr || up == nullptr || w_gate == nullptr || w_up == nullptr ||
+        w_down == nullptr)
+        return reject(SBNET_ERR_INVALID_ARGUMENT, "%s: null tensor pointer", op);
+    const uintptr_t inputs = address(dy) | address(x) | address(w_gate) | address(w_up) | address(w_down);
+    if ((inputs & 1) || ((address(gate) | address(up)) & 15))
+        return reject(SBNET_ERR_INVALID_ARGUMENT, "%s: tensor pointer not aligned to its element size (gate, up: 16 bytes)", op);
+    const size_t bytes = (size_t)rows * C * 2, wbytes = (size_t)F * C * 2, hbytes = (size_t)rows * ((F + 7) / 8 * 8) * 2;
+    const struct { const void* p; size_t n; } in[] = {{dy, bytes}, {x, bytes}, {gate, hbytes}, {up, hbytes},
+                                                      {w_gate, wbytes}, {w_up, wbytes}, {w_down, wbytes}},
+                                              out[] = {{dx, bytes}, {dw_gate, wbytes}, {dw_up, wbytes}, {dw_down, wbytes}};
+    for (const auto& o : out)
+        for (const auto& i : in)
+            if (o.p != nullptr && address(o.p) < address(i.p) + i.n && address(i.p) < address(o.p) + o.n)
+                return reject(SBNET_ERR_INVALID_ARGUMENT, "%s: an output must not overlap an input", op);
+    if (int rc = check_workspace(op, workspace, workspace_bytes,
+                                 sbnet::gated_ffn_workspace(rows, C, F, true, (inputs & 15) == 0)))
+        return rc;
+    sbnet::FfnArgs f = {};
+    f.dy = dy, f.x = x, f.gate = const_cast<void*>(gate), f.up = const_cast<void*>(up);
+    f.w_gate = w_gate, f.w_up = w_up, f.w_down = w_down;
+    f.dx = dx, f.dw_gate = dw_gate, f.dw_up = dw_up, f.dw_down = dw_down;
+    f.workspace = workspace, f.rows = rows, f.rowsPerBlock = 1, f.C = C, f.F = F, f.act = act;
+    return cuda_status(sbnet::launch_gated_ffn_grad(f, dtype, s));
 }

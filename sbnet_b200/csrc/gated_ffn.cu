@@ -1,0 +1,758 @@
+// The gated feed-forward block over a list of rows, forward and backward, on the fifth-generation tensor cores:
+//
+//   G = X Wg^T   U = X Wu^T   H = act(G) * U   Y = H Wd^T               X [R,C], Wg and Wu [F,C], Wd [C,F]
+//   dH = dY Wd   dU = dH * act(G)   dG = dH * U * act'(G)
+//   dX = dG Wg + dU Wu    dWg = dG^T X    dWu = dU^T X    dWd = dY^T H
+//
+// One kernel, gemm_kernel, computes all of them as D[m,n] = sum_k A[m,k] B[n,k]; what differs is which
+// operand's memory order has the reduction contiguous ("K-major") or not ("MN-major") and what the epilogue
+// does with an accumulator tile:
+//
+//   kGate   both projections at once: a tile's B operand is 128 rows of Wg followed by 128 rows of Wu, so G and
+//           U of the same 128 x 128 positions come out of one instruction stream side by side in TMEM and the
+//           epilogue writes H (and, in training, G and U) without either having been to memory
+//   kGrad   dH stays in TMEM; the epilogue reads G and U and writes dG, dU and H
+//   kStore  a plain product, rounded once
+//
+// G, U, H, dG and dU are held between kernels in the type of X (they are operands of the next product, and the
+// tensor cores multiply 16-bit types); accumulators and every element-wise step are fp32.
+//
+// Structure: persistent CTAs (one per SM) over 128 x 256 (or 128 x 128) output tiles; one thread feeds a ring of
+// shared-memory stages by TMA (64 reduction steps each, 128-byte swizzle; rows and columns past the matrix read
+// as zero), one thread issues tcgen05.mma, eight warps run the epilogue on one TMEM accumulator while the other
+// is being filled.  Tiles are walked in groups of 16 row tiles so that the operands of neighbouring CTAs meet in
+// L2.  Where a product has fewer tiles than the GPU has SMs, the reduction is split: every piece writes fp32
+// partial sums to the workspace and a second kernel adds them in a fixed order (no atomics: the same call gives
+// the same bits).
+//
+// A matrix whose rows do not start on 16-byte boundaries cannot be read by TMA; it is first copied to the
+// workspace at the next pitch that can.
+//
+// Waits are bounded; a wait that gives up raises a CTA-wide flag, counts itself, and the CTA lets its copies and
+// matrix instructions land, frees its TMEM and returns.
+#include <cuda.h>
+#include <cudaTypedefs.h>
+
+#include <algorithm>
+
+#include "common.cuh"
+#include "kernels.h"
+#include "tensor_ptx.cuh"
+
+namespace sbnet {
+namespace {
+
+constexpr int kTileM = 128;
+constexpr int kStepK = 64;                       // reduction steps of a stage (128 bytes)
+constexpr int kEpiWarps = 8;
+constexpr int kGemmThreads = (2 + kEpiWarps) * 32;
+constexpr int kStagingBytes = kEpiWarps * 4096;  // two 32 x 32 tiles of 16-bit elements per epilogue warp
+constexpr int kGroupM = 16;
+
+__device__ unsigned int g_ffn_timeouts = 0;
+
+enum Epilogue { kStore, kGate, kGrad };
+enum Act { kSilu = 0, kGelu = 1, kRelu = 2 };
+
+struct Maps {
+    CUtensorMap a[2], b[2];
+};
+
+struct Plan {
+    int mTiles, nTiles;            // tiles of D
+    int batch;                     // products of one shape in this launch: product z reads a[z], b[z], writes out[z]
+    int segs;                      // reduction segments: segment s reads a[s], b[s]  (batch == 1)
+    int kIters;                    // stages of one segment
+    int splits;                    // pieces of the reduction (> 1: fp32 partials)
+    int N;                         // columns of the output
+    long long M;                   // rows of the output
+    const int32_t* num_blocks_dev; // live rows = min(count * rowsPerBlock, M), or nullptr
+    int rowsPerBlock;
+    int act;
+    void* out[2];                  // kStore: D of product z.  kGate: H
+    long long ldo;
+    void *gate, *up;               // kGate: written unless null.  kGrad: read
+    void *dgate, *dup, *hid;       // kGrad: written
+    long long ldh;                 // pitch of gate .. hid (a multiple of 8)
+    float* partials;               // splits > 1: [splits][batch][mTiles * 128][nTiles * BN]
+};
+
+template <int BN> constexpr int kStages = BN == 256 ? 4 : 6;
+template <int BN> constexpr int kStageBytes = (kTileM + BN) * kStepK * 2;
+template <int BN> constexpr int kGemmSmem = 1024 + kStages<BN> * kStageBytes<BN> + kStagingBytes + 256;
+
+template <typename T> __device__ __forceinline__ uint32_t pack2(float lo, float hi);
+template <> __device__ __forceinline__ uint32_t pack2<__half>(float lo, float hi)
+{
+    const __half2 v = __floats2half2_rn(lo, hi);
+    return *reinterpret_cast<const uint32_t*>(&v);
+}
+template <> __device__ __forceinline__ uint32_t pack2<__nv_bfloat16>(float lo, float hi)
+{
+    const __nv_bfloat162 v = __floats2bfloat162_rn(lo, hi);
+    return *reinterpret_cast<const uint32_t*>(&v);
+}
+template <typename T> __device__ __forceinline__ float2 unpack2(uint32_t v);
+template <> __device__ __forceinline__ float2 unpack2<__half>(uint32_t v)
+{
+    return __half22float2(*reinterpret_cast<const __half2*>(&v));
+}
+template <> __device__ __forceinline__ float2 unpack2<__nv_bfloat16>(uint32_t v)
+{
+    return __bfloat1622float2(*reinterpret_cast<const __nv_bfloat162*>(&v));
+}
+
+// act(g), and its derivative where it is asked for.
+template <int ACT, bool SLOPE> __device__ __forceinline__ float activate(float g, float& slope)
+{
+    if constexpr (ACT == kSilu) {
+        const float s = __fdividef(1.f, 1.f + __expf(-g));
+        if (SLOPE)
+            slope = s * (1.f + g * (1.f - s));
+        return g * s;
+    } else if constexpr (ACT == kGelu) {
+        const float cdf = 0.5f * (1.f + erff(g * 0.70710678118654752f));
+        if (SLOPE)
+            slope = cdf + g * 0.3989422804014327f * __expf(-0.5f * g * g);
+        return g * cdf;
+    } else {
+        if (SLOPE)
+            slope = g > 0.f ? 1.f : 0.f;
+        return g != g ? g : fmaxf(g, 0.f);
+    }
+}
+
+// ---- 32 x 32 tiles of 16-bit elements between registers (one row per lane) and memory -----------------------
+// Staged through 2 KB of shared memory so that global accesses are 64 contiguous bytes per row.  16-byte pieces
+// are swizzled by row: eight lanes touch eight different pieces of 128 bytes whichever way the tile is walked.
+__device__ __forceinline__ uint32_t piece(uint32_t buf, int row, int c) { return buf + row * 64 + ((c ^ ((row >> 1) & 3)) << 4); }
+
+__device__ __forceinline__ void stage_rows(uint32_t buf, int lane, const uint32_t (&w)[16])
+{
+#pragma unroll
+    for (int c = 0; c < 4; ++c)
+        sts128(piece(buf, lane, c), make_uint4(w[4 * c], w[4 * c + 1], w[4 * c + 2], w[4 * c + 3]));
+}
+__device__ __forceinline__ void unstage_rows(uint32_t buf, int lane, uint32_t (&w)[16])
+{
+#pragma unroll
+    for (int c = 0; c < 4; ++c) {
+        const uint4 v = lds128(piece(buf, lane, c));
+        w[4 * c] = v.x, w[4 * c + 1] = v.y, w[4 * c + 2] = v.z, w[4 * c + 3] = v.w;
+    }
+}
+// tile -> memory: rows row0.. (below rowEnd), columns col0.. (below N) of a matrix of pitch ld
+template <typename T>
+__device__ __forceinline__ void store_tile(T* out, long long ld, long long row0, long long rowEnd, int col0, int N, bool wide,
+                                           uint32_t buf, int lane)
+{
+    const int c = lane & 3, col = col0 + c * 8;
+#pragma unroll
+    for (int i = 0; i < 4; ++i) {
+        const int r = i * 8 + (lane >> 2);
+        const uint4 v = lds128(piece(buf, r, c));
+        if (row0 + r >= rowEnd)
+            continue;
+        T* dst = out + (row0 + r) * ld + col;
+        if (wide && col + 8 <= N) {
+            *reinterpret_cast<uint4*>(dst) = v;
+        } else {
+            const T* e = reinterpret_cast<const T*>(&v);
+#pragma unroll
+            for (int k = 0; k < 8; ++k)
+                if (col + k < N)
+                    dst[k] = e[k];
+        }
+    }
+}
+// memory -> tile, from a matrix whose pitch is a multiple of 8 elements and covers the piece that holds column N - 1
+template <typename T>
+__device__ __forceinline__ void load_tile(const T* in, long long ld, long long row0, long long rowEnd, int col0, int N,
+                                          uint32_t buf, int lane)
+{
+    const int c = lane & 3, col = col0 + c * 8;
+#pragma unroll
+    for (int i = 0; i < 4; ++i) {
+        const int r = i * 8 + (lane >> 2);
+        uint4 v = make_uint4(0, 0, 0, 0);
+        if (row0 + r < rowEnd && col < N)
+            v = *reinterpret_cast<const uint4*>(in + (row0 + r) * ld + col);
+        sts128(piece(buf, r, c), v);
+    }
+}
+
+template <typename T, int ACT>
+__device__ __forceinline__ void gate_chunk(const uint32_t (&g)[32], const uint32_t (&u)[32], uint32_t (&h)[16])
+{
+    float unused;
+#pragma unroll
+    for (int i = 0; i < 16; ++i)
+        h[i] = pack2<T>(activate<ACT, false>(__uint_as_float(g[2 * i]), unused) * __uint_as_float(u[2 * i]),
+                        activate<ACT, false>(__uint_as_float(g[2 * i + 1]), unused) * __uint_as_float(u[2 * i + 1]));
+}
+// g and u are replaced by dG and dU
+template <typename T, int ACT>
+__device__ __forceinline__ void grad_chunk(const uint32_t (&dh)[32], uint32_t (&g)[16], uint32_t (&u)[16], uint32_t (&h)[16])
+{
+#pragma unroll
+    for (int i = 0; i < 16; ++i) {
+        const float2 gg = unpack2<T>(g[i]), uu = unpack2<T>(u[i]);
+        const float d0 = __uint_as_float(dh[2 * i]), d1 = __uint_as_float(dh[2 * i + 1]);
+        float s0, s1;
+        const float a0 = activate<ACT, true>(gg.x, s0), a1 = activate<ACT, true>(gg.y, s1);
+        h[i] = pack2<T>(a0 * uu.x, a1 * uu.y);
+        u[i] = pack2<T>(d0 * a0, d1 * a1);
+        g[i] = pack2<T>(d0 * uu.x * s0, d1 * uu.y * s1);
+    }
+}
+
+struct Tile {
+    int m, n, z, s;
+};
+__device__ __forceinline__ Tile tile_at(int t, const Plan& p, int mTiles)
+{
+    Tile r;
+    const int plane = mTiles * p.nTiles;
+    const int q = t / plane;
+    t -= q * plane;
+    r.s = q / p.batch, r.z = q - r.s * p.batch;
+    const int group = t / (kGroupM * p.nTiles), inside = t - group * kGroupM * p.nTiles;
+    const int rows = min(kGroupM, mTiles - group * kGroupM);
+    r.n = inside / rows, r.m = group * kGroupM + inside - r.n * rows;
+    return r;
+}
+
+// A_MN / B_MN: the operand's reduction runs along its rows' pitch, not along its rows.
+template <typename T, bool A_MN, bool B_MN, int EPI, int BN>
+__global__ void __launch_bounds__(kGemmThreads, 1) gemm_kernel(const __grid_constant__ Maps maps, const __grid_constant__ Plan p)
+{
+    constexpr int S = kStages<BN>;
+    extern __shared__ uint8_t smem_raw[];
+    const uint32_t smem = (smem_u32(smem_raw) + 1023) & ~1023u;
+    const uint32_t staging = smem + S * kStageBytes<BN>;
+    const uint32_t bars = staging + kStagingBytes;           // full[S], empty[S], accFull[2], accEmpty[2], drain
+    const uint32_t full = bars, empty = bars + 8 * S, accFull = bars + 16 * S, accEmpty = accFull + 16, drain = accEmpty + 16;
+    __shared__ uint32_t tmemSlot;
+    __shared__ int abortFlag;
+    const int warp = threadIdx.x >> 5, lane = threadIdx.x & 31;
+
+    if (threadIdx.x == 0) {
+        for (int i = 0; i < S; ++i)
+            mbar_init(full + 8 * i, 1), mbar_init(empty + 8 * i, 1);
+        for (int i = 0; i < 2; ++i)
+            mbar_init(accFull + 8 * i, 1), mbar_init(accEmpty + 8 * i, kEpiWarps);
+        mbar_init(drain, 1);
+        mbar_init_fence();
+        abortFlag = 0;
+        for (int i = 0; i < 2; ++i)
+            prefetch_map(&maps.a[i]), prefetch_map(&maps.b[i]);
+    }
+    if (warp == 1) {
+        tmem_alloc(smem_u32(&tmemSlot), 2 * BN);
+        tmem_relinquish();
+        tc_fence_before();
+    }
+    __syncthreads();
+    tc_fence_after();
+    const uint32_t tmem = *const_cast<volatile uint32_t*>(&tmemSlot);
+    volatile int* abort = &abortFlag;
+    pdl_wait();
+    pdl_launch_dependents();
+
+    long long rowEnd = p.M;
+    if (p.num_blocks_dev != nullptr)
+        rowEnd = min(rowEnd, (long long)max(*p.num_blocks_dev, 0) * p.rowsPerBlock);
+    const int mTiles = (int)((rowEnd + kTileM - 1) / kTileM);
+    const int tiles = mTiles * p.nTiles * p.batch * p.splits;
+    const int kAll = p.kIters * p.segs;
+
+    if (warp == 0 && lane == 0) {
+        // ---- producer ----
+        uint32_t issued = 0;
+        bool ok = true;
+        for (int t = blockIdx.x; ok && t < tiles; t += gridDim.x) {
+            const Tile w = tile_at(t, p, mTiles);
+            const int k0 = (int)((long long)kAll * w.s / p.splits), k1 = (int)((long long)kAll * (w.s + 1) / p.splits);
+            for (int k = k0; k < k1; ++k, ++issued) {
+                const uint32_t st = issued % S, turn = issued / S;
+                if (turn > 0 && !mbar_wait_bounded(empty + 8 * st, (turn - 1) & 1, abort, &g_ffn_timeouts)) {
+                    ok = false;
+                    break;
+                }
+                const int seg = p.segs > 1 ? k / p.kIters : 0;
+                const int kk = (k - seg * p.kIters) * kStepK;
+                const int which = p.segs > 1 ? seg : w.z;
+                const uint32_t a = smem + st * kStageBytes<BN>, b = a + kTileM * kStepK * 2, bar = full + 8 * st;
+                mbar_expect_tx(bar, kStageBytes<BN>);
+                if (A_MN) {
+                    for (int i = 0; i < kTileM / 64; ++i)
+                        tma_load_2d(a + i * 8192, &maps.a[which], w.m * kTileM + i * 64, kk, bar);
+                } else {
+                    tma_load_2d(a, &maps.a[which], kk, w.m * kTileM, bar);
+                }
+                if (EPI == kGate) {
+                    tma_load_2d(b, &maps.b[0], kk, w.n * 128, bar);
+                    tma_load_2d(b + 128 * kStepK * 2, &maps.b[1], kk, w.n * 128, bar);
+                } else if (B_MN) {
+                    for (int i = 0; i < BN / 64; ++i)
+                        tma_load_2d(b + i * 8192, &maps.b[which], w.n * BN + i * 64, kk, bar);
+                } else {
+                    tma_load_2d(b, &maps.b[which], kk, w.n * BN, bar);
+                }
+            }
+        }
+        if (*abort) {   // shared memory is not given back with copies in flight
+            int own = 0;
+            for (uint32_t i = issued > S ? issued - S : 0; i < issued; ++i)
+                mbar_wait_bounded(full + 8 * (i % S), (i / S) & 1, &own, &g_ffn_timeouts);
+        }
+    } else if (warp == 1 && lane == 0) {
+        // ---- matrix instructions ----
+        constexpr uint32_t idesc0 = instr_desc<A_MN, B_MN>(0, BN), idesc1 = instr_desc<A_MN, B_MN>(1, BN);
+        constexpr uint32_t idesc = sizeof(T) == 2 && std::is_same<T, __nv_bfloat16>::value ? idesc1 : idesc0;
+        uint32_t used = 0, turn = 0;
+        bool ok = true;
+        for (int t = blockIdx.x; ok && t < tiles; t += gridDim.x, ++turn) {
+            const Tile w = tile_at(t, p, mTiles);
+            const int k0 = (int)((long long)kAll * w.s / p.splits), k1 = (int)((long long)kAll * (w.s + 1) / p.splits);
+            const uint32_t acc = turn & 1, d = tmem + acc * BN;
+            if (turn > 1 && !mbar_wait_bounded(accEmpty + 8 * acc, ((turn >> 1) - 1) & 1, abort, &g_ffn_timeouts))
+                break;
+            tc_fence_after();
+            for (int k = k0; k < k1; ++k, ++used) {
+                const uint32_t st = used % S;
+                if (!mbar_wait_bounded(full + 8 * st, (used / S) & 1, abort, &g_ffn_timeouts)) {
+                    ok = false;
+                    break;
+                }
+                tc_fence_after();
+                const uint32_t a = smem + st * kStageBytes<BN>;
+                const uint64_t da = operand_desc<A_MN>(a), db = operand_desc<B_MN>(a + kTileM * kStepK * 2);
+#pragma unroll
+                for (int j = 0; j < kStepK / 16; ++j)
+                    mma_f16(d, da + j * kDescStep<A_MN>, db + j * kDescStep<B_MN>, idesc, k > k0 || j > 0);
+                mma_commit(empty + 8 * st);
+            }
+            if (ok)
+                mma_commit(accFull + 8 * acc);
+        }
+        if (*abort) {
+            int own = 0;
+            mma_commit(drain);
+            mbar_wait_bounded(drain, 0, &own, &g_ffn_timeouts);
+        }
+    } else if (warp >= 2) {
+        // ---- epilogue: warp w may touch TMEM lanes 32 (w % 4) ..; two warps share each quarter, half the columns each ----
+        const int quarter = warp & 3, half = (warp - 2) >> 2;
+        const uint32_t buf0 = staging + (warp - 2) * 4096, buf1 = buf0 + 2048;
+        uint32_t turn = 0;
+        for (int t = blockIdx.x; t < tiles; t += gridDim.x, ++turn) {
+            const Tile w = tile_at(t, p, mTiles);
+            const uint32_t acc = turn & 1, d = tmem + acc * BN + ((uint32_t)(quarter * 32) << 16);
+            if (!mbar_wait_bounded(accFull + 8 * acc, (turn >> 1) & 1, abort, &g_ffn_timeouts))
+                break;
+            tc_fence_after();
+            const long long row0 = (long long)w.m * kTileM + quarter * 32;
+            if (p.splits > 1) {
+                float* part = p.partials + ((long long)w.s * p.batch + w.z) * p.mTiles * kTileM * (p.nTiles * BN) +
+                              (row0 + lane) * (p.nTiles * BN) + w.n * BN + half * (BN / 2);
+#pragma unroll 1
+                for (int c = 0; c < BN / 2; c += 32) {
+                    uint32_t v[32];
+                    tmem_load32(d + half * (BN / 2) + c, v);
+                    tmem_wait_load();
+#pragma unroll
+                    for (int i = 0; i < 8; ++i)
+                        *reinterpret_cast<uint4*>(part + c + 4 * i) = make_uint4(v[4 * i], v[4 * i + 1], v[4 * i + 2], v[4 * i + 3]);
+                }
+            } else if (EPI == kGate) {
+#pragma unroll 1
+                for (int c = half * 64; c < half * 64 + 64; c += 32) {
+                    uint32_t g[32], u[32], h[16];
+                    tmem_load32(d + c, g);
+                    tmem_load32(d + 128 + c, u);
+                    tmem_wait_load();
+                    if (p.act == kSilu)
+                        gate_chunk<T, kSilu>(g, u, h);
+                    else if (p.act == kGelu)
+                        gate_chunk<T, kGelu>(g, u, h);
+                    else
+                        gate_chunk<T, kRelu>(g, u, h);
+                    const int col = w.n * 128 + c;
+                    stage_rows(buf0, lane, h);
+                    if (p.gate != nullptr) {
+#pragma unroll
+                        for (int i = 0; i < 16; ++i)
+                            h[i] = pack2<T>(__uint_as_float(g[2 * i]), __uint_as_float(g[2 * i + 1]));
+                        stage_rows(buf1, lane, h);
+                    }
+                    __syncwarp();
+                    store_tile<T>(static_cast<T*>(p.out[0]), p.ldo, row0, rowEnd, col, p.N, true, buf0, lane);
+                    if (p.gate != nullptr) {
+                        store_tile<T>(static_cast<T*>(p.gate), p.ldh, row0, rowEnd, col, p.N, true, buf1, lane);
+#pragma unroll
+                        for (int i = 0; i < 16; ++i)
+                            h[i] = pack2<T>(__uint_as_float(u[2 * i]), __uint_as_float(u[2 * i + 1]));
+                        __syncwarp();
+                        stage_rows(buf0, lane, h);
+                        __syncwarp();
+                        store_tile<T>(static_cast<T*>(p.up), p.ldh, row0, rowEnd, col, p.N, true, buf0, lane);
+                    }
+                    __syncwarp();
+                }
+            } else if (EPI == kGrad) {
+#pragma unroll 1
+                for (int c = half * (BN / 2); c < (half + 1) * (BN / 2); c += 32) {
+                    const int col = w.n * BN + c;
+                    uint32_t dh[32], g[16], u[16], h[16];
+                    load_tile<T>(static_cast<const T*>(p.gate), p.ldh, row0, rowEnd, col, p.N, buf0, lane);
+                    load_tile<T>(static_cast<const T*>(p.up), p.ldh, row0, rowEnd, col, p.N, buf1, lane);
+                    tmem_load32(d + c, dh);
+                    tmem_wait_load();
+                    __syncwarp();
+                    unstage_rows(buf0, lane, g);
+                    unstage_rows(buf1, lane, u);
+                    if (p.act == kSilu)
+                        grad_chunk<T, kSilu>(dh, g, u, h);
+                    else if (p.act == kGelu)
+                        grad_chunk<T, kGelu>(dh, g, u, h);
+                    else
+                        grad_chunk<T, kRelu>(dh, g, u, h);
+                    __syncwarp();
+                    stage_rows(buf0, lane, g);
+                    stage_rows(buf1, lane, u);
+                    __syncwarp();
+                    store_tile<T>(static_cast<T*>(p.dgate), p.ldh, row0, rowEnd, col, p.N, true, buf0, lane);
+                    store_tile<T>(static_cast<T*>(p.dup), p.ldh, row0, rowEnd, col, p.N, true, buf1, lane);
+                    __syncwarp();
+                    stage_rows(buf0, lane, h);
+                    __syncwarp();
+                    store_tile<T>(static_cast<T*>(p.hid), p.ldh, row0, rowEnd, col, p.N, true, buf0, lane);
+                    __syncwarp();
+                }
+            } else {
+                T* out = static_cast<T*>(p.out[w.z]);
+                const bool wide = ((p.ldo & 7) == 0) && (reinterpret_cast<uintptr_t>(out) & 15) == 0;
+#pragma unroll 1
+                for (int c = half * (BN / 2); c < (half + 1) * (BN / 2); c += 32) {
+                    uint32_t v[32], h[16];
+                    tmem_load32(d + c, v);
+                    tmem_wait_load();
+#pragma unroll
+                    for (int i = 0; i < 16; ++i)
+                        h[i] = pack2<T>(__uint_as_float(v[2 * i]), __uint_as_float(v[2 * i + 1]));
+                    stage_rows(buf0, lane, h);
+                    __syncwarp();
+                    store_tile<T>(out, p.ldo, row0, rowEnd, w.n * BN + c, p.N, wide, buf0, lane);
+                    __syncwarp();
+                }
+            }
+            tc_fence_before();
+            if (lane == 0)
+                mbar_arrive(accEmpty + 8 * acc);
+        }
+    }
+    __syncthreads();
+    if (warp == 1) {
+        __syncwarp();
+        tc_fence_after();
+        tmem_free(tmem, 2 * BN);
+    }
+}
+
+// Adds the partial sums of a split reduction in the order of the pieces and finishes the elements as the epilogue
+// would have.  One thread per element.
+template <typename T, int EPI> __global__ void __launch_bounds__(256) finish_kernel(const __grid_constant__ Plan p, int bn)
+{
+    pdl_wait();
+    pdl_launch_dependents();
+    long long rowEnd = p.M;
+    if (p.num_blocks_dev != nullptr)
+        rowEnd = min(rowEnd, (long long)max(*p.num_blocks_dev, 0) * p.rowsPerBlock);
+    const long long pitch = (long long)p.nTiles * bn, plane = (long long)p.mTiles * kTileM * pitch;
+    const long long n = rowEnd * p.N;
+    for (long long i = (long long)blockIdx.x * 256 + threadIdx.x; i < n * p.batch; i += (long long)gridDim.x * 256) {
+        const int z = (int)(i / n);
+        const long long row = (i - z * n) / p.N;
+        const int col = (int)((i - z * n) - row * p.N);
+        if (EPI == kGate) {
+            const float* q = p.partials + row * pitch + (col >> 7) * 256 + (col & 127);
+            float g = 0.f, u = 0.f, unused;
+            for (int s = 0; s < p.splits; ++s)
+                g += q[s * plane], u += q[s * plane + 128];
+            const float a = p.act == kSilu   ? activate<kSilu, false>(g, unused)
+                            : p.act == kGelu ? activate<kGelu, false>(g, unused)
+                                             : activate<kRelu, false>(g, unused);
+            static_cast<T*>(p.out[0])[row * p.ldo + col] = T(a * u);
+            if (p.gate != nullptr) {
+                static_cast<T*>(p.gate)[row * p.ldh + col] = T(g);
+                static_cast<T*>(p.up)[row * p.ldh + col] = T(u);
+            }
+        } else {
+            const float* q = p.partials + z * plane + row * pitch + col;
+            float v = 0.f;
+            for (int s = 0; s < p.splits; ++s)
+                v += q[s * p.batch * plane];
+            static_cast<T*>(p.out[z])[row * p.ldo + col] = T(v);
+        }
+    }
+}
+
+// Rows of `cols` 16-bit elements, pitch `cols` -> pitch `ld` (a multiple of 8).  One warp per row.
+__global__ void __launch_bounds__(256) repack_kernel(const uint16_t* src, long long rows, int cols, uint16_t* dst, int ld)
+{
+    pdl_wait();
+    pdl_launch_dependents();
+    const int lane = threadIdx.x & 31;
+    for (long long r = (long long)blockIdx.x * 8 + (threadIdx.x >> 5); r < rows; r += (long long)gridDim.x * 8)
+        for (int c = lane; c < cols; c += 32)
+            dst[r * ld + c] = src[r * cols + c];
+}
+
+// ---- host side -------------------------------------------------------------------------------------------
+PFN_cuTensorMapEncodeTiled encoder()
+{
+    static const PFN_cuTensorMapEncodeTiled fn = [] {
+        void* ptr = nullptr;
+        cudaDriverEntryPointQueryResult q;
+        if (cudaGetDriverEntryPoint("cuTensorMapEncodeTiled", &ptr, cudaEnableDefault, &q) == cudaSuccess &&
+            q == cudaDriverEntryPointSuccess)
+            return reinterpret_cast<PFN_cuTensorMapEncodeTiled>(ptr);
+        (void)cudaGetLastError();
+        return static_cast<PFN_cuTensorMapEncodeTiled>(nullptr);
+    }();
+    return fn;
+}
+
+// A row-major matrix of 16-bit elements as TMA reads it: boxes of 64 columns x boxRows rows.
+struct Matrix {
+    const void* ptr;
+    long long rows;
+    int cols;
+    long long ld;
+};
+cudaError_t encode(const Matrix& m, int boxRows, CUtensorMap* out)
+{
+    PFN_cuTensorMapEncodeTiled enc = encoder();
+    if (enc == nullptr)
+        return cudaErrorNotSupported;
+    const cuuint64_t dims[2] = {(cuuint64_t)m.cols, (cuuint64_t)m.rows}, strides[1] = {(cuuint64_t)m.ld * 2};
+    const cuuint32_t box[2] = {(cuuint32_t)kStepK, (cuuint32_t)boxRows}, estr[2] = {1, 1};
+    return enc(out, CU_TENSOR_MAP_DATA_TYPE_UINT16, 2, const_cast<void*>(m.ptr), dims, strides, box, estr,
+               CU_TENSOR_MAP_INTERLEAVE_NONE, CU_TENSOR_MAP_SWIZZLE_128B, CU_TENSOR_MAP_L2_PROMOTION_L2_256B,
+               CU_TENSOR_MAP_FLOAT_OOB_FILL_NONE) == CUDA_SUCCESS
+               ? cudaSuccess
+               : cudaErrorInvalidValue;
+}
+
+int ceil_div(long long a, long long b) { return (int)((a + b - 1) / b); }
+
+// Column tile of a plain product: 256 wide unless the matrix is narrow.
+int tile_n(int N) { return N <= 128 ? 128 : 256; }
+
+// Pieces of the reduction.  One piece fills the machine when there are enough tiles; with fewer, the pieces make
+// up for it as long as each keeps at least four stages.  `most`: what the caller's workspace can hold.
+int split_count(long long tiles, int kIters)
+{
+    const int sms = sm_count();
+    if (tiles * 2 > sms)
+        return 1;
+    return (int)std::max<long long>(1, std::min<long long>(sms / tiles, kIters / 4));
+}
+
+template <typename T, bool A_MN, bool B_MN, int EPI, int BN>
+cudaError_t launch_gemm(const Matrix (&a)[2], const Matrix (&b)[2], Plan& p, cudaStream_t stream)
+{
+    Maps maps;
+    const int n = std::max(p.batch, std::max(p.segs, EPI == kGate ? 2 : 1));
+    for (int i = 0; i < 2; ++i) {
+        const int j = i < n ? i : 0;
+        if (cudaError_t e = encode(a[EPI == kGate ? 0 : j], A_MN ? kStepK : kTileM, &maps.a[i]))
+            return e;
+        if (cudaError_t e = encode(b[j], B_MN ? kStepK : (EPI == kGate ? 128 : BN), &maps.b[i]))
+            return e;
+    }
+    auto kernel = gemm_kernel<T, A_MN, B_MN, EPI, BN>;
+    if (cudaError_t e = cudaFuncSetAttribute(kernel, cudaFuncAttributeMaxDynamicSharedMemorySize, kGemmSmem<BN>))
+        return e;
+    const long long tiles = (long long)p.mTiles * p.nTiles * p.batch * p.splits;
+    const int grid = (int)std::min<long long>(tiles, sm_count());
+    if (cudaError_t e = launch_pdl(kernel, dim3(grid), dim3(kGemmThreads), kGemmSmem<BN>, stream, maps, p))
+        return e;
+    if (p.splits == 1)
+        return cudaSuccess;
+    const long long items = p.M * p.N * p.batch;
+    const int fgrid = (int)std::min<long long>((items + 255) / 256, (long long)sm_count() * 8);
+    if constexpr (EPI != kGrad)
+        return launch_pdl(finish_kernel<T, EPI>, dim3(fgrid), dim3(256), 0, stream, p, BN);
+    return cudaErrorInvalidValue;
+}
+
+// A plain product D[m,n] of one or two products (batch) or segments.
+template <typename T, bool A_MN, bool B_MN>
+cudaError_t product(const Matrix (&a)[2], const Matrix (&b)[2], int batch, int segs, long long M, int N, long long K,
+                    void* out0, void* out1, float* partials, const FfnArgs& f, bool rowsOfX, cudaStream_t stream)
+{
+    Plan p = {};
+    const int bn = tile_n(N);
+    p.mTiles = ceil_div(M, kTileM), p.nTiles = ceil_div(N, bn), p.batch = batch, p.segs = segs;
+    p.kIters = ceil_div(K, kStepK);
+    p.splits = split_count((long long)p.mTiles * p.nTiles * batch, p.kIters * segs);
+    p.N = N, p.M = M, p.out[0] = out0, p.out[1] = out1, p.ldo = N, p.partials = partials;
+    if (rowsOfX)
+        p.num_blocks_dev = f.num_blocks_dev, p.rowsPerBlock = f.rowsPerBlock;
+    return bn == 128 ? launch_gemm<T, A_MN, B_MN, kStore, 128>(a, b, p, stream)
+                     : launch_gemm<T, A_MN, B_MN, kStore, 256>(a, b, p, stream);
+}
+size_t product_partials(int batch, int segs, long long M, int N, long long K)
+{
+    const int bn = tile_n(N);
+    const long long mT = ceil_div(M, kTileM), nT = ceil_div(N, bn);
+    const int s = split_count(mT * nT * batch, ceil_div(K, kStepK) * segs);
+    return s == 1 ? 0 : sizeof(float) * s * batch * mT * kTileM * nT * bn;
+}
+size_t gate_partials(long long R, int F, int C)
+{
+    const long long mT = ceil_div(R, kTileM), nT = ceil_div(F, 128);
+    const int s = split_count(mT * nT, ceil_div(C, kStepK));
+    return s == 1 ? 0 : sizeof(float) * s * mT * kTileM * nT * 256;
+}
+
+// Hands out the caller's workspace in 256-byte aligned pieces; without a base it only counts.
+struct Bump {
+    uint8_t* base;
+    size_t used;
+    void* take(size_t bytes)
+    {
+        void* p = base == nullptr ? nullptr : base + used;
+        used += (bytes + 255) & ~(size_t)255;
+        return p;
+    }
+};
+int padded(int n) { return (n + 7) & ~7; }
+
+struct Layout {
+    Bump bump;
+    bool aligned;      // base addresses are multiples of 16
+    // pitch at which a [rows, cols] input is read, and room for a copy where that is not its own pitch
+    Matrix plan(const void* src, long long rows, int cols)
+    {
+        Matrix m = {src, rows, cols, cols};
+        const bool fits = cols % 8 == 0 && (bump.base == nullptr ? aligned : (reinterpret_cast<uintptr_t>(src) & 15) == 0);
+        if (!fits) {
+            m.ld = padded(cols);
+            m.ptr = bump.take((size_t)rows * m.ld * 2);
+        }
+        return m;
+    }
+};
+cudaError_t repack(const void* src, const Matrix& m, cudaStream_t stream)
+{
+    if (m.ptr == src)
+        return cudaSuccess;
+    const int grid = (int)std::min<long long>((m.rows + 7) / 8, (long long)sm_count() * 8);
+    return launch_pdl(repack_kernel, dim3(grid), dim3(256), 0, stream, static_cast<const uint16_t*>(src), m.rows, m.cols,
+                      static_cast<uint16_t*>(const_cast<void*>(m.ptr)), (int)m.ld);
+}
+
+#define SBNET_TRY(call)                  \
+    do {                                 \
+        if (cudaError_t e_ = (call))     \
+            return e_;                   \
+    } while (0)
+
+// run == false: only counts the workspace.
+template <typename T> cudaError_t forward(const FfnArgs& f, Layout& l, bool run, cudaStream_t stream)
+{
+    const long long R = f.rows;
+    const int C = f.C, F = f.F, Fp = padded(F);
+    const Matrix x = l.plan(f.x, R, C), wg = l.plan(f.w_gate, F, C), wu = l.plan(f.w_up, F, C), wd = l.plan(f.w_down, C, F);
+    const Matrix h = {l.bump.take((size_t)R * Fp * 2), R, F, Fp};
+    float* parts = static_cast<float*>(l.bump.take(std::max(gate_partials(R, F, C), product_partials(1, 1, R, C, F))));
+    if (!run)
+        return cudaSuccess;
+    note_site("gated_ffn repack");
+    SBNET_TRY(repack(f.x, x, stream));
+    SBNET_TRY(repack(f.w_gate, wg, stream));
+    SBNET_TRY(repack(f.w_up, wu, stream));
+    SBNET_TRY(repack(f.w_down, wd, stream));
+    note_site("gated_ffn projections");
+    Plan p = {};
+    p.mTiles = ceil_div(R, kTileM), p.nTiles = ceil_div(F, 128), p.batch = 1, p.segs = 1, p.kIters = ceil_div(C, kStepK);
+    p.splits = split_count((long long)p.mTiles * p.nTiles, p.kIters);
+    p.N = F, p.M = R, p.num_blocks_dev = f.num_blocks_dev, p.rowsPerBlock = f.rowsPerBlock, p.act = f.act;
+    p.out[0] = const_cast<void*>(h.ptr), p.ldo = Fp, p.gate = f.gate, p.up = f.up, p.ldh = Fp, p.partials = parts;
+    SBNET_TRY((launch_gemm<T, false, false, kGate, 256>({x, x}, {wg, wu}, p, stream)));
+    note_site("gated_ffn output");
+    return product<T, false, false>({h, h}, {wd, wd}, 1, 1, R, C, F, f.y, nullptr, parts, f, true, stream);
+}
+
+template <typename T> cudaError_t backward(const FfnArgs& f, Layout& l, bool run, cudaStream_t stream)
+{
+    const long long R = f.rows;
+    const int C = f.C, F = f.F, Fp = padded(F);
+    const Matrix x = l.plan(f.x, R, C), dy = l.plan(f.dy, R, C), wg = l.plan(f.w_gate, F, C), wu = l.plan(f.w_up, F, C),
+                 wd = l.plan(f.w_down, C, F);
+    const size_t mid = (size_t)R * Fp * 2;
+    const Matrix dg = {l.bump.take(mid), R, F, Fp}, du = {l.bump.take(mid), R, F, Fp}, h = {l.bump.take(mid), R, F, Fp};
+    float* parts = static_cast<float*>(l.bump.take(std::max(
+        product_partials(1, 2, R, C, F), std::max(product_partials(2, 1, F, C, R), product_partials(1, 1, C, F, R)))));
+    if (!run)
+        return cudaSuccess;
+    note_site("gated_ffn_grad repack");
+    SBNET_TRY(repack(f.x, x, stream));
+    SBNET_TRY(repack(f.dy, dy, stream));
+    SBNET_TRY(repack(f.w_gate, wg, stream));
+    SBNET_TRY(repack(f.w_up, wu, stream));
+    SBNET_TRY(repack(f.w_down, wd, stream));
+    note_site("gated_ffn_grad hidden gradients");
+    Plan p = {};
+    p.mTiles = ceil_div(R, kTileM), p.nTiles = ceil_div(F, 256), p.batch = 1, p.segs = 1, p.kIters = ceil_div(C, kStepK);
+    p.splits = 1, p.N = F, p.M = R, p.act = f.act;
+    p.gate = f.gate, p.up = f.up, p.ldh = Fp;
+    p.dgate = const_cast<void*>(dg.ptr), p.dup = const_cast<void*>(du.ptr), p.hid = const_cast<void*>(h.ptr);
+    SBNET_TRY((launch_gemm<T, false, true, kGrad, 256>({dy, dy}, {wd, wd}, p, stream)));
+    if (f.dx != nullptr) {
+        note_site("gated_ffn_grad dx");
+        SBNET_TRY((product<T, false, true>({dg, du}, {wg, wu}, 1, 2, R, C, F, f.dx, nullptr, parts, f, false, stream)));
+    }
+    if (f.dw_gate != nullptr) {
+        note_site("gated_ffn_grad dw_gate, dw_up");
+        SBNET_TRY((product<T, true, true>({dg, du}, {x, x}, 2, 1, F, C, R, f.dw_gate, f.dw_up, parts, f, false, stream)));
+    }
+    if (f.dw_down != nullptr) {
+        note_site("gated_ffn_grad dw_down");
+        SBNET_TRY((product<T, true, true>({dy, dy}, {h, h}, 1, 1, C, F, R, f.dw_down, nullptr, parts, f, false, stream)));
+    }
+    return cudaSuccess;
+}
+
+} // namespace
+
+size_t gated_ffn_workspace(long long rows, int C, int F, bool grad, bool aligned)
+{
+    FfnArgs f = {};
+    f.rows = rows, f.C = C, f.F = F;
+    Layout l = {{nullptr, 0}, aligned};
+    if (grad)
+        backward<__half>(f, l, false, nullptr);
+    else
+        forward<__half>(f, l, false, nullptr);
+    return l.bump.used;
+}
+
+cudaError_t launch_gated_ffn(const FfnArgs& f, int dtype, cudaStream_t stream)
+{
+    Layout l = {{static_cast<uint8_t*>(f.workspace), 0}, true};
+    return dtype == 1 ? forward<__half>(f, l, true, stream) : forward<__nv_bfloat16>(f, l, true, stream);
+}
+
+cudaError_t launch_gated_ffn_grad(const FfnArgs& f, int dtype, cudaStream_t stream)
+{
+    Layout l = {{static_cast<uint8_t*>(f.workspace), 0}, true};
+    return dtype == 1 ? backward<__half>(f, l, true, stream) : backward<__nv_bfloat16>(f, l, true, stream);
+}
+
+cudaError_t read_ffn_wait_timeouts(unsigned int* out) { return cudaMemcpyFromSymbol(out, g_ffn_timeouts, sizeof(*out)); }
+
+} // namespace sbnet

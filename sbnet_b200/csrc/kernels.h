@@ -53,6 +53,24 @@ cudaError_t launch_layer_norm(const NormArgs& a, int dtype, cudaStream_t stream)
 cudaError_t launch_layer_norm_grad(const NormArgs& a, int dtype, cudaStream_t stream);
 int layer_norm_grad_parts(long long rows, int C);
 
+// The gated feed-forward block (gated_ffn.cu): 16-bit types only.  act: 0 silu, 1 gelu (erf), 2 relu.
+struct FfnArgs {
+    const void* x;                             // [rows, C]
+    const void *w_gate, *w_up, *w_down;        // [F, C], [F, C], [C, F]
+    void* y;                                   // forward: [rows, C]
+    void *gate, *up;                           // [rows, F rounded up to 8]: forward writes them unless null, backward reads
+    const void* dy;                            // backward: [rows, C]
+    void *dx, *dw_gate, *dw_up, *dw_down;      // backward: written unless null (dw_gate and dw_up go together)
+    const int32_t* num_blocks_dev;             // forward: live blocks of rowsPerBlock rows, or nullptr (all rows)
+    void* workspace;                           // gated_ffn_workspace() bytes, 256-byte aligned
+    long long rows;
+    int rowsPerBlock, C, F, act;
+};
+size_t gated_ffn_workspace(long long rows, int C, int F, bool grad, bool aligned);
+cudaError_t launch_gated_ffn(const FfnArgs& f, int dtype, cudaStream_t stream);
+cudaError_t launch_gated_ffn_grad(const FfnArgs& f, int dtype, cudaStream_t stream);
+cudaError_t read_ffn_wait_timeouts(unsigned int* out);
+
 int sm_count();
 
 // Sets the calling thread's sbnet_last_error() text.

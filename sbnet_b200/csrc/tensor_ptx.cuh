@@ -1,0 +1,89 @@
+// Thin wrappers over the tcgen05 (fifth-generation tensor core) and TMEM instructions, shared-memory
+// operand descriptors and two-dimensional TMA loads used by the matrix kernels.  sm_100a only.
+#pragma once
+#include "async_ptx.cuh"
+
+namespace sbnet {
+
+// ---- tensor memory -------------------------------------------------------------------------------
+// Whole-warp calls; `cols` is a power of two >= 32.  The warp that allocates also frees.
+__device__ __forceinline__ void tmem_alloc(uint32_t slot, uint32_t cols)
+{
+    asm volatile("tcgen05.alloc.cta_group::1.sync.aligned.shared::cta.b32 [%0], %1;" ::"r"(slot), "r"(cols) : "memory");
+}
+__device__ __forceinline__ void tmem_relinquish()
+{
+    asm volatile("tcgen05.relinquish_alloc_permit.cta_group::1.sync.aligned;" ::: "memory");
+}
+__device__ __forceinline__ void tmem_free(uint32_t addr, uint32_t cols)
+{
+    asm volatile("tcgen05.dealloc.cta_group::1.sync.aligned.b32 %0, %1;" ::"r"(addr), "r"(cols) : "memory");
+}
+// 32 lanes x 32 columns of 32-bit words: lane i of the warp gets row i (of the warp's quarter of the lanes).
+__device__ __forceinline__ void tmem_load32(uint32_t addr, uint32_t (&r)[32])
+{
+    asm volatile(
+        "tcgen05.ld.sync.aligned.32x32b.x32.b32 "
+        "{%0,%1,%2,%3,%4,%5,%6,%7,%8,%9,%10,%11,%12,%13,%14,%15,%16,%17,%18,%19,%20,%21,%22,%23,%24,%25,%26,%27,%28,%29,%30,%31}, [%32];"
+        : "=r"(r[0]), "=r"(r[1]), "=r"(r[2]), "=r"(r[3]), "=r"(r[4]), "=r"(r[5]), "=r"(r[6]), "=r"(r[7]), "=r"(r[8]),
+          "=r"(r[9]), "=r"(r[10]), "=r"(r[11]), "=r"(r[12]), "=r"(r[13]), "=r"(r[14]), "=r"(r[15]), "=r"(r[16]), "=r"(r[17]),
+          "=r"(r[18]), "=r"(r[19]), "=r"(r[20]), "=r"(r[21]), "=r"(r[22]), "=r"(r[23]), "=r"(r[24]), "=r"(r[25]), "=r"(r[26]),
+          "=r"(r[27]), "=r"(r[28]), "=r"(r[29]), "=r"(r[30]), "=r"(r[31])
+        : "r"(addr));
+}
+__device__ __forceinline__ void tmem_wait_load() { asm volatile("tcgen05.wait::ld.sync.aligned;" ::: "memory"); }
+
+__device__ __forceinline__ void tc_fence_before() { asm volatile("tcgen05.fence::before_thread_sync;" ::: "memory"); }
+__device__ __forceinline__ void tc_fence_after() { asm volatile("tcgen05.fence::after_thread_sync;" ::: "memory"); }
+
+// ---- matrix multiply ------------------------------------------------------------------------------
+// Shared-memory operand of 16-bit elements in the 128-byte swizzle.  A tile arrives by TMA as boxes of
+// 64 elements (128 bytes) x rows; eight rows (1,024 bytes) are the swizzle's repeating unit.
+//  K-major : a box row is one row of the matrix, 64 steps of the reduction; the next eight rows are 1,024
+//            bytes on (stride offset).  One instruction takes 16 reduction steps: 32 bytes along the row.
+//  MN-major: a box row is one step of the reduction, 64 rows of the matrix; the next eight steps are 1,024
+//            bytes on (stride offset), the next 64 rows are the next box, 64 steps * 128 bytes on (leading
+//            offset).  16 reduction steps are 2,048 bytes.
+template <bool MN> __device__ __forceinline__ uint64_t operand_desc(uint32_t smem)
+{
+    const uint64_t lead = MN ? 8192 >> 4 : 1, stride = 1024 >> 4;
+    return (uint64_t)((smem & 0x3ffff) >> 4) | (lead << 16) | (stride << 32) | (1ull << 46) | (2ull << 61);
+}
+template <bool MN> constexpr uint32_t kDescStep = MN ? 2048 >> 4 : 32 >> 4;
+
+// kind::f16, fp32 accumulators; format 0 = f16, 1 = bf16 (both operands); M = 128.
+template <bool A_MN, bool B_MN> __device__ __forceinline__ constexpr uint32_t instr_desc(int format, int n)
+{
+    return (1u << 4) | ((uint32_t)format << 7) | ((uint32_t)format << 10) | ((A_MN ? 1u : 0u) << 15) |
+           ((B_MN ? 1u : 0u) << 16) | ((uint32_t)(n >> 3) << 17) | (8u << 24);
+}
+__device__ __forceinline__ void mma_f16(uint32_t d, uint64_t a, uint64_t b, uint32_t idesc, bool accumulate)
+{
+    asm volatile(
+        "{\n\t.reg .pred p;\n\t"
+        "setp.ne.u32 p, %4, 0;\n\t"
+        "tcgen05.mma.cta_group::1.kind::f16 [%0], %1, %2, %3, p;\n\t}" ::"r"(d),
+        "l"(a), "l"(b), "r"(idesc), "r"((uint32_t)accumulate)
+        : "memory");
+}
+// Arrives on the barrier once every tcgen05.mma this thread has issued is done.
+__device__ __forceinline__ void mma_commit(uint32_t bar)
+{
+    asm volatile("tcgen05.commit.cta_group::1.mbarrier::arrive::one.shared::cluster.b64 [%0];" ::"r"(bar) : "memory");
+}
+
+// ---- loads ------------------------------------------------------------------------------------------
+// c0 (the contiguous coordinate) times the element size is a multiple of 16 bytes at every call.
+__device__ __forceinline__ void tma_load_2d(uint32_t dst, const CUtensorMap* map, int c0, int c1, uint32_t bar)
+{
+    asm volatile(
+        "cp.async.bulk.tensor.2d.shared::cluster.global.tile.mbarrier::complete_tx::bytes [%0], [%1, {%2, %3}], [%4];" ::"r"(dst),
+        "l"(reinterpret_cast<uint64_t>(map)), "r"(c0), "r"(c1), "r"(bar)
+        : "memory");
+}
+__device__ __forceinline__ void prefetch_map(const CUtensorMap* map)
+{
+    asm volatile("prefetch.tensormap [%0];" ::"l"(reinterpret_cast<uint64_t>(map)) : "memory");
+}
+
+} // namespace sbnet

@@ -19,6 +19,7 @@ SBNET_COUNT_YIELD = 8
 SBNET_COUNT_NOWAIT = 16
 SBNET_COUNT_PENDING = -(2 ** 31)
 SBNET_REDUCE_MASK_SCRATCH_INTS = 4
+SBNET_ACT = {"silu": 0, "gelu": 1, "relu": 2}
 
 _i, _f, _p, _sz, _l = C.c_int, C.c_float, C.c_void_p, C.c_size_t, C.c_int64
 _GEOM = [_i] * 6
@@ -43,6 +44,10 @@ SIGNATURES = {
     "sbnet_layer_norm": (_i, [_p, _i, _l, _i, _p, _p, _i, _f, _p, _p, _p, _p]),
     "sbnet_layer_norm_dyn": (_i, [_p, _i, _l, _i, _p, _i, _p, _p, _i, _f, _p, _p, _p, _p]),
     "sbnet_layer_norm_grad_workspace": (_sz, [_l, _i]),
+    "sbnet_gated_ffn_workspace": (_sz, [_l, _i, _i, _i, _i]),
+    "sbnet_gated_ffn": (_i, [_p, _i, _l, _i, _i, _p, _p, _p, _i, _p, _p, _p, _p, _sz, _p]),
+    "sbnet_gated_ffn_dyn": (_i, [_p, _i, _l, _i, _p, _i, _i, _p, _p, _p, _i, _p, _p, _sz, _p]),
+    "sbnet_gated_ffn_grad": (_i, [_p, _p, _p, _p, _i, _l, _i, _i, _p, _p, _p, _i, _p, _p, _p, _p, _p, _sz, _p]),
     "sbnet_layer_norm_grad": (_i, [_p, _p, _i, _l, _i, _p, _i, _p, _p, _p, _p, _p, _p, _sz, _p]),
 }
 

@@ -490,6 +490,105 @@ def layer_norm_grad(grad: torch.Tensor, x: torch.Tensor, mean: torch.Tensor, rst
     return dx, dw, db
 
 
+def _check_ffn(x, w_gate, w_up, w_down, activation):
+    """Rules of the gated feed-forward block's arguments; returns ``(rows, C, F, activation code)``."""
+    rows, channels = _check_rows(x, "x")
+    if x.dtype == torch.float32:
+        raise ValueError("gated_ffn takes float16 and bfloat16 (the tensor cores' operand types)")
+    act = _lib.SBNET_ACT.get(activation)
+    if act is None:
+        raise ValueError(f"activation must be one of {', '.join(sorted(_lib.SBNET_ACT))}, got {activation!r}")
+    if w_gate.dim() != 2 or w_gate.shape[1] != channels or w_gate.shape[0] < 1:
+        raise ValueError(f"w_gate must be [hidden, {channels}]")
+    hidden = w_gate.shape[0]
+    for t, name, shape in ((w_gate, "w_gate", (hidden, channels)), (w_up, "w_up", (hidden, channels)),
+                           (w_down, "w_down", (channels, hidden))):
+        if t.dim() != 2 or t.shape[0] != shape[0] or t.shape[1] != shape[1]:
+            raise ValueError(f"{name} must be [{shape[0]}, {shape[1]}]")
+        if t.dtype != x.dtype or t.device != x.device or not t.is_contiguous():
+            raise ValueError(f"{name} must be contiguous and of the dtype and device of the input")
+    return rows, channels, hidden, act
+
+
+def _workspace(rows, channels, hidden, grad, tensors, device):
+    """Device memory for one call (the caching allocator's: on the current stream, and a capturing graph's own)."""
+    bits = 0
+    for t in tensors:
+        bits |= t.data_ptr()
+    need = _lib.load().sbnet_gated_ffn_workspace(rows, channels, hidden, grad, int(bits & 15 == 0))
+    return torch.empty(need, dtype=torch.uint8, device=device), need
+
+
+def _gated_ffn_call(x, w_gate, w_up, w_down, activation, out, train, count_dev):
+    rows, channels, hidden, act = _check_ffn(x, w_gate, w_up, w_down, activation)
+    if count_dev is not None:
+        _check_count_dev(count_dev, x)
+        blocks, per = _blocks_of(x)
+    if out is not None:
+        _check_like(out, "out", x)
+    _require_cuda(x, "x")
+    with _on(x.device):
+        y = torch.empty_like(x) if out is None else out
+        gate = up = None
+        if train:
+            both = torch.empty((2, rows, (hidden + 7) // 8 * 8), dtype=x.dtype, device=x.device)
+            gate, up = both[0], both[1]
+        ws, need = _workspace(rows, channels, hidden, 0, (x, w_gate, w_up, w_down), x.device)
+        head = (channels, hidden, w_gate.data_ptr(), w_up.data_ptr(), w_down.data_ptr(), act, y.data_ptr())
+        tail = (ws.data_ptr(), need, _stream(x.device))
+        if count_dev is None:
+            _lib.check(_lib.load().sbnet_gated_ffn(x.data_ptr(), _DTYPES[x.dtype], rows, *head, _ptr(gate), _ptr(up), *tail))
+        else:
+            _lib.check(_lib.load().sbnet_gated_ffn_dyn(x.data_ptr(), _DTYPES[x.dtype], blocks, per, count_dev.data_ptr(),
+                                                       *head, *tail))
+    return (y, gate, up) if train else y
+
+
+def gated_ffn(x: torch.Tensor, w_gate: torch.Tensor, w_up: torch.Tensor, w_down: torch.Tensor, activation: str = "silu",
+              out=None) -> torch.Tensor:
+    """Gated feed-forward block over the rows of ``x`` (``[..., C]``, float16 or bfloat16):
+    ``(act(x @ w_gate.T) * (x @ w_up.T)) @ w_down.T`` with ``w_gate``, ``w_up`` ``[F, C]`` and ``w_down``
+    ``[C, F]`` of the same type; ``activation``: "silu", "gelu" (by the error function) or "relu".  Sums are fp32,
+    the gated product is rounded to the type of ``x`` once.  ``out`` must not overlap an input."""
+    return _gated_ffn_call(x, w_gate, w_up, w_down, activation, out, False, None)
+
+
+def gated_ffn_dyn(x: torch.Tensor, count_dev: torch.Tensor, w_gate, w_up, w_down, activation: str = "silu", out=None):
+    """:func:`gated_ffn` of the first ``count_dev[0]`` blocks of a stack ``[maxBlocks, ..., C]``, the count read on
+    the device; the rest of the result (of ``out``) is left as it was."""
+    if count_dev is None:
+        raise ValueError("count_dev must be an int32 tensor with at least one element")
+    return _gated_ffn_call(x, w_gate, w_up, w_down, activation, out, False, count_dev)
+
+
+def gated_ffn_train(x: torch.Tensor, w_gate, w_up, w_down, activation: str = "silu"):
+    """:func:`gated_ffn` that also returns what :func:`gated_ffn_grad` needs: ``(y, gate, up)``, the two
+    projections as ``[rows, F rounded up to a multiple of 8]`` (columns past F are undefined)."""
+    return _gated_ffn_call(x, w_gate, w_up, w_down, activation, None, True, None)
+
+
+def gated_ffn_grad(grad: torch.Tensor, x: torch.Tensor, gate: torch.Tensor, up: torch.Tensor, w_gate, w_up, w_down,
+                   activation: str = "silu", need_x: bool = True, need_gate_up: bool = True, need_down: bool = True):
+    """Backward pass of :func:`gated_ffn_train`: ``(dx, dw_gate, dw_up, dw_down)``, None where not asked for."""
+    rows, channels, hidden, act = _check_ffn(x, w_gate, w_up, w_down, activation)
+    _check_like(grad, "grad", x)
+    for t, name in ((gate, "gate"), (up, "up")):
+        if tuple(t.shape) != (rows, (hidden + 7) // 8 * 8) or t.dtype != x.dtype or t.device != x.device or not t.is_contiguous():
+            raise ValueError(f"{name} must be what gated_ffn_train returned")
+    _require_cuda(x, "x")
+    with _on(x.device):
+        dx = torch.empty_like(x) if need_x else None
+        dwg = torch.empty_like(w_gate) if need_gate_up else None
+        dwu = torch.empty_like(w_up) if need_gate_up else None
+        dwd = torch.empty_like(w_down) if need_down else None
+        ws, need = _workspace(rows, channels, hidden, 1, (grad, x, w_gate, w_up, w_down), x.device)
+        _lib.check(_lib.load().sbnet_gated_ffn_grad(
+            grad.data_ptr(), x.data_ptr(), gate.data_ptr(), up.data_ptr(), _DTYPES[x.dtype], rows, channels, hidden,
+            w_gate.data_ptr(), w_up.data_ptr(), w_down.data_ptr(), act, _ptr(dx), _ptr(dwg), _ptr(dwu), _ptr(dwd),
+            ws.data_ptr(), need, _stream(x.device)))
+    return dx, dwg, dwu, dwd
+
+
 # ---- pre-validated calls for hot loops ---------------------------------------------------------------
 # The wrappers above re-check every argument on every call (about 7 us of interpreter time each, beside
 # the ~5 us of the foreign call itself).  A loop that calls the same op on the same buffers with the
