@@ -17,11 +17,13 @@
 // G, U, H, dG and dU are held between kernels in the type of X (they are operands of the next product, and the
 // tensor cores multiply 16-bit types); accumulators and every element-wise step are fp32.
 //
-// Structure: persistent CTAs (one per SM) over 128 x 256 (or 128 x 128) output tiles; one thread feeds a ring of
-// shared-memory stages by TMA (64 reduction steps each, 128-byte swizzle; rows and columns past the matrix read
-// as zero), one thread issues tcgen05.mma, eight warps run the epilogue on one TMEM accumulator while the other
-// is being filled.  Tiles are walked in groups of 16 row tiles so that the operands of neighbouring CTAs meet in
-// L2.  Where a product has fewer tiles than the GPU has SMs, the reduction is split: every piece writes fp32
+// Structure: persistent pairs of CTAs (one CTA per SM) over 256 x 256 (or 256 x 128) output tiles.  A pair
+// multiplies as one (cta_group::2): each CTA holds its own 128 rows of A and half of B, so a stage of 64
+// reduction steps costs 32 KB of L2 reads per SM where single CTAs with 128 x 256 tiles need 48 KB.  In each
+// CTA one thread feeds a ring of shared-memory stages by TMA (128-byte swizzle; rows and columns past the
+// matrix read as zero); one thread of the first CTA issues tcgen05.mma; eight warps run the epilogue on one
+// TMEM accumulator while the other is being filled.  Tiles are walked in groups of 8 row tiles so that the
+// operands of neighbouring pairs meet in L2.  Where a product has fewer tiles than the GPU has SMs, the reduction is split: every piece writes fp32
 // partial sums to the workspace and a second kernel adds them in a fixed order (no atomics: the same call gives
 // the same bits).
 //
@@ -42,12 +44,13 @@
 namespace sbnet {
 namespace {
 
-constexpr int kTileM = 128;
+constexpr int kTileM = 256;                      // rows of a tile
+constexpr int kCtaM = 128;                       // ... in each CTA of the pair
 constexpr int kStepK = 64;                       // reduction steps of a stage (128 bytes)
 constexpr int kEpiWarps = 8;
 constexpr int kGemmThreads = (2 + kEpiWarps) * 32;
 constexpr int kStagingBytes = kEpiWarps * 4096;  // two 32 x 32 tiles of 16-bit elements per epilogue warp
-constexpr int kGroupM = 16;
+constexpr int kGroupM = 8;
 
 __device__ unsigned int g_ffn_timeouts = 0;
 
@@ -74,11 +77,11 @@ struct Plan {
     void *gate, *up;               // kGate: written unless null.  kGrad: read
     void *dgate, *dup, *hid;       // kGrad: written
     long long ldh;                 // pitch of gate .. hid (a multiple of 8)
-    float* partials;               // splits > 1: [splits][batch][mTiles * 128][nTiles * BN]
+    float* partials;               // splits > 1: [splits][batch][mTiles * 256][nTiles * BN]
 };
 
-template <int BN> constexpr int kStages = BN == 256 ? 4 : 6;
-template <int BN> constexpr int kStageBytes = (kTileM + BN) * kStepK * 2;
+template <int BN> constexpr int kStages = BN == 256 ? 6 : 8;
+template <int BN> constexpr int kStageBytes = (kCtaM + BN / 2) * kStepK * 2;    // of one CTA
 template <int BN> constexpr int kGemmSmem = 1024 + kStages<BN> * kStageBytes<BN> + kStagingBytes + 256;
 
 template <typename T> __device__ __forceinline__ uint32_t pack2(float lo, float hi);
@@ -235,12 +238,13 @@ __global__ void __launch_bounds__(kGemmThreads, 1) gemm_kernel(const __grid_cons
     __shared__ uint32_t tmemSlot;
     __shared__ int abortFlag;
     const int warp = threadIdx.x >> 5, lane = threadIdx.x & 31;
+    const int rank = (int)cluster_rank();      // of this CTA in its pair
 
     if (threadIdx.x == 0) {
         for (int i = 0; i < S; ++i)
             mbar_init(full + 8 * i, 1), mbar_init(empty + 8 * i, 1);
         for (int i = 0; i < 2; ++i)
-            mbar_init(accFull + 8 * i, 1), mbar_init(accEmpty + 8 * i, kEpiWarps);
+            mbar_init(accFull + 8 * i, 1), mbar_init(accEmpty + 8 * i, 2 * kEpiWarps);
         mbar_init(drain, 1);
         mbar_init_fence();
         abortFlag = 0;
@@ -253,6 +257,7 @@ __global__ void __launch_bounds__(kGemmThreads, 1) gemm_kernel(const __grid_cons
         tc_fence_before();
     }
     __syncthreads();
+    cluster_sync();     // the other CTA's barriers are initialised too
     tc_fence_after();
     const uint32_t tmem = *const_cast<volatile uint32_t*>(&tmemSlot);
     volatile int* abort = &abortFlag;
@@ -268,11 +273,15 @@ __global__ void __launch_bounds__(kGemmThreads, 1) gemm_kernel(const __grid_cons
 
     if (warp == 0 && lane == 0) {
         // ---- producer ----
+        // The second CTA's copies are counted on the first CTA's barrier as well: bytes may arrive there before the
+        // stage's count has been announced, but a stage is not filled again before both CTAs know it was consumed.
+        const uint32_t fullFirst = in_first_cta(full);
         uint32_t issued = 0;
         bool ok = true;
-        for (int t = blockIdx.x; ok && t < tiles; t += gridDim.x) {
+        for (int t = blockIdx.x >> 1; ok && t < tiles; t += gridDim.x >> 1) {
             const Tile w = tile_at(t, p, mTiles);
             const int k0 = (int)((long long)kAll * w.s / p.splits), k1 = (int)((long long)kAll * (w.s + 1) / p.splits);
+            const int row = w.m * kTileM + rank * kCtaM;
             for (int k = k0; k < k1; ++k, ++issued) {
                 const uint32_t st = issued % S, turn = issued / S;
                 if (turn > 0 && !mbar_wait_bounded(empty + 8 * st, (turn - 1) & 1, abort, &g_ffn_timeouts)) {
@@ -282,37 +291,37 @@ __global__ void __launch_bounds__(kGemmThreads, 1) gemm_kernel(const __grid_cons
                 const int seg = p.segs > 1 ? k / p.kIters : 0;
                 const int kk = (k - seg * p.kIters) * kStepK;
                 const int which = p.segs > 1 ? seg : w.z;
-                const uint32_t a = smem + st * kStageBytes<BN>, b = a + kTileM * kStepK * 2, bar = full + 8 * st;
-                mbar_expect_tx(bar, kStageBytes<BN>);
+                const uint32_t a = smem + st * kStageBytes<BN>, b = a + kCtaM * kStepK * 2, bar = fullFirst + 8 * st;
+                if (rank == 0)
+                    mbar_expect_tx(full + 8 * st, 2 * kStageBytes<BN>);
                 if (A_MN) {
-                    for (int i = 0; i < kTileM / 64; ++i)
-                        tma_load_2d(a + i * 8192, &maps.a[which], w.m * kTileM + i * 64, kk, bar);
+                    for (int i = 0; i < kCtaM / 64; ++i)
+                        tma_load_2d(a + i * 8192, &maps.a[which], row + i * 64, kk, bar);
                 } else {
-                    tma_load_2d(a, &maps.a[which], kk, w.m * kTileM, bar);
+                    tma_load_2d(a, &maps.a[which], kk, row, bar);
                 }
-                if (EPI == kGate) {
-                    tma_load_2d(b, &maps.b[0], kk, w.n * 128, bar);
-                    tma_load_2d(b + 128 * kStepK * 2, &maps.b[1], kk, w.n * 128, bar);
+                if (EPI == kGate) {     // Wg's rows are the first CTA's half of B, Wu's the second's
+                    tma_load_2d(b, &maps.b[rank], kk, w.n * 128, bar);
                 } else if (B_MN) {
-                    for (int i = 0; i < BN / 64; ++i)
-                        tma_load_2d(b + i * 8192, &maps.b[which], w.n * BN + i * 64, kk, bar);
+                    for (int i = 0; i < BN / 2 / 64; ++i)
+                        tma_load_2d(b + i * 8192, &maps.b[which], w.n * BN + rank * (BN / 2) + i * 64, kk, bar);
                 } else {
-                    tma_load_2d(b, &maps.b[which], kk, w.n * BN, bar);
+                    tma_load_2d(b, &maps.b[which], kk, w.n * BN + rank * (BN / 2), bar);
                 }
             }
         }
-        if (*abort) {   // shared memory is not given back with copies in flight
+        if (*abort && rank == 0) {   // shared memory is not given back with copies (of either CTA) in flight
             int own = 0;
             for (uint32_t i = issued > S ? issued - S : 0; i < issued; ++i)
                 mbar_wait_bounded(full + 8 * (i % S), (i / S) & 1, &own, &g_ffn_timeouts);
         }
-    } else if (warp == 1 && lane == 0) {
-        // ---- matrix instructions ----
+    } else if (warp == 1 && lane == 0 && rank == 0) {
+        // ---- matrix instructions: the first CTA's, for both ----
         constexpr uint32_t idesc0 = instr_desc<A_MN, B_MN>(0, BN), idesc1 = instr_desc<A_MN, B_MN>(1, BN);
         constexpr uint32_t idesc = sizeof(T) == 2 && std::is_same<T, __nv_bfloat16>::value ? idesc1 : idesc0;
         uint32_t used = 0, turn = 0;
         bool ok = true;
-        for (int t = blockIdx.x; ok && t < tiles; t += gridDim.x, ++turn) {
+        for (int t = blockIdx.x >> 1; ok && t < tiles; t += gridDim.x >> 1, ++turn) {
             const Tile w = tile_at(t, p, mTiles);
             const int k0 = (int)((long long)kAll * w.s / p.splits), k1 = (int)((long long)kAll * (w.s + 1) / p.splits);
             const uint32_t acc = turn & 1, d = tmem + acc * BN;
@@ -327,32 +336,33 @@ __global__ void __launch_bounds__(kGemmThreads, 1) gemm_kernel(const __grid_cons
                 }
                 tc_fence_after();
                 const uint32_t a = smem + st * kStageBytes<BN>;
-                const uint64_t da = operand_desc<A_MN>(a), db = operand_desc<B_MN>(a + kTileM * kStepK * 2);
+                const uint64_t da = operand_desc<A_MN>(a), db = operand_desc<B_MN>(a + kCtaM * kStepK * 2);
 #pragma unroll
                 for (int j = 0; j < kStepK / 16; ++j)
                     mma_f16(d, da + j * kDescStep<A_MN>, db + j * kDescStep<B_MN>, idesc, k > k0 || j > 0);
-                mma_commit(empty + 8 * st);
+                mma_commit_pair(empty + 8 * st);
             }
             if (ok)
-                mma_commit(accFull + 8 * acc);
+                mma_commit_pair(accFull + 8 * acc);
         }
         if (*abort) {
             int own = 0;
-            mma_commit(drain);
+            mma_commit_pair(drain);
             mbar_wait_bounded(drain, 0, &own, &g_ffn_timeouts);
         }
     } else if (warp >= 2) {
         // ---- epilogue: warp w may touch TMEM lanes 32 (w % 4) ..; two warps share each quarter, half the columns each ----
         const int quarter = warp & 3, half = (warp - 2) >> 2;
         const uint32_t buf0 = staging + (warp - 2) * 4096, buf1 = buf0 + 2048;
+        const uint32_t accEmptyFirst = in_first_cta(accEmpty);
         uint32_t turn = 0;
-        for (int t = blockIdx.x; t < tiles; t += gridDim.x, ++turn) {
+        for (int t = blockIdx.x >> 1; t < tiles; t += gridDim.x >> 1, ++turn) {
             const Tile w = tile_at(t, p, mTiles);
             const uint32_t acc = turn & 1, d = tmem + acc * BN + ((uint32_t)(quarter * 32) << 16);
             if (!mbar_wait_bounded(accFull + 8 * acc, (turn >> 1) & 1, abort, &g_ffn_timeouts))
                 break;
             tc_fence_after();
-            const long long row0 = (long long)w.m * kTileM + quarter * 32;
+            const long long row0 = (long long)w.m * kTileM + rank * kCtaM + quarter * 32;
             if (p.splits > 1) {
                 float* part = p.partials + ((long long)w.s * p.batch + w.z) * p.mTiles * kTileM * (p.nTiles * BN) +
                               (row0 + lane) * (p.nTiles * BN) + w.n * BN + half * (BN / 2);
@@ -449,10 +459,14 @@ __global__ void __launch_bounds__(kGemmThreads, 1) gemm_kernel(const __grid_cons
             }
             tc_fence_before();
             if (lane == 0)
-                mbar_arrive(accEmpty + 8 * acc);
+                mbar_arrive_cluster(accEmptyFirst + 8 * acc);
         }
     }
+    // every role's waits are bounded, so both CTAs get here; neither frees TMEM or leaves while the other may still
+    // signal its barriers or multiply out of its shared memory
+    tc_fence_before();
     __syncthreads();
+    cluster_sync();
     if (warp == 1) {
         __syncwarp();
         tc_fence_after();
@@ -554,10 +568,10 @@ int tile_n(int N) { return N <= 128 ? 128 : 256; }
 // up for it as long as each keeps at least four stages.  `most`: what the caller's workspace can hold.
 int split_count(long long tiles, int kIters)
 {
-    const int sms = sm_count();
-    if (tiles * 2 > sms)
+    const int pairs = sm_count() / 2;
+    if (tiles * 2 > pairs)
         return 1;
-    return (int)std::max<long long>(1, std::min<long long>(sms / tiles, kIters / 4));
+    return (int)std::max<long long>(1, std::min<long long>(pairs / tiles, kIters / 4));
 }
 
 template <typename T, bool A_MN, bool B_MN, int EPI, int BN>
@@ -567,17 +581,25 @@ cudaError_t launch_gemm(const Matrix (&a)[2], const Matrix (&b)[2], Plan& p, cud
     const int n = std::max(p.batch, std::max(p.segs, EPI == kGate ? 2 : 1));
     for (int i = 0; i < 2; ++i) {
         const int j = i < n ? i : 0;
-        if (cudaError_t e = encode(a[EPI == kGate ? 0 : j], A_MN ? kStepK : kTileM, &maps.a[i]))
+        if (cudaError_t e = encode(a[EPI == kGate ? 0 : j], A_MN ? kStepK : kCtaM, &maps.a[i]))
             return e;
-        if (cudaError_t e = encode(b[j], B_MN ? kStepK : (EPI == kGate ? 128 : BN), &maps.b[i]))
+        if (cudaError_t e = encode(b[j], B_MN ? kStepK : BN / 2, &maps.b[i]))
             return e;
     }
     auto kernel = gemm_kernel<T, A_MN, B_MN, EPI, BN>;
     if (cudaError_t e = cudaFuncSetAttribute(kernel, cudaFuncAttributeMaxDynamicSharedMemorySize, kGemmSmem<BN>))
         return e;
     const long long tiles = (long long)p.mTiles * p.nTiles * p.batch * p.splits;
-    const int grid = (int)std::min<long long>(tiles, sm_count());
-    if (cudaError_t e = launch_pdl(kernel, dim3(grid), dim3(kGemmThreads), kGemmSmem<BN>, stream, maps, p))
+    cudaLaunchConfig_t cfg = {};
+    cfg.gridDim = dim3(2 * (unsigned)std::min<long long>(tiles, sm_count() / 2)), cfg.blockDim = dim3(kGemmThreads);
+    cfg.dynamicSmemBytes = kGemmSmem<BN>, cfg.stream = stream;
+    cudaLaunchAttribute attr[2];
+    attr[0].id = cudaLaunchAttributeClusterDimension;
+    attr[0].val.clusterDim.x = 2, attr[0].val.clusterDim.y = 1, attr[0].val.clusterDim.z = 1;
+    attr[1].id = cudaLaunchAttributeProgrammaticStreamSerialization;
+    attr[1].val.programmaticStreamSerializationAllowed = 1;
+    cfg.attrs = attr, cfg.numAttrs = options().pdl ? 2 : 1;
+    if (cudaError_t e = cudaLaunchKernelEx(&cfg, kernel, maps, p))
         return e;
     if (p.splits == 1)
         return cudaSuccess;

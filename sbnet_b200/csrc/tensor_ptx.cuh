@@ -1,23 +1,26 @@
 // Thin wrappers over the tcgen05 (fifth-generation tensor core) and TMEM instructions, shared-memory
-// operand descriptors and two-dimensional TMA loads used by the matrix kernels.  sm_100a only.
+// operand descriptors, two-dimensional TMA loads and the cluster controls used by the matrix kernels, which
+// run as pairs of CTAs (cta_group::2): one instruction multiplies 256 rows, 128 of them in each CTA's shared
+// memory and TMEM, and each CTA holds half of the other operand.  sm_100a only.
 #pragma once
 #include "async_ptx.cuh"
 
 namespace sbnet {
 
 // ---- tensor memory -------------------------------------------------------------------------------
-// Whole-warp calls; `cols` is a power of two >= 32.  The warp that allocates also frees.
+// Whole-warp calls, made by one warp of each CTA of the pair; `cols` is a power of two >= 32.  The warp that
+// allocates also frees.
 __device__ __forceinline__ void tmem_alloc(uint32_t slot, uint32_t cols)
 {
-    asm volatile("tcgen05.alloc.cta_group::1.sync.aligned.shared::cta.b32 [%0], %1;" ::"r"(slot), "r"(cols) : "memory");
+    asm volatile("tcgen05.alloc.cta_group::2.sync.aligned.shared::cta.b32 [%0], %1;" ::"r"(slot), "r"(cols) : "memory");
 }
 __device__ __forceinline__ void tmem_relinquish()
 {
-    asm volatile("tcgen05.relinquish_alloc_permit.cta_group::1.sync.aligned;" ::: "memory");
+    asm volatile("tcgen05.relinquish_alloc_permit.cta_group::2.sync.aligned;" ::: "memory");
 }
 __device__ __forceinline__ void tmem_free(uint32_t addr, uint32_t cols)
 {
-    asm volatile("tcgen05.dealloc.cta_group::1.sync.aligned.b32 %0, %1;" ::"r"(addr), "r"(cols) : "memory");
+    asm volatile("tcgen05.dealloc.cta_group::2.sync.aligned.b32 %0, %1;" ::"r"(addr), "r"(cols) : "memory");
 }
 // 32 lanes x 32 columns of 32-bit words: lane i of the warp gets row i (of the warp's quarter of the lanes).
 __device__ __forceinline__ void tmem_load32(uint32_t addr, uint32_t (&r)[32])
@@ -51,33 +54,61 @@ template <bool MN> __device__ __forceinline__ uint64_t operand_desc(uint32_t sme
 }
 template <bool MN> constexpr uint32_t kDescStep = MN ? 2048 >> 4 : 32 >> 4;
 
-// kind::f16, fp32 accumulators; format 0 = f16, 1 = bf16 (both operands); M = 128.
+// kind::f16, fp32 accumulators; format 0 = f16, 1 = bf16 (both operands); M = 256 over the pair.
 template <bool A_MN, bool B_MN> __device__ __forceinline__ constexpr uint32_t instr_desc(int format, int n)
 {
     return (1u << 4) | ((uint32_t)format << 7) | ((uint32_t)format << 10) | ((A_MN ? 1u : 0u) << 15) |
-           ((B_MN ? 1u : 0u) << 16) | ((uint32_t)(n >> 3) << 17) | (8u << 24);
+           ((B_MN ? 1u : 0u) << 16) | ((uint32_t)(n >> 3) << 17) | (16u << 24);
 }
 __device__ __forceinline__ void mma_f16(uint32_t d, uint64_t a, uint64_t b, uint32_t idesc, bool accumulate)
 {
     asm volatile(
         "{\n\t.reg .pred p;\n\t"
         "setp.ne.u32 p, %4, 0;\n\t"
-        "tcgen05.mma.cta_group::1.kind::f16 [%0], %1, %2, %3, p;\n\t}" ::"r"(d),
+        "tcgen05.mma.cta_group::2.kind::f16 [%0], %1, %2, %3, p;\n\t}" ::"r"(d),
         "l"(a), "l"(b), "r"(idesc), "r"((uint32_t)accumulate)
         : "memory");
 }
-// Arrives on the barrier once every tcgen05.mma this thread has issued is done.
-__device__ __forceinline__ void mma_commit(uint32_t bar)
+// Arrives on the barrier at this offset in both CTAs once every tcgen05.mma this thread has issued is done.
+__device__ __forceinline__ void mma_commit_pair(uint32_t bar)
 {
-    asm volatile("tcgen05.commit.cta_group::1.mbarrier::arrive::one.shared::cluster.b64 [%0];" ::"r"(bar) : "memory");
+    asm volatile("tcgen05.commit.cta_group::2.mbarrier::arrive::one.shared::cluster.multicast::cluster.b64 [%0], %1;" ::"r"(bar),
+                 "h"((uint16_t)3)
+                 : "memory");
+}
+
+// ---- the pair -----------------------------------------------------------------------------------------
+__device__ __forceinline__ uint32_t cluster_rank()
+{
+    uint32_t r;
+    asm volatile("mov.u32 %0, %%cluster_ctarank;" : "=r"(r));
+    return r;
+}
+// Address, in the cluster's shared window, of this offset in the first CTA of the pair.
+__device__ __forceinline__ uint32_t in_first_cta(uint32_t addr)
+{
+    uint32_t r;
+    asm volatile("mapa.shared::cluster.u32 %0, %1, %2;" : "=r"(r) : "r"(addr), "r"(0));
+    return r;
+}
+__device__ __forceinline__ void mbar_arrive_cluster(uint32_t addr)
+{
+    asm volatile("mbarrier.arrive.release.cluster.shared::cluster.b64 _, [%0];" ::"r"(addr) : "memory");
+}
+__device__ __forceinline__ void cluster_sync()
+{
+    asm volatile("barrier.cluster.arrive.release;" ::: "memory");
+    asm volatile("barrier.cluster.wait.acquire;" ::: "memory");
 }
 
 // ---- loads ------------------------------------------------------------------------------------------
-// c0 (the contiguous coordinate) times the element size is a multiple of 16 bytes at every call.
+// Into this CTA's shared memory; the bytes are counted on a barrier of either CTA of the pair (a cluster
+// address).  c0 (the contiguous coordinate) times the element size is a multiple of 16 bytes at every call.
 __device__ __forceinline__ void tma_load_2d(uint32_t dst, const CUtensorMap* map, int c0, int c1, uint32_t bar)
 {
     asm volatile(
-        "cp.async.bulk.tensor.2d.shared::cluster.global.tile.mbarrier::complete_tx::bytes [%0], [%1, {%2, %3}], [%4];" ::"r"(dst),
+        "cp.async.bulk.tensor.2d.shared::cluster.global.tile.mbarrier::complete_tx::bytes.cta_group::2 "
+        "[%0], [%1, {%2, %3}], [%4];" ::"r"(dst),
         "l"(reinterpret_cast<uint64_t>(map)), "r"(c0), "r"(c1), "r"(bar)
         : "memory");
 }
