@@ -159,6 +159,13 @@ static __device__ __noinline__ bool mbar_wait_bounded(uint32_t bar, uint32_t par
     return false;
 }
 
+// The same wait with its first look inlined: for loops where the barrier has usually completed already.
+static __device__ __forceinline__ bool mbar_wait_quick(uint32_t bar, uint32_t parity, volatile int* abortFlag,
+                                                       unsigned int* timeouts)
+{
+    return mbar_try_wait(bar, parity) || mbar_wait_bounded(bar, parity, abortFlag, timeouts);
+}
+
 // ---- loads through the TMA engine (this GPU's memory only; never multicast) -----------------------
 __device__ __forceinline__ void tma_load_4d(uint32_t dst, const CUtensorMap* map, int c0, int c1, int c2,
                                             int c3, uint32_t bar)

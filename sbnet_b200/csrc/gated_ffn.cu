@@ -271,11 +271,14 @@ __global__ void __launch_bounds__(kGemmThreads, 1) gemm_kernel(const __grid_cons
     const int tiles = mTiles * p.nTiles * p.batch * p.splits;
     const int kAll = p.kIters * p.segs;
 
-    if (warp == 0 && lane == 0) {
+    // The two single-thread roles run their loops as whole warps (addresses stay in uniform registers) and let one
+    // lane issue.
+    if (warp == 0) {
         // ---- producer ----
         // The second CTA's copies are counted on the first CTA's barrier as well: bytes may arrive there before the
         // stage's count has been announced, but a stage is not filled again before both CTAs know it was consumed.
         const uint32_t fullFirst = in_first_cta(full);
+        const bool lead = elect_one();
         uint32_t issued = 0;
         bool ok = true;
         for (int t = blockIdx.x >> 1; ok && t < tiles; t += gridDim.x >> 1) {
@@ -284,7 +287,7 @@ __global__ void __launch_bounds__(kGemmThreads, 1) gemm_kernel(const __grid_cons
             const int row = w.m * kTileM + rank * kCtaM;
             for (int k = k0; k < k1; ++k, ++issued) {
                 const uint32_t st = issued % S, turn = issued / S;
-                if (turn > 0 && !mbar_wait_bounded(empty + 8 * st, (turn - 1) & 1, abort, &g_ffn_timeouts)) {
+                if (turn > 0 && !mbar_wait_warp(empty + 8 * st, (turn - 1) & 1, abort, &g_ffn_timeouts)) {
                     ok = false;
                     break;
                 }
@@ -292,22 +295,25 @@ __global__ void __launch_bounds__(kGemmThreads, 1) gemm_kernel(const __grid_cons
                 const int kk = (k - seg * p.kIters) * kStepK;
                 const int which = p.segs > 1 ? seg : w.z;
                 const uint32_t a = smem + st * kStageBytes<BN>, b = a + kCtaM * kStepK * 2, bar = fullFirst + 8 * st;
-                if (rank == 0)
-                    mbar_expect_tx(full + 8 * st, 2 * kStageBytes<BN>);
-                if (A_MN) {
-                    for (int i = 0; i < kCtaM / 64; ++i)
-                        tma_load_2d(a + i * 8192, &maps.a[which], row + i * 64, kk, bar);
-                } else {
-                    tma_load_2d(a, &maps.a[which], kk, row, bar);
+                if (lead) {
+                    if (rank == 0)
+                        mbar_expect_tx(full + 8 * st, 2 * kStageBytes<BN>);
+                    if (A_MN) {
+                        for (int i = 0; i < kCtaM / 64; ++i)
+                            tma_load_2d(a + i * 8192, &maps.a[which], row + i * 64, kk, bar);
+                    } else {
+                        tma_load_2d(a, &maps.a[which], kk, row, bar);
+                    }
+                    if (EPI == kGate) {     // Wg's rows are the first CTA's half of B, Wu's the second's
+                        tma_load_2d(b, &maps.b[rank], kk, w.n * 128, bar);
+                    } else if (B_MN) {
+                        for (int i = 0; i < BN / 2 / 64; ++i)
+                            tma_load_2d(b + i * 8192, &maps.b[which], w.n * BN + rank * (BN / 2) + i * 64, kk, bar);
+                    } else {
+                        tma_load_2d(b, &maps.b[which], kk, w.n * BN + rank * (BN / 2), bar);
+                    }
                 }
-                if (EPI == kGate) {     // Wg's rows are the first CTA's half of B, Wu's the second's
-                    tma_load_2d(b, &maps.b[rank], kk, w.n * 128, bar);
-                } else if (B_MN) {
-                    for (int i = 0; i < BN / 2 / 64; ++i)
-                        tma_load_2d(b + i * 8192, &maps.b[which], w.n * BN + rank * (BN / 2) + i * 64, kk, bar);
-                } else {
-                    tma_load_2d(b, &maps.b[which], kk, w.n * BN + rank * (BN / 2), bar);
-                }
+                __syncwarp();
             }
         }
         if (*abort && rank == 0) {   // shared memory is not given back with copies (of either CTA) in flight
@@ -315,39 +321,45 @@ __global__ void __launch_bounds__(kGemmThreads, 1) gemm_kernel(const __grid_cons
             for (uint32_t i = issued > S ? issued - S : 0; i < issued; ++i)
                 mbar_wait_bounded(full + 8 * (i % S), (i / S) & 1, &own, &g_ffn_timeouts);
         }
-    } else if (warp == 1 && lane == 0 && rank == 0) {
+    } else if (warp == 1 && rank == 0) {
         // ---- matrix instructions: the first CTA's, for both ----
         constexpr uint32_t idesc0 = instr_desc<A_MN, B_MN>(0, BN), idesc1 = instr_desc<A_MN, B_MN>(1, BN);
         constexpr uint32_t idesc = sizeof(T) == 2 && std::is_same<T, __nv_bfloat16>::value ? idesc1 : idesc0;
+        const bool lead = elect_one();
         uint32_t used = 0, turn = 0;
         bool ok = true;
         for (int t = blockIdx.x >> 1; ok && t < tiles; t += gridDim.x >> 1, ++turn) {
             const Tile w = tile_at(t, p, mTiles);
             const int k0 = (int)((long long)kAll * w.s / p.splits), k1 = (int)((long long)kAll * (w.s + 1) / p.splits);
             const uint32_t acc = turn & 1, d = tmem + acc * BN;
-            if (turn > 1 && !mbar_wait_bounded(accEmpty + 8 * acc, ((turn >> 1) - 1) & 1, abort, &g_ffn_timeouts))
+            if (turn > 1 && !mbar_wait_warp(accEmpty + 8 * acc, ((turn >> 1) - 1) & 1, abort, &g_ffn_timeouts))
                 break;
             tc_fence_after();
             for (int k = k0; k < k1; ++k, ++used) {
                 const uint32_t st = used % S;
-                if (!mbar_wait_bounded(full + 8 * st, (used / S) & 1, abort, &g_ffn_timeouts)) {
+                if (!mbar_wait_warp(full + 8 * st, (used / S) & 1, abort, &g_ffn_timeouts)) {
                     ok = false;
                     break;
                 }
                 tc_fence_after();
                 const uint32_t a = smem + st * kStageBytes<BN>;
                 const uint64_t da = operand_desc<A_MN>(a), db = operand_desc<B_MN>(a + kCtaM * kStepK * 2);
+                if (lead) {
 #pragma unroll
-                for (int j = 0; j < kStepK / 16; ++j)
-                    mma_f16(d, da + j * kDescStep<A_MN>, db + j * kDescStep<B_MN>, idesc, k > k0 || j > 0);
-                mma_commit_pair(empty + 8 * st);
+                    for (int j = 0; j < kStepK / 16; ++j)
+                        mma_f16(d, da + j * kDescStep<A_MN>, db + j * kDescStep<B_MN>, idesc, k > k0 || j > 0);
+                    mma_commit_pair(empty + 8 * st);
+                }
+                __syncwarp();
             }
-            if (ok)
+            if (ok && lead)
                 mma_commit_pair(accFull + 8 * acc);
+            __syncwarp();
         }
         if (*abort) {
             int own = 0;
-            mma_commit_pair(drain);
+            if (lead)
+                mma_commit_pair(drain);
             mbar_wait_bounded(drain, 0, &own, &g_ffn_timeouts);
         }
     } else if (warp >= 2) {
@@ -359,7 +371,7 @@ __global__ void __launch_bounds__(kGemmThreads, 1) gemm_kernel(const __grid_cons
         for (int t = blockIdx.x >> 1; t < tiles; t += gridDim.x >> 1, ++turn) {
             const Tile w = tile_at(t, p, mTiles);
             const uint32_t acc = turn & 1, d = tmem + acc * BN + ((uint32_t)(quarter * 32) << 16);
-            if (!mbar_wait_bounded(accFull + 8 * acc, (turn >> 1) & 1, abort, &g_ffn_timeouts))
+            if (!mbar_wait_warp(accFull + 8 * acc, (turn >> 1) & 1, abort, &g_ffn_timeouts))
                 break;
             tc_fence_after();
             const long long row0 = (long long)w.m * kTileM + rank * kCtaM + quarter * 32;

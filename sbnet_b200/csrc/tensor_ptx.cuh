@@ -7,6 +7,22 @@
 
 namespace sbnet {
 
+// One lane of a converged warp, chosen by the hardware.
+__device__ __forceinline__ bool elect_one()
+{
+    uint32_t r;
+    asm volatile("{\n\t.reg .pred p;\n\telect.sync _|p, 0xffffffff;\n\tselp.u32 %0, 1, 0, p;\n\t}" : "=r"(r));
+    return r != 0;
+}
+
+// A bounded wait made by a whole warp, with one outcome for all of its lanes (a lane that gave up alone would
+// leave the others behind at the next warp-wide instruction).
+static __device__ __forceinline__ bool mbar_wait_warp(uint32_t bar, uint32_t parity, volatile int* abortFlag,
+                                                      unsigned int* timeouts)
+{
+    return __all_sync(0xffffffffu, mbar_wait_quick(bar, parity, abortFlag, timeouts));
+}
+
 // ---- tensor memory -------------------------------------------------------------------------------
 // Whole-warp calls, made by one warp of each CTA of the pair; `cols` is a power of two >= 32.  The warp that
 // allocates also frees.
