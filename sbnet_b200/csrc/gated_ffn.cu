@@ -375,6 +375,12 @@ __global__ void __launch_bounds__(kGemmThreads, 1) gemm_kernel(const __grid_cons
                 break;
             tc_fence_after();
             const long long row0 = (long long)w.m * kTileM + rank * kCtaM + quarter * 32;
+            // after the last read of the accumulator: the next tile may be multiplied into it
+            auto release = [&] {
+                tc_fence_before();
+                if (lane == 0)
+                    mbar_arrive_cluster(accEmptyFirst + 8 * acc);
+            };
             if (p.splits > 1) {
                 float* part = p.partials + ((long long)w.s * p.batch + w.z) * p.mTiles * kTileM * (p.nTiles * BN) +
                               (row0 + lane) * (p.nTiles * BN) + w.n * BN + half * (BN / 2);
@@ -383,6 +389,8 @@ __global__ void __launch_bounds__(kGemmThreads, 1) gemm_kernel(const __grid_cons
                     uint32_t v[32];
                     tmem_load32(d + half * (BN / 2) + c, v);
                     tmem_wait_load();
+                    if (c + 32 == BN / 2)
+                        release();
 #pragma unroll
                     for (int i = 0; i < 8; ++i)
                         *reinterpret_cast<uint4*>(part + c + 4 * i) = make_uint4(v[4 * i], v[4 * i + 1], v[4 * i + 2], v[4 * i + 3]);
@@ -394,6 +402,8 @@ __global__ void __launch_bounds__(kGemmThreads, 1) gemm_kernel(const __grid_cons
                     tmem_load32(d + c, g);
                     tmem_load32(d + 128 + c, u);
                     tmem_wait_load();
+                    if (c + 32 == half * 64 + 64)
+                        release();
                     if (p.act == kSilu)
                         gate_chunk<T, kSilu>(g, u, h);
                     else if (p.act == kGelu)
@@ -431,6 +441,8 @@ __global__ void __launch_bounds__(kGemmThreads, 1) gemm_kernel(const __grid_cons
                     load_tile<T>(static_cast<const T*>(p.up), p.ldh, row0, rowEnd, col, p.N, buf1, lane);
                     tmem_load32(d + c, dh);
                     tmem_wait_load();
+                    if (c + 32 == (half + 1) * (BN / 2))
+                        release();
                     __syncwarp();
                     unstage_rows(buf0, lane, g);
                     unstage_rows(buf1, lane, u);
@@ -460,6 +472,8 @@ __global__ void __launch_bounds__(kGemmThreads, 1) gemm_kernel(const __grid_cons
                     uint32_t v[32], h[16];
                     tmem_load32(d + c, v);
                     tmem_wait_load();
+                    if (c + 32 == (half + 1) * (BN / 2))
+                        release();
 #pragma unroll
                     for (int i = 0; i < 16; ++i)
                         h[i] = pack2<T>(__uint_as_float(v[2 * i]), __uint_as_float(v[2 * i + 1]));
@@ -469,9 +483,6 @@ __global__ void __launch_bounds__(kGemmThreads, 1) gemm_kernel(const __grid_cons
                     __syncwarp();
                 }
             }
-            tc_fence_before();
-            if (lane == 0)
-                mbar_arrive_cluster(accEmptyFirst + 8 * acc);
         }
     }
     // every role's waits are bounded, so both CTAs get here; neither frees TMEM or leaves while the other may still
@@ -487,7 +498,29 @@ __global__ void __launch_bounds__(kGemmThreads, 1) gemm_kernel(const __grid_cons
 }
 
 // Adds the partial sums of a split reduction in the order of the pieces and finishes the elements as the epilogue
-// would have.  One thread per element.
+// would have.  A thread takes four neighbouring columns of a row; blocks of 32 x 8 threads cover 128 columns x 8 rows.
+__device__ __forceinline__ float4 sum_pieces(const float* q, long long step, int pieces)
+{
+    float4 v = make_float4(0.f, 0.f, 0.f, 0.f);
+#pragma unroll 4
+    for (int s = 0; s < pieces; ++s) {
+        const float4 w = *reinterpret_cast<const float4*>(q + s * step);
+        v.x += w.x, v.y += w.y, v.z += w.z, v.w += w.w;
+    }
+    return v;
+}
+template <typename T> __device__ __forceinline__ void store4(T* dst, float4 v, int n, bool wide)
+{
+    if (wide && n >= 4) {
+        *reinterpret_cast<uint2*>(dst) = make_uint2(pack2<T>(v.x, v.y), pack2<T>(v.z, v.w));
+        return;
+    }
+    const float e[4] = {v.x, v.y, v.z, v.w};
+#pragma unroll
+    for (int i = 0; i < 4; ++i)
+        if (i < n)
+            dst[i] = T(e[i]);
+}
 template <typename T, int EPI> __global__ void __launch_bounds__(256) finish_kernel(const __grid_constant__ Plan p, int bn)
 {
     pdl_wait();
@@ -496,43 +529,56 @@ template <typename T, int EPI> __global__ void __launch_bounds__(256) finish_ker
     if (p.num_blocks_dev != nullptr)
         rowEnd = min(rowEnd, (long long)max(*p.num_blocks_dev, 0) * p.rowsPerBlock);
     const long long pitch = (long long)p.nTiles * bn, plane = (long long)p.mTiles * kTileM * pitch;
-    const long long n = rowEnd * p.N;
-    for (long long i = (long long)blockIdx.x * 256 + threadIdx.x; i < n * p.batch; i += (long long)gridDim.x * 256) {
-        const int z = (int)(i / n);
-        const long long row = (i - z * n) / p.N;
-        const int col = (int)((i - z * n) - row * p.N);
+    const int col = blockIdx.x * 128 + threadIdx.x * 4, z = blockIdx.z, n = p.N - col;
+    if (n <= 0)
+        return;
+    T* out = static_cast<T*>(p.out[z]);
+    const bool wide = (p.ldo & 3) == 0 && (reinterpret_cast<uintptr_t>(out) & 7) == 0;
+    for (long long row = (long long)blockIdx.y * 8 + threadIdx.y; row < rowEnd; row += (long long)gridDim.y * 8) {
         if (EPI == kGate) {
             const float* q = p.partials + row * pitch + (col >> 7) * 256 + (col & 127);
-            float g = 0.f, u = 0.f, unused;
-            for (int s = 0; s < p.splits; ++s)
-                g += q[s * plane], u += q[s * plane + 128];
-            const float a = p.act == kSilu   ? activate<kSilu, false>(g, unused)
-                            : p.act == kGelu ? activate<kGelu, false>(g, unused)
-                                             : activate<kRelu, false>(g, unused);
-            static_cast<T*>(p.out[0])[row * p.ldo + col] = T(a * u);
+            const float4 g = sum_pieces(q, plane, p.splits), u = sum_pieces(q + 128, plane, p.splits);
+            float4 h;
+            float unused;
+            auto gated = [&](float a, float b) {
+                return b * (p.act == kSilu   ? activate<kSilu, false>(a, unused)
+                            : p.act == kGelu ? activate<kGelu, false>(a, unused)
+                                             : activate<kRelu, false>(a, unused));
+            };
+            h.x = gated(g.x, u.x), h.y = gated(g.y, u.y), h.z = gated(g.z, u.z), h.w = gated(g.w, u.w);
+            store4<T>(out + row * p.ldo + col, h, n, wide);
             if (p.gate != nullptr) {
-                static_cast<T*>(p.gate)[row * p.ldh + col] = T(g);
-                static_cast<T*>(p.up)[row * p.ldh + col] = T(u);
+                store4<T>(static_cast<T*>(p.gate) + row * p.ldh + col, g, n, true);
+                store4<T>(static_cast<T*>(p.up) + row * p.ldh + col, u, n, true);
             }
         } else {
-            const float* q = p.partials + z * plane + row * pitch + col;
-            float v = 0.f;
-            for (int s = 0; s < p.splits; ++s)
-                v += q[s * p.batch * plane];
-            static_cast<T*>(p.out[z])[row * p.ldo + col] = T(v);
+            const float4 v = sum_pieces(p.partials + z * plane + row * pitch + col, p.batch * plane, p.splits);
+            store4<T>(out + row * p.ldo + col, v, n, wide);
         }
     }
 }
 
-// Rows of `cols` 16-bit elements, pitch `cols` -> pitch `ld` (a multiple of 8).  One warp per row.
-__global__ void __launch_bounds__(256) repack_kernel(const uint16_t* src, long long rows, int cols, uint16_t* dst, int ld)
+// Copies matrices of 16-bit elements to another pitch (a multiple of 8), all of a call's in one launch: grid.y is the
+// matrix, a warp takes a row.
+constexpr int kMaxRepack = 5;
+struct Repack {
+    const uint16_t* src[kMaxRepack];
+    uint16_t* dst[kMaxRepack];
+    long long rows[kMaxRepack];
+    int cols[kMaxRepack], ld[kMaxRepack];
+};
+__global__ void __launch_bounds__(256) repack_kernel(const __grid_constant__ Repack r)
 {
     pdl_wait();
     pdl_launch_dependents();
-    const int lane = threadIdx.x & 31;
-    for (long long r = (long long)blockIdx.x * 8 + (threadIdx.x >> 5); r < rows; r += (long long)gridDim.x * 8)
+    const int m = blockIdx.y, lane = threadIdx.x & 31, cols = r.cols[m];
+    for (long long row = (long long)blockIdx.x * 8 + (threadIdx.x >> 5); row < r.rows[m]; row += (long long)gridDim.x * 8) {
+        const uint16_t* src = r.src[m] + row * cols;
+        uint16_t* dst = r.dst[m] + row * r.ld[m];
+#pragma unroll 4
         for (int c = lane; c < cols; c += 32)
-            dst[r * ld + c] = src[r * cols + c];
+            dst[c] = src[c];
+    }
 }
 
 // ---- host side -------------------------------------------------------------------------------------------
@@ -576,31 +622,46 @@ int ceil_div(long long a, long long b) { return (int)((a + b - 1) / b); }
 // Column tile of a plain product: 256 wide unless the matrix is narrow.
 int tile_n(int N) { return N <= 128 ? 128 : 256; }
 
-// Pieces of the reduction.  One piece fills the machine when there are enough tiles; with fewer, the pieces make
-// up for it as long as each keeps at least four stages.  `most`: what the caller's workspace can hold.
+// Pieces of the reduction.  One piece fills the machine when there are enough tiles.  With fewer, and a reduction of
+// more than 16 stages (5 us; the second kernel that adds the pieces costs about as much), pieces of at least 8 stages
+// make up for it.
 int split_count(long long tiles, int kIters)
 {
     const int pairs = sm_count() / 2;
-    if (tiles * 2 > pairs)
+    if (tiles * 2 > pairs || kIters <= 16)
         return 1;
-    return (int)std::max<long long>(1, std::min<long long>(pairs / tiles, kIters / 4));
+    return (int)std::max<long long>(1, std::min<long long>(pairs / tiles, kIters / 8));
 }
 
 template <typename T, bool A_MN, bool B_MN, int EPI, int BN>
 cudaError_t launch_gemm(const Matrix (&a)[2], const Matrix (&b)[2], Plan& p, cudaStream_t stream)
 {
     Maps maps;
-    const int n = std::max(p.batch, std::max(p.segs, EPI == kGate ? 2 : 1));
-    for (int i = 0; i < 2; ++i) {
-        const int j = i < n ? i : 0;
-        if (cudaError_t e = encode(a[EPI == kGate ? 0 : j], A_MN ? kStepK : kCtaM, &maps.a[i]))
+    const int n = std::max(p.batch, p.segs);
+    for (int i = 0; i < n; ++i)
+        if (cudaError_t e = encode(a[i], A_MN ? kStepK : kCtaM, &maps.a[i]))
             return e;
-        if (cudaError_t e = encode(b[j], B_MN ? kStepK : BN / 2, &maps.b[i]))
+    for (int i = 0; i < (EPI == kGate ? 2 : n); ++i) {
+        if (i > 0 && b[i].ptr == b[0].ptr)
+            maps.b[i] = maps.b[0];
+        else if (cudaError_t e = encode(b[i], B_MN ? kStepK : BN / 2, &maps.b[i]))
             return e;
     }
+    if (n == 1)     // the kernel never reads the second map, but prefetches both
+        maps.a[1] = maps.a[0];
+    if (n == 1 && EPI != kGate)
+        maps.b[1] = maps.b[0];
     auto kernel = gemm_kernel<T, A_MN, B_MN, EPI, BN>;
-    if (cudaError_t e = cudaFuncSetAttribute(kernel, cudaFuncAttributeMaxDynamicSharedMemorySize, kGemmSmem<BN>))
+    static bool raised[64] = {};       // per device; a race only repeats the call
+    int device = 0;
+    if (cudaError_t e = cudaGetDevice(&device))
         return e;
+    if (device >= 64 || !raised[device]) {
+        if (cudaError_t e = cudaFuncSetAttribute(kernel, cudaFuncAttributeMaxDynamicSharedMemorySize, kGemmSmem<BN>))
+            return e;
+        if (device < 64)
+            raised[device] = true;
+    }
     const long long tiles = (long long)p.mTiles * p.nTiles * p.batch * p.splits;
     cudaLaunchConfig_t cfg = {};
     cfg.gridDim = dim3(2 * (unsigned)std::min<long long>(tiles, sm_count() / 2)), cfg.blockDim = dim3(kGemmThreads);
@@ -615,10 +676,9 @@ cudaError_t launch_gemm(const Matrix (&a)[2], const Matrix (&b)[2], Plan& p, cud
         return e;
     if (p.splits == 1)
         return cudaSuccess;
-    const long long items = p.M * p.N * p.batch;
-    const int fgrid = (int)std::min<long long>((items + 255) / 256, (long long)sm_count() * 8);
+    const dim3 fgrid((unsigned)ceil_div(p.N, 128), (unsigned)std::min<long long>((p.M + 7) / 8, 65535), (unsigned)p.batch);
     if constexpr (EPI != kGrad)
-        return launch_pdl(finish_kernel<T, EPI>, dim3(fgrid), dim3(256), 0, stream, p, BN);
+        return launch_pdl(finish_kernel<T, EPI>, fgrid, dim3(32, 8), 0, stream, p, BN);
     return cudaErrorInvalidValue;
 }
 
@@ -680,14 +740,26 @@ struct Layout {
         return m;
     }
 };
-cudaError_t repack(const void* src, const Matrix& m, cudaStream_t stream)
-{
-    if (m.ptr == src)
-        return cudaSuccess;
-    const int grid = (int)std::min<long long>((m.rows + 7) / 8, (long long)sm_count() * 8);
-    return launch_pdl(repack_kernel, dim3(grid), dim3(256), 0, stream, static_cast<const uint16_t*>(src), m.rows, m.cols,
-                      static_cast<uint16_t*>(const_cast<void*>(m.ptr)), (int)m.ld);
-}
+struct Repacks {
+    Repack r = {};
+    int n = 0;
+    long long most = 0;
+    void add(const void* src, const Matrix& m)
+    {
+        if (m.ptr == src)
+            return;
+        r.src[n] = static_cast<const uint16_t*>(src), r.dst[n] = static_cast<uint16_t*>(const_cast<void*>(m.ptr));
+        r.rows[n] = m.rows, r.cols[n] = m.cols, r.ld[n] = (int)m.ld;
+        most = std::max(most, m.rows), ++n;
+    }
+    cudaError_t run(cudaStream_t stream) const
+    {
+        if (n == 0)
+            return cudaSuccess;
+        const unsigned grid = (unsigned)std::min<long long>((most + 7) / 8, (long long)sm_count() * 8);
+        return launch_pdl(repack_kernel, dim3(grid, n), dim3(256), 0, stream, r);
+    }
+};
 
 #define SBNET_TRY(call)                  \
     do {                                 \
@@ -706,10 +778,9 @@ template <typename T> cudaError_t forward(const FfnArgs& f, Layout& l, bool run,
     if (!run)
         return cudaSuccess;
     note_site("gated_ffn repack");
-    SBNET_TRY(repack(f.x, x, stream));
-    SBNET_TRY(repack(f.w_gate, wg, stream));
-    SBNET_TRY(repack(f.w_up, wu, stream));
-    SBNET_TRY(repack(f.w_down, wd, stream));
+    Repacks copies;
+    copies.add(f.x, x), copies.add(f.w_gate, wg), copies.add(f.w_up, wu), copies.add(f.w_down, wd);
+    SBNET_TRY(copies.run(stream));
     note_site("gated_ffn projections");
     Plan p = {};
     p.mTiles = ceil_div(R, kTileM), p.nTiles = ceil_div(F, 128), p.batch = 1, p.segs = 1, p.kIters = ceil_div(C, kStepK);
@@ -734,11 +805,9 @@ template <typename T> cudaError_t backward(const FfnArgs& f, Layout& l, bool run
     if (!run)
         return cudaSuccess;
     note_site("gated_ffn_grad repack");
-    SBNET_TRY(repack(f.x, x, stream));
-    SBNET_TRY(repack(f.dy, dy, stream));
-    SBNET_TRY(repack(f.w_gate, wg, stream));
-    SBNET_TRY(repack(f.w_up, wu, stream));
-    SBNET_TRY(repack(f.w_down, wd, stream));
+    Repacks copies;
+    copies.add(f.x, x), copies.add(f.dy, dy), copies.add(f.w_gate, wg), copies.add(f.w_up, wu), copies.add(f.w_down, wd);
+    SBNET_TRY(copies.run(stream));
     note_site("gated_ffn_grad hidden gradients");
     Plan p = {};
     p.mTiles = ceil_div(R, kTileM), p.nTiles = ceil_div(F, 256), p.batch = 1, p.segs = 1, p.kIters = ceil_div(C, kStepK);

@@ -107,9 +107,11 @@ __device__ __forceinline__ uint32_t in_first_cta(uint32_t addr)
     asm volatile("mapa.shared::cluster.u32 %0, %1, %2;" : "=r"(r) : "r"(addr), "r"(0));
     return r;
 }
+// Relaxed: hands over TMEM, which tcgen05.wait::ld and the tcgen05 fences order.  A release at cluster scope would
+// wait for this thread's global stores as well.
 __device__ __forceinline__ void mbar_arrive_cluster(uint32_t addr)
 {
-    asm volatile("mbarrier.arrive.release.cluster.shared::cluster.b64 _, [%0];" ::"r"(addr) : "memory");
+    asm volatile("mbarrier.arrive.relaxed.cluster.shared::cluster.b64 _, [%0];" ::"r"(addr) : "memory");
 }
 __device__ __forceinline__ void cluster_sync()
 {
