@@ -13,8 +13,8 @@
 // Work split.  `threads per row` T is a power of two and every thread owns the same E = 8 or 16 channels of
 // every row it meets, in vectors of VE elements spread T apart, so w, b and the gradient sums of those
 // channels stay in registers for the whole kernel.  Up to 512 channels a row belongs to a part of a warp
-// (T <= 32: reductions are shuffles, a warp works on 32/T rows at once); wider rows belong to a whole CTA
-// (T = 64 .. 1024, one shared-memory exchange per reduction).  Rows of more than 16,384 channels re-read
+// (T <= 32: reductions are shuffles, a warp works on 32/T rows at once and has several such sets in flight);
+// wider rows belong to a whole CTA (T = 64 .. 1024, one barrier a row, the next row loading behind it).  Rows of more than 16,384 channels re-read
 // the row from L2 in a plain loop.  The vector width is the widest that the row pitch and the base
 // addresses allow: 16 bytes, 4 bytes (two 16-bit elements) or one element.
 //
@@ -31,6 +31,8 @@ namespace sbnet {
 namespace {
 
 constexpr int kWarpThreads = 256;   // CTA size where a row belongs to (part of) a warp
+constexpr int kFwdCtas = 3;         // ... and such CTAs per SM, all resident: forward
+constexpr int kGradCtas = 3;        // ... backward
 
 template <typename T> __device__ __forceinline__ float to_f(T v);
 template <> __device__ __forceinline__ float to_f<float>(float v) { return v; }
@@ -40,6 +42,47 @@ template <typename T> __device__ __forceinline__ T from_f(float v);
 template <> __device__ __forceinline__ float from_f<float>(float v) { return v; }
 template <> __device__ __forceinline__ __half from_f<__half>(float v) { return __float2half_rn(v); }
 template <> __device__ __forceinline__ __nv_bfloat16 from_f<__nv_bfloat16>(float v) { return __float2bfloat16_rn(v); }
+
+// Two fp32 values in a 64-bit register: sm_100 adds and multiplies such pairs in one instruction, and these kernels
+// are as close to the issue limit as to HBM's.
+struct F2 {
+    unsigned long long v;
+};
+__device__ __forceinline__ F2 f2(float a, float b)
+{
+    F2 r;
+    asm("mov.b64 %0, {%1, %2};" : "=l"(r.v) : "f"(a), "f"(b));
+    return r;
+}
+__device__ __forceinline__ float2 unpair(F2 a)
+{
+    float2 r;
+    asm("mov.b64 {%0, %1}, %2;" : "=f"(r.x), "=f"(r.y) : "l"(a.v));
+    return r;
+}
+__device__ __forceinline__ float both(F2 a)
+{
+    const float2 r = unpair(a);
+    return r.x + r.y;
+}
+__device__ __forceinline__ F2 add2(F2 a, F2 b)
+{
+    F2 r;
+    asm("add.rn.f32x2 %0, %1, %2;" : "=l"(r.v) : "l"(a.v), "l"(b.v));
+    return r;
+}
+__device__ __forceinline__ F2 mul2(F2 a, F2 b)
+{
+    F2 r;
+    asm("mul.rn.f32x2 %0, %1, %2;" : "=l"(r.v) : "l"(a.v), "l"(b.v));
+    return r;
+}
+__device__ __forceinline__ F2 fma2(F2 a, F2 b, F2 c)
+{
+    F2 r;
+    asm("fma.rn.f32x2 %0, %1, %2, %3;" : "=l"(r.v) : "l"(a.v), "l"(b.v), "l"(c.v));
+    return r;
+}
 
 // VE elements as raw words; kept packed until they are used.
 template <typename T, int VE> struct Pack {
@@ -51,7 +94,40 @@ template <typename T, int VE> struct Pack {
     __device__ __forceinline__ void clear() { raw = vzero<kBytes>(); }
     __device__ __forceinline__ float get(int i) const { return to_f<T>(reinterpret_cast<const T*>(&raw)[i]); }
     __device__ __forceinline__ void set(int i, float v) { reinterpret_cast<T*>(&raw)[i] = from_f<T>(v); }
+    __device__ __forceinline__ void set2(int i, float2 v)    // elements i and i + 1, i even
+    {
+        if constexpr (std::is_same<T, __half>::value)
+            reinterpret_cast<__half2*>(&raw)[i / 2] = __floats2half2_rn(v.x, v.y);
+        else if constexpr (std::is_same<T, __nv_bfloat16>::value)
+            reinterpret_cast<__nv_bfloat162*>(&raw)[i / 2] = __floats2bfloat162_rn(v.x, v.y);
+        else
+            reinterpret_cast<float2*>(&raw)[i / 2] = v;
+    }
 };
+
+// A thread's E = NV * VE channels of a row as E / 2 pairs, and back.
+template <typename T, int VE, int NV> __device__ __forceinline__ F2 pair_of(const Pack<T, VE> (&v)[NV], int j)
+{
+    return f2(v[2 * j / VE].get(2 * j % VE), v[(2 * j + 1) / VE].get((2 * j + 1) % VE));
+}
+template <typename T, int VE, int NV>
+__device__ __forceinline__ void store_pairs(T* row, const F2 (&o)[NV * VE / 2], int t, int tpr, int C)
+{
+#pragma unroll
+    for (int k = 0; k < NV; ++k) {
+        const int c = (k * tpr + t) * VE;
+        Pack<T, VE> p;
+        if constexpr (VE == 1) {
+            p.set(0, k % 2 ? unpair(o[k / 2]).y : unpair(o[k / 2]).x);
+        } else {
+#pragma unroll
+            for (int i = 0; i < VE; i += 2)
+                p.set2(i, unpair(o[(k * VE + i) / 2]));
+        }
+        if (c < C)
+            p.store(row + c);
+    }
+}
 
 __device__ __forceinline__ float load_param(const void* p, int dtype, int i)
 {
@@ -105,87 +181,180 @@ template <int N> __device__ __forceinline__ void cta_sum(float (&v)[N], float* b
         v[k] = group_sum(lane < warps ? buf[k * 32 + lane] : 0.f, 32);
 }
 
-// CTA == false: `tpr` threads (<= 32) share a row.  CTA == true: the whole CTA does (tpr == blockDim.x).
-template <typename T, int VE, int NV, bool CTA> __global__ void __launch_bounds__(CTA ? 1024 : kWarpThreads)
-layer_norm_kernel(NormArgs a, int tpr)
+// This thread's channels of a row; zeros past the end of the row and for rows that are not there.
+template <typename T, int VE, int NV>
+__device__ __forceinline__ void load_row(Pack<T, VE> (&v)[NV], const T* row, bool live, int t, int tpr, int C)
 {
-    __shared__ float red[4][32];
+#pragma unroll
+    for (int k = 0; k < NV; ++k) {
+        const int c = (k * tpr + t) * VE;
+        if (live && c < C)
+            v[k].load(row + c);
+        else
+            v[k].clear();
+    }
+}
+
+// The row as pairs; returns its sum.
+template <typename T, int VE, int NV>
+__device__ __forceinline__ float row_sum(const Pack<T, VE> (&v)[NV], F2 (&f)[NV * VE / 2])
+{
+    F2 s = f2(0.f, 0.f);
+#pragma unroll
+    for (int j = 0; j < NV * VE / 2; ++j) {
+        f[j] = pair_of<T, VE, NV>(v, j);
+        s = add2(s, f[j]);
+    }
+    return both(s);
+}
+// Replaces the row by its distances from `mean` (zero past the row's end); returns the sum of their squares.
+template <int VE, int NV>
+__device__ __forceinline__ float row_spread(F2 (&f)[NV * VE / 2], float mean, int t, int tpr, int C)
+{
+    const F2 m = f2(-mean, -mean);
+#pragma unroll
+    for (int j = 0; j < NV * VE / 2; ++j)
+        f[j] = add2(f[j], m);
+    if (tpr * NV * VE != C) {    // some threads reach past the end
+#pragma unroll
+        for (int j = 0; j < NV * VE / 2; ++j) {
+            float2 d = unpair(f[j]);
+            if ((2 * j / VE * tpr + t) * VE >= C)
+                d.x = 0.f;
+            if (((2 * j + 1) / VE * tpr + t) * VE >= C)
+                d.y = 0.f;
+            f[j] = f2(d.x, d.y);
+        }
+    }
+    F2 s = f2(0.f, 0.f);
+#pragma unroll
+    for (int j = 0; j < NV * VE / 2; ++j)
+        s = fma2(f[j], f[j], s);
+    return both(s);
+}
+
+template <int VE, int NV>
+__device__ __forceinline__ void load_params(F2 (&w)[NV * VE / 2], const void* p, float dflt, int dtype, int t, int tpr, int C)
+{
+    auto at = [&](int e) {
+        const int c = (e / VE * tpr + t) * VE + e % VE;
+        return (p != nullptr && c < C) ? load_param(p, dtype, c) : dflt;
+    };
+#pragma unroll
+    for (int j = 0; j < NV * VE / 2; ++j)
+        w[j] = f2(at(2 * j), at(2 * j + 1));
+}
+
+// f: distances from the row's mean + `shift`
+template <typename T, int VE, int NV>
+__device__ __forceinline__ void store_normed(T* y, F2 (&f)[NV * VE / 2], float shift, float rstd, const F2 (&w)[NV * VE / 2],
+                                             const F2 (&b)[NV * VE / 2], int t, int tpr, int C)
+{
+    const F2 m = f2(-shift, -shift), r = f2(rstd, rstd);
+#pragma unroll
+    for (int j = 0; j < NV * VE / 2; ++j)
+        f[j] = fma2(mul2(shift == 0.f ? f[j] : add2(f[j], m), r), w[j], b[j]);
+    store_pairs<T, VE, NV>(y, f, t, tpr, C);
+}
+
+// `tpr` threads (<= 32) share a row; every turn takes ROWS rows per group so that their loads are in flight together.
+template <typename T, int VE, int NV, int ROWS> __global__ void __launch_bounds__(kWarpThreads, kFwdCtas) layer_norm_warp_kernel(NormArgs a, int tpr)
+{
     pdl_wait();
     pdl_launch_dependents();
-    const int t = CTA ? threadIdx.x : (threadIdx.x & (tpr - 1));
-    const long long perPass = CTA ? gridDim.x : (long long)gridDim.x * (kWarpThreads / tpr);
-    const long long first = CTA ? blockIdx.x : (long long)blockIdx.x * (kWarpThreads / tpr) + threadIdx.x / tpr;
+    const int t = threadIdx.x & (tpr - 1);
+    const long long groups = (long long)gridDim.x * (kWarpThreads / tpr);
+    const long long first = (long long)blockIdx.x * (kWarpThreads / tpr) + threadIdx.x / tpr;
     const long long rows = live_rows(a);
     const float inv = 1.f / (float)a.C;
-    float w[NV * VE], b[NV * VE];
-#pragma unroll
-    for (int k = 0; k < NV; ++k)
-#pragma unroll
-        for (int i = 0; i < VE; ++i) {
-            const int c = (k * tpr + t) * VE + i;
-            w[k * VE + i] = (a.weight != nullptr && c < a.C) ? load_param(a.weight, a.wdtype, c) : 1.f;
-            b[k * VE + i] = (a.bias != nullptr && c < a.C) ? load_param(a.bias, a.wdtype, c) : 0.f;
-        }
+    F2 w[NV * VE / 2], b[NV * VE / 2];
+    load_params<VE, NV>(w, a.weight, 1.f, a.wdtype, t, tpr, a.C);
+    load_params<VE, NV>(b, a.bias, 0.f, a.wdtype, t, tpr, a.C);
     // all lanes of a warp make the same number of turns (the shuffles need every lane); a lane without a
     // row of its own works on zeros and stores nothing
-    const long long turns = (rows + perPass - 1) / perPass;
-    int flip = 0;
+    const long long turns = (rows + groups * ROWS - 1) / (groups * ROWS);
     for (long long turn = 0; turn < turns; ++turn) {
-        const long long row = first + turn * perPass;
-        const bool live = row < rows;
-        if (CTA && !live)
-            break;      // the whole CTA leaves
-        const T* x = static_cast<const T*>(a.x) + row * a.C;
-        Pack<T, VE> v[NV];
-        float s[1] = {0.f};
+        const long long row0 = turn * ROWS * groups + first;
+        Pack<T, VE> v[ROWS][NV];
+        F2 f[ROWS][NV * VE / 2];
+        float mean[ROWS], rstd[ROWS];
 #pragma unroll
-        for (int k = 0; k < NV; ++k) {
-            const int c = (k * tpr + t) * VE;
-            if (live && c < a.C)
-                v[k].load(x + c);
-            else
-                v[k].clear();
+        for (int r = 0; r < ROWS; ++r)
+            load_row<T, VE, NV>(v[r], static_cast<const T*>(a.x) + (row0 + r * groups) * a.C, row0 + r * groups < rows, t, tpr, a.C);
+#pragma unroll
+        for (int r = 0; r < ROWS; ++r)
+            mean[r] = row_sum<T, VE, NV>(v[r], f[r]);
+        for (int m = tpr >> 1; m > 0; m >>= 1)
+#pragma unroll
+            for (int r = 0; r < ROWS; ++r)
+                mean[r] += __shfl_xor_sync(0xffffffffu, mean[r], m);
+#pragma unroll
+        for (int r = 0; r < ROWS; ++r) {
+            mean[r] *= inv;
+            rstd[r] = row_spread<VE, NV>(f[r], mean[r], t, tpr, a.C);
         }
+        for (int m = tpr >> 1; m > 0; m >>= 1)
 #pragma unroll
-        for (int k = 0; k < NV; ++k)
+            for (int r = 0; r < ROWS; ++r)
+                rstd[r] += __shfl_xor_sync(0xffffffffu, rstd[r], m);
 #pragma unroll
-            for (int i = 0; i < VE; ++i)
-                s[0] += v[k].get(i);
-        if (CTA)
-            cta_sum(s, red[flip]);
-        else
-            s[0] = group_sum(s[0], tpr);
-        const float mean = s[0] * inv;
-        s[0] = 0.f;
-#pragma unroll
-        for (int k = 0; k < NV; ++k)
-            if ((k * tpr + t) * VE < a.C)
-#pragma unroll
-                for (int i = 0; i < VE; ++i) {
-                    const float d = v[k].get(i) - mean;
-                    s[0] += d * d;
-                }
-        if (CTA)
-            cta_sum(s, red[flip + 1]);
-        else
-            s[0] = group_sum(s[0], tpr);
-        flip ^= 2;
-        const float rstd = rsqrtf(s[0] * inv + a.eps);
-        if (live) {
-            T* y = static_cast<T*>(a.y) + row * a.C;
-#pragma unroll
-            for (int k = 0; k < NV; ++k) {
-                const int c = (k * tpr + t) * VE;
-                Pack<T, VE> o;
-#pragma unroll
-                for (int i = 0; i < VE; ++i)
-                    o.set(i, (v[k].get(i) - mean) * rstd * w[k * VE + i] + b[k * VE + i]);
-                if (c < a.C)
-                    o.store(y + c);
-            }
+        for (int r = 0; r < ROWS; ++r) {
+            const long long row = row0 + r * groups;
+            if (row >= rows)
+                continue;
+            rstd[r] = rsqrtf(rstd[r] * inv + a.eps);
+            store_normed<T, VE, NV>(static_cast<T*>(a.y) + row * a.C, f[r], 0.f, rstd[r], w, b, t, tpr, a.C);
             if (t == 0 && a.mean != nullptr)
-                a.mean[row] = mean, a.rstd[row] = rstd;
+                a.mean[row] = mean[r], a.rstd[row] = rstd[r];
         }
+    }
+}
+
+// The whole CTA shares a row.  Each warp takes mean and spread of its own channels, and the warps' results are joined
+// (mean = sum n_w mean_w / C, spread = sum spread_w + n_w (mean_w - mean)^2), which needs one barrier a row; the next
+// row's loads are issued before it.
+template <typename T, int VE, int NV, int MAXT> __global__ void __launch_bounds__(MAXT) layer_norm_cta_kernel(NormArgs a)
+{
+    __shared__ float red[2][64];
+    pdl_wait();
+    pdl_launch_dependents();
+    const int t = threadIdx.x, tpr = blockDim.x, lane = t & 31, warp = t >> 5, warps = tpr >> 5;
+    const long long rows = live_rows(a);
+    const float inv = 1.f / (float)a.C;
+    F2 w[NV * VE / 2], b[NV * VE / 2];
+    load_params<VE, NV>(w, a.weight, 1.f, a.wdtype, t, tpr, a.C);
+    load_params<VE, NV>(b, a.bias, 0.f, a.wdtype, t, tpr, a.C);
+    // channels of warp q: of each of the NV vectors, those of its 32 threads that the row reaches
+    auto channels = [&](int q) {
+        int n = 0;
+#pragma unroll
+        for (int k = 0; k < NV; ++k)
+            n += min(max(a.C - (k * tpr + q * 32) * VE, 0), 32 * VE);
+        return (float)n;
+    };
+    const float own = channels(warp), ownInv = own > 0.f ? 1.f / own : 0.f, laneCount = lane < warps ? channels(lane) : 0.f;
+    long long row = blockIdx.x;
+    Pack<T, VE> v[NV], next[NV];
+    load_row<T, VE, NV>(v, static_cast<const T*>(a.x) + row * a.C, row < rows, t, tpr, a.C);
+    for (int flip = 0; row < rows; row += gridDim.x, flip ^= 1) {
+        const long long ahead = row + gridDim.x;
+        load_row<T, VE, NV>(next, static_cast<const T*>(a.x) + ahead * a.C, ahead < rows, t, tpr, a.C);
+        F2 f[NV * VE / 2];
+        const float m = group_sum(row_sum<T, VE, NV>(v, f), 32) * ownInv;
+        const float q = group_sum(row_spread<VE, NV>(f, m, t, tpr, a.C), 32);
+        if (lane == 0)
+            red[flip][warp] = m, red[flip][32 + warp] = q;
+        __syncthreads();
+        const float mw = lane < warps ? red[flip][lane] : 0.f, qw = lane < warps ? red[flip][32 + lane] : 0.f;
+        const float mean = group_sum(mw * laneCount, 32) * inv;
+        const float spread = group_sum(qw + laneCount * (mw - mean) * (mw - mean), 32);
+        const float rstd = rsqrtf(spread * inv + a.eps);
+        store_normed<T, VE, NV>(static_cast<T*>(a.y) + row * a.C, f, mean - m, rstd, w, b, t, tpr, a.C);
+        if (t == 0 && a.mean != nullptr)
+            a.mean[row] = mean, a.rstd[row] = rstd;
+#pragma unroll
+        for (int k = 0; k < NV; ++k)
+            v[k] = next[k];
     }
 }
 
@@ -224,109 +393,154 @@ template <typename T> __global__ void __launch_bounds__(1024) layer_norm_loop_ke
 }
 
 // ---- backward --------------------------------------------------------------------------------------
-template <typename T, int VE, int NV, bool CTA> __global__ void __launch_bounds__(CTA ? 1024 : kWarpThreads)
-layer_norm_grad_kernel(NormArgs a, int tpr)
+template <int E> __device__ __forceinline__ float element(const F2 (&v)[E / 2], int e)
+{
+    const float2 p = unpair(v[e / 2]);
+    return e % 2 ? p.y : p.x;
+}
+
+// One row's products: adds to the column sums, keeps xh and gw, and returns sum(gw) and sum(gw * xh) of this thread's
+// channels (g reads as zero past the row's end and for rows that are not there).
+template <typename T, int VE, int NV>
+__device__ __forceinline__ void grad_sums(const Pack<T, VE> (&xv)[NV], const Pack<T, VE> (&gv)[NV], float mean, float rstd,
+                                          const F2 (&w)[NV * VE / 2], F2 (&dw)[NV * VE / 2], F2 (&db)[NV * VE / 2],
+                                          F2 (&xh)[NV * VE / 2], F2 (&gw)[NV * VE / 2], float& s0, float& s1)
+{
+    const F2 m = f2(-mean, -mean), r = f2(rstd, rstd);
+    F2 a0 = f2(0.f, 0.f), a1 = a0;
+#pragma unroll
+    for (int j = 0; j < NV * VE / 2; ++j) {
+        const F2 gi = pair_of<T, VE, NV>(gv, j);
+        xh[j] = mul2(add2(pair_of<T, VE, NV>(xv, j), m), r), gw[j] = mul2(gi, w[j]);
+        dw[j] = fma2(gi, xh[j], dw[j]), db[j] = add2(db[j], gi);
+        a0 = add2(a0, gw[j]), a1 = fma2(gw[j], xh[j], a1);
+    }
+    s0 = both(a0), s1 = both(a1);
+}
+template <typename T, int VE, int NV>
+__device__ __forceinline__ void store_dx(T* dx, F2 (&xh)[NV * VE / 2], const F2 (&gw)[NV * VE / 2], float rstd, float m0, float m1,
+                                         int t, int tpr, int C)
+{
+    const F2 r = f2(rstd, rstd), n0 = f2(-m0, -m0), n1 = f2(-m1, -m1);
+#pragma unroll
+    for (int j = 0; j < NV * VE / 2; ++j)
+        xh[j] = mul2(r, fma2(xh[j], n1, add2(gw[j], n0)));
+    store_pairs<T, VE, NV>(dx, xh, t, tpr, C);
+}
+
+template <typename T, int VE, int NV, int ROWS> __global__ void __launch_bounds__(kWarpThreads, kGradCtas) layer_norm_grad_warp_kernel(NormArgs a, int tpr)
 {
     constexpr int E = NV * VE;
-    __shared__ float red[2][64];
-    extern __shared__ float cols[];     // CTA == false: [rows at once][2][tpr * E] column sums
+    extern __shared__ float cols[];     // [groups of the CTA][2][tpr * E] column sums
     pdl_wait();
     pdl_launch_dependents();
-    const int t = CTA ? threadIdx.x : (threadIdx.x & (tpr - 1));
-    const long long perPass = CTA ? gridDim.x : (long long)gridDim.x * (kWarpThreads / tpr);
-    const long long first = CTA ? blockIdx.x : (long long)blockIdx.x * (kWarpThreads / tpr) + threadIdx.x / tpr;
+    const int t = threadIdx.x & (tpr - 1);
+    const long long groups = (long long)gridDim.x * (kWarpThreads / tpr);
+    const long long first = (long long)blockIdx.x * (kWarpThreads / tpr) + threadIdx.x / tpr;
     const float inv = 1.f / (float)a.C;
-    float w[E], dw[E], db[E];
-#pragma unroll
-    for (int k = 0; k < NV; ++k)
-#pragma unroll
-        for (int i = 0; i < VE; ++i) {
-            const int c = (k * tpr + t) * VE + i;
-            w[k * VE + i] = (a.weight != nullptr && c < a.C) ? load_param(a.weight, a.wdtype, c) : 1.f;
-            dw[k * VE + i] = 0.f, db[k * VE + i] = 0.f;
-        }
-    const long long turns = (a.rows + perPass - 1) / perPass;
-    int flip = 0;
+    F2 w[E / 2], dw[E / 2] = {}, db[E / 2] = {};
+    load_params<VE, NV>(w, a.weight, 1.f, a.wdtype, t, tpr, a.C);
+    const long long turns = (a.rows + groups * ROWS - 1) / (groups * ROWS);
     for (long long turn = 0; turn < turns; ++turn) {
-        const long long row = first + turn * perPass;
-        const bool live = row < a.rows;
-        if (CTA && !live)
-            break;
-        const T* x = static_cast<const T*>(a.x) + row * a.C;
-        const T* g = static_cast<const T*>(a.g) + row * a.C;
-        Pack<T, VE> xv[NV], gv[NV];
+        const long long row0 = turn * ROWS * groups + first;
+        Pack<T, VE> xv[ROWS][NV], gv[ROWS][NV];
+        F2 xh[ROWS][E / 2], gw[ROWS][E / 2];
+        float mean[ROWS], rstd[ROWS], s0[ROWS], s1[ROWS];
 #pragma unroll
-        for (int k = 0; k < NV; ++k) {
-            const int c = (k * tpr + t) * VE;
-            if (live && c < a.C)
-                xv[k].load(x + c), gv[k].load(g + c);
-            else
-                xv[k].clear(), gv[k].clear();
+        for (int r = 0; r < ROWS; ++r) {
+            const long long row = row0 + r * groups;
+            const bool live = row < a.rows;
+            load_row<T, VE, NV>(xv[r], static_cast<const T*>(a.x) + row * a.C, live, t, tpr, a.C);
+            load_row<T, VE, NV>(gv[r], static_cast<const T*>(a.g) + row * a.C, live, t, tpr, a.C);
+            mean[r] = live ? a.mean[row] : 0.f, rstd[r] = live ? a.rstd[row] : 0.f;
         }
-        const float mean = live ? a.mean[row] : 0.f, rstd = live ? a.rstd[row] : 0.f;
-        float s[2] = {0.f, 0.f};
 #pragma unroll
-        for (int k = 0; k < NV; ++k)
+        for (int r = 0; r < ROWS; ++r)
+            grad_sums<T, VE, NV>(xv[r], gv[r], mean[r], rstd[r], w, dw, db, xh[r], gw[r], s0[r], s1[r]);
+        for (int m = tpr >> 1; m > 0; m >>= 1)
 #pragma unroll
-            for (int i = 0; i < VE; ++i) {
-                const float xh = (xv[k].get(i) - mean) * rstd, gi = gv[k].get(i);    // gi == 0 past the row's end
-                const float gw = gi * w[k * VE + i];
-                dw[k * VE + i] += gi * xh, db[k * VE + i] += gi;
-                s[0] += gw, s[1] += gw * xh;
+            for (int r = 0; r < ROWS; ++r) {
+                s0[r] += __shfl_xor_sync(0xffffffffu, s0[r], m);
+                s1[r] += __shfl_xor_sync(0xffffffffu, s1[r], m);
             }
-        if (CTA)
-            cta_sum(s, red[flip]);
-        else
-            s[0] = group_sum(s[0], tpr), s[1] = group_sum(s[1], tpr);
-        flip ^= 1;
-        if (live) {
-            T* dx = static_cast<T*>(a.y) + row * a.C;
-            const float m0 = s[0] * inv, m1 = s[1] * inv;
 #pragma unroll
-            for (int k = 0; k < NV; ++k) {
-                const int c = (k * tpr + t) * VE;
-                Pack<T, VE> o;
-#pragma unroll
-                for (int i = 0; i < VE; ++i) {
-                    const float xh = (xv[k].get(i) - mean) * rstd;
-                    o.set(i, rstd * (gv[k].get(i) * w[k * VE + i] - m0 - xh * m1));
-                }
-                if (c < a.C)
-                    o.store(dx + c);
-            }
+        for (int r = 0; r < ROWS; ++r) {
+            const long long row = row0 + r * groups;
+            if (row < a.rows)
+                store_dx<T, VE, NV>(static_cast<T*>(a.y) + row * a.C, xh[r], gw[r], rstd[r], s0[r] * inv, s1[r] * inv, t, tpr, a.C);
         }
     }
     if (a.partials == nullptr)
         return;
     float* pw = a.partials + (long long)blockIdx.x * 2 * a.C;
-    if (CTA) {
+    const int inCta = kWarpThreads / tpr, grp = threadIdx.x / tpr, width = tpr * E;
 #pragma unroll
-        for (int k = 0; k < NV; ++k)
+    for (int k = 0; k < NV; ++k)
 #pragma unroll
-            for (int i = 0; i < VE; ++i) {
-                const int c = (k * tpr + t) * VE + i;
-                if (c < a.C)
-                    pw[c] = dw[k * VE + i], pw[a.C + c] = db[k * VE + i];
-            }
-    } else {
-        const int groups = kWarpThreads / tpr, grp = threadIdx.x / tpr, width = tpr * E;
-#pragma unroll
-        for (int k = 0; k < NV; ++k)
-#pragma unroll
-            for (int i = 0; i < VE; ++i) {
-                const int c = (k * tpr + t) * VE + i;
-                cols[(grp * 2 + 0) * width + c] = dw[k * VE + i];
-                cols[(grp * 2 + 1) * width + c] = db[k * VE + i];
-            }
-        __syncthreads();
-        for (int c = threadIdx.x; c < 2 * a.C; c += kWarpThreads) {
-            const int half = c >= a.C, cc = c - half * a.C;
-            float s = 0.f;
-            for (int q = 0; q < groups; ++q)
-                s += cols[(q * 2 + half) * width + cc];
-            pw[c] = s;
+        for (int i = 0; i < VE; ++i) {
+            const int c = (k * tpr + t) * VE + i;
+            cols[(grp * 2 + 0) * width + c] = element<E>(dw, k * VE + i);
+            cols[(grp * 2 + 1) * width + c] = element<E>(db, k * VE + i);
         }
+    __syncthreads();
+    for (int c = threadIdx.x; c < 2 * a.C; c += kWarpThreads) {
+        const int half = c >= a.C, cc = c - half * a.C;
+        float s = 0.f;
+        for (int q = 0; q < inCta; ++q)
+            s += cols[(q * 2 + half) * width + cc];
+        pw[c] = s;
     }
+}
+
+// AHEAD: the next row's loads are issued before this row's barrier (where the registers allow it).
+template <typename T, int VE, int NV, int MAXT, bool AHEAD> __global__ void __launch_bounds__(MAXT) layer_norm_grad_cta_kernel(NormArgs a)
+{
+    constexpr int E = NV * VE;
+    __shared__ float red[2][64];
+    pdl_wait();
+    pdl_launch_dependents();
+    const int t = threadIdx.x, tpr = blockDim.x;
+    const float inv = 1.f / (float)a.C;
+    F2 w[E / 2], dw[E / 2] = {}, db[E / 2] = {};
+    load_params<VE, NV>(w, a.weight, 1.f, a.wdtype, t, tpr, a.C);
+    const T *x = static_cast<const T*>(a.x), *g = static_cast<const T*>(a.g);
+    long long row = blockIdx.x;
+    Pack<T, VE> xv[NV], gv[NV], xn[NV], gn[NV];
+    if (AHEAD) {
+        load_row<T, VE, NV>(xv, x + row * a.C, row < a.rows, t, tpr, a.C);
+        load_row<T, VE, NV>(gv, g + row * a.C, row < a.rows, t, tpr, a.C);
+    }
+    for (int flip = 0; row < a.rows; row += gridDim.x, flip ^= 1) {
+        const float mean = a.mean[row], rstd = a.rstd[row];
+        if (AHEAD) {
+            const long long ahead = row + gridDim.x;
+            load_row<T, VE, NV>(xn, x + ahead * a.C, ahead < a.rows, t, tpr, a.C);
+            load_row<T, VE, NV>(gn, g + ahead * a.C, ahead < a.rows, t, tpr, a.C);
+        } else {
+            load_row<T, VE, NV>(xv, x + row * a.C, true, t, tpr, a.C);
+            load_row<T, VE, NV>(gv, g + row * a.C, true, t, tpr, a.C);
+        }
+        F2 xh[E / 2], gw[E / 2];
+        float s[2];
+        grad_sums<T, VE, NV>(xv, gv, mean, rstd, w, dw, db, xh, gw, s[0], s[1]);
+        cta_sum(s, red[flip]);
+        store_dx<T, VE, NV>(static_cast<T*>(a.y) + row * a.C, xh, gw, rstd, s[0] * inv, s[1] * inv, t, tpr, a.C);
+        if (AHEAD)
+#pragma unroll
+            for (int k = 0; k < NV; ++k)
+                xv[k] = xn[k], gv[k] = gn[k];
+    }
+    if (a.partials == nullptr)
+        return;
+    float* pw = a.partials + (long long)blockIdx.x * 2 * a.C;
+#pragma unroll
+    for (int k = 0; k < NV; ++k)
+#pragma unroll
+        for (int i = 0; i < VE; ++i) {
+            const int c = (k * tpr + t) * VE + i;
+            if (c < a.C)
+                pw[c] = element<E>(dw, k * VE + i), pw[a.C + c] = element<E>(db, k * VE + i);
+        }
 }
 
 template <typename T> __global__ void __launch_bounds__(1024) layer_norm_grad_loop_kernel(NormArgs a)
@@ -394,7 +608,11 @@ struct NormShape {
     bool cta;
 };
 
-NormShape pick(int C, int itemsize, uintptr_t bits)
+// Up to 512 channels a row stays inside a warp, 16 channels a thread where that leaves at least 8 threads a row (fewer
+// exchanges per channel); in the backward pass the column sums leave registers for 8 up to 256 channels.  Then whole
+// CTAs: 8 a thread up to 2,048 channels, 16 beyond (half the threads, so that two or more rows share an SM), in the
+// backward pass 8 until the CTA is full.
+NormShape pick(int C, int itemsize, uintptr_t bits, bool grad)
 {
     NormShape s = {itemsize, 0, 0, false};
     const uintptr_t all = bits | (uintptr_t)((long long)C * itemsize);
@@ -402,15 +620,14 @@ NormShape pick(int C, int itemsize, uintptr_t bits)
         s.vecBytes = 16;
     else if (itemsize == 2 && (all & 3) == 0)
         s.vecBytes = 4;
-    // up to 256 channels: 8 a thread; up to 512: 16 a thread, still inside a warp; then whole CTAs
     if (C <= 512) {
-        s.elems = C <= 256 ? 8 : 16;
+        s.elems = C <= (grad ? 256 : 64) ? 8 : 16;
         s.tpr = 4;
         while (s.tpr * s.elems < C)
             s.tpr *= 2;
     } else if (C <= 16384) {
         s.cta = true;
-        s.elems = C <= 8192 ? 8 : 16;
+        s.elems = C <= (grad ? 8192 : 2048) ? 8 : 16;
         s.tpr = 64;
         while (s.tpr * s.elems < C)
             s.tpr *= 2;
@@ -420,26 +637,35 @@ NormShape pick(int C, int itemsize, uintptr_t bits)
 
 template <typename T, int VE, int NV> cudaError_t launch_fwd(const NormArgs& a, const NormShape& s, cudaStream_t stream)
 {
+    constexpr int E = VE * NV;
     if (s.cta) {
-        const long long grid = std::min<long long>(a.rows, (long long)sm_count() * (2048 / s.tpr) * 4);
-        return launch_pdl(layer_norm_kernel<T, VE, NV, true>, dim3((unsigned)grid), dim3(s.tpr), 0, stream, a, s.tpr);
+        const long long grid = std::min<long long>(a.rows, (long long)sm_count() * (2048 / s.tpr));
+        return launch_pdl(layer_norm_cta_kernel<T, VE, NV, E == 8 ? 256 : 1024>, dim3((unsigned)grid), dim3(s.tpr), 0, stream, a);
     }
+    constexpr int ROWS = E == 8 ? 4 : 2;
+    // one row a group while that leaves SMs empty, ROWS in flight per group otherwise
     const long long ctas = (a.rows * s.tpr + kWarpThreads - 1) / kWarpThreads;
-    const long long grid = std::min<long long>(ctas, (long long)sm_count() * 8);
-    return launch_pdl(layer_norm_kernel<T, VE, NV, false>, dim3((unsigned)grid), dim3(kWarpThreads), 0, stream, a, s.tpr);
+    if (ctas <= (long long)sm_count() * kFwdCtas)
+        return launch_pdl(layer_norm_warp_kernel<T, VE, NV, 1>, dim3((unsigned)ctas), dim3(kWarpThreads), 0, stream, a, s.tpr);
+    const long long grid = std::min<long long>(ctas, (long long)sm_count() * kFwdCtas);
+    return launch_pdl(layer_norm_warp_kernel<T, VE, NV, ROWS>, dim3((unsigned)grid), dim3(kWarpThreads), 0, stream, a, s.tpr);
 }
 
 template <typename T, int VE, int NV> cudaError_t launch_bwd(const NormArgs& a, const NormShape& s, int grid, cudaStream_t stream)
 {
-    if (s.cta)
-        return launch_pdl(layer_norm_grad_kernel<T, VE, NV, true>, dim3(grid), dim3(s.tpr), 0, stream, a, s.tpr);
-    const size_t smem = a.partials == nullptr ? 0 : sizeof(float) * 2 * kWarpThreads * NV * VE;
-    return launch_pdl(layer_norm_grad_kernel<T, VE, NV, false>, dim3(grid), dim3(kWarpThreads), smem, stream, a, s.tpr);
+    constexpr int E = VE * NV;
+    if (s.cta) {
+        if (E == 8 && s.tpr <= 256)
+            return launch_pdl(layer_norm_grad_cta_kernel<T, VE, NV, 256, true>, dim3(grid), dim3(s.tpr), 0, stream, a);
+        return launch_pdl(layer_norm_grad_cta_kernel<T, VE, NV, 1024, E == 8 && sizeof(T) == 2>, dim3(grid), dim3(s.tpr), 0, stream, a);
+    }
+    const size_t smem = a.partials == nullptr ? 0 : sizeof(float) * 2 * kWarpThreads * E;
+    return launch_pdl(layer_norm_grad_warp_kernel<T, VE, NV, E == 8 ? 2 : 1>, dim3(grid), dim3(kWarpThreads), smem, stream, a, s.tpr);
 }
 
 template <typename T> cudaError_t run_fwd(const NormArgs& a, cudaStream_t stream)
 {
-    const NormShape s = pick(a.C, sizeof(T), reinterpret_cast<uintptr_t>(a.x) | reinterpret_cast<uintptr_t>(a.y));
+    const NormShape s = pick(a.C, sizeof(T), reinterpret_cast<uintptr_t>(a.x) | reinterpret_cast<uintptr_t>(a.y), false);
     constexpr int V16 = 16 / (int)sizeof(T);
     if (s.tpr == 0)
         return launch_pdl(layer_norm_loop_kernel<T>, dim3((unsigned)std::min<long long>(a.rows, sm_count() * 2)), dim3(1024),
@@ -455,7 +681,7 @@ template <typename T> cudaError_t run_fwd(const NormArgs& a, cudaStream_t stream
 template <typename T> cudaError_t run_bwd(const NormArgs& a, int grid, cudaStream_t stream)
 {
     const NormShape s = pick(a.C, sizeof(T), reinterpret_cast<uintptr_t>(a.x) | reinterpret_cast<uintptr_t>(a.y) |
-                                                 reinterpret_cast<uintptr_t>(a.g));
+                                                 reinterpret_cast<uintptr_t>(a.g), true);
     constexpr int V16 = 16 / (int)sizeof(T);
     if (s.tpr == 0)
         return launch_pdl(layer_norm_grad_loop_kernel<T>, dim3(grid), dim3(1024), 0, stream, a);
@@ -472,12 +698,12 @@ template <typename T> cudaError_t run_bwd(const NormArgs& a, int grid, cudaStrea
 // CTAs of the backward kernel = partial rows of the column sums.  Depends on the sizes only.
 int layer_norm_grad_parts(long long rows, int C)
 {
-    const NormShape s = pick(C, 4, 0);
+    const NormShape s = pick(C, 4, 0, true);
     if (s.tpr == 0)
         return (int)std::min<long long>(rows, sm_count());
     if (s.cta)
         return (int)std::min<long long>(rows, (long long)sm_count() * std::max(1, 1024 / s.tpr));
-    return (int)std::min<long long>((rows * s.tpr + kWarpThreads - 1) / kWarpThreads, (long long)sm_count() * 4);
+    return (int)std::min<long long>((rows * s.tpr + kWarpThreads - 1) / kWarpThreads, (long long)sm_count() * kGradCtas);
 }
 
 cudaError_t launch_layer_norm(const NormArgs& a, int dtype, cudaStream_t stream)
