@@ -32,7 +32,8 @@ namespace {
 
 constexpr int kWarpThreads = 256;   // CTA size where a row belongs to (part of) a warp
 constexpr int kFwdCtas = 3;         // ... and such CTAs per SM, all resident: forward
-constexpr int kGradCtas = 3;        // ... backward
+constexpr int kGradCtas = 3;        // ... backward with 8 channels a thread
+constexpr int kGradCtas16 = 2;      // ... with 16
 
 template <typename T> __device__ __forceinline__ float to_f(T v);
 template <> __device__ __forceinline__ float to_f<float>(float v) { return v; }
@@ -195,6 +196,55 @@ __device__ __forceinline__ void load_row(Pack<T, VE> (&v)[NV], const T* row, boo
     }
 }
 
+// Loads that run ahead of their use through shared memory: every thread copies its own vectors of the turns to come
+// (cp.async) into slots of its own and reads them back itself, so nothing but the thread's own wait is needed and no
+// registers are held meanwhile.  Vectors of one 16-bit element are too narrow for cp.async and are loaded when used.
+constexpr int kAhead = 3;      // turns in shared memory: the current one and two in flight
+constexpr int kAheadCta = 2;   // the same in the whole-CTA backward kernel, whose turns are two rows of two tensors
+template <typename T, int VE> constexpr bool kCanRunAhead = VE * sizeof(T) >= 4;
+template <typename T, int VE> constexpr int kSlotBytes = kCanRunAhead<T, VE> ? VE * (int)sizeof(T) : 0;
+
+template <typename T, int VE, int NV>
+__device__ __forceinline__ void copy_row(uint32_t slots, const T* row, bool live, int t, int tpr, int C)
+{
+    if constexpr (kCanRunAhead<T, VE>) {
+#pragma unroll
+        for (int k = 0; k < NV; ++k) {
+            const int c = (k * tpr + t) * VE;
+            const uint32_t dst = slots + k * blockDim.x * kSlotBytes<T, VE>;
+            if (live && c < C) {
+                if constexpr (VE * sizeof(T) == 16)
+                    asm volatile("cp.async.cg.shared.global [%0], [%1], 16;" ::"r"(dst), "l"(row + c) : "memory");
+                else
+                    asm volatile("cp.async.ca.shared.global [%0], [%1], 4;" ::"r"(dst), "l"(row + c) : "memory");
+            }
+        }
+    }
+}
+template <typename T, int VE, int NV>
+__device__ __forceinline__ void take_row(Pack<T, VE> (&v)[NV], uint32_t slots, const T* row, bool live, int t, int tpr, int C)
+{
+    if constexpr (kCanRunAhead<T, VE>) {
+#pragma unroll
+        for (int k = 0; k < NV; ++k) {
+            const uint32_t src = slots + k * blockDim.x * kSlotBytes<T, VE>;
+            v[k].clear();
+            if (live && (k * tpr + t) * VE < C) {
+                if constexpr (VE * sizeof(T) == 16)
+                    v[k].raw = lds128(src);
+                else
+                    v[k].raw = lds32(src);
+            }
+        }
+    } else {
+        load_row<T, VE, NV>(v, row, live, t, tpr, C);
+    }
+}
+__device__ __forceinline__ void copies_commit() { asm volatile("cp.async.commit_group;" ::: "memory"); }
+__device__ __forceinline__ void copies_wait() { asm volatile("cp.async.wait_group %0;" ::"n"(kAhead - 1) : "memory"); }
+// Shared memory of `rows` rows (or pairs of rows) per turn and thread.
+template <typename T, int VE, int NV> constexpr int slots_bytes(int threads, int rows) { return kAhead * rows * NV * threads * kSlotBytes<T, VE>; }
+
 // The row as pairs; returns its sum.
 template <typename T, int VE, int NV>
 __device__ __forceinline__ float row_sum(const Pack<T, VE> (&v)[NV], F2 (&f)[NV * VE / 2])
@@ -257,9 +307,11 @@ __device__ __forceinline__ void store_normed(T* y, F2 (&f)[NV * VE / 2], float s
     store_pairs<T, VE, NV>(y, f, t, tpr, C);
 }
 
-// `tpr` threads (<= 32) share a row; every turn takes ROWS rows per group so that their loads are in flight together.
-template <typename T, int VE, int NV, int ROWS> __global__ void __launch_bounds__(kWarpThreads, kFwdCtas) layer_norm_warp_kernel(NormArgs a, int tpr)
+// `tpr` threads (<= 32) share a row; every turn takes ROWS rows per group.
+template <typename T, int VE, int NV, int ROWS>
+__global__ void __launch_bounds__(kWarpThreads, kFwdCtas) layer_norm_warp_kernel(NormArgs a, int tpr)
 {
+    extern __shared__ __align__(16) uint8_t dyn[];
     pdl_wait();
     pdl_launch_dependents();
     const int t = threadIdx.x & (tpr - 1);
@@ -267,23 +319,42 @@ template <typename T, int VE, int NV, int ROWS> __global__ void __launch_bounds_
     const long long first = (long long)blockIdx.x * (kWarpThreads / tpr) + threadIdx.x / tpr;
     const long long rows = live_rows(a);
     const float inv = 1.f / (float)a.C;
-    F2 w[NV * VE / 2], b[NV * VE / 2];
-    load_params<VE, NV>(w, a.weight, 1.f, a.wdtype, t, tpr, a.C);
-    load_params<VE, NV>(b, a.bias, 0.f, a.wdtype, t, tpr, a.C);
+    const T* x = static_cast<const T*>(a.x);
+    constexpr int rowBytes = NV * kWarpThreads * kSlotBytes<T, VE>;
+    const uint32_t slots = smem_u32(dyn) + threadIdx.x * kSlotBytes<T, VE>;
     // all lanes of a warp make the same number of turns (the shuffles need every lane); a lane without a
     // row of its own works on zeros and stores nothing
     const long long turns = (rows + groups * ROWS - 1) / (groups * ROWS);
-    for (long long turn = 0; turn < turns; ++turn) {
+    auto fetch = [&](long long turn, uint32_t stage) {
+        const uint32_t at = slots + stage * ROWS * rowBytes;
+#pragma unroll
+        for (int r = 0; r < ROWS; ++r) {
+            const long long row = (turn * ROWS + r) * groups + first;
+            copy_row<T, VE, NV>(at + r * rowBytes, x + row * a.C, row < rows, t, tpr, a.C);
+        }
+        copies_commit();
+    };
+#pragma unroll
+    for (int i = 0; i < kAhead - 1; ++i)
+        fetch(i, i);
+    F2 w[NV * VE / 2], b[NV * VE / 2];
+    load_params<VE, NV>(w, a.weight, 1.f, a.wdtype, t, tpr, a.C);
+    load_params<VE, NV>(b, a.bias, 0.f, a.wdtype, t, tpr, a.C);
+    uint32_t stage = 0;
+    for (long long turn = 0; turn < turns; ++turn, stage = stage + 1 == kAhead ? 0 : stage + 1) {
         const long long row0 = turn * ROWS * groups + first;
-        Pack<T, VE> v[ROWS][NV];
+        fetch(turn + kAhead - 1, stage == 0 ? kAhead - 1 : stage - 1);
+        copies_wait();
+        const uint32_t at = slots + stage * ROWS * rowBytes;
         F2 f[ROWS][NV * VE / 2];
         float mean[ROWS], rstd[ROWS];
 #pragma unroll
-        for (int r = 0; r < ROWS; ++r)
-            load_row<T, VE, NV>(v[r], static_cast<const T*>(a.x) + (row0 + r * groups) * a.C, row0 + r * groups < rows, t, tpr, a.C);
-#pragma unroll
-        for (int r = 0; r < ROWS; ++r)
-            mean[r] = row_sum<T, VE, NV>(v[r], f[r]);
+        for (int r = 0; r < ROWS; ++r) {
+            const long long row = row0 + r * groups;
+            Pack<T, VE> v[NV];
+            take_row<T, VE, NV>(v, at + r * rowBytes, x + row * a.C, row < rows, t, tpr, a.C);
+            mean[r] = row_sum<T, VE, NV>(v, f[r]);
+        }
         for (int m = tpr >> 1; m > 0; m >>= 1)
 #pragma unroll
             for (int r = 0; r < ROWS; ++r)
@@ -311,16 +382,25 @@ template <typename T, int VE, int NV, int ROWS> __global__ void __launch_bounds_
 }
 
 // The whole CTA shares a row.  Each warp takes mean and spread of its own channels, and the warps' results are joined
-// (mean = sum n_w mean_w / C, spread = sum spread_w + n_w (mean_w - mean)^2), which needs one barrier a row; the next
-// row's loads are issued before it.
-template <typename T, int VE, int NV, int MAXT> __global__ void __launch_bounds__(MAXT) layer_norm_cta_kernel(NormArgs a)
+// (mean = sum n_w mean_w / C, spread = sum spread_w + n_w (mean_w - mean)^2), which needs one barrier a row.
+template <typename T, int VE, int NV, int MAXT> __global__ void __launch_bounds__(MAXT, MAXT == 1024 ? 1 : 1024 / MAXT) layer_norm_cta_kernel(NormArgs a)
 {
+    extern __shared__ __align__(16) uint8_t dyn[];
     __shared__ float red[2][64];
     pdl_wait();
     pdl_launch_dependents();
     const int t = threadIdx.x, tpr = blockDim.x, lane = t & 31, warp = t >> 5, warps = tpr >> 5;
     const long long rows = live_rows(a);
     const float inv = 1.f / (float)a.C;
+    const T* x = static_cast<const T*>(a.x);
+    const uint32_t rowBytes = NV * tpr * kSlotBytes<T, VE>, slots = smem_u32(dyn) + t * kSlotBytes<T, VE>;
+    auto fetch = [&](long long row, uint32_t stage) {
+        copy_row<T, VE, NV>(slots + stage * rowBytes, x + row * a.C, row < rows, t, tpr, a.C);
+        copies_commit();
+    };
+#pragma unroll
+    for (int i = 0; i < kAhead - 1; ++i)
+        fetch(blockIdx.x + (long long)i * gridDim.x, i);
     F2 w[NV * VE / 2], b[NV * VE / 2];
     load_params<VE, NV>(w, a.weight, 1.f, a.wdtype, t, tpr, a.C);
     load_params<VE, NV>(b, a.bias, 0.f, a.wdtype, t, tpr, a.C);
@@ -333,12 +413,13 @@ template <typename T, int VE, int NV, int MAXT> __global__ void __launch_bounds_
         return (float)n;
     };
     const float own = channels(warp), ownInv = own > 0.f ? 1.f / own : 0.f, laneCount = lane < warps ? channels(lane) : 0.f;
-    long long row = blockIdx.x;
-    Pack<T, VE> v[NV], next[NV];
-    load_row<T, VE, NV>(v, static_cast<const T*>(a.x) + row * a.C, row < rows, t, tpr, a.C);
-    for (int flip = 0; row < rows; row += gridDim.x, flip ^= 1) {
-        const long long ahead = row + gridDim.x;
-        load_row<T, VE, NV>(next, static_cast<const T*>(a.x) + ahead * a.C, ahead < rows, t, tpr, a.C);
+    uint32_t stage = 0;
+    int flip = 0;
+    for (long long row = blockIdx.x; row < rows; row += gridDim.x, flip ^= 1, stage = stage + 1 == kAhead ? 0 : stage + 1) {
+        fetch(row + (kAhead - 1ll) * gridDim.x, stage == 0 ? kAhead - 1 : stage - 1);
+        copies_wait();
+        Pack<T, VE> v[NV];
+        take_row<T, VE, NV>(v, slots + stage * rowBytes, x + row * a.C, true, t, tpr, a.C);
         F2 f[NV * VE / 2];
         const float m = group_sum(row_sum<T, VE, NV>(v, f), 32) * ownInv;
         const float q = group_sum(row_spread<VE, NV>(f, m, t, tpr, a.C), 32);
@@ -352,9 +433,6 @@ template <typename T, int VE, int NV, int MAXT> __global__ void __launch_bounds_
         store_normed<T, VE, NV>(static_cast<T*>(a.y) + row * a.C, f, mean - m, rstd, w, b, t, tpr, a.C);
         if (t == 0 && a.mean != nullptr)
             a.mean[row] = mean, a.rstd[row] = rstd;
-#pragma unroll
-        for (int k = 0; k < NV; ++k)
-            v[k] = next[k];
     }
 }
 
@@ -428,35 +506,66 @@ __device__ __forceinline__ void store_dx(T* dx, F2 (&xh)[NV * VE / 2], const F2 
     store_pairs<T, VE, NV>(dx, xh, t, tpr, C);
 }
 
-template <typename T, int VE, int NV, int ROWS> __global__ void __launch_bounds__(kWarpThreads, kGradCtas) layer_norm_grad_warp_kernel(NormArgs a, int tpr)
+template <typename T, int VE, int NV, int ROWS>
+__global__ void __launch_bounds__(kWarpThreads, NV * VE == 8 ? kGradCtas : kGradCtas16) layer_norm_grad_warp_kernel(NormArgs a, int tpr)
 {
     constexpr int E = NV * VE;
-    extern __shared__ float cols[];     // [groups of the CTA][2][tpr * E] column sums
+    extern __shared__ __align__(16) uint8_t dyn[];   // the slots, then [groups of the CTA][2][tpr * E] column sums
+    float* cols = reinterpret_cast<float*>(dyn);
     pdl_wait();
     pdl_launch_dependents();
     const int t = threadIdx.x & (tpr - 1);
     const long long groups = (long long)gridDim.x * (kWarpThreads / tpr);
     const long long first = (long long)blockIdx.x * (kWarpThreads / tpr) + threadIdx.x / tpr;
     const float inv = 1.f / (float)a.C;
+    const T *x = static_cast<const T*>(a.x), *g = static_cast<const T*>(a.g);
+    constexpr int rowBytes = NV * kWarpThreads * kSlotBytes<T, VE>;
+    const uint32_t slots = smem_u32(dyn) + threadIdx.x * kSlotBytes<T, VE>;
+    const long long turns = (a.rows + groups * ROWS - 1) / (groups * ROWS);
+    float meanNext[ROWS], rstdNext[ROWS];
+    auto fetch = [&](long long turn, uint32_t stage) {
+        const uint32_t at = slots + stage * 2 * ROWS * rowBytes;
+#pragma unroll
+        for (int r = 0; r < ROWS; ++r) {
+            const long long row = (turn * ROWS + r) * groups + first;
+            copy_row<T, VE, NV>(at + 2 * r * rowBytes, x + row * a.C, row < a.rows, t, tpr, a.C);
+            copy_row<T, VE, NV>(at + (2 * r + 1) * rowBytes, g + row * a.C, row < a.rows, t, tpr, a.C);
+        }
+        copies_commit();
+    };
+    auto stats = [&](long long turn) {      // of the next turn: their latency passes behind this one's work
+#pragma unroll
+        for (int r = 0; r < ROWS; ++r) {
+            const long long row = (turn * ROWS + r) * groups + first;
+            meanNext[r] = row < a.rows ? a.mean[row] : 0.f, rstdNext[r] = row < a.rows ? a.rstd[row] : 0.f;
+        }
+    };
+#pragma unroll
+    for (int i = 0; i < kAhead - 1; ++i)
+        fetch(i, i);
+    stats(0);
     F2 w[E / 2], dw[E / 2] = {}, db[E / 2] = {};
     load_params<VE, NV>(w, a.weight, 1.f, a.wdtype, t, tpr, a.C);
-    const long long turns = (a.rows + groups * ROWS - 1) / (groups * ROWS);
-    for (long long turn = 0; turn < turns; ++turn) {
+    uint32_t stage = 0;
+    for (long long turn = 0; turn < turns; ++turn, stage = stage + 1 == kAhead ? 0 : stage + 1) {
         const long long row0 = turn * ROWS * groups + first;
-        Pack<T, VE> xv[ROWS][NV], gv[ROWS][NV];
-        F2 xh[ROWS][E / 2], gw[ROWS][E / 2];
+        fetch(turn + kAhead - 1, stage == 0 ? kAhead - 1 : stage - 1);
         float mean[ROWS], rstd[ROWS], s0[ROWS], s1[ROWS];
+#pragma unroll
+        for (int r = 0; r < ROWS; ++r)
+            mean[r] = meanNext[r], rstd[r] = rstdNext[r];
+        stats(turn + 1);
+        copies_wait();
+        const uint32_t at = slots + stage * 2 * ROWS * rowBytes;
+        F2 xh[ROWS][E / 2], gw[ROWS][E / 2];
 #pragma unroll
         for (int r = 0; r < ROWS; ++r) {
             const long long row = row0 + r * groups;
-            const bool live = row < a.rows;
-            load_row<T, VE, NV>(xv[r], static_cast<const T*>(a.x) + row * a.C, live, t, tpr, a.C);
-            load_row<T, VE, NV>(gv[r], static_cast<const T*>(a.g) + row * a.C, live, t, tpr, a.C);
-            mean[r] = live ? a.mean[row] : 0.f, rstd[r] = live ? a.rstd[row] : 0.f;
+            Pack<T, VE> xv[NV], gv[NV];
+            take_row<T, VE, NV>(xv, at + 2 * r * rowBytes, x + row * a.C, row < a.rows, t, tpr, a.C);
+            take_row<T, VE, NV>(gv, at + (2 * r + 1) * rowBytes, g + row * a.C, row < a.rows, t, tpr, a.C);
+            grad_sums<T, VE, NV>(xv, gv, mean[r], rstd[r], w, dw, db, xh[r], gw[r], s0[r], s1[r]);
         }
-#pragma unroll
-        for (int r = 0; r < ROWS; ++r)
-            grad_sums<T, VE, NV>(xv[r], gv[r], mean[r], rstd[r], w, dw, db, xh[r], gw[r], s0[r], s1[r]);
         for (int m = tpr >> 1; m > 0; m >>= 1)
 #pragma unroll
             for (int r = 0; r < ROWS; ++r) {
@@ -470,6 +579,9 @@ template <typename T, int VE, int NV, int ROWS> __global__ void __launch_bounds_
                 store_dx<T, VE, NV>(static_cast<T*>(a.y) + row * a.C, xh[r], gw[r], rstd[r], s0[r] * inv, s1[r] * inv, t, tpr, a.C);
         }
     }
+    // no copy is in flight into the slots that the sums go over: the last ones issued had no row
+    asm volatile("cp.async.wait_all;" ::: "memory");
+    __syncthreads();
     if (a.partials == nullptr)
         return;
     float* pw = a.partials + (long long)blockIdx.x * 2 * a.C;
@@ -492,43 +604,82 @@ template <typename T, int VE, int NV, int ROWS> __global__ void __launch_bounds_
     }
 }
 
-// AHEAD: the next row's loads are issued before this row's barrier (where the registers allow it).
-template <typename T, int VE, int NV, int MAXT, bool AHEAD> __global__ void __launch_bounds__(MAXT) layer_norm_grad_cta_kernel(NormArgs a)
+// Rows that share a barrier: two, or what shared memory holds.
+template <typename T, int MAXT> constexpr int kCtaRows = sizeof(T) == 4 && MAXT == 1024 ? 1 : 2;
+
+// The whole CTA shares a row; two rows at a time share a barrier.  Their products are computed twice, before and after
+// it, from the copies in shared memory: two rows of them would not fit the registers beside w, dw and db.
+template <typename T, int VE, int NV, int MAXT> __global__ void __launch_bounds__(MAXT) layer_norm_grad_cta_kernel(NormArgs a)
 {
-    constexpr int E = NV * VE;
-    __shared__ float red[2][64];
+    constexpr int E = NV * VE, ROWS = kCtaRows<T, MAXT>;
+    extern __shared__ __align__(16) uint8_t dyn[];
+    __shared__ float red[2][64 * ROWS];
     pdl_wait();
     pdl_launch_dependents();
     const int t = threadIdx.x, tpr = blockDim.x;
     const float inv = 1.f / (float)a.C;
+    const T *x = static_cast<const T*>(a.x), *g = static_cast<const T*>(a.g);
+    const uint32_t rowBytes = NV * tpr * kSlotBytes<T, VE>, slots = smem_u32(dyn) + t * kSlotBytes<T, VE>;
+    float meanNext[ROWS], rstdNext[ROWS];
+    auto fetch = [&](long long row0, uint32_t stage) {
+        const uint32_t at = slots + stage * 2 * ROWS * rowBytes;
+#pragma unroll
+        for (int r = 0; r < ROWS; ++r) {
+            const long long row = row0 + (long long)r * gridDim.x;
+            copy_row<T, VE, NV>(at + 2 * r * rowBytes, x + row * a.C, row < a.rows, t, tpr, a.C);
+            copy_row<T, VE, NV>(at + (2 * r + 1) * rowBytes, g + row * a.C, row < a.rows, t, tpr, a.C);
+        }
+        copies_commit();
+    };
+    auto stats = [&](long long row0) {
+#pragma unroll
+        for (int r = 0; r < ROWS; ++r) {
+            const long long row = row0 + (long long)r * gridDim.x;
+            meanNext[r] = row < a.rows ? a.mean[row] : 0.f, rstdNext[r] = row < a.rows ? a.rstd[row] : 0.f;
+        }
+    };
+    const long long step = (long long)ROWS * gridDim.x;
+#pragma unroll
+    for (int i = 0; i < kAheadCta - 1; ++i)
+        fetch(blockIdx.x + i * step, i);
+    stats(blockIdx.x);
     F2 w[E / 2], dw[E / 2] = {}, db[E / 2] = {};
     load_params<VE, NV>(w, a.weight, 1.f, a.wdtype, t, tpr, a.C);
-    const T *x = static_cast<const T*>(a.x), *g = static_cast<const T*>(a.g);
-    long long row = blockIdx.x;
-    Pack<T, VE> xv[NV], gv[NV], xn[NV], gn[NV];
-    if (AHEAD) {
-        load_row<T, VE, NV>(xv, x + row * a.C, row < a.rows, t, tpr, a.C);
-        load_row<T, VE, NV>(gv, g + row * a.C, row < a.rows, t, tpr, a.C);
-    }
-    for (int flip = 0; row < a.rows; row += gridDim.x, flip ^= 1) {
-        const float mean = a.mean[row], rstd = a.rstd[row];
-        if (AHEAD) {
-            const long long ahead = row + gridDim.x;
-            load_row<T, VE, NV>(xn, x + ahead * a.C, ahead < a.rows, t, tpr, a.C);
-            load_row<T, VE, NV>(gn, g + ahead * a.C, ahead < a.rows, t, tpr, a.C);
-        } else {
-            load_row<T, VE, NV>(xv, x + row * a.C, true, t, tpr, a.C);
-            load_row<T, VE, NV>(gv, g + row * a.C, true, t, tpr, a.C);
-        }
-        F2 xh[E / 2], gw[E / 2];
-        float s[2];
-        grad_sums<T, VE, NV>(xv, gv, mean, rstd, w, dw, db, xh, gw, s[0], s[1]);
-        cta_sum(s, red[flip]);
-        store_dx<T, VE, NV>(static_cast<T*>(a.y) + row * a.C, xh, gw, rstd, s[0] * inv, s[1] * inv, t, tpr, a.C);
-        if (AHEAD)
+    uint32_t stage = 0;
+    int flip = 0;
+    for (long long row0 = blockIdx.x; row0 < a.rows; row0 += step, flip ^= 1, stage = stage + 1 == kAheadCta ? 0 : stage + 1) {
+        fetch(row0 + (kAheadCta - 1) * step, stage == 0 ? kAheadCta - 1 : stage - 1);
+        float mean[ROWS], rstd[ROWS], s[2 * ROWS];
 #pragma unroll
-            for (int k = 0; k < NV; ++k)
-                xv[k] = xn[k], gv[k] = gn[k];
+        for (int r = 0; r < ROWS; ++r)
+            mean[r] = meanNext[r], rstd[r] = rstdNext[r];
+        stats(row0 + step);
+        asm volatile("cp.async.wait_group %0;" ::"n"(kAheadCta - 1) : "memory");
+        const uint32_t at = slots + stage * 2 * ROWS * rowBytes;
+        Pack<T, VE> xv[NV], gv[NV];
+#pragma unroll
+        for (int r = 0; r < ROWS; ++r) {
+            const long long row = row0 + (long long)r * gridDim.x;
+            take_row<T, VE, NV>(xv, at + 2 * r * rowBytes, x + row * a.C, row < a.rows, t, tpr, a.C);
+            take_row<T, VE, NV>(gv, at + (2 * r + 1) * rowBytes, g + row * a.C, row < a.rows, t, tpr, a.C);
+            F2 xh[E / 2], gw[E / 2];
+            grad_sums<T, VE, NV>(xv, gv, mean[r], rstd[r], w, dw, db, xh, gw, s[2 * r], s[2 * r + 1]);
+        }
+        cta_sum(s, red[flip]);
+#pragma unroll
+        for (int r = 0; r < ROWS; ++r) {
+            const long long row = row0 + (long long)r * gridDim.x;
+            if (row >= a.rows)
+                continue;
+            take_row<T, VE, NV>(xv, at + 2 * r * rowBytes, x + row * a.C, true, t, tpr, a.C);
+            take_row<T, VE, NV>(gv, at + (2 * r + 1) * rowBytes, g + row * a.C, true, t, tpr, a.C);
+            F2 xh[E / 2], gw[E / 2];
+            const F2 m = f2(-mean[r], -mean[r]), rs = f2(rstd[r], rstd[r]);
+#pragma unroll
+            for (int j = 0; j < E / 2; ++j)
+                xh[j] = mul2(add2(pair_of<T, VE, NV>(xv, j), m), rs), gw[j] = mul2(pair_of<T, VE, NV>(gv, j), w[j]);
+            store_dx<T, VE, NV>(static_cast<T*>(a.y) + row * a.C, xh, gw, rstd[r], s[2 * r] * inv, s[2 * r + 1] * inv, t, tpr, a.C);
+        }
     }
     if (a.partials == nullptr)
         return;
@@ -610,8 +761,8 @@ struct NormShape {
 
 // Up to 512 channels a row stays inside a warp, 16 channels a thread where that leaves at least 8 threads a row (fewer
 // exchanges per channel); in the backward pass the column sums leave registers for 8 up to 256 channels.  Then whole
-// CTAs: 8 a thread up to 2,048 channels, 16 beyond (half the threads, so that two or more rows share an SM), in the
-// backward pass 8 until the CTA is full.
+// CTAs: 8 a thread up to 2,048 channels, 16 beyond (half the threads: fewer exchanges, and in the forward pass two or
+// more rows share an SM); fp32 rows keep 8 in the backward pass.
 NormShape pick(int C, int itemsize, uintptr_t bits, bool grad)
 {
     NormShape s = {itemsize, 0, 0, false};
@@ -625,9 +776,9 @@ NormShape pick(int C, int itemsize, uintptr_t bits, bool grad)
         s.tpr = 4;
         while (s.tpr * s.elems < C)
             s.tpr *= 2;
-    } else if (C <= 16384) {
+    } else if (C <= (grad ? 8192 : 16384)) {   // backward: what shared memory holds
         s.cta = true;
-        s.elems = C <= (grad ? 8192 : 2048) ? 8 : 16;
+        s.elems = C <= 2048 || (grad && itemsize == 4) ? 8 : 16;
         s.tpr = 64;
         while (s.tpr * s.elems < C)
             s.tpr *= 2;
@@ -635,32 +786,95 @@ NormShape pick(int C, int itemsize, uintptr_t bits, bool grad)
     return s;
 }
 
+// Raises a kernel's shared-memory limit once per device (a race only repeats the call).
+template <typename K> cudaError_t allow_smem(K kernel, int bytes, int (&done)[64])
+{
+    if (bytes <= 40 * 1024)     // with the static arrays, inside the 48 KB that need no asking
+        return cudaSuccess;
+    int device = 0;
+    if (cudaError_t e = cudaGetDevice(&device))
+        return e;
+    if (device < 64 && done[device] >= bytes)
+        return cudaSuccess;
+    if (cudaError_t e = cudaFuncSetAttribute(kernel, cudaFuncAttributeMaxDynamicSharedMemorySize, bytes))
+        return e;
+    if (device < 64)
+        done[device] = bytes;
+    return cudaSuccess;
+}
+
+template <typename T, int VE, int NV, int MAXT> cudaError_t launch_fwd_cta(const NormArgs& a, const NormShape& s, cudaStream_t stream)
+{
+    auto kernel = layer_norm_cta_kernel<T, VE, NV, MAXT>;
+    static int done[64] = {};
+    const int smem = slots_bytes<T, VE, NV>(s.tpr, 1);
+    if (cudaError_t e = allow_smem(kernel, smem, done))
+        return e;
+    const long long grid = std::min<long long>(a.rows, (long long)sm_count() * (1024 / s.tpr));
+    return launch_pdl(kernel, dim3((unsigned)grid), dim3(s.tpr), smem, stream, a);
+}
+
 template <typename T, int VE, int NV> cudaError_t launch_fwd(const NormArgs& a, const NormShape& s, cudaStream_t stream)
 {
     constexpr int E = VE * NV;
     if (s.cta) {
-        const long long grid = std::min<long long>(a.rows, (long long)sm_count() * (2048 / s.tpr));
-        return launch_pdl(layer_norm_cta_kernel<T, VE, NV, E == 8 ? 256 : 1024>, dim3((unsigned)grid), dim3(s.tpr), 0, stream, a);
+        if (E == 8 || s.tpr <= 512)
+            return launch_fwd_cta<T, VE, NV, E == 8 ? 256 : 512>(a, s, stream);
+        return launch_fwd_cta<T, VE, NV, 1024>(a, s, stream);
     }
-    constexpr int ROWS = E == 8 ? 4 : 2;
-    // one row a group while that leaves SMs empty, ROWS in flight per group otherwise
+    // one row a group while that leaves SMs empty, two in flight per group and turn otherwise
     const long long ctas = (a.rows * s.tpr + kWarpThreads - 1) / kWarpThreads;
-    if (ctas <= (long long)sm_count() * kFwdCtas)
-        return launch_pdl(layer_norm_warp_kernel<T, VE, NV, 1>, dim3((unsigned)ctas), dim3(kWarpThreads), 0, stream, a, s.tpr);
     const long long grid = std::min<long long>(ctas, (long long)sm_count() * kFwdCtas);
-    return launch_pdl(layer_norm_warp_kernel<T, VE, NV, ROWS>, dim3((unsigned)grid), dim3(kWarpThreads), 0, stream, a, s.tpr);
+    if (ctas <= (long long)sm_count() * kFwdCtas) {
+        auto kernel = layer_norm_warp_kernel<T, VE, NV, 1>;
+        static int done[64] = {};
+        constexpr int smem = slots_bytes<T, VE, NV>(kWarpThreads, 1);
+        if (cudaError_t e = allow_smem(kernel, smem, done))
+            return e;
+        return launch_pdl(kernel, dim3((unsigned)grid), dim3(kWarpThreads), smem, stream, a, s.tpr);
+    }
+    constexpr int ROWS = sizeof(T) == 4 && E == 16 ? 1 : 2;     // 48 KB of slots a CTA
+    auto kernel = layer_norm_warp_kernel<T, VE, NV, ROWS>;
+    static int done[64] = {};
+    constexpr int smem = slots_bytes<T, VE, NV>(kWarpThreads, ROWS);
+    if (cudaError_t e = allow_smem(kernel, smem, done))
+        return e;
+    return launch_pdl(kernel, dim3((unsigned)grid), dim3(kWarpThreads), smem, stream, a, s.tpr);
+}
+
+template <typename T, int VE, int NV, int MAXT>
+cudaError_t launch_bwd_cta(const NormArgs& a, const NormShape& s, int grid, cudaStream_t stream)
+{
+    auto kernel = layer_norm_grad_cta_kernel<T, VE, NV, MAXT>;
+    static int done[64] = {};
+    const int smem = kAheadCta * 2 * kCtaRows<T, MAXT> * NV * s.tpr * kSlotBytes<T, VE>;
+    if (cudaError_t e = allow_smem(kernel, smem, done))
+        return e;
+    return launch_pdl(kernel, dim3(grid), dim3(s.tpr), smem, stream, a);
 }
 
 template <typename T, int VE, int NV> cudaError_t launch_bwd(const NormArgs& a, const NormShape& s, int grid, cudaStream_t stream)
 {
     constexpr int E = VE * NV;
     if (s.cta) {
-        if (E == 8 && s.tpr <= 256)
-            return launch_pdl(layer_norm_grad_cta_kernel<T, VE, NV, 256, true>, dim3(grid), dim3(s.tpr), 0, stream, a);
-        return launch_pdl(layer_norm_grad_cta_kernel<T, VE, NV, 1024, E == 8 && sizeof(T) == 2>, dim3(grid), dim3(s.tpr), 0, stream, a);
+        if constexpr (E == 8) {
+            if (s.tpr <= 256)
+                return launch_bwd_cta<T, VE, NV, 256>(a, s, grid, stream);
+            if constexpr (sizeof(T) == 4)
+                return s.tpr <= 512 ? launch_bwd_cta<T, VE, NV, 512>(a, s, grid, stream)
+                                    : launch_bwd_cta<T, VE, NV, 1024>(a, s, grid, stream);
+        } else if constexpr (sizeof(T) == 2) {
+            return launch_bwd_cta<T, VE, NV, 512>(a, s, grid, stream);
+        }
+        return cudaErrorInvalidValue;    // no shape that pick() makes
     }
-    const size_t smem = a.partials == nullptr ? 0 : sizeof(float) * 2 * kWarpThreads * E;
-    return launch_pdl(layer_norm_grad_warp_kernel<T, VE, NV, E == 8 ? 2 : 1>, dim3(grid), dim3(kWarpThreads), smem, stream, a, s.tpr);
+    constexpr int ROWS = E == 8 && sizeof(T) == 2 ? 2 : 1;
+    auto kernel = layer_norm_grad_warp_kernel<T, VE, NV, ROWS>;
+    static int done[64] = {};
+    constexpr int smem = std::max(slots_bytes<T, VE, NV>(kWarpThreads, 2 * ROWS), (int)sizeof(float) * 2 * kWarpThreads * E);
+    if (cudaError_t e = allow_smem(kernel, smem, done))
+        return e;
+    return launch_pdl(kernel, dim3(grid), dim3(kWarpThreads), smem, stream, a, s.tpr);
 }
 
 template <typename T> cudaError_t run_fwd(const NormArgs& a, cudaStream_t stream)
@@ -698,12 +912,12 @@ template <typename T> cudaError_t run_bwd(const NormArgs& a, int grid, cudaStrea
 // CTAs of the backward kernel = partial rows of the column sums.  Depends on the sizes only.
 int layer_norm_grad_parts(long long rows, int C)
 {
-    const NormShape s = pick(C, 4, 0, true);
+    const NormShape s = pick(C, 4, 0, true);    // the fewest CTAs of wide rows that either element size asks for
     if (s.tpr == 0)
         return (int)std::min<long long>(rows, sm_count());
     if (s.cta)
         return (int)std::min<long long>(rows, (long long)sm_count() * std::max(1, 1024 / s.tpr));
-    return (int)std::min<long long>((rows * s.tpr + kWarpThreads - 1) / kWarpThreads, (long long)sm_count() * kGradCtas);
+    return (int)std::min<long long>((rows * s.tpr + kWarpThreads - 1) / kWarpThreads, (long long)sm_count() * (s.elems == 8 ? kGradCtas : kGradCtas16));
 }
 
 cudaError_t launch_layer_norm(const NormArgs& a, int dtype, cudaStream_t stream)
