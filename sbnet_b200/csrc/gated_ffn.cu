@@ -37,8 +37,7 @@
 
 #include <algorithm>
 
-#include "common.cuh"
-#include "kernels.h"
+#include "gated_ffn.cuh"
 #include "tensor_ptx.cuh"
 
 namespace sbnet {
@@ -55,7 +54,6 @@ constexpr int kGroupM = 8;
 __device__ unsigned int g_ffn_timeouts = 0;
 
 enum Epilogue { kStore, kGate, kGrad };
-enum Act { kSilu = 0, kGelu = 1, kRelu = 2 };
 
 struct Maps {
     CUtensorMap a[2], b[2];
@@ -83,47 +81,6 @@ struct Plan {
 template <int BN> constexpr int kStages = BN == 256 ? 6 : 8;
 template <int BN> constexpr int kStageBytes = (kCtaM + BN / 2) * kStepK * 2;    // of one CTA
 template <int BN> constexpr int kGemmSmem = 1024 + kStages<BN> * kStageBytes<BN> + kStagingBytes + 256;
-
-template <typename T> __device__ __forceinline__ uint32_t pack2(float lo, float hi);
-template <> __device__ __forceinline__ uint32_t pack2<__half>(float lo, float hi)
-{
-    const __half2 v = __floats2half2_rn(lo, hi);
-    return *reinterpret_cast<const uint32_t*>(&v);
-}
-template <> __device__ __forceinline__ uint32_t pack2<__nv_bfloat16>(float lo, float hi)
-{
-    const __nv_bfloat162 v = __floats2bfloat162_rn(lo, hi);
-    return *reinterpret_cast<const uint32_t*>(&v);
-}
-template <typename T> __device__ __forceinline__ float2 unpack2(uint32_t v);
-template <> __device__ __forceinline__ float2 unpack2<__half>(uint32_t v)
-{
-    return __half22float2(*reinterpret_cast<const __half2*>(&v));
-}
-template <> __device__ __forceinline__ float2 unpack2<__nv_bfloat16>(uint32_t v)
-{
-    return __bfloat1622float2(*reinterpret_cast<const __nv_bfloat162*>(&v));
-}
-
-// act(g), and its derivative where it is asked for.
-template <int ACT, bool SLOPE> __device__ __forceinline__ float activate(float g, float& slope)
-{
-    if constexpr (ACT == kSilu) {
-        const float s = __fdividef(1.f, 1.f + __expf(-g));
-        if (SLOPE)
-            slope = s * (1.f + g * (1.f - s));
-        return g * s;
-    } else if constexpr (ACT == kGelu) {
-        const float cdf = 0.5f * (1.f + erff(g * 0.70710678118654752f));
-        if (SLOPE)
-            slope = cdf + g * 0.3989422804014327f * __expf(-0.5f * g * g);
-        return g * cdf;
-    } else {
-        if (SLOPE)
-            slope = g > 0.f ? 1.f : 0.f;
-        return g != g ? g : fmaxf(g, 0.f);
-    }
-}
 
 // ---- 32 x 32 tiles of 16-bit elements between registers (one row per lane) and memory -----------------------
 // Staged through 2 KB of shared memory so that global accesses are 64 contiguous bytes per row.  16-byte pieces
@@ -264,9 +221,7 @@ __global__ void __launch_bounds__(kGemmThreads, 1) gemm_kernel(const __grid_cons
     pdl_wait();
     pdl_launch_dependents();
 
-    long long rowEnd = p.M;
-    if (p.num_blocks_dev != nullptr)
-        rowEnd = min(rowEnd, (long long)max(*p.num_blocks_dev, 0) * p.rowsPerBlock);
+    const long long rowEnd = live_rows(p.M, p.num_blocks_dev, p.rowsPerBlock);
     const int mTiles = (int)((rowEnd + kTileM - 1) / kTileM);
     const int tiles = mTiles * p.nTiles * p.batch * p.splits;
     const int kAll = p.kIters * p.segs;
@@ -525,9 +480,7 @@ template <typename T, int EPI> __global__ void __launch_bounds__(256) finish_ker
 {
     pdl_wait();
     pdl_launch_dependents();
-    long long rowEnd = p.M;
-    if (p.num_blocks_dev != nullptr)
-        rowEnd = min(rowEnd, (long long)max(*p.num_blocks_dev, 0) * p.rowsPerBlock);
+    const long long rowEnd = live_rows(p.M, p.num_blocks_dev, p.rowsPerBlock);
     const long long pitch = (long long)p.nTiles * bn, plane = (long long)p.mTiles * kTileM * pitch;
     const int col = blockIdx.x * 128 + threadIdx.x * 4, z = blockIdx.z, n = p.N - col;
     if (n <= 0)
@@ -539,12 +492,7 @@ template <typename T, int EPI> __global__ void __launch_bounds__(256) finish_ker
             const float* q = p.partials + row * pitch + (col >> 7) * 256 + (col & 127);
             const float4 g = sum_pieces(q, plane, p.splits), u = sum_pieces(q + 128, plane, p.splits);
             float4 h;
-            float unused;
-            auto gated = [&](float a, float b) {
-                return b * (p.act == kSilu   ? activate<kSilu, false>(a, unused)
-                            : p.act == kGelu ? activate<kGelu, false>(a, unused)
-                                             : activate<kRelu, false>(a, unused));
-            };
+            auto gated = [&](float a, float b) { return activate_any(p.act, a) * b; };
             h.x = gated(g.x, u.x), h.y = gated(g.y, u.y), h.z = gated(g.z, u.z), h.w = gated(g.w, u.w);
             store4<T>(out + row * p.ldo + col, h, n, wide);
             if (p.gate != nullptr) {
@@ -776,6 +724,10 @@ template <typename T> cudaError_t forward(const FfnArgs& f, Layout& l, bool run,
     const Matrix h = {l.bump.take((size_t)R * Fp * 2), R, F, Fp};
     float* parts = static_cast<float*>(l.bump.take(std::max(gate_partials(R, F, C), product_partials(1, 1, R, C, F))));
     if (!run)
+        return cudaSuccess;
+    bool taken = false;
+    SBNET_TRY(launch_ffn_few<T>(f, const_cast<void*>(h.ptr), stream, &taken));
+    if (taken)
         return cudaSuccess;
     note_site("gated_ffn repack");
     Repacks copies;
