@@ -346,6 +346,7 @@ __global__ void __launch_bounds__(kGemmThreads, 1) gemm_kernel(const __grid_cons
                     tmem_wait_load();
                     if (c + 32 == BN / 2)
                         release();
+                    if (row0 + lane < rowEnd)
 #pragma unroll
                     for (int i = 0; i < 8; ++i)
                         *reinterpret_cast<uint4*>(part + c + 4 * i) = make_uint4(v[4 * i], v[4 * i + 1], v[4 * i + 2], v[4 * i + 3]);
@@ -570,15 +571,23 @@ int ceil_div(long long a, long long b) { return (int)((a + b - 1) / b); }
 // Column tile of a plain product: 256 wide unless the matrix is narrow.
 int tile_n(int N) { return N <= 128 ? 128 : 256; }
 
-// Pieces of the reduction.  One piece fills the machine when there are enough tiles.  With fewer, and a reduction of
-// more than 16 stages (5 us; the second kernel that adds the pieces costs about as much), pieces of at least 8 stages
-// make up for it.
-int split_count(long long tiles, int kIters)
+// Pieces of the reduction: what a small model of the two kernels' times says is quickest.  A round of tiles over the
+// pairs of SMs costs 0.35 us a stage (tensor cores under the power cap; a stage's B from HBM takes as long) and 1.5 us
+// to fill and drain; adding up pieces costs a launch, 4 us, and the partial sums' way to memory and back at 2.5 TB/s.
+int split_count(long long rows, long long N, long long tiles, int kIters)
 {
     const int pairs = sm_count() / 2;
-    if (tiles * 2 > pairs || kIters <= 16)
-        return 1;
-    return (int)std::max<long long>(1, std::min<long long>(pairs / tiles, kIters / 8));
+    int best = 1;
+    double least = 1e30;
+    for (int s = 1; s <= 64 && (s == 1 || kIters / s >= 4); ++s) {
+        const double rounds = (double)((tiles * s + pairs - 1) / pairs);
+        double t = rounds * ((double)((kIters + s - 1) / s) * 0.35 + 1.5);
+        if (s > 1)
+            t += 4 + 8e-6 * (double)s * (double)rows * (double)N / 2.5;
+        if (t < least * 0.97)
+            least = t, best = s;
+    }
+    return best;
 }
 
 template <typename T, bool A_MN, bool B_MN, int EPI, int BN>
@@ -639,7 +648,7 @@ cudaError_t product(const Matrix (&a)[2], const Matrix (&b)[2], int batch, int s
     const int bn = tile_n(N);
     p.mTiles = ceil_div(M, kTileM), p.nTiles = ceil_div(N, bn), p.batch = batch, p.segs = segs;
     p.kIters = ceil_div(K, kStepK);
-    p.splits = split_count((long long)p.mTiles * p.nTiles * batch, p.kIters * segs);
+    p.splits = split_count(M, (long long)N * batch, (long long)p.mTiles * p.nTiles * batch, p.kIters * segs);
     p.N = N, p.M = M, p.out[0] = out0, p.out[1] = out1, p.ldo = N, p.partials = partials;
     if (rowsOfX)
         p.num_blocks_dev = f.num_blocks_dev, p.rowsPerBlock = f.rowsPerBlock;
@@ -650,13 +659,13 @@ size_t product_partials(int batch, int segs, long long M, int N, long long K)
 {
     const int bn = tile_n(N);
     const long long mT = ceil_div(M, kTileM), nT = ceil_div(N, bn);
-    const int s = split_count(mT * nT * batch, ceil_div(K, kStepK) * segs);
+    const int s = split_count(M, (long long)N * batch, mT * nT * batch, ceil_div(K, kStepK) * segs);
     return s == 1 ? 0 : sizeof(float) * s * batch * mT * kTileM * nT * bn;
 }
 size_t gate_partials(long long R, int F, int C)
 {
     const long long mT = ceil_div(R, kTileM), nT = ceil_div(F, 128);
-    const int s = split_count(mT * nT, ceil_div(C, kStepK));
+    const int s = split_count(R, 2ll * F, mT * nT, ceil_div(C, kStepK));
     return s == 1 ? 0 : sizeof(float) * s * mT * kTileM * nT * 256;
 }
 
@@ -736,7 +745,7 @@ template <typename T> cudaError_t forward(const FfnArgs& f, Layout& l, bool run,
     note_site("gated_ffn projections");
     Plan p = {};
     p.mTiles = ceil_div(R, kTileM), p.nTiles = ceil_div(F, 128), p.batch = 1, p.segs = 1, p.kIters = ceil_div(C, kStepK);
-    p.splits = split_count((long long)p.mTiles * p.nTiles, p.kIters);
+    p.splits = split_count(R, 2ll * F, (long long)p.mTiles * p.nTiles, p.kIters);
     p.N = F, p.M = R, p.num_blocks_dev = f.num_blocks_dev, p.rowsPerBlock = f.rowsPerBlock, p.act = f.act;
     p.out[0] = const_cast<void*>(h.ptr), p.ldo = Fp, p.gate = f.gate, p.up = f.up, p.ldh = Fp, p.partials = parts;
     SBNET_TRY((launch_gemm<T, false, false, kGate, 256>({x, x}, {wg, wu}, p, stream)));

@@ -62,7 +62,7 @@ __device__ __forceinline__ long long live_rows(long long rows, const int32_t* bl
     return blocks == nullptr ? rows : min(rows, (long long)max(*blocks, 0) * rowsPerBlock);
 }
 
-// Up to 64 rows (gated_ffn_few.cu): h [rows, F] is scratch.  *taken tells whether the sizes suit the kernels.
+// Up to 32 rows (gated_ffn_few.cu): h [rows, F] is scratch.  *taken tells whether the sizes suit the kernels.
 template <typename T> cudaError_t launch_ffn_few(const FfnArgs& f, void* h, cudaStream_t stream, bool* taken);
 
 } // namespace sbnet

@@ -1,4 +1,4 @@
-// The gated feed-forward block for up to 64 rows (single positions of a batch): every weight is read once for a handful
+// The gated feed-forward block for up to 32 rows (single positions of a batch): every weight is read once for a handful
 // of rows, so the two kernels are weight streams and bound by HBM.
 //
 //   gate kernel: H = act(X Wg^T) * (X Wu^T)        output kernel: Y = H Wd^T
@@ -27,7 +27,7 @@ namespace {
 constexpr int kWarps = 8;
 constexpr int kThreads = kWarps * 32;
 constexpr int kBatch = 4;            // pieces of 64 that a warp loads ahead
-constexpr int kMaxRows = 64;
+constexpr int kMaxRows = 32;
 constexpr int kSmemLimit = 224 * 1024, kSmemHalf = 110 * 1024;     // of a CTA that has an SM alone, or shares it
 
 struct FewArgs {
@@ -113,18 +113,30 @@ template <typename T, int MT, bool GATE> __global__ void __launch_bounds__(kThre
         pdl_wait();
     pdl_launch_dependents();
 
-    // X of this CTA's pieces; zeros past the end of the reduction
-    for (int i = threadIdx.x; i < M * p.perCta * 8; i += kThreads) {
-        const int row = i / (p.perCta * 8), q = i - row * (p.perCta * 8), k = c0 * 64 + q * 8;
-        const uint32_t dst = xs + row * pitch + q * 16;
-        if (k < p.K)
-            asm volatile("cp.async.ca.shared.global [%0], [%1], 16;" ::"r"(dst), "l"(static_cast<const T*>(p.x) + (long long)row * p.K + k)
-                         : "memory");
-        else
-            sts128(dst, make_uint4(0, 0, 0, 0));
-    }
-    asm volatile("cp.async.wait_all;" ::: "memory");
-    __syncthreads();
+    // X of this CTA's pieces; zeros past the end of the reduction.  Every warp copies what it will read itself, its first
+    // batch as a group of its own, so that nobody waits for all of X.
+    auto stage_x = [&](int from, int to) {
+        for (int j = from; j < to; ++j) {
+            const int piece = warp + kWarps * j;
+            if (piece >= nPieces)
+                break;
+            const int k = (c0 + piece) * 64 + (lane & 7) * 8;
+            const T* src = static_cast<const T*>(p.x) + k;
+            const uint32_t dst = xs + piece * 128 + (lane & 7) * 16;
+#pragma unroll 4
+            for (int row = lane >> 3; row < M; row += 4) {
+                if (k < p.K)
+                    asm volatile("cp.async.ca.shared.global [%0], [%1], 16;" ::"r"(dst + row * pitch), "l"(src + (long long)row * p.K) : "memory");
+                else
+                    sts128(dst + row * pitch, make_uint4(0, 0, 0, 0));
+            }
+        }
+        asm volatile("cp.async.commit_group;" ::: "memory");
+    };
+    stage_x(0, kBatch);
+    stage_x(kBatch, batches * kBatch);
+    asm volatile("cp.async.wait_group 1;" ::: "memory");
+    __syncwarp();
 
     const int rowEnd = (int)live_rows(p.M, p.num_blocks_dev, p.rowsPerBlock);
     auto finish = [&](int group, int tok, int r, float s0, float s1) {      // r < 8: weight rows r and r + 8 of the group
@@ -149,6 +161,10 @@ template <typename T, int MT, bool GATE> __global__ void __launch_bounds__(kThre
         float acc[MT][2][4] = {};
         for (int b = 0; b < batches; ++b) {
             const bool last = b + 1 == batches;
+            if (gi == 0 && b == 1) {
+                asm volatile("cp.async.wait_all;" ::: "memory");
+                __syncwarp();
+            }
 #pragma unroll
             for (int c = 0; c < kBatch; ++c) {
                 const int piece = warp + kWarps * (b * kBatch + c);
@@ -332,21 +348,18 @@ template <typename T, int MT> cudaError_t both(const FfnArgs& f, void* h, cudaSt
 
 } // namespace
 
-// 16-byte loads need rows of a multiple of 8 elements on 16-byte boundaries.
+// Taken for up to 32 rows of at most 2^17 elements of X or H together; 16-byte loads need rows of a multiple of 8 elements
+// on 16-byte boundaries.  With more of X to keep in shared memory the clusters' pieces become so short that the sums per
+// group cost more than the tensor cores' padding (4096 x 12288 fp16: 1 row 56 against 94 us, 8 rows 67 against 75, 16 rows
+// 83 against 75; 2048 x 8192: 16 rows 32 against 36, 32 rows 36 either way; 1024 x 4096: 32 rows 20 against 23).
 template <typename T> cudaError_t launch_ffn_few(const FfnArgs& f, void* h, cudaStream_t stream, bool* taken)
 {
     *taken = false;
     const uintptr_t bits = reinterpret_cast<uintptr_t>(f.x) | reinterpret_cast<uintptr_t>(f.w_gate) |
                            reinterpret_cast<uintptr_t>(f.w_up) | reinterpret_cast<uintptr_t>(f.w_down);
-    if (f.rows > kMaxRows || f.C % 8 != 0 || f.F % 8 != 0 || (bits & 15) != 0)
+    if (f.rows > kMaxRows || f.rows * std::max(f.C, f.F) > (1 << 17) || f.C % 8 != 0 || f.F % 8 != 0 || (bits & 15) != 0)
         return cudaSuccess;
-    if (f.rows <= 16)
-        return both<T, 1>(f, h, stream, taken);
-    if (f.rows <= 32)
-        return both<T, 2>(f, h, stream, taken);
-    if (f.rows <= 48)
-        return both<T, 3>(f, h, stream, taken);
-    return both<T, 4>(f, h, stream, taken);
+    return f.rows <= 16 ? both<T, 1>(f, h, stream, taken) : both<T, 2>(f, h, stream, taken);
 }
 template cudaError_t launch_ffn_few<__half>(const FfnArgs&, void*, cudaStream_t, bool*);
 template cudaError_t launch_ffn_few<__nv_bfloat16>(const FfnArgs&, void*, cudaStream_t, bool*);
