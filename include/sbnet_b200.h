@@ -292,7 +292,8 @@ int sbnet_gated_ffn_dyn(const void* x, int dtype, int64_t maxBlocks, int rowsPer
                         int C, int F, const void* w_gate, const void* w_up, const void* w_down, int act, void* y,
                         void* workspace, size_t workspace_bytes, void* stream);
 /*
- * Backward pass from dy, x and the forward pass' gate and up.  dx [rows,C], dw_gate and dw_up [F,C], dw_down [C,F]
+ * Backward pass from dy, x and the forward pass' gate and up, which are multiplied again from x where both are NULL
+ * (4*C operations per hidden element instead of 4 bytes kept, written and read; quicker up to some 512 channels).  dx [rows,C], dw_gate and dw_up [F,C], dw_down [C,F]
  * are each skipped where NULL (dw_gate and dw_up go together); no output may overlap an input.  With rows == 0 the
  * weight gradients are set to zero.
  */

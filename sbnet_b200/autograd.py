@@ -100,12 +100,19 @@ def layer_norm(x, weight=None, bias=None, eps=1e-5):
     return _LayerNorm.apply(x, weight, bias, eps)
 
 
+# Up to this many channels the backward pass of the gated feed-forward block multiplies the two projections again
+# instead of keeping them (4*C operations per hidden element against writing, keeping and reading 4 bytes).
+RECOMPUTE_CHANNELS = 512
+
+
 class _GatedFfn(torch.autograd.Function):
     @staticmethod
     def forward(ctx, x, w_gate, w_up, w_down, activation):
-        if not any(ctx.needs_input_grad):
-            return ops.gated_ffn(x, w_gate, w_up, w_down, activation)
-        y, gate, up = ops.gated_ffn_train(x, w_gate, w_up, w_down, activation)
+        gate = up = None
+        if x.shape[-1] <= RECOMPUTE_CHANNELS or not any(ctx.needs_input_grad):
+            y = ops.gated_ffn(x, w_gate, w_up, w_down, activation)
+        else:
+            y, gate, up = ops.gated_ffn_train(x, w_gate, w_up, w_down, activation)
         ctx.save_for_backward(x, w_gate, w_up, w_down, gate, up)
         ctx.activation = activation
         return y

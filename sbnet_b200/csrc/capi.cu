@@ -589,8 +589,9 @@ SBNET_EXPORT int sbnet_gated_ffn_grad(const void* dy, const void* x, const void*
                     return cuda_status(e);
         return SBNET_OK;
     }
-    if (dy == nullptr || x == nullptr || gate == nullptr || up == nullptr || w_gate == nullptr || w_up == nullptr ||
-        w_down == nullptr)
+    if ((gate == nullptr) != (up == nullptr))
+        return reject(SBNET_ERR_INVALID_ARGUMENT, "%s: gate and up go together", op);
+    if (dy == nullptr || x == nullptr || w_gate == nullptr || w_up == nullptr || w_down == nullptr)
         return reject(SBNET_ERR_INVALID_ARGUMENT, "%s: null tensor pointer", op);
     const uintptr_t inputs = address(dy) | address(x) | address(w_gate) | address(w_up) | address(w_down);
     if ((inputs & 1) || ((address(gate) | address(up)) & 15))
@@ -601,7 +602,7 @@ SBNET_EXPORT int sbnet_gated_ffn_grad(const void* dy, const void* x, const void*
                                               out[] = {{dx, bytes}, {dw_gate, wbytes}, {dw_up, wbytes}, {dw_down, wbytes}};
     for (const auto& o : out)
         for (const auto& i : in)
-            if (o.p != nullptr && address(o.p) < address(i.p) + i.n && address(i.p) < address(o.p) + o.n)
+            if (o.p != nullptr && i.p != nullptr && address(o.p) < address(i.p) + i.n && address(i.p) < address(o.p) + o.n)
                 return reject(SBNET_ERR_INVALID_ARGUMENT, "%s: an output must not overlap an input", op);
     if (int rc = check_workspace(op, workspace, workspace_bytes,
                                  sbnet::gated_ffn_workspace(rows, C, F, true, (inputs & 15) == 0)))

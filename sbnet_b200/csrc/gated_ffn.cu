@@ -12,6 +12,9 @@
 //           U of the same 128 x 128 positions come out of one instruction stream side by side in TMEM and the
 //           epilogue writes H (and, in training, G and U) without either having been to memory
 //   kGrad   dH stays in TMEM; the epilogue reads G and U and writes dG, dU and H
+//   kRegrad the same without G and U from the forward pass: a tile multiplies dH (128 columns), then G and U again
+//           (256 columns), and the epilogue takes all three from TMEM.  With few channels that costs less than
+//           writing and reading G and U: 4 C operations per hidden element against 8 bytes of HBM traffic
 //   kStore  a plain product, rounded once
 //
 // G, U, H, dG and dU are held between kernels in the type of X (they are operands of the next product, and the
@@ -46,17 +49,18 @@ namespace {
 constexpr int kTileM = 256;                      // rows of a tile
 constexpr int kCtaM = 128;                       // ... in each CTA of the pair
 constexpr int kStepK = 64;                       // reduction steps of a stage (128 bytes)
-constexpr int kEpiWarps = 8;
-constexpr int kGemmThreads = (2 + kEpiWarps) * 32;
-constexpr int kStagingBytes = kEpiWarps * 4096;  // two 32 x 32 tiles of 16-bit elements per epilogue warp
+enum Epilogue { kStore, kGate, kGrad, kRegrad };
+// Epilogue warps: the element-wise epilogues are chains of special functions, shared and global accesses, which four
+// warps per scheduler hide better than two.
+template <int EPI> constexpr int kEpiWarps = EPI == kStore ? 8 : 16;
+template <int EPI> constexpr int kGemmThreads = (2 + kEpiWarps<EPI>) * 32;
+template <int EPI> constexpr int kStagingBytes = kEpiWarps<EPI> * 4096;  // two 32 x 32 tiles of 16-bit elements per warp
 constexpr int kGroupM = 8;
 
 __device__ unsigned int g_ffn_timeouts = 0;
 
-enum Epilogue { kStore, kGate, kGrad };
-
 struct Maps {
-    CUtensorMap a[2], b[2];
+    CUtensorMap a[2], b[2], c;     // c: kRegrad's Wd
 };
 
 struct Plan {
@@ -78,9 +82,9 @@ struct Plan {
     float* partials;               // splits > 1: [splits][batch][mTiles * 256][nTiles * BN]
 };
 
-template <int BN> constexpr int kStages = BN == 256 ? 6 : 8;
+template <int EPI, int BN> constexpr int kStages = EPI != kStore ? 5 : BN == 256 ? 6 : 8;
 template <int BN> constexpr int kStageBytes = (kCtaM + BN / 2) * kStepK * 2;    // of one CTA
-template <int BN> constexpr int kGemmSmem = 1024 + kStages<BN> * kStageBytes<BN> + kStagingBytes + 256;
+template <int EPI, int BN> constexpr int kGemmSmem = 1024 + kStages<EPI, BN> * kStageBytes<BN> + kStagingBytes<EPI> + 256;
 
 // ---- 32 x 32 tiles of 16-bit elements between registers (one row per lane) and memory -----------------------
 // Staged through 2 KB of shared memory so that global accesses are 64 contiguous bytes per row.  16-byte pieces
@@ -166,6 +170,22 @@ __device__ __forceinline__ void grad_chunk(const uint32_t (&dh)[32], uint32_t (&
     }
 }
 
+// The same from fp32 G and U; their first 16 words are replaced by dG and dU
+template <typename T, int ACT>
+__device__ __forceinline__ void regrad_chunk(const uint32_t (&dh)[32], uint32_t (&g)[32], uint32_t (&u)[32], uint32_t (&h)[16])
+{
+#pragma unroll
+    for (int i = 0; i < 16; ++i) {
+        const float d0 = __uint_as_float(dh[2 * i]), d1 = __uint_as_float(dh[2 * i + 1]);
+        const float u0 = __uint_as_float(u[2 * i]), u1 = __uint_as_float(u[2 * i + 1]);
+        float s0, s1;
+        const float a0 = activate<ACT, true>(__uint_as_float(g[2 * i]), s0), a1 = activate<ACT, true>(__uint_as_float(g[2 * i + 1]), s1);
+        h[i] = pack2<T>(a0 * u0, a1 * u1);
+        u[i] = pack2<T>(d0 * a0, d1 * a1);
+        g[i] = pack2<T>(d0 * u0 * s0, d1 * u1 * s1);
+    }
+}
+
 struct Tile {
     int m, n, z, s;
 };
@@ -184,13 +204,13 @@ __device__ __forceinline__ Tile tile_at(int t, const Plan& p, int mTiles)
 
 // A_MN / B_MN: the operand's reduction runs along its rows' pitch, not along its rows.
 template <typename T, bool A_MN, bool B_MN, int EPI, int BN>
-__global__ void __launch_bounds__(kGemmThreads, 1) gemm_kernel(const __grid_constant__ Maps maps, const __grid_constant__ Plan p)
+__global__ void __launch_bounds__(kGemmThreads<EPI>, 1) gemm_kernel(const __grid_constant__ Maps maps, const __grid_constant__ Plan p)
 {
-    constexpr int S = kStages<BN>;
+    constexpr int S = kStages<EPI, BN>, W = kEpiWarps<EPI>;
     extern __shared__ uint8_t smem_raw[];
     const uint32_t smem = (smem_u32(smem_raw) + 1023) & ~1023u;
     const uint32_t staging = smem + S * kStageBytes<BN>;
-    const uint32_t bars = staging + kStagingBytes;           // full[S], empty[S], accFull[2], accEmpty[2], drain
+    const uint32_t bars = staging + kStagingBytes<EPI>;           // full[S], empty[S], accFull[2], accEmpty[2], drain
     const uint32_t full = bars, empty = bars + 8 * S, accFull = bars + 16 * S, accEmpty = accFull + 16, drain = accEmpty + 16;
     __shared__ uint32_t tmemSlot;
     __shared__ int abortFlag;
@@ -201,7 +221,7 @@ __global__ void __launch_bounds__(kGemmThreads, 1) gemm_kernel(const __grid_cons
         for (int i = 0; i < S; ++i)
             mbar_init(full + 8 * i, 1), mbar_init(empty + 8 * i, 1);
         for (int i = 0; i < 2; ++i)
-            mbar_init(accFull + 8 * i, 1), mbar_init(accEmpty + 8 * i, 2 * kEpiWarps);
+            mbar_init(accFull + 8 * i, 1), mbar_init(accEmpty + 8 * i, 2 * W);
         mbar_init(drain, 1);
         mbar_init_fence();
         abortFlag = 0;
@@ -250,7 +270,15 @@ __global__ void __launch_bounds__(kGemmThreads, 1) gemm_kernel(const __grid_cons
                 const int kk = (k - seg * p.kIters) * kStepK;
                 const int which = p.segs > 1 ? seg : w.z;
                 const uint32_t a = smem + st * kStageBytes<BN>, b = a + kCtaM * kStepK * 2, bar = fullFirst + 8 * st;
-                if (lead) {
+                if (lead && EPI == kRegrad) {    // segment 0: dY and 64 columns of Wd; segment 1: X and 128 rows of Wg or Wu
+                    if (rank == 0)
+                        mbar_expect_tx(full + 8 * st, seg == 0 ? 2 * (kCtaM + 64) * kStepK * 2 : 2 * kStageBytes<BN>);
+                    tma_load_2d(a, &maps.a[seg], kk, row, bar);
+                    if (seg == 0)
+                        tma_load_2d(b, &maps.c, w.n * 128 + rank * 64, kk, bar);
+                    else
+                        tma_load_2d(b, &maps.b[rank], kk, w.n * 128, bar);
+                } else if (lead) {
                     if (rank == 0)
                         mbar_expect_tx(full + 8 * st, 2 * kStageBytes<BN>);
                     if (A_MN) {
@@ -286,8 +314,9 @@ __global__ void __launch_bounds__(kGemmThreads, 1) gemm_kernel(const __grid_cons
         for (int t = blockIdx.x >> 1; ok && t < tiles; t += gridDim.x >> 1, ++turn) {
             const Tile w = tile_at(t, p, mTiles);
             const int k0 = (int)((long long)kAll * w.s / p.splits), k1 = (int)((long long)kAll * (w.s + 1) / p.splits);
-            const uint32_t acc = turn & 1, d = tmem + acc * BN;
-            if (turn > 1 && !mbar_wait_warp(accEmpty + 8 * acc, ((turn >> 1) - 1) & 1, abort, &g_ffn_timeouts))
+            // kRegrad: G and U have columns 0 .. 255, dH 256 .. 383 or 384 .. 511 in turn, and one pair of barriers
+            const uint32_t acc = EPI == kRegrad ? 0 : turn & 1, d = EPI == kRegrad ? tmem + 256 + 128 * (turn & 1) : tmem + acc * BN;
+            if (EPI != kRegrad && turn > 1 && !mbar_wait_warp(accEmpty + 8 * acc, ((turn >> 1) - 1) & 1, abort, &g_ffn_timeouts))
                 break;
             tc_fence_after();
             for (int k = k0; k < k1; ++k, ++used) {
@@ -298,6 +327,35 @@ __global__ void __launch_bounds__(kGemmThreads, 1) gemm_kernel(const __grid_cons
                 }
                 tc_fence_after();
                 const uint32_t a = smem + st * kStageBytes<BN>;
+                if constexpr (EPI == kRegrad) {
+                    // dH of the next tile is multiplied while the epilogue still reads G and U of this one
+                    if (k == p.kIters) {
+                        if (turn > 0 && !mbar_wait_warp(accEmpty, (turn - 1) & 1, abort, &g_ffn_timeouts)) {
+                            ok = false;
+                            break;
+                        }
+                        tc_fence_after();
+                    }
+                    constexpr int format = std::is_same<T, __nv_bfloat16>::value ? 1 : 0;
+                    if (lead) {
+                        const uint64_t da = operand_desc<false>(a);
+                        if (k < p.kIters) {
+                            const uint64_t db = operand_desc<true>(a + kCtaM * kStepK * 2);
+#pragma unroll
+                            for (int j = 0; j < kStepK / 16; ++j)
+                                mma_f16(d, da + j * kDescStep<false>, db + j * kDescStep<true>, instr_desc<false, true>(format, 128), k > 0 || j > 0);
+                        } else {
+                            const uint64_t db = operand_desc<false>(a + kCtaM * kStepK * 2);
+#pragma unroll
+                            for (int j = 0; j < kStepK / 16; ++j)
+                                mma_f16(tmem, da + j * kDescStep<false>, db + j * kDescStep<false>, instr_desc<false, false>(format, 256),
+                                        k > p.kIters || j > 0);
+                        }
+                        mma_commit_pair(empty + 8 * st);
+                    }
+                    __syncwarp();
+                    continue;
+                }
                 const uint64_t da = operand_desc<A_MN>(a), db = operand_desc<B_MN>(a + kCtaM * kStepK * 2);
                 if (lead) {
 #pragma unroll
@@ -318,15 +376,15 @@ __global__ void __launch_bounds__(kGemmThreads, 1) gemm_kernel(const __grid_cons
             mbar_wait_bounded(drain, 0, &own, &g_ffn_timeouts);
         }
     } else if (warp >= 2) {
-        // ---- epilogue: warp w may touch TMEM lanes 32 (w % 4) ..; two warps share each quarter, half the columns each ----
-        const int quarter = warp & 3, half = (warp - 2) >> 2;
+        // ---- epilogue: warp w may touch TMEM lanes 32 (w % 4) ..; W / 4 warps share each quarter and split its columns ----
+        const int quarter = warp & 3, share = (warp - 2) >> 2;
         const uint32_t buf0 = staging + (warp - 2) * 4096, buf1 = buf0 + 2048;
         const uint32_t accEmptyFirst = in_first_cta(accEmpty);
         uint32_t turn = 0;
         for (int t = blockIdx.x >> 1; t < tiles; t += gridDim.x >> 1, ++turn) {
             const Tile w = tile_at(t, p, mTiles);
-            const uint32_t acc = turn & 1, d = tmem + acc * BN + ((uint32_t)(quarter * 32) << 16);
-            if (!mbar_wait_warp(accFull + 8 * acc, (turn >> 1) & 1, abort, &g_ffn_timeouts))
+            const uint32_t acc = EPI == kRegrad ? 0 : turn & 1, d = tmem + acc * BN + ((uint32_t)(quarter * 32) << 16);
+            if (!mbar_wait_warp(accFull + 8 * acc, (EPI == kRegrad ? turn : turn >> 1) & 1, abort, &g_ffn_timeouts))
                 break;
             tc_fence_after();
             const long long row0 = (long long)w.m * kTileM + rank * kCtaM + quarter * 32;
@@ -338,13 +396,13 @@ __global__ void __launch_bounds__(kGemmThreads, 1) gemm_kernel(const __grid_cons
             };
             if (p.splits > 1) {
                 float* part = p.partials + ((long long)w.s * p.batch + w.z) * p.mTiles * kTileM * (p.nTiles * BN) +
-                              (row0 + lane) * (p.nTiles * BN) + w.n * BN + half * (BN / 2);
+                              (row0 + lane) * (p.nTiles * BN) + w.n * BN + share * (BN * 4 / W);
 #pragma unroll 1
-                for (int c = 0; c < BN / 2; c += 32) {
+                for (int c = 0; c < BN * 4 / W; c += 32) {
                     uint32_t v[32];
-                    tmem_load32(d + half * (BN / 2) + c, v);
+                    tmem_load32(d + share * (BN * 4 / W) + c, v);
                     tmem_wait_load();
-                    if (c + 32 == BN / 2)
+                    if (c + 32 == BN * 4 / W)
                         release();
                     if (row0 + lane < rowEnd)
 #pragma unroll
@@ -353,12 +411,12 @@ __global__ void __launch_bounds__(kGemmThreads, 1) gemm_kernel(const __grid_cons
                 }
             } else if (EPI == kGate) {
 #pragma unroll 1
-                for (int c = half * 64; c < half * 64 + 64; c += 32) {
+                for (int c = share * (512 / W); c < (share + 1) * (512 / W); c += 32) {
                     uint32_t g[32], u[32], h[16];
                     tmem_load32(d + c, g);
                     tmem_load32(d + 128 + c, u);
                     tmem_wait_load();
-                    if (c + 32 == half * 64 + 64)
+                    if (c + 32 == (share + 1) * (512 / W))
                         release();
                     if (p.act == kSilu)
                         gate_chunk<T, kSilu>(g, u, h);
@@ -388,16 +446,40 @@ __global__ void __launch_bounds__(kGemmThreads, 1) gemm_kernel(const __grid_cons
                     }
                     __syncwarp();
                 }
+            } else if (EPI == kRegrad) {     // one chunk of 32 columns a warp: TMEM is free again after three loads
+                const int c = share * 32, col = w.n * 128 + c;
+                uint32_t dh[32], g[32], u[32], h[16];
+                tmem_load32(d + c, g);
+                tmem_load32(d + 128 + c, u);
+                tmem_load32(d + 256 + 128 * (turn & 1) + c, dh);
+                tmem_wait_load();
+                release();
+                if (p.act == kSilu)
+                    regrad_chunk<T, kSilu>(dh, g, u, h);
+                else if (p.act == kGelu)
+                    regrad_chunk<T, kGelu>(dh, g, u, h);
+                else
+                    regrad_chunk<T, kRelu>(dh, g, u, h);
+                stage_rows(buf0, lane, h);
+                stage_rows(buf1, lane, reinterpret_cast<const uint32_t(&)[16]>(g));
+                __syncwarp();
+                store_tile<T>(static_cast<T*>(p.hid), p.ldh, row0, rowEnd, col, p.N, true, buf0, lane);
+                store_tile<T>(static_cast<T*>(p.dgate), p.ldh, row0, rowEnd, col, p.N, true, buf1, lane);
+                __syncwarp();
+                stage_rows(buf0, lane, reinterpret_cast<const uint32_t(&)[16]>(u));
+                __syncwarp();
+                store_tile<T>(static_cast<T*>(p.dup), p.ldh, row0, rowEnd, col, p.N, true, buf0, lane);
+                __syncwarp();
             } else if (EPI == kGrad) {
 #pragma unroll 1
-                for (int c = half * (BN / 2); c < (half + 1) * (BN / 2); c += 32) {
+                for (int c = share * (BN * 4 / W); c < (share + 1) * (BN * 4 / W); c += 32) {
                     const int col = w.n * BN + c;
                     uint32_t dh[32], g[16], u[16], h[16];
                     load_tile<T>(static_cast<const T*>(p.gate), p.ldh, row0, rowEnd, col, p.N, buf0, lane);
                     load_tile<T>(static_cast<const T*>(p.up), p.ldh, row0, rowEnd, col, p.N, buf1, lane);
                     tmem_load32(d + c, dh);
                     tmem_wait_load();
-                    if (c + 32 == (half + 1) * (BN / 2))
+                    if (c + 32 == (share + 1) * (BN * 4 / W))
                         release();
                     __syncwarp();
                     unstage_rows(buf0, lane, g);
@@ -424,11 +506,11 @@ __global__ void __launch_bounds__(kGemmThreads, 1) gemm_kernel(const __grid_cons
                 T* out = static_cast<T*>(p.out[w.z]);
                 const bool wide = ((p.ldo & 7) == 0) && (reinterpret_cast<uintptr_t>(out) & 15) == 0;
 #pragma unroll 1
-                for (int c = half * (BN / 2); c < (half + 1) * (BN / 2); c += 32) {
+                for (int c = share * (BN * 4 / W); c < (share + 1) * (BN * 4 / W); c += 32) {
                     uint32_t v[32], h[16];
                     tmem_load32(d + c, v);
                     tmem_wait_load();
-                    if (c + 32 == (half + 1) * (BN / 2))
+                    if (c + 32 == (share + 1) * (BN * 4 / W))
                         release();
 #pragma unroll
                     for (int i = 0; i < 16; ++i)
@@ -591,6 +673,40 @@ int split_count(long long rows, long long N, long long tiles, int kIters)
 }
 
 template <typename T, bool A_MN, bool B_MN, int EPI, int BN>
+cudaError_t launch_maps(const Maps& maps, Plan& p, cudaStream_t stream)
+{
+    auto kernel = gemm_kernel<T, A_MN, B_MN, EPI, BN>;
+    static bool raised[64] = {};       // per device; a race only repeats the call
+    int device = 0;
+    if (cudaError_t e = cudaGetDevice(&device))
+        return e;
+    if (device >= 64 || !raised[device]) {
+        if (cudaError_t e = cudaFuncSetAttribute(kernel, cudaFuncAttributeMaxDynamicSharedMemorySize, kGemmSmem<EPI, BN>))
+            return e;
+        if (device < 64)
+            raised[device] = true;
+    }
+    const long long tiles = (long long)p.mTiles * p.nTiles * p.batch * p.splits;
+    cudaLaunchConfig_t cfg = {};
+    cfg.gridDim = dim3(2 * (unsigned)std::min<long long>(tiles, sm_count() / 2)), cfg.blockDim = dim3(kGemmThreads<EPI>);
+    cfg.dynamicSmemBytes = kGemmSmem<EPI, BN>, cfg.stream = stream;
+    cudaLaunchAttribute attr[2];
+    attr[0].id = cudaLaunchAttributeClusterDimension;
+    attr[0].val.clusterDim.x = 2, attr[0].val.clusterDim.y = 1, attr[0].val.clusterDim.z = 1;
+    attr[1].id = cudaLaunchAttributeProgrammaticStreamSerialization;
+    attr[1].val.programmaticStreamSerializationAllowed = 1;
+    cfg.attrs = attr, cfg.numAttrs = options().pdl ? 2 : 1;
+    if (cudaError_t e = cudaLaunchKernelEx(&cfg, kernel, maps, p))
+        return e;
+    if (p.splits == 1)
+        return cudaSuccess;
+    const dim3 fgrid((unsigned)ceil_div(p.N, 128), (unsigned)std::min<long long>((p.M + 7) / 8, 65535), (unsigned)p.batch);
+    if constexpr (EPI == kStore || EPI == kGate)
+        return launch_pdl(finish_kernel<T, EPI>, fgrid, dim3(32, 8), 0, stream, p, BN);
+    return cudaErrorInvalidValue;
+}
+
+template <typename T, bool A_MN, bool B_MN, int EPI, int BN>
 cudaError_t launch_gemm(const Matrix (&a)[2], const Matrix (&b)[2], Plan& p, cudaStream_t stream)
 {
     Maps maps;
@@ -608,35 +724,25 @@ cudaError_t launch_gemm(const Matrix (&a)[2], const Matrix (&b)[2], Plan& p, cud
         maps.a[1] = maps.a[0];
     if (n == 1 && EPI != kGate)
         maps.b[1] = maps.b[0];
-    auto kernel = gemm_kernel<T, A_MN, B_MN, EPI, BN>;
-    static bool raised[64] = {};       // per device; a race only repeats the call
-    int device = 0;
-    if (cudaError_t e = cudaGetDevice(&device))
+    return launch_maps<T, A_MN, B_MN, EPI, BN>(maps, p, stream);
+}
+
+// Hidden gradients with G and U multiplied again.
+template <typename T>
+cudaError_t launch_regrad(const Matrix& dy, const Matrix& x, const Matrix& wd, const Matrix& wg, const Matrix& wu, Plan& p, cudaStream_t stream)
+{
+    Maps maps;
+    if (cudaError_t e = encode(dy, kCtaM, &maps.a[0]))
         return e;
-    if (device >= 64 || !raised[device]) {
-        if (cudaError_t e = cudaFuncSetAttribute(kernel, cudaFuncAttributeMaxDynamicSharedMemorySize, kGemmSmem<BN>))
-            return e;
-        if (device < 64)
-            raised[device] = true;
-    }
-    const long long tiles = (long long)p.mTiles * p.nTiles * p.batch * p.splits;
-    cudaLaunchConfig_t cfg = {};
-    cfg.gridDim = dim3(2 * (unsigned)std::min<long long>(tiles, sm_count() / 2)), cfg.blockDim = dim3(kGemmThreads);
-    cfg.dynamicSmemBytes = kGemmSmem<BN>, cfg.stream = stream;
-    cudaLaunchAttribute attr[2];
-    attr[0].id = cudaLaunchAttributeClusterDimension;
-    attr[0].val.clusterDim.x = 2, attr[0].val.clusterDim.y = 1, attr[0].val.clusterDim.z = 1;
-    attr[1].id = cudaLaunchAttributeProgrammaticStreamSerialization;
-    attr[1].val.programmaticStreamSerializationAllowed = 1;
-    cfg.attrs = attr, cfg.numAttrs = options().pdl ? 2 : 1;
-    if (cudaError_t e = cudaLaunchKernelEx(&cfg, kernel, maps, p))
+    if (cudaError_t e = encode(x, kCtaM, &maps.a[1]))
         return e;
-    if (p.splits == 1)
-        return cudaSuccess;
-    const dim3 fgrid((unsigned)ceil_div(p.N, 128), (unsigned)std::min<long long>((p.M + 7) / 8, 65535), (unsigned)p.batch);
-    if constexpr (EPI != kGrad)
-        return launch_pdl(finish_kernel<T, EPI>, fgrid, dim3(32, 8), 0, stream, p, BN);
-    return cudaErrorInvalidValue;
+    if (cudaError_t e = encode(wg, 128, &maps.b[0]))
+        return e;
+    if (cudaError_t e = encode(wu, 128, &maps.b[1]))
+        return e;
+    if (cudaError_t e = encode(wd, kStepK, &maps.c))
+        return e;
+    return launch_maps<T, false, false, kRegrad, 256>(maps, p, stream);
 }
 
 // A plain product D[m,n] of one or two products (batch) or segments.
@@ -775,7 +881,12 @@ template <typename T> cudaError_t backward(const FfnArgs& f, Layout& l, bool run
     p.splits = 1, p.N = F, p.M = R, p.act = f.act;
     p.gate = f.gate, p.up = f.up, p.ldh = Fp;
     p.dgate = const_cast<void*>(dg.ptr), p.dup = const_cast<void*>(du.ptr), p.hid = const_cast<void*>(h.ptr);
-    SBNET_TRY((launch_gemm<T, false, true, kGrad, 256>({dy, dy}, {wd, wd}, p, stream)));
+    if (f.gate != nullptr) {
+        SBNET_TRY((launch_gemm<T, false, true, kGrad, 256>({dy, dy}, {wd, wd}, p, stream)));
+    } else {
+        p.nTiles = ceil_div(F, 128), p.segs = 2;
+        SBNET_TRY(launch_regrad<T>(dy, x, wd, wg, wu, p, stream));
+    }
     if (f.dx != nullptr) {
         note_site("gated_ffn_grad dx");
         SBNET_TRY((product<T, false, true>({dg, du}, {wg, wu}, 1, 2, R, C, F, f.dx, nullptr, parts, f, false, stream)));

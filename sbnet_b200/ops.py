@@ -569,11 +569,15 @@ def gated_ffn_train(x: torch.Tensor, w_gate, w_up, w_down, activation: str = "si
 
 def gated_ffn_grad(grad: torch.Tensor, x: torch.Tensor, gate: torch.Tensor, up: torch.Tensor, w_gate, w_up, w_down,
                    activation: str = "silu", need_x: bool = True, need_gate_up: bool = True, need_down: bool = True):
-    """Backward pass of :func:`gated_ffn_train`: ``(dx, dw_gate, dw_up, dw_down)``, None where not asked for."""
+    """Backward pass of :func:`gated_ffn_train` -- or of :func:`gated_ffn`, with ``gate`` and ``up`` None: they are then
+    multiplied again.  Returns ``(dx, dw_gate, dw_up, dw_down)``, None where not asked for."""
     rows, channels, hidden, act = _check_ffn(x, w_gate, w_up, w_down, activation)
     _check_like(grad, "grad", x)
+    if (gate is None) != (up is None):
+        raise ValueError("gate and up go together")
     for t, name in ((gate, "gate"), (up, "up")):
-        if tuple(t.shape) != (rows, (hidden + 7) // 8 * 8) or t.dtype != x.dtype or t.device != x.device or not t.is_contiguous():
+        if t is not None and (tuple(t.shape) != (rows, (hidden + 7) // 8 * 8) or t.dtype != x.dtype or
+                              t.device != x.device or not t.is_contiguous()):
             raise ValueError(f"{name} must be what gated_ffn_train returned")
     _require_cuda(x, "x")
     with _on(x.device):
@@ -583,7 +587,7 @@ def gated_ffn_grad(grad: torch.Tensor, x: torch.Tensor, gate: torch.Tensor, up: 
         dwd = torch.empty_like(w_down) if need_down else None
         ws, need = _workspace(rows, channels, hidden, 1, (grad, x, w_gate, w_up, w_down), x.device)
         _lib.check(_lib.load().sbnet_gated_ffn_grad(
-            grad.data_ptr(), x.data_ptr(), gate.data_ptr(), up.data_ptr(), _DTYPES[x.dtype], rows, channels, hidden,
+            grad.data_ptr(), x.data_ptr(), _ptr(gate), _ptr(up), _DTYPES[x.dtype], rows, channels, hidden,
             w_gate.data_ptr(), w_up.data_ptr(), w_down.data_ptr(), act, _ptr(dx), _ptr(dwg), _ptr(dwu), _ptr(dwd),
             ws.data_ptr(), need, _stream(x.device)))
     return dx, dwg, dwu, dwd

@@ -114,6 +114,21 @@ def test_forward_and_backward(cuda_ops, dtype, size):
     assert lib.wait_timeouts() == 0
 
 
+@pytest.mark.parametrize("size", SIZES, ids=str)
+@pytest.mark.parametrize("dtype", [torch.float16, torch.bfloat16])
+def test_backward_that_multiplies_the_projections_again(cuda_ops, dtype, size):
+    """The same bounds hold without the saved projections' rounding."""
+    act = ("silu", "gelu", "relu")[sum(size) % 3]
+    x, wg, wu, wd, dy = _inputs(*size, dtype, seed=sum(size) + 1)
+    exp = _expected(act, x, wg, wu, wd, dy)
+    got = ops.gated_ffn_grad(dy, x, None, None, wg, wu, wd, act)
+    for n, v in zip(NAMES[1:], got):
+        _check(v, exp, n, dtype)
+    again = ops.gated_ffn_grad(dy, x, None, None, wg, wu, wd, act)
+    assert all(torch.equal(a, b) for a, b in zip(got, again))
+    assert lib.wait_timeouts() == 0
+
+
 @pytest.mark.parametrize("act", ["silu", "gelu", "relu"])
 @pytest.mark.parametrize("dtype", [torch.float16, torch.bfloat16])
 @pytest.mark.parametrize("rows", [4, 40, 260])
@@ -125,8 +140,11 @@ def test_activations_over_their_range(cuda_ops, act, dtype, rows):
     exp = _expected(act, x, wg, wu, wd, dy)
     _check(ops.gated_ffn(x, wg, wu, wd, act), exp, "y", dtype, norm=False)
     got = _run(act, x, wg, wu, wd, dy)
+    got.update(zip(("dx2", "dwg2", "dwu2", "dwd2"), ops.gated_ffn_grad(dy, x, None, None, wg, wu, wd, act)))
     for n in NAMES:
         _check(got[n], exp, n, dtype, norm=False)
+    for n, again in zip(NAMES[1:], ("dx2", "dwg2", "dwu2", "dwd2")):
+        _check(got[again], exp, n, dtype, norm=False)
 
 
 @pytest.mark.parametrize("rows", [1, 2, 3, 4, 5, 8, 9, 16, 17, 31, 32, 33, 48, 64, 65, 96, 128])
