@@ -65,6 +65,7 @@ struct Maps {
 
 struct Plan {
     int mTiles, nTiles;            // tiles of D
+    FastDiv perGroup;              // kGroupM * nTiles
     int batch;                     // products of one shape in this launch: product z reads a[z], b[z], writes out[z]
     int segs;                      // reduction segments: segment s reads a[s], b[s]  (batch == 1)
     int kIters;                    // stages of one segment
@@ -105,43 +106,48 @@ __device__ __forceinline__ void unstage_rows(uint32_t buf, int lane, uint32_t (&
         w[4 * c] = v.x, w[4 * c + 1] = v.y, w[4 * c + 2] = v.z, w[4 * c + 3] = v.w;
     }
 }
-// tile -> memory: rows row0.. (below rowEnd), columns col0.. (below N) of a matrix of pitch ld
-template <typename T>
-__device__ __forceinline__ void store_tile(T* out, long long ld, long long row0, long long rowEnd, int col0, int N, bool wide,
-                                           uint32_t buf, int lane)
+// Where a lane's pieces of a tile lie in a matrix of pitch ld: rows r, r + 8, .. r + 24 (r = lane / 4) of row0.., of which
+// the first `rows` pieces are below rowEnd, and columns col.., of which `cols` are below N.
+struct Spot {
+    long long at, step;
+    int rows, cols;
+};
+__device__ __forceinline__ Spot spot(long long ld, long long row0, long long rowEnd, int col0, int N, int lane)
 {
-    const int c = lane & 3, col = col0 + c * 8;
+    const int r = lane >> 2, col = col0 + (lane & 3) * 8;
+    const long long left = rowEnd - row0 - r;
+    return {(row0 + r) * ld + col, 8 * ld, left <= 0 ? 0 : left >= 32 ? 4 : ((int)left + 7) >> 3, N - col};
+}
+// tile -> memory
+template <typename T> __device__ __forceinline__ void store_tile(void* out, const Spot& s, bool wide, uint32_t buf, int lane)
+{
+    T* dst = static_cast<T*>(out) + s.at;
 #pragma unroll
-    for (int i = 0; i < 4; ++i) {
-        const int r = i * 8 + (lane >> 2);
-        const uint4 v = lds128(piece(buf, r, c));
-        if (row0 + r >= rowEnd)
+    for (int i = 0; i < 4; ++i, dst += s.step) {
+        const uint4 v = lds128(piece(buf, i * 8 + (lane >> 2), lane & 3));
+        if (i >= s.rows)
             continue;
-        T* dst = out + (row0 + r) * ld + col;
-        if (wide && col + 8 <= N) {
+        if (wide && s.cols >= 8) {
             *reinterpret_cast<uint4*>(dst) = v;
         } else {
             const T* e = reinterpret_cast<const T*>(&v);
 #pragma unroll
             for (int k = 0; k < 8; ++k)
-                if (col + k < N)
+                if (k < s.cols)
                     dst[k] = e[k];
         }
     }
 }
 // memory -> tile, from a matrix whose pitch is a multiple of 8 elements and covers the piece that holds column N - 1
-template <typename T>
-__device__ __forceinline__ void load_tile(const T* in, long long ld, long long row0, long long rowEnd, int col0, int N,
-                                          uint32_t buf, int lane)
+template <typename T> __device__ __forceinline__ void load_tile(const void* in, const Spot& s, uint32_t buf, int lane)
 {
-    const int c = lane & 3, col = col0 + c * 8;
+    const T* src = static_cast<const T*>(in) + s.at;
 #pragma unroll
-    for (int i = 0; i < 4; ++i) {
-        const int r = i * 8 + (lane >> 2);
+    for (int i = 0; i < 4; ++i, src += s.step) {
         uint4 v = make_uint4(0, 0, 0, 0);
-        if (row0 + r < rowEnd && col < N)
-            v = *reinterpret_cast<const uint4*>(in + (row0 + r) * ld + col);
-        sts128(piece(buf, r, c), v);
+        if (i < s.rows && s.cols > 0)
+            v = *reinterpret_cast<const uint4*>(src);
+        sts128(piece(buf, i * 8 + (lane >> 2), lane & 3), v);
     }
 }
 
@@ -170,19 +176,20 @@ __device__ __forceinline__ void grad_chunk(const uint32_t (&dh)[32], uint32_t (&
     }
 }
 
-// The same from fp32 G and U; their first 16 words are replaced by dG and dU
+// The same for 16 columns from fp32 G and U
 template <typename T, int ACT>
-__device__ __forceinline__ void regrad_chunk(const uint32_t (&dh)[32], uint32_t (&g)[32], uint32_t (&u)[32], uint32_t (&h)[16])
+__device__ __forceinline__ void regrad_chunk(const uint32_t (&dh)[16], const uint32_t (&g)[16], const uint32_t (&u)[16], uint32_t (&h)[8],
+                                             uint32_t (&dg)[8], uint32_t* du)
 {
 #pragma unroll
-    for (int i = 0; i < 16; ++i) {
+    for (int i = 0; i < 8; ++i) {
         const float d0 = __uint_as_float(dh[2 * i]), d1 = __uint_as_float(dh[2 * i + 1]);
         const float u0 = __uint_as_float(u[2 * i]), u1 = __uint_as_float(u[2 * i + 1]);
         float s0, s1;
         const float a0 = activate<ACT, true>(__uint_as_float(g[2 * i]), s0), a1 = activate<ACT, true>(__uint_as_float(g[2 * i + 1]), s1);
         h[i] = pack2<T>(a0 * u0, a1 * u1);
-        u[i] = pack2<T>(d0 * a0, d1 * a1);
-        g[i] = pack2<T>(d0 * u0 * s0, d1 * u1 * s1);
+        du[i] = pack2<T>(d0 * a0, d1 * a1);
+        dg[i] = pack2<T>(d0 * u0 * s0, d1 * u1 * s1);
     }
 }
 
@@ -192,13 +199,17 @@ struct Tile {
 __device__ __forceinline__ Tile tile_at(int t, const Plan& p, int mTiles)
 {
     Tile r;
-    const int plane = mTiles * p.nTiles;
-    const int q = t / plane;
-    t -= q * plane;
-    r.s = q / p.batch, r.z = q - r.s * p.batch;
-    const int group = t / (kGroupM * p.nTiles), inside = t - group * kGroupM * p.nTiles;
-    const int rows = min(kGroupM, mTiles - group * kGroupM);
-    r.n = inside / rows, r.m = group * kGroupM + inside - r.n * rows;
+    r.z = r.s = 0;
+    if (p.batch * p.splits > 1) {
+        const int plane = mTiles * p.nTiles, q = t / plane;
+        t -= q * plane;
+        r.s = q / p.batch, r.z = q - r.s * p.batch;
+    }
+    uint32_t group, inside;
+    p.perGroup.divmod((uint32_t)t, group, inside);
+    const int rows = mTiles - (int)group * kGroupM;
+    r.n = rows >= kGroupM ? (int)inside / kGroupM : (int)inside / rows;      // only the last group divides
+    r.m = (int)group * kGroupM + (int)inside - r.n * min(rows, kGroupM);
     return r;
 }
 
@@ -424,7 +435,6 @@ __global__ void __launch_bounds__(kGemmThreads<EPI>, 1) gemm_kernel(const __grid
                         gate_chunk<T, kGelu>(g, u, h);
                     else
                         gate_chunk<T, kRelu>(g, u, h);
-                    const int col = w.n * 128 + c;
                     stage_rows(buf0, lane, h);
                     if (p.gate != nullptr) {
 #pragma unroll
@@ -433,50 +443,60 @@ __global__ void __launch_bounds__(kGemmThreads<EPI>, 1) gemm_kernel(const __grid
                         stage_rows(buf1, lane, h);
                     }
                     __syncwarp();
-                    store_tile<T>(static_cast<T*>(p.out[0]), p.ldo, row0, rowEnd, col, p.N, true, buf0, lane);
+                    const Spot at = spot(p.ldh, row0, rowEnd, w.n * 128 + c, p.N, lane);
+                    store_tile<T>(p.out[0], at, true, buf0, lane);
                     if (p.gate != nullptr) {
-                        store_tile<T>(static_cast<T*>(p.gate), p.ldh, row0, rowEnd, col, p.N, true, buf1, lane);
+                        store_tile<T>(p.gate, at, true, buf1, lane);
 #pragma unroll
                         for (int i = 0; i < 16; ++i)
                             h[i] = pack2<T>(__uint_as_float(u[2 * i]), __uint_as_float(u[2 * i + 1]));
                         __syncwarp();
                         stage_rows(buf0, lane, h);
                         __syncwarp();
-                        store_tile<T>(static_cast<T*>(p.up), p.ldh, row0, rowEnd, col, p.N, true, buf0, lane);
+                        store_tile<T>(p.up, at, true, buf0, lane);
                     }
                     __syncwarp();
                 }
             } else if (EPI == kRegrad) {     // one chunk of 32 columns a warp: TMEM is free again after three loads
-                const int c = share * 32, col = w.n * 128 + c;
-                uint32_t dh[32], g[32], u[32], h[16];
-                tmem_load32(d + c, g);
-                tmem_load32(d + 128 + c, u);
-                tmem_load32(d + 256 + 128 * (turn & 1) + c, dh);
-                tmem_wait_load();
-                release();
-                if (p.act == kSilu)
-                    regrad_chunk<T, kSilu>(dh, g, u, h);
-                else if (p.act == kGelu)
-                    regrad_chunk<T, kGelu>(dh, g, u, h);
-                else
-                    regrad_chunk<T, kRelu>(dh, g, u, h);
-                stage_rows(buf0, lane, h);
-                stage_rows(buf1, lane, reinterpret_cast<const uint32_t(&)[16]>(g));
+                const int c = share * 32;
+                uint32_t du[16];
+#pragma unroll
+                for (int i = 0; i < 2; ++i) {       // 16 columns at a time: 32 of all three would not fit the registers
+                    uint32_t dh[16], g[16], u[16], h[8], dg[8];
+                    tmem_load16(d + c + 16 * i, g);
+                    tmem_load16(d + 128 + c + 16 * i, u);
+                    tmem_load16(d + 256 + 128 * (turn & 1) + c + 16 * i, dh);
+                    tmem_wait_load();
+                    if (i == 1)
+                        release();
+                    if (p.act == kSilu)
+                        regrad_chunk<T, kSilu>(dh, g, u, h, dg, du + 8 * i);
+                    else if (p.act == kGelu)
+                        regrad_chunk<T, kGelu>(dh, g, u, h, dg, du + 8 * i);
+                    else
+                        regrad_chunk<T, kRelu>(dh, g, u, h, dg, du + 8 * i);
+#pragma unroll
+                    for (int q = 0; q < 2; ++q) {
+                        sts128(piece(buf0, lane, 2 * i + q), make_uint4(h[4 * q], h[4 * q + 1], h[4 * q + 2], h[4 * q + 3]));
+                        sts128(piece(buf1, lane, 2 * i + q), make_uint4(dg[4 * q], dg[4 * q + 1], dg[4 * q + 2], dg[4 * q + 3]));
+                    }
+                }
                 __syncwarp();
-                store_tile<T>(static_cast<T*>(p.hid), p.ldh, row0, rowEnd, col, p.N, true, buf0, lane);
-                store_tile<T>(static_cast<T*>(p.dgate), p.ldh, row0, rowEnd, col, p.N, true, buf1, lane);
+                const Spot at = spot(p.ldh, row0, rowEnd, w.n * 128 + c, p.N, lane);
+                store_tile<T>(p.hid, at, true, buf0, lane);
+                store_tile<T>(p.dgate, at, true, buf1, lane);
                 __syncwarp();
-                stage_rows(buf0, lane, reinterpret_cast<const uint32_t(&)[16]>(u));
+                stage_rows(buf0, lane, du);
                 __syncwarp();
-                store_tile<T>(static_cast<T*>(p.dup), p.ldh, row0, rowEnd, col, p.N, true, buf0, lane);
+                store_tile<T>(p.dup, at, true, buf0, lane);
                 __syncwarp();
             } else if (EPI == kGrad) {
 #pragma unroll 1
                 for (int c = share * (BN * 4 / W); c < (share + 1) * (BN * 4 / W); c += 32) {
-                    const int col = w.n * BN + c;
+                    const Spot at = spot(p.ldh, row0, rowEnd, w.n * BN + c, p.N, lane);
                     uint32_t dh[32], g[16], u[16], h[16];
-                    load_tile<T>(static_cast<const T*>(p.gate), p.ldh, row0, rowEnd, col, p.N, buf0, lane);
-                    load_tile<T>(static_cast<const T*>(p.up), p.ldh, row0, rowEnd, col, p.N, buf1, lane);
+                    load_tile<T>(p.gate, at, buf0, lane);
+                    load_tile<T>(p.up, at, buf1, lane);
                     tmem_load32(d + c, dh);
                     tmem_wait_load();
                     if (c + 32 == (share + 1) * (BN * 4 / W))
@@ -494,12 +514,12 @@ __global__ void __launch_bounds__(kGemmThreads<EPI>, 1) gemm_kernel(const __grid
                     stage_rows(buf0, lane, g);
                     stage_rows(buf1, lane, u);
                     __syncwarp();
-                    store_tile<T>(static_cast<T*>(p.dgate), p.ldh, row0, rowEnd, col, p.N, true, buf0, lane);
-                    store_tile<T>(static_cast<T*>(p.dup), p.ldh, row0, rowEnd, col, p.N, true, buf1, lane);
+                    store_tile<T>(p.dgate, at, true, buf0, lane);
+                    store_tile<T>(p.dup, at, true, buf1, lane);
                     __syncwarp();
                     stage_rows(buf0, lane, h);
                     __syncwarp();
-                    store_tile<T>(static_cast<T*>(p.hid), p.ldh, row0, rowEnd, col, p.N, true, buf0, lane);
+                    store_tile<T>(p.hid, at, true, buf0, lane);
                     __syncwarp();
                 }
             } else {
@@ -517,7 +537,7 @@ __global__ void __launch_bounds__(kGemmThreads<EPI>, 1) gemm_kernel(const __grid
                         h[i] = pack2<T>(__uint_as_float(v[2 * i]), __uint_as_float(v[2 * i + 1]));
                     stage_rows(buf0, lane, h);
                     __syncwarp();
-                    store_tile<T>(out, p.ldo, row0, rowEnd, w.n * BN + c, p.N, wide, buf0, lane);
+                    store_tile<T>(out, spot(p.ldo, row0, rowEnd, w.n * BN + c, p.N, lane), wide, buf0, lane);
                     __syncwarp();
                 }
             }
@@ -687,6 +707,7 @@ cudaError_t launch_maps(const Maps& maps, Plan& p, cudaStream_t stream)
             raised[device] = true;
     }
     const long long tiles = (long long)p.mTiles * p.nTiles * p.batch * p.splits;
+    p.perGroup = FastDiv((uint32_t)(kGroupM * p.nTiles));
     cudaLaunchConfig_t cfg = {};
     cfg.gridDim = dim3(2 * (unsigned)std::min<long long>(tiles, sm_count() / 2)), cfg.blockDim = dim3(kGemmThreads<EPI>);
     cfg.dynamicSmemBytes = kGemmSmem<EPI, BN>, cfg.stream = stream;
@@ -853,7 +874,7 @@ template <typename T> cudaError_t forward(const FfnArgs& f, Layout& l, bool run,
     p.mTiles = ceil_div(R, kTileM), p.nTiles = ceil_div(F, 128), p.batch = 1, p.segs = 1, p.kIters = ceil_div(C, kStepK);
     p.splits = split_count(R, 2ll * F, (long long)p.mTiles * p.nTiles, p.kIters);
     p.N = F, p.M = R, p.num_blocks_dev = f.num_blocks_dev, p.rowsPerBlock = f.rowsPerBlock, p.act = f.act;
-    p.out[0] = const_cast<void*>(h.ptr), p.ldo = Fp, p.gate = f.gate, p.up = f.up, p.ldh = Fp, p.partials = parts;
+    p.out[0] = const_cast<void*>(h.ptr), p.ldo = Fp /* = ldh */, p.gate = f.gate, p.up = f.up, p.ldh = Fp, p.partials = parts;
     SBNET_TRY((launch_gemm<T, false, false, kGate, 256>({x, x}, {wg, wu}, p, stream)));
     note_site("gated_ffn output");
     return product<T, false, false>({h, h}, {wd, wd}, 1, 1, R, C, F, f.y, nullptr, parts, f, true, stream);
