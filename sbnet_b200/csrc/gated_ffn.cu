@@ -54,13 +54,16 @@ enum Epilogue { kStore, kGate, kGrad, kRegrad };
 // warps per scheduler hide better than two.
 template <int EPI> constexpr int kEpiWarps = EPI == kStore ? 8 : 16;
 template <int EPI> constexpr int kGemmThreads = (2 + kEpiWarps<EPI>) * 32;
-template <int EPI> constexpr int kStagingBytes = kEpiWarps<EPI> * 4096;  // two 32 x 32 tiles of 16-bit elements per warp
+// 32 x 32 tiles of 16-bit elements (2 KB) that a warp stages between registers and memory
+template <int EPI> constexpr int kStaged = EPI == kStore ? 1 : EPI == kGrad ? 3 : 2;
+template <int EPI> constexpr int kStagingBytes = kEpiWarps<EPI> * kStaged<EPI> * 2048;
 constexpr int kGroupM = 8;
 
 __device__ unsigned int g_ffn_timeouts = 0;
 
 struct Maps {
     CUtensorMap a[2], b[2], c;     // c: kRegrad's Wd
+    CUtensorMap out[3];            // what kGate (H, G, U) and kGrad (H, dG, dU) write by TMA
 };
 
 struct Plan {
@@ -83,13 +86,14 @@ struct Plan {
     float* partials;               // splits > 1: [splits][batch][mTiles * 256][nTiles * BN]
 };
 
-template <int EPI, int BN> constexpr int kStages = EPI != kStore ? 5 : BN == 256 ? 6 : 8;
+template <int EPI, int BN> constexpr int kStages = EPI == kGrad ? 4 : EPI != kStore ? 5 : BN == 256 ? 6 : 8;
 template <int BN> constexpr int kStageBytes = (kCtaM + BN / 2) * kStepK * 2;    // of one CTA
 template <int EPI, int BN> constexpr int kGemmSmem = 1024 + kStages<EPI, BN> * kStageBytes<BN> + kStagingBytes<EPI> + 256;
 
 // ---- 32 x 32 tiles of 16-bit elements between registers (one row per lane) and memory -----------------------
 // Staged through 2 KB of shared memory so that global accesses are 64 contiguous bytes per row.  16-byte pieces
-// are swizzled by row: eight lanes touch eight different pieces of 128 bytes whichever way the tile is walked.
+// are swizzled by row as TMA's 64-byte mode does it: eight lanes touch eight different pieces of 128 bytes whichever
+// way the tile is walked, and two of the epilogues send their tiles by TMA straight from here.
 __device__ __forceinline__ uint32_t piece(uint32_t buf, int row, int c) { return buf + row * 64 + ((c ^ ((row >> 1) & 3)) << 4); }
 
 __device__ __forceinline__ void stage_rows(uint32_t buf, int lane, const uint32_t (&w)[16])
@@ -154,11 +158,12 @@ template <typename T> __device__ __forceinline__ void load_tile(const void* in, 
 template <typename T, int ACT>
 __device__ __forceinline__ void gate_chunk(const uint32_t (&g)[32], const uint32_t (&u)[32], uint32_t (&h)[16])
 {
-    float unused;
 #pragma unroll
-    for (int i = 0; i < 16; ++i)
-        h[i] = pack2<T>(activate<ACT, false>(__uint_as_float(g[2 * i]), unused) * __uint_as_float(u[2 * i]),
-                        activate<ACT, false>(__uint_as_float(g[2 * i + 1]), unused) * __uint_as_float(u[2 * i + 1]));
+    for (int i = 0; i < 16; ++i) {
+        float a0, a1, unused;
+        activate2<ACT, false>(__uint_as_float(g[2 * i]), __uint_as_float(g[2 * i + 1]), a0, a1, unused, unused);
+        h[i] = pack2<T>(a0 * __uint_as_float(u[2 * i]), a1 * __uint_as_float(u[2 * i + 1]));
+    }
 }
 // g and u are replaced by dG and dU
 template <typename T, int ACT>
@@ -168,8 +173,8 @@ __device__ __forceinline__ void grad_chunk(const uint32_t (&dh)[32], uint32_t (&
     for (int i = 0; i < 16; ++i) {
         const float2 gg = unpack2<T>(g[i]), uu = unpack2<T>(u[i]);
         const float d0 = __uint_as_float(dh[2 * i]), d1 = __uint_as_float(dh[2 * i + 1]);
-        float s0, s1;
-        const float a0 = activate<ACT, true>(gg.x, s0), a1 = activate<ACT, true>(gg.y, s1);
+        float a0, a1, s0, s1;
+        activate2<ACT, true>(gg.x, gg.y, a0, a1, s0, s1);
         h[i] = pack2<T>(a0 * uu.x, a1 * uu.y);
         u[i] = pack2<T>(d0 * a0, d1 * a1);
         g[i] = pack2<T>(d0 * uu.x * s0, d1 * uu.y * s1);
@@ -185,12 +190,31 @@ __device__ __forceinline__ void regrad_chunk(const uint32_t (&dh)[16], const uin
     for (int i = 0; i < 8; ++i) {
         const float d0 = __uint_as_float(dh[2 * i]), d1 = __uint_as_float(dh[2 * i + 1]);
         const float u0 = __uint_as_float(u[2 * i]), u1 = __uint_as_float(u[2 * i + 1]);
-        float s0, s1;
-        const float a0 = activate<ACT, true>(__uint_as_float(g[2 * i]), s0), a1 = activate<ACT, true>(__uint_as_float(g[2 * i + 1]), s1);
+        float a0, a1, s0, s1;
+        activate2<ACT, true>(__uint_as_float(g[2 * i]), __uint_as_float(g[2 * i + 1]), a0, a1, s0, s1);
         h[i] = pack2<T>(a0 * u0, a1 * u1);
         du[i] = pack2<T>(d0 * a0, d1 * a1);
         dg[i] = pack2<T>(d0 * u0 * s0, d1 * u1 * s1);
     }
+}
+
+// A staged tile into one of the scratch matrices (rows past the live ones, inside the matrix, may be written: nobody
+// reads them).
+__device__ __forceinline__ void send_tile(const CUtensorMap* map, uint32_t buf, int col0, int row0, int lane)
+{
+    fence_async_smem();
+    __syncwarp();
+    if (lane == 0) {
+        tma_store_2d(map, buf, col0, row0);
+        bulk_commit();
+    }
+}
+// Before a warp stages into a buffer again: all but the last KEEP tiles it sent have been read.
+template <int KEEP> __device__ __forceinline__ void wait_sent(int lane)
+{
+    if (lane == 0)
+        bulk_wait_read<KEEP>();
+    __syncwarp();
 }
 
 struct Tile {
@@ -208,8 +232,11 @@ __device__ __forceinline__ Tile tile_at(int t, const Plan& p, int mTiles)
     uint32_t group, inside;
     p.perGroup.divmod((uint32_t)t, group, inside);
     const int rows = mTiles - (int)group * kGroupM;
-    r.n = rows >= kGroupM ? (int)inside / kGroupM : (int)inside / rows;      // only the last group divides
-    r.m = (int)group * kGroupM + (int)inside - r.n * min(rows, kGroupM);
+    if (rows >= kGroupM) {
+        r.n = (int)(inside / kGroupM), r.m = (int)(group * kGroupM + inside % kGroupM);
+    } else {        // the last group
+        r.n = (int)inside / rows, r.m = (int)group * kGroupM + (int)inside - r.n * rows;
+    }
     return r;
 }
 
@@ -389,7 +416,7 @@ __global__ void __launch_bounds__(kGemmThreads<EPI>, 1) gemm_kernel(const __grid
     } else if (warp >= 2) {
         // ---- epilogue: warp w may touch TMEM lanes 32 (w % 4) ..; W / 4 warps share each quarter and split its columns ----
         const int quarter = warp & 3, share = (warp - 2) >> 2;
-        const uint32_t buf0 = staging + (warp - 2) * 4096, buf1 = buf0 + 2048;
+        const uint32_t buf0 = staging + (warp - 2) * (kStaged<EPI> * 2048), buf1 = buf0 + 2048, buf2 = buf0 + 4096;
         const uint32_t accEmptyFirst = in_first_cta(accEmpty);
         uint32_t turn = 0;
         for (int t = blockIdx.x >> 1; t < tiles; t += gridDim.x >> 1, ++turn) {
@@ -404,6 +431,7 @@ __global__ void __launch_bounds__(kGemmThreads<EPI>, 1) gemm_kernel(const __grid
                 tc_fence_before();
                 if (lane == 0)
                     mbar_arrive_cluster(accEmptyFirst + 8 * acc);
+                __syncwarp();
             };
             if (p.splits > 1) {
                 float* part = p.partials + ((long long)w.s * p.batch + w.z) * p.mTiles * kTileM * (p.nTiles * BN) +
@@ -435,27 +463,28 @@ __global__ void __launch_bounds__(kGemmThreads<EPI>, 1) gemm_kernel(const __grid
                         gate_chunk<T, kGelu>(g, u, h);
                     else
                         gate_chunk<T, kRelu>(g, u, h);
+                    const int col = w.n * 128 + c;
+                    if (p.gate == nullptr) {    // the two buffers in turn
+                        const uint32_t buf = turn & 1 ? buf1 : buf0;
+                        wait_sent<1>(lane);
+                        stage_rows(buf, lane, h);
+                        send_tile(&maps.out[0], buf, col, (int)row0, lane);
+                        continue;
+                    }
+                    wait_sent<0>(lane);
                     stage_rows(buf0, lane, h);
-                    if (p.gate != nullptr) {
+                    send_tile(&maps.out[0], buf0, col, (int)row0, lane);
 #pragma unroll
-                        for (int i = 0; i < 16; ++i)
-                            h[i] = pack2<T>(__uint_as_float(g[2 * i]), __uint_as_float(g[2 * i + 1]));
-                        stage_rows(buf1, lane, h);
-                    }
-                    __syncwarp();
-                    const Spot at = spot(p.ldh, row0, rowEnd, w.n * 128 + c, p.N, lane);
-                    store_tile<T>(p.out[0], at, true, buf0, lane);
-                    if (p.gate != nullptr) {
-                        store_tile<T>(p.gate, at, true, buf1, lane);
+                    for (int i = 0; i < 16; ++i)
+                        h[i] = pack2<T>(__uint_as_float(g[2 * i]), __uint_as_float(g[2 * i + 1]));
+                    stage_rows(buf1, lane, h);
+                    send_tile(&maps.out[1], buf1, col, (int)row0, lane);
 #pragma unroll
-                        for (int i = 0; i < 16; ++i)
-                            h[i] = pack2<T>(__uint_as_float(u[2 * i]), __uint_as_float(u[2 * i + 1]));
-                        __syncwarp();
-                        stage_rows(buf0, lane, h);
-                        __syncwarp();
-                        store_tile<T>(p.up, at, true, buf0, lane);
-                    }
-                    __syncwarp();
+                    for (int i = 0; i < 16; ++i)
+                        h[i] = pack2<T>(__uint_as_float(u[2 * i]), __uint_as_float(u[2 * i + 1]));
+                    wait_sent<1>(lane);
+                    stage_rows(buf0, lane, h);
+                    send_tile(&maps.out[2], buf0, col, (int)row0, lane);
                 }
             } else if (EPI == kRegrad) {     // one chunk of 32 columns a warp: TMEM is free again after three loads
                 const int c = share * 32;
@@ -494,7 +523,9 @@ __global__ void __launch_bounds__(kGemmThreads<EPI>, 1) gemm_kernel(const __grid
 #pragma unroll 1
                 for (int c = share * (BN * 4 / W); c < (share + 1) * (BN * 4 / W); c += 32) {
                     const Spot at = spot(p.ldh, row0, rowEnd, w.n * BN + c, p.N, lane);
+                    const int col = w.n * BN + c;
                     uint32_t dh[32], g[16], u[16], h[16];
+                    wait_sent<0>(lane);
                     load_tile<T>(p.gate, at, buf0, lane);
                     load_tile<T>(p.up, at, buf1, lane);
                     tmem_load32(d + c, dh);
@@ -511,16 +542,12 @@ __global__ void __launch_bounds__(kGemmThreads<EPI>, 1) gemm_kernel(const __grid
                     else
                         grad_chunk<T, kRelu>(dh, g, u, h);
                     __syncwarp();
-                    stage_rows(buf0, lane, g);
-                    stage_rows(buf1, lane, u);
-                    __syncwarp();
-                    store_tile<T>(p.dgate, at, true, buf0, lane);
-                    store_tile<T>(p.dup, at, true, buf1, lane);
-                    __syncwarp();
-                    stage_rows(buf0, lane, h);
-                    __syncwarp();
-                    store_tile<T>(p.hid, at, true, buf0, lane);
-                    __syncwarp();
+                    stage_rows(buf1, lane, g);
+                    send_tile(&maps.out[1], buf1, col, (int)row0, lane);
+                    stage_rows(buf0, lane, u);
+                    send_tile(&maps.out[2], buf0, col, (int)row0, lane);
+                    stage_rows(buf2, lane, h);
+                    send_tile(&maps.out[0], buf2, col, (int)row0, lane);
                 }
             } else {
                 T* out = static_cast<T*>(p.out[w.z]);
@@ -542,6 +569,8 @@ __global__ void __launch_bounds__(kGemmThreads<EPI>, 1) gemm_kernel(const __grid
                 }
             }
         }
+        if ((EPI == kGate || EPI == kGrad) && lane == 0)
+            bulk_wait_all();     // shared memory is read until then
     }
     // every role's waits are bounded, so both CTAs get here; neither frees TMEM or leaves while the other may still
     // signal its barriers or multiply out of its shared memory
@@ -647,22 +676,23 @@ PFN_cuTensorMapEncodeTiled encoder()
     return fn;
 }
 
-// A row-major matrix of 16-bit elements as TMA reads it: boxes of 64 columns x boxRows rows.
+// A row-major matrix of 16-bit elements as TMA reads it, boxes of 64 columns x boxRows rows, or writes it, 32 x 32.
 struct Matrix {
     const void* ptr;
     long long rows;
     int cols;
     long long ld;
 };
-cudaError_t encode(const Matrix& m, int boxRows, CUtensorMap* out)
+cudaError_t encode(const Matrix& m, int boxRows, CUtensorMap* out, int boxCols = kStepK)
 {
     PFN_cuTensorMapEncodeTiled enc = encoder();
     if (enc == nullptr)
         return cudaErrorNotSupported;
     const cuuint64_t dims[2] = {(cuuint64_t)m.cols, (cuuint64_t)m.rows}, strides[1] = {(cuuint64_t)m.ld * 2};
-    const cuuint32_t box[2] = {(cuuint32_t)kStepK, (cuuint32_t)boxRows}, estr[2] = {1, 1};
+    const cuuint32_t box[2] = {(cuuint32_t)boxCols, (cuuint32_t)boxRows}, estr[2] = {1, 1};
     return enc(out, CU_TENSOR_MAP_DATA_TYPE_UINT16, 2, const_cast<void*>(m.ptr), dims, strides, box, estr,
-               CU_TENSOR_MAP_INTERLEAVE_NONE, CU_TENSOR_MAP_SWIZZLE_128B, CU_TENSOR_MAP_L2_PROMOTION_L2_256B,
+               CU_TENSOR_MAP_INTERLEAVE_NONE, boxCols == 32 ? CU_TENSOR_MAP_SWIZZLE_64B : CU_TENSOR_MAP_SWIZZLE_128B,
+               CU_TENSOR_MAP_L2_PROMOTION_L2_256B,
                CU_TENSOR_MAP_FLOAT_OOB_FILL_NONE) == CUDA_SUCCESS
                ? cudaSuccess
                : cudaErrorInvalidValue;
@@ -727,6 +757,19 @@ cudaError_t launch_maps(const Maps& maps, Plan& p, cudaStream_t stream)
     return cudaErrorInvalidValue;
 }
 
+// The scratch matrices that the epilogue writes by TMA (none where the reduction is split).
+template <int EPI> cudaError_t encode_outputs(const Plan& p, Maps* maps)
+{
+    if ((EPI != kGate && EPI != kGrad) || p.splits > 1)
+        return cudaSuccess;
+    const void* m[3] = {EPI == kGate ? p.out[0] : p.hid, EPI == kGate ? p.gate : p.dgate, EPI == kGate ? p.up : p.dup};
+    for (int i = 0; i < 3; ++i)
+        if (m[i] != nullptr)
+            if (cudaError_t e = encode({m[i], p.M, p.N, p.ldh}, 32, &maps->out[i], 32))
+                return e;
+    return cudaSuccess;
+}
+
 template <typename T, bool A_MN, bool B_MN, int EPI, int BN>
 cudaError_t launch_gemm(const Matrix (&a)[2], const Matrix (&b)[2], Plan& p, cudaStream_t stream)
 {
@@ -745,6 +788,8 @@ cudaError_t launch_gemm(const Matrix (&a)[2], const Matrix (&b)[2], Plan& p, cud
         maps.a[1] = maps.a[0];
     if (n == 1 && EPI != kGate)
         maps.b[1] = maps.b[0];
+    if (cudaError_t e = encode_outputs<EPI>(p, &maps))
+        return e;
     return launch_maps<T, A_MN, B_MN, EPI, BN>(maps, p, stream);
 }
 

@@ -29,31 +29,62 @@ template <> __device__ __forceinline__ float2 unpack2<__nv_bfloat16>(uint32_t v)
     return __bfloat1622float2(*reinterpret_cast<const __nv_bfloat162*>(&v));
 }
 
-// act(g), and its derivative where it is asked for.
-template <int ACT, bool SLOPE> __device__ __forceinline__ float activate(float g, float& slope)
+__device__ __forceinline__ float exp2_fast(float x)
+{
+    float r;
+    asm("ex2.approx.ftz.f32 %0, %1;" : "=f"(r) : "f"(x));
+    return r;
+}
+__device__ __forceinline__ float recip_fast(float x)
+{
+    float r;
+    asm("rcp.approx.ftz.f32 %0, %1;" : "=f"(r) : "f"(x));
+    return r;
+}
+
+// act of two values, and the derivatives where they are asked for.  The epilogues are bound by the special-function unit
+// (16 operations a clock and SM) and by issue slots, hence:
+//  silu: both sigmoids from one reciprocal, 1 / ((1 + e0)(1 + e1)); 2^60 bounds each factor (sigmoids below 2^-60 read
+//        as 2^-60, an error of |g| 2^-60).
+//  gelu: Phi(g) by the rational approximation of Abramowitz and Stegun 7.1.26 for erfc (|error| <= 1.5e-7), whose
+//        exponential is the density that the derivative needs.
+template <int ACT, bool SLOPE> __device__ __forceinline__ void activate2(float g0, float g1, float& a0, float& a1, float& s0, float& s1)
 {
     if constexpr (ACT == kSilu) {
-        const float s = __fdividef(1.f, 1.f + __expf(-g));
+        const float f0 = 1.f + exp2_fast(fminf(g0 * -1.4426950408889634f, 60.f));
+        const float f1 = 1.f + exp2_fast(fminf(g1 * -1.4426950408889634f, 60.f));
+        const float r = recip_fast(f0 * f1), p0 = r * f1, p1 = r * f0;
+        a0 = g0 * p0, a1 = g1 * p1;
         if (SLOPE)
-            slope = s * (1.f + g * (1.f - s));
-        return g * s;
+            s0 = p0 + a0 * (1.f - p0), s1 = p1 + a1 * (1.f - p1);
     } else if constexpr (ACT == kGelu) {
-        const float cdf = 0.5f * (1.f + erff(g * 0.70710678118654752f));
-        if (SLOPE)
-            slope = cdf + g * 0.3989422804014327f * __expf(-0.5f * g * g);
-        return g * cdf;
+        auto one = [](float g, float& a, float& s) {
+            const float z = fabsf(g) * 0.70710678118654752f, t = recip_fast(1.f + 0.3275911f * z);
+            const float e = exp2_fast(g * g * -0.72134752044448170f);        // exp(-g^2 / 2)
+            const float q = 0.5f * e * t *
+                            (0.254829592f + t * (-0.284496736f + t * (1.421413741f + t * (-1.453152027f + t * 1.061405429f))));
+            const float cdf = g < 0.f ? q : 1.f - q;
+            a = g * cdf;
+            if (SLOPE)
+                s = cdf + g * 0.3989422804014327f * e;
+        };
+        one(g0, a0, s0), one(g1, a1, s1);
     } else {
+        a0 = g0 != g0 ? g0 : fmaxf(g0, 0.f), a1 = g1 != g1 ? g1 : fmaxf(g1, 0.f);
         if (SLOPE)
-            slope = g > 0.f ? 1.f : 0.f;
-        return g != g ? g : fmaxf(g, 0.f);
+            s0 = g0 > 0.f ? 1.f : 0.f, s1 = g1 > 0.f ? 1.f : 0.f;
     }
 }
 __device__ __forceinline__ float activate_any(int act, float g)
 {
-    float unused;
-    return act == kSilu   ? activate<kSilu, false>(g, unused)
-           : act == kGelu ? activate<kGelu, false>(g, unused)
-                          : activate<kRelu, false>(g, unused);
+    float a, unused;
+    if (act == kSilu)
+        activate2<kSilu, false>(g, 0.f, a, unused, unused, unused);
+    else if (act == kGelu)
+        activate2<kGelu, false>(g, 0.f, a, unused, unused, unused);
+    else
+        activate2<kRelu, false>(g, 0.f, a, unused, unused, unused);
+    return a;
 }
 
 // Rows to work on: all of them, or those of the live blocks of a stack whose count is on the device.
