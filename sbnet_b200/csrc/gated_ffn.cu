@@ -35,20 +35,15 @@
 //
 // Waits are bounded; a wait that gives up raises a CTA-wide flag, counts itself, and the CTA lets its copies and
 // matrix instructions land, frees its TMEM and returns.
-#include <cuda.h>
-#include <cudaTypedefs.h>
-
 #include <algorithm>
 
 #include "gated_ffn.cuh"
-#include "tensor_ptx.cuh"
 
 namespace sbnet {
 namespace {
 
 constexpr int kTileM = 256;                      // rows of a tile
 constexpr int kCtaM = 128;                       // ... in each CTA of the pair
-constexpr int kStepK = 64;                       // reduction steps of a stage (128 bytes)
 enum Epilogue { kStore, kGate, kGrad, kRegrad };
 // Epilogue warps: the element-wise epilogues are chains of special functions, shared and global accesses, which four
 // warps per scheduler hide better than two.
@@ -89,71 +84,6 @@ struct Plan {
 template <int EPI, int BN> constexpr int kStages = EPI == kGrad ? 4 : EPI != kStore ? 5 : BN == 256 ? 6 : 8;
 template <int BN> constexpr int kStageBytes = (kCtaM + BN / 2) * kStepK * 2;    // of one CTA
 template <int EPI, int BN> constexpr int kGemmSmem = 1024 + kStages<EPI, BN> * kStageBytes<BN> + kStagingBytes<EPI> + 256;
-
-// ---- 32 x 32 tiles of 16-bit elements between registers (one row per lane) and memory -----------------------
-// Staged through 2 KB of shared memory so that global accesses are 64 contiguous bytes per row.  16-byte pieces
-// are swizzled by row as TMA's 64-byte mode does it: eight lanes touch eight different pieces of 128 bytes whichever
-// way the tile is walked, and two of the epilogues send their tiles by TMA straight from here.
-__device__ __forceinline__ uint32_t piece(uint32_t buf, int row, int c) { return buf + row * 64 + ((c ^ ((row >> 1) & 3)) << 4); }
-
-__device__ __forceinline__ void stage_rows(uint32_t buf, int lane, const uint32_t (&w)[16])
-{
-#pragma unroll
-    for (int c = 0; c < 4; ++c)
-        sts128(piece(buf, lane, c), make_uint4(w[4 * c], w[4 * c + 1], w[4 * c + 2], w[4 * c + 3]));
-}
-__device__ __forceinline__ void unstage_rows(uint32_t buf, int lane, uint32_t (&w)[16])
-{
-#pragma unroll
-    for (int c = 0; c < 4; ++c) {
-        const uint4 v = lds128(piece(buf, lane, c));
-        w[4 * c] = v.x, w[4 * c + 1] = v.y, w[4 * c + 2] = v.z, w[4 * c + 3] = v.w;
-    }
-}
-// Where a lane's pieces of a tile lie in a matrix of pitch ld: rows r, r + 8, .. r + 24 (r = lane / 4) of row0.., of which
-// the first `rows` pieces are below rowEnd, and columns col.., of which `cols` are below N.
-struct Spot {
-    long long at, step;
-    int rows, cols;
-};
-__device__ __forceinline__ Spot spot(long long ld, long long row0, long long rowEnd, int col0, int N, int lane)
-{
-    const int r = lane >> 2, col = col0 + (lane & 3) * 8;
-    const long long left = rowEnd - row0 - r;
-    return {(row0 + r) * ld + col, 8 * ld, left <= 0 ? 0 : left >= 32 ? 4 : ((int)left + 7) >> 3, N - col};
-}
-// tile -> memory
-template <typename T> __device__ __forceinline__ void store_tile(void* out, const Spot& s, bool wide, uint32_t buf, int lane)
-{
-    T* dst = static_cast<T*>(out) + s.at;
-#pragma unroll
-    for (int i = 0; i < 4; ++i, dst += s.step) {
-        const uint4 v = lds128(piece(buf, i * 8 + (lane >> 2), lane & 3));
-        if (i >= s.rows)
-            continue;
-        if (wide && s.cols >= 8) {
-            *reinterpret_cast<uint4*>(dst) = v;
-        } else {
-            const T* e = reinterpret_cast<const T*>(&v);
-#pragma unroll
-            for (int k = 0; k < 8; ++k)
-                if (k < s.cols)
-                    dst[k] = e[k];
-        }
-    }
-}
-// memory -> tile, from a matrix whose pitch is a multiple of 8 elements and covers the piece that holds column N - 1
-template <typename T> __device__ __forceinline__ void load_tile(const void* in, const Spot& s, uint32_t buf, int lane)
-{
-    const T* src = static_cast<const T*>(in) + s.at;
-#pragma unroll
-    for (int i = 0; i < 4; ++i, src += s.step) {
-        uint4 v = make_uint4(0, 0, 0, 0);
-        if (i < s.rows && s.cols > 0)
-            v = *reinterpret_cast<const uint4*>(src);
-        sts128(piece(buf, i * 8 + (lane >> 2), lane & 3), v);
-    }
-}
 
 template <typename T, int ACT>
 __device__ __forceinline__ void gate_chunk(const uint32_t (&g)[32], const uint32_t (&u)[32], uint32_t (&h)[16])
@@ -662,44 +592,6 @@ __global__ void __launch_bounds__(256) repack_kernel(const __grid_constant__ Rep
 }
 
 // ---- host side -------------------------------------------------------------------------------------------
-PFN_cuTensorMapEncodeTiled encoder()
-{
-    static const PFN_cuTensorMapEncodeTiled fn = [] {
-        void* ptr = nullptr;
-        cudaDriverEntryPointQueryResult q;
-        if (cudaGetDriverEntryPoint("cuTensorMapEncodeTiled", &ptr, cudaEnableDefault, &q) == cudaSuccess &&
-            q == cudaDriverEntryPointSuccess)
-            return reinterpret_cast<PFN_cuTensorMapEncodeTiled>(ptr);
-        (void)cudaGetLastError();
-        return static_cast<PFN_cuTensorMapEncodeTiled>(nullptr);
-    }();
-    return fn;
-}
-
-// A row-major matrix of 16-bit elements as TMA reads it, boxes of 64 columns x boxRows rows, or writes it, 32 x 32.
-struct Matrix {
-    const void* ptr;
-    long long rows;
-    int cols;
-    long long ld;
-};
-cudaError_t encode(const Matrix& m, int boxRows, CUtensorMap* out, int boxCols = kStepK)
-{
-    PFN_cuTensorMapEncodeTiled enc = encoder();
-    if (enc == nullptr)
-        return cudaErrorNotSupported;
-    const cuuint64_t dims[2] = {(cuuint64_t)m.cols, (cuuint64_t)m.rows}, strides[1] = {(cuuint64_t)m.ld * 2};
-    const cuuint32_t box[2] = {(cuuint32_t)boxCols, (cuuint32_t)boxRows}, estr[2] = {1, 1};
-    return enc(out, CU_TENSOR_MAP_DATA_TYPE_UINT16, 2, const_cast<void*>(m.ptr), dims, strides, box, estr,
-               CU_TENSOR_MAP_INTERLEAVE_NONE, boxCols == 32 ? CU_TENSOR_MAP_SWIZZLE_64B : CU_TENSOR_MAP_SWIZZLE_128B,
-               CU_TENSOR_MAP_L2_PROMOTION_L2_256B,
-               CU_TENSOR_MAP_FLOAT_OOB_FILL_NONE) == CUDA_SUCCESS
-               ? cudaSuccess
-               : cudaErrorInvalidValue;
-}
-
-int ceil_div(long long a, long long b) { return (int)((a + b - 1) / b); }
-
 // Column tile of a plain product: 256 wide unless the matrix is narrow.
 int tile_n(int N) { return N <= 128 ? 128 : 256; }
 
@@ -914,6 +806,9 @@ template <typename T> cudaError_t forward(const FfnArgs& f, Layout& l, bool run,
     Repacks copies;
     copies.add(f.x, x), copies.add(f.w_gate, wg), copies.add(f.w_up, wu), copies.add(f.w_down, wd);
     SBNET_TRY(copies.run(stream));
+    SBNET_TRY(launch_ffn_fused<T>(f, x, wg, wu, wd, stream, &taken));
+    if (taken)
+        return cudaSuccess;
     note_site("gated_ffn projections");
     Plan p = {};
     p.mTiles = ceil_div(R, kTileM), p.nTiles = ceil_div(F, 128), p.batch = 1, p.segs = 1, p.kIters = ceil_div(C, kStepK);
@@ -994,6 +889,14 @@ cudaError_t launch_gated_ffn_grad(const FfnArgs& f, int dtype, cudaStream_t stre
     return dtype == 1 ? backward<__half>(f, l, true, stream) : backward<__nv_bfloat16>(f, l, true, stream);
 }
 
-cudaError_t read_ffn_wait_timeouts(unsigned int* out) { return cudaMemcpyFromSymbol(out, g_ffn_timeouts, sizeof(*out)); }
+cudaError_t read_ffn_wait_timeouts(unsigned int* out)
+{
+    unsigned int fused = 0;
+    cudaError_t e = cudaMemcpyFromSymbol(out, g_ffn_timeouts, sizeof(*out));
+    if (e == cudaSuccess)
+        e = read_ffn_fused_wait_timeouts(&fused);
+    *out += fused;
+    return e;
+}
 
 } // namespace sbnet

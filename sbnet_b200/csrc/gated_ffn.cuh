@@ -1,12 +1,18 @@
 // What the kernels of the gated feed-forward block share: the activation, conversions between fp32 and pairs of 16-bit
-// elements, and the launcher of the few-row kernels.
+// elements, tiles staged between registers and memory, tensor maps, and the launchers of the special cases.
 #pragma once
+#include <cuda.h>
+#include <cudaTypedefs.h>
+
 #include "common.cuh"
 #include "kernels.h"
+#include "tensor_ptx.cuh"
 
 namespace sbnet {
 
 enum Act { kSilu = 0, kGelu = 1, kRelu = 2 };
+
+constexpr int kStepK = 64;      // reduction steps of a shared-memory stage (128 bytes)
 
 template <typename T> __device__ __forceinline__ uint32_t pack2(float lo, float hi);
 template <> __device__ __forceinline__ uint32_t pack2<__half>(float lo, float hi)
@@ -93,7 +99,119 @@ __device__ __forceinline__ long long live_rows(long long rows, const int32_t* bl
     return blocks == nullptr ? rows : min(rows, (long long)max(*blocks, 0) * rowsPerBlock);
 }
 
+// ---- 32 x 32 tiles of 16-bit elements between registers (one row per lane) and memory -----------------------
+// Staged through 2 KB of shared memory so that global accesses are 64 contiguous bytes per row.  16-byte pieces
+// are swizzled by row as TMA's 64-byte mode does it: eight lanes touch eight different pieces of 128 bytes whichever
+// way the tile is walked, and two of the epilogues send their tiles by TMA straight from here.
+__device__ __forceinline__ uint32_t piece(uint32_t buf, int row, int c) { return buf + row * 64 + ((c ^ ((row >> 1) & 3)) << 4); }
+
+__device__ __forceinline__ void stage_rows(uint32_t buf, int lane, const uint32_t (&w)[16])
+{
+#pragma unroll
+    for (int c = 0; c < 4; ++c)
+        sts128(piece(buf, lane, c), make_uint4(w[4 * c], w[4 * c + 1], w[4 * c + 2], w[4 * c + 3]));
+}
+__device__ __forceinline__ void unstage_rows(uint32_t buf, int lane, uint32_t (&w)[16])
+{
+#pragma unroll
+    for (int c = 0; c < 4; ++c) {
+        const uint4 v = lds128(piece(buf, lane, c));
+        w[4 * c] = v.x, w[4 * c + 1] = v.y, w[4 * c + 2] = v.z, w[4 * c + 3] = v.w;
+    }
+}
+// Where a lane's pieces of a tile lie in a matrix of pitch ld: rows r, r + 8, .. r + 24 (r = lane / 4) of row0.., of which
+// the first `rows` pieces are below rowEnd, and columns col.., of which `cols` are below N.
+struct Spot {
+    long long at, step;
+    int rows, cols;
+};
+__device__ __forceinline__ Spot spot(long long ld, long long row0, long long rowEnd, int col0, int N, int lane)
+{
+    const int r = lane >> 2, col = col0 + (lane & 3) * 8;
+    const long long left = rowEnd - row0 - r;
+    return {(row0 + r) * ld + col, 8 * ld, left <= 0 ? 0 : left >= 32 ? 4 : ((int)left + 7) >> 3, N - col};
+}
+// tile -> memory
+template <typename T> __device__ __forceinline__ void store_tile(void* out, const Spot& s, bool wide, uint32_t buf, int lane)
+{
+    T* dst = static_cast<T*>(out) + s.at;
+#pragma unroll
+    for (int i = 0; i < 4; ++i, dst += s.step) {
+        const uint4 v = lds128(piece(buf, i * 8 + (lane >> 2), lane & 3));
+        if (i >= s.rows)
+            continue;
+        if (wide && s.cols >= 8) {
+            *reinterpret_cast<uint4*>(dst) = v;
+        } else {
+            const T* e = reinterpret_cast<const T*>(&v);
+#pragma unroll
+            for (int k = 0; k < 8; ++k)
+                if (k < s.cols)
+                    dst[k] = e[k];
+        }
+    }
+}
+// memory -> tile, from a matrix whose pitch is a multiple of 8 elements and covers the piece that holds column N - 1
+template <typename T> __device__ __forceinline__ void load_tile(const void* in, const Spot& s, uint32_t buf, int lane)
+{
+    const T* src = static_cast<const T*>(in) + s.at;
+#pragma unroll
+    for (int i = 0; i < 4; ++i, src += s.step) {
+        uint4 v = make_uint4(0, 0, 0, 0);
+        if (i < s.rows && s.cols > 0)
+            v = *reinterpret_cast<const uint4*>(src);
+        sts128(piece(buf, i * 8 + (lane >> 2), lane & 3), v);
+    }
+}
+
+// ---- host side ----
+inline PFN_cuTensorMapEncodeTiled encoder()
+{
+    static const PFN_cuTensorMapEncodeTiled fn = [] {
+        void* ptr = nullptr;
+        cudaDriverEntryPointQueryResult q;
+        if (cudaGetDriverEntryPoint("cuTensorMapEncodeTiled", &ptr, cudaEnableDefault, &q) == cudaSuccess &&
+            q == cudaDriverEntryPointSuccess)
+            return reinterpret_cast<PFN_cuTensorMapEncodeTiled>(ptr);
+        (void)cudaGetLastError();
+        return static_cast<PFN_cuTensorMapEncodeTiled>(nullptr);
+    }();
+    return fn;
+}
+
+// A row-major matrix of 16-bit elements as TMA reads it, boxes of 64 columns x boxRows rows, or writes it, 32 x 32.
+struct Matrix {
+    const void* ptr;
+    long long rows;
+    int cols;
+    long long ld;
+};
+inline cudaError_t encode(const Matrix& m, int boxRows, CUtensorMap* out, int boxCols = kStepK)
+{
+    PFN_cuTensorMapEncodeTiled enc = encoder();
+    if (enc == nullptr)
+        return cudaErrorNotSupported;
+    const cuuint64_t dims[2] = {(cuuint64_t)m.cols, (cuuint64_t)m.rows}, strides[1] = {(cuuint64_t)m.ld * 2};
+    const cuuint32_t box[2] = {(cuuint32_t)boxCols, (cuuint32_t)boxRows}, estr[2] = {1, 1};
+    return enc(out, CU_TENSOR_MAP_DATA_TYPE_UINT16, 2, const_cast<void*>(m.ptr), dims, strides, box, estr,
+               CU_TENSOR_MAP_INTERLEAVE_NONE, boxCols == 32 ? CU_TENSOR_MAP_SWIZZLE_64B : CU_TENSOR_MAP_SWIZZLE_128B,
+               CU_TENSOR_MAP_L2_PROMOTION_L2_256B,
+               CU_TENSOR_MAP_FLOAT_OOB_FILL_NONE) == CUDA_SUCCESS
+               ? cudaSuccess
+               : cudaErrorInvalidValue;
+}
+
+inline int ceil_div(long long a, long long b) { return (int)((a + b - 1) / b); }
+
 // Up to 32 rows (gated_ffn_few.cu): h [rows, F] is scratch.  *taken tells whether the sizes suit the kernels.
 template <typename T> cudaError_t launch_ffn_few(const FfnArgs& f, void* h, cudaStream_t stream, bool* taken);
+
+// Up to 256 channels and many rows, both products in one kernel (gated_ffn_fused.cu).  The matrices are what TMA can
+// read.  *taken tells whether the sizes suit it.
+template <typename T>
+cudaError_t launch_ffn_fused(const FfnArgs& f, const Matrix& x, const Matrix& wg, const Matrix& wu, const Matrix& wd,
+                             cudaStream_t stream, bool* taken);
+bool ffn_fused_suits(long long rows, int C);
+cudaError_t read_ffn_fused_wait_timeouts(unsigned int* out);
 
 } // namespace sbnet

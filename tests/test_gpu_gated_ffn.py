@@ -159,7 +159,31 @@ def test_few_rows(cuda_ops, rows, c, f):
     assert torch.equal(y, again)
 
 
-@pytest.mark.parametrize("rows,block", [(4, 1), (12, 3), (300, 100), (1280, 256), (2048, 64)])
+# many rows and up to 256 channels: both products in one kernel; a last tile of one row and of all but one, channel counts
+# around every 64, hidden counts of less than one chunk of 64, of an odd and an even number of chunks
+@pytest.mark.parametrize("rows", [9217, 19200, 40191])
+@pytest.mark.parametrize("c", [8, 33, 64, 72, 128, 136, 192, 200, 256])
+@pytest.mark.parametrize("f", [24, 64, 130, 192, 333])
+def test_many_rows_of_few_channels(cuda_ops, rows, c, f):
+    act, dtype = ("silu", "gelu", "relu")[(rows + c + f) % 3], (torch.float16, torch.bfloat16)[(c + f) % 2]
+    x, wg, wu, wd, _ = _inputs(rows, c, f, dtype, seed=c + f)
+    exp = _expected(act, x, wg, wu, wd)
+    y = ops.gated_ffn(x, wg, wu, wd, act)
+    _check(y, exp, "y", dtype)
+    assert torch.equal(y, ops.gated_ffn(x, wg, wu, wd, act)) and lib.wait_timeouts() == 0
+
+
+def test_many_rows_of_few_channels_stay_alone(cuda_ops):
+    x, wg, wu, wd, _ = _inputs(12_000, 128, 256, torch.float16)
+    want = ops.gated_ffn(x, wg, wu, wd)
+    x[5000, 3], x[11999, 0] = math.nan, math.nan
+    y = ops.gated_ffn(x, wg, wu, wd)
+    keep = torch.ones(12_000, dtype=torch.bool, device="cuda")
+    keep[5000] = keep[11999] = False
+    assert torch.equal(y[keep], want[keep]) and torch.isnan(y[~keep]).all()
+
+
+@pytest.mark.parametrize("rows,block", [(4, 1), (12, 3), (300, 100), (1280, 256), (2048, 64), (12_000, 100)])
 @pytest.mark.parametrize("c,f", [(64, 128), (128, 512), (136, 264), (45, 70), (512, 1024)])
 @pytest.mark.parametrize("part", [0.0, 0.4, 1.0, 5.0])
 def test_device_count(cuda_ops, rows, block, c, f, part):
@@ -288,7 +312,7 @@ def test_another_stream_and_captured_graphs(cuda_ops):
 
 def test_many_rows(cuda_ops):
     """Row offsets past 2^31 elements of the hidden products."""
-    rows, c, f = 140_000, 64, 16_384
+    rows, c, f = 140_000, 264, 16_384
     x, wg, wu, wd, _ = _inputs(256, c, f, torch.bfloat16, seed=4)
     big = torch.zeros((rows, c), dtype=x.dtype, device="cuda")
     big[-256:] = x
