@@ -9,7 +9,7 @@
 //   Y    += H(j) Wd_j^T            256 x C accumulator in TMEM
 //
 // so that X and Y move once and the weights stream out of L2 (each CTA of the pair loads half of every weight tile:
-// rows of Wg or of Wu, half the rows of Wd).  The products are issued one chunk apart -- GU(j), Y(j-1), GU(j+1), .. -- and
+// rows of Wg or of Wu, half the rows of Wd).  The products are issued two chunks apart -- GU(j), Y(j-2), GU(j+1), .. -- and
 // two groups of eight epilogue warps take the chunks in turn, so the tensor cores, the special-function units (two
 // exponentials and a reciprocal for two values of H: the bound of this kernel at C = 128) and the loads overlap.
 // Waits are bounded as in the other matrix kernels.
@@ -25,7 +25,9 @@ __device__ unsigned int g_fused_timeouts = 0;
 constexpr int kRows = 256, kCtaRows = 128;      // of a tile, and of each CTA of the pair
 constexpr int kChunk = 64;                      // hidden channels of a step
 constexpr int kGroupWarps = 8;                  // epilogue warps of each of the two groups
-constexpr int kThreads = (2 + 2 * kGroupWarps) * 32;
+constexpr int kWdWarp = 2 + 2 * kGroupWarps;    // loads, matrix instructions, the epilogue, loads of Wd
+constexpr int kThreads = (kWdWarp + 1) * 32;
+constexpr int kLag = 2;                         // chunks between a GU product and the Y product that uses it
 
 // KC: 64-channel pieces of C.  Stage counts and buffers by what shared memory holds.
 template <int KC> struct Fused {
@@ -115,7 +117,7 @@ __global__ void __launch_bounds__(kThreads, 1) fused_kernel(const __grid_constan
     auto wait = [&](int i, uint32_t parity) { return mbar_wait_warp(bar(i), parity & 1, abort, &g_fused_timeouts); };
 
     if (warp == 0) {
-        // ---- loads: X of a tile, then per chunk the weights of GU and of Y ----
+        // ---- loads: X of a tile, then per chunk the weights of GU ----
         const bool lead = elect_one();
         const uint32_t first = in_first_cta(bars);
         uint32_t turn = 0, q = 0;
@@ -144,6 +146,27 @@ __global__ void __launch_bounds__(kThreads, 1) fused_kernel(const __grid_constan
                                     first + 8 * (B::w1Full + st));
                 }
                 __syncwarp();
+            }
+        }
+        if (*abort && rank == 0) {      // shared memory is not given back with copies (of either CTA) in flight
+            int own = 0;
+            for (int i = 0; i < S; ++i) {
+                if (q > (uint32_t)i)
+                    mbar_wait_bounded(bar(B::w1Full + i), ((q - 1 - i) / S) & 1, &own, &g_fused_timeouts);
+            }
+            for (int i = 0; i < L::kXBufs; ++i)
+                if (turn > (uint32_t)i)
+                    mbar_wait_bounded(bar(B::xFull + i), ((turn - 1 - i) / L::kXBufs) & 1, &own, &g_fused_timeouts);
+        }
+    } else if (warp == kWdWarp) {
+        // ---- loads of Wd, which run kLag chunks behind: a warp of their own keeps them from holding up the others ----
+        const bool lead = elect_one();
+        const uint32_t first = in_first_cta(bars);
+        uint32_t q = 0;
+        bool ok = true;
+        for (int t = pair; ok && t < tiles; t += pairs)
+            for (int j = 0; j < n; ++j, ++q) {
+                const uint32_t st = q % S, again = q / S;
                 if (again > 0 && !(ok = wait(B::wdEmpty + st, again - 1)))
                     break;
                 if (lead) {
@@ -153,27 +176,20 @@ __global__ void __launch_bounds__(kThreads, 1) fused_kernel(const __grid_constan
                 }
                 __syncwarp();
             }
-        }
-        if (*abort && rank == 0) {      // shared memory is not given back with copies (of either CTA) in flight
+        if (*abort && rank == 0) {
             int own = 0;
-            for (int i = 0; i < S; ++i) {
-                if (q > (uint32_t)i)
-                    mbar_wait_bounded(bar(B::w1Full + i), ((q - 1 - i) / S) & 1, &own, &g_fused_timeouts);
+            for (int i = 0; i < S; ++i)
                 if (q > (uint32_t)i)
                     mbar_wait_bounded(bar(B::wdFull + i), ((q - 1 - i) / S) & 1, &own, &g_fused_timeouts);
-            }
-            for (int i = 0; i < L::kXBufs; ++i)
-                if (turn > (uint32_t)i)
-                    mbar_wait_bounded(bar(B::xFull + i), ((turn - 1 - i) / L::kXBufs) & 1, &own, &g_fused_timeouts);
         }
     } else if (warp == 1 && rank == 0) {
         // ---- matrix instructions: the first CTA's, for both ----
         const bool lead = elect_one();
         constexpr int format = std::is_same<T, __nv_bfloat16>::value ? 1 : 0;
         constexpr uint32_t idescGU = instr_desc<false, false>(format, 2 * kChunk), idescY = instr_desc<false, false>(format, L::kYCols);
-        // Y(j - 1) of the tile whose number is `turn`; i: the chunk's number over all tiles
-        auto issue_y = [&](uint32_t i, int j, uint32_t turn) -> bool {
-            const uint32_t st = i % S, hb = i & 1, yb = turn % L::kYBufs;
+        // Y's product of chunk number i (over all tiles)
+        auto issue_y = [&](uint32_t i) -> bool {
+            const uint32_t turn = i / n, j = i - turn * n, st = i % S, hb = i & 1, yb = turn % L::kYBufs;
             if (j == 0 && turn >= L::kYBufs && !wait(B::yEmpty + yb, turn / L::kYBufs - 1))
                 return false;
             if (!wait(B::wdFull + st, i / S) || !wait(B::hFull + hb, i >> 1))
@@ -186,20 +202,21 @@ __global__ void __launch_bounds__(kThreads, 1) fused_kernel(const __grid_constan
                     mma_f16(tmem + 256 + yb * L::kYCols, da + k * kDescStep<false>, db + k * kDescStep<false>, idescY, j > 0 || k > 0);
                 mma_commit_pair(bar(B::wdEmpty + st));
                 mma_commit_pair(bar(B::hEmpty + hb));
-                if (j == n - 1)
+                if (j == n - 1u)
                     mma_commit_pair(bar(B::yFull + yb));
             }
             __syncwarp();
             return true;
         };
-        uint32_t turn = 0, q = 0;
+        // Y runs kLag chunks behind GU, across tiles, so that an epilogue has the time of kLag products
+        uint32_t turn = 0, q = 0, done = 0;     // chunks of GU and of Y issued
         bool ok = true;
         for (int t = pair; ok && t < tiles; t += pairs, ++turn) {
             const uint32_t xb = turn % L::kXBufs;
-            // with one buffer X of this tile is still on its way: the last tile's last product goes first
-            if (L::kXBufs == 1 && turn > 0 && !(ok = issue_y(q - 1, n - 1, turn - 1)))
-                break;
-            if (!(ok = wait(B::xFull + xb, turn / L::kXBufs)))
+            // with one buffer X of this tile is still on its way: the last tile's products go first
+            while (L::kXBufs == 1 && ok && done < q)
+                ok = issue_y(done++);
+            if (!ok || !(ok = wait(B::xFull + xb, turn / L::kXBufs)))
                 break;
             for (int j = 0; j < n; ++j, ++q) {
                 const uint32_t st = q % S, gb = q & 1;
@@ -223,24 +240,19 @@ __global__ void __launch_bounds__(kThreads, 1) fused_kernel(const __grid_constan
                         mma_commit_pair(bar(B::xEmpty + xb));
                 }
                 __syncwarp();
-                // the chunk before this one, maybe the last of the tile before
-                if (j > 0)
-                    ok = issue_y(q - 1, j - 1, turn);
-                else if (turn > 0 && L::kXBufs > 1)
-                    ok = issue_y(q - 1, n - 1, turn - 1);
-                if (!ok)
+                if (done + kLag <= q && !(ok = issue_y(done++)))
                     break;
             }
         }
-        if (ok && turn > 0)
-            issue_y(q - 1, n - 1, turn - 1);
+        while (ok && done < q)
+            ok = issue_y(done++);
         if (*abort) {
             int own = 0;
             if (lead)
                 mma_commit_pair(bar(B::drain));
             mbar_wait_bounded(bar(B::drain), 0, &own, &g_fused_timeouts);
         }
-    } else if (warp >= 2) {
+    } else if (warp >= 2 && warp < kWdWarp) {
         // ---- epilogue: group 0 takes the even chunks (over all tiles), group 1 the odd ones; of a chunk's 64 columns a warp
         // has 32, of Y's columns every fourth 32 ----
         const int e = warp - 2, quarter = warp & 3, group = e >> 3, share = (e >> 2) & 1, all = group * 2 + share;

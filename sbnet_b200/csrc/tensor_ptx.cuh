@@ -121,10 +121,11 @@ __device__ __forceinline__ void mbar_arrive_cluster(uint32_t addr)
 {
     asm volatile("mbarrier.arrive.relaxed.cluster.shared::cluster.b64 _, [%0];" ::"r"(addr) : "memory");
 }
-// Hands over shared memory as well (behind fence_async_smem when the tensor cores read it).
+// Behind fence_async_smem: hands this CTA's shared memory to the tensor cores.  Released at CTA scope: what is handed
+// over is read by this SM; at cluster scope the arrival would wait for the thread's global stores.
 __device__ __forceinline__ void mbar_arrive_cluster_release(uint32_t addr)
 {
-    asm volatile("mbarrier.arrive.release.cluster.shared::cluster.b64 _, [%0];" ::"r"(addr) : "memory");
+    asm volatile("mbarrier.arrive.shared::cluster.b64 _, [%0];" ::"r"(addr) : "memory");
 }
 __device__ __forceinline__ void cluster_sync()
 {
