@@ -6,6 +6,7 @@
 
 #include "common.cuh"
 #include "kernels.h"
+#include "pairs.cuh"
 #include "tensor_ptx.cuh"
 
 namespace sbnet {
@@ -57,12 +58,16 @@ __device__ __forceinline__ float recip_fast(float x)
 template <int ACT, bool SLOPE> __device__ __forceinline__ void activate2(float g0, float g1, float& a0, float& a1, float& s0, float& s1)
 {
     if constexpr (ACT == kSilu) {
-        const float f0 = 1.f + exp2_fast(fminf(g0 * -1.4426950408889634f, 60.f));
-        const float f1 = 1.f + exp2_fast(fminf(g1 * -1.4426950408889634f, 60.f));
-        const float r = recip_fast(f0 * f1), p0 = r * f1, p1 = r * f0;
-        a0 = g0 * p0, a1 = g1 * p1;
-        if (SLOPE)
-            s0 = p0 + a0 * (1.f - p0), s1 = p1 + a1 * (1.f - p1);
+        const F2 g = f2(g0, g1);
+        const float2 x = unpair(mul2(g, f2(-1.4426950408889634f, -1.4426950408889634f)));
+        const float2 f = unpair(add2(f2(exp2_fast(fminf(x.x, 60.f)), exp2_fast(fminf(x.y, 60.f))), f2(1.f, 1.f)));
+        const float r = recip_fast(f.x * f.y);
+        const F2 sig = mul2(f2(r, r), f2(f.y, f.x)), a = mul2(g, sig);
+        a0 = unpair(a).x, a1 = unpair(a).y;
+        if (SLOPE) {    // sig + a (1 - sig)
+            const F2 s = fma2(a, fma2(sig, f2(-1.f, -1.f), f2(1.f, 1.f)), sig);
+            s0 = unpair(s).x, s1 = unpair(s).y;
+        }
     } else if constexpr (ACT == kGelu) {
         auto one = [](float g, float& a, float& s) {
             const float z = fabsf(g) * 0.70710678118654752f, t = recip_fast(1.f + 0.3275911f * z);

@@ -259,9 +259,40 @@ __global__ void __launch_bounds__(kThreads, 1) fused_kernel(const __grid_constan
         const uint32_t lanes = (uint32_t)(quarter * 32) << 16, first = in_first_cta(bars);
         const uint32_t staging = smem + L::kStage + e * 2048;
         const int row = quarter * 32 + lane;
-        uint32_t turn = 0, q = 0;
+        const bool wide = (p.C & 7) == 0 && (reinterpret_cast<uintptr_t>(p.y) & 15) == 0;
+        uint32_t turn = 0, q = 0, stored = 0;
         bool ok = true;
+        // Y of the oldest tile that is not stored yet
+        auto finish = [&]() -> bool {
+            if (stored == turn)
+                return true;
+            const uint32_t yb = stored % L::kYBufs;
+            if (!wait(B::yFull + yb, stored / L::kYBufs))
+                return false;
+            tc_fence_after();
+            const long long row0 = (long long)(pair + (int)stored * pairs) * kRows + rank * kCtaRows + quarter * 32;
+#pragma unroll 1
+            for (int c = all * 32; c < L::kYCols; c += 128) {
+                uint32_t v[32], h[16];
+                tmem_load32(tmem + lanes + 256 + yb * L::kYCols + c, v);
+                tmem_wait_load();
+#pragma unroll
+                for (int i = 0; i < 16; ++i)
+                    h[i] = pack2<T>(__uint_as_float(v[2 * i]), __uint_as_float(v[2 * i + 1]));
+                stage_rows(staging, lane, h);
+                __syncwarp();
+                store_tile<T>(p.y, spot(p.C, row0, rowEnd, c, p.C, lane), wide, staging, lane);
+                __syncwarp();
+            }
+            tc_fence_before();
+            if (lane == 0)
+                mbar_arrive_cluster(first + 8 * (B::yEmpty + yb));
+            __syncwarp();
+            ++stored;
+            return true;
+        };
         for (int t = pair; ok && t < tiles; t += pairs, ++turn) {
+            bool taken = false;     // a chunk of this tile: Y of the tile before is stored behind it, when it has long been done
             for (int j = 0; j < n; ++j, ++q) {
                 if ((int)(q & 1) != group)
                     continue;
@@ -294,31 +325,15 @@ __global__ void __launch_bounds__(kThreads, 1) fused_kernel(const __grid_constan
                 if (lane == 0)
                     mbar_arrive_cluster_release(first + 8 * (B::hFull + group));
                 __syncwarp();
+                if (!taken && !(ok = finish()))
+                    break;
+                taken = true;
             }
-            const uint32_t yb = turn % L::kYBufs;
-            if (!ok || !(ok = wait(B::yFull + yb, turn / L::kYBufs)))
+            if (!ok || (!taken && !(ok = finish())))
                 break;
-            tc_fence_after();
-            const long long row0 = (long long)t * kRows + rank * kCtaRows + quarter * 32;
-            const bool wide = (p.C & 7) == 0 && (reinterpret_cast<uintptr_t>(p.y) & 15) == 0;
-#pragma unroll 1
-            for (int c = all * 32; c < L::kYCols; c += 128) {
-                uint32_t v[32], h[16];
-                tmem_load32(tmem + lanes + 256 + yb * L::kYCols + c, v);
-                tmem_wait_load();
-#pragma unroll
-                for (int i = 0; i < 16; ++i)
-                    h[i] = pack2<T>(__uint_as_float(v[2 * i]), __uint_as_float(v[2 * i + 1]));
-                stage_rows(staging, lane, h);
-                __syncwarp();
-                store_tile<T>(p.y, spot(p.C, row0, rowEnd, c, p.C, lane), wide, staging, lane);
-                __syncwarp();
-            }
-            tc_fence_before();
-            if (lane == 0)
-                mbar_arrive_cluster(first + 8 * (B::yEmpty + yb));
-            __syncwarp();
         }
+        if (ok && turn > 0)
+            finish();
     }
     // every wait is bounded, so both CTAs get here; neither leaves while the other may still signal its barriers or multiply
     // out of its shared memory

@@ -26,6 +26,7 @@
 #include "async_ptx.cuh"
 #include "common.cuh"
 #include "kernels.h"
+#include "pairs.cuh"
 
 namespace sbnet {
 namespace {
@@ -43,47 +44,6 @@ template <typename T> __device__ __forceinline__ T from_f(float v);
 template <> __device__ __forceinline__ float from_f<float>(float v) { return v; }
 template <> __device__ __forceinline__ __half from_f<__half>(float v) { return __float2half_rn(v); }
 template <> __device__ __forceinline__ __nv_bfloat16 from_f<__nv_bfloat16>(float v) { return __float2bfloat16_rn(v); }
-
-// Two fp32 values in a 64-bit register: sm_100 adds and multiplies such pairs in one instruction, and these kernels
-// are as close to the issue limit as to HBM's.
-struct F2 {
-    unsigned long long v;
-};
-__device__ __forceinline__ F2 f2(float a, float b)
-{
-    F2 r;
-    asm("mov.b64 %0, {%1, %2};" : "=l"(r.v) : "f"(a), "f"(b));
-    return r;
-}
-__device__ __forceinline__ float2 unpair(F2 a)
-{
-    float2 r;
-    asm("mov.b64 {%0, %1}, %2;" : "=f"(r.x), "=f"(r.y) : "l"(a.v));
-    return r;
-}
-__device__ __forceinline__ float both(F2 a)
-{
-    const float2 r = unpair(a);
-    return r.x + r.y;
-}
-__device__ __forceinline__ F2 add2(F2 a, F2 b)
-{
-    F2 r;
-    asm("add.rn.f32x2 %0, %1, %2;" : "=l"(r.v) : "l"(a.v), "l"(b.v));
-    return r;
-}
-__device__ __forceinline__ F2 mul2(F2 a, F2 b)
-{
-    F2 r;
-    asm("mul.rn.f32x2 %0, %1, %2;" : "=l"(r.v) : "l"(a.v), "l"(b.v));
-    return r;
-}
-__device__ __forceinline__ F2 fma2(F2 a, F2 b, F2 c)
-{
-    F2 r;
-    asm("fma.rn.f32x2 %0, %1, %2, %3;" : "=l"(r.v) : "l"(a.v), "l"(b.v), "l"(c.v));
-    return r;
-}
 
 // VE elements as raw words; kept packed until they are used.
 template <typename T, int VE> struct Pack {
