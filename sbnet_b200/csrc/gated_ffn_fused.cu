@@ -9,9 +9,9 @@
 //   Y    += H(j) Wd_j^T            256 x C accumulator in TMEM
 //
 // so that X and Y move once and the weights stream out of L2 (each CTA of the pair loads half of every weight tile:
-// rows of Wg or of Wu, half the rows of Wd).  The products are issued two chunks apart -- GU(j), Y(j-2), GU(j+1), .. -- and
-// two groups of eight epilogue warps take the chunks in turn, so the tensor cores, the special-function units (two
-// exponentials and a reciprocal for two values of H: the bound of this kernel at C = 128) and the loads overlap.
+// rows of Wg or of Wu, half the rows of Wd).  GU and Y are issued by a
+// warp each, GU up to two chunks ahead, and two groups of eight epilogue warps take the chunks in turn, so the tensor
+// cores, the special-function units (two exponentials and a reciprocal for two values of H) and the loads overlap.
 // Waits are bounded as in the other matrix kernels.
 #include <algorithm>
 
@@ -25,9 +25,8 @@ __device__ unsigned int g_fused_timeouts = 0;
 constexpr int kRows = 256, kCtaRows = 128;      // of a tile, and of each CTA of the pair
 constexpr int kChunk = 64;                      // hidden channels of a step
 constexpr int kGroupWarps = 8;                  // epilogue warps of each of the two groups
-constexpr int kWdWarp = 2 + 2 * kGroupWarps;    // loads, matrix instructions, the epilogue, loads of Wd
-constexpr int kThreads = (kWdWarp + 1) * 32;
-constexpr int kLag = 2;                         // chunks between a GU product and the Y product that uses it
+// Warps: 0 loads X and the weights of GU, 1 issues GU, then the epilogue's, then one that loads Wd and one that issues Y.
+constexpr int kWdWarp = 2 + 2 * kGroupWarps, kYWarp = kWdWarp + 1, kThreads = (kYWarp + 1) * 32;
 
 // KC: 64-channel pieces of C.  Stage counts and buffers by what shared memory holds.
 template <int KC> struct Fused {
@@ -70,7 +69,7 @@ __device__ __forceinline__ void gate_words(const uint32_t (&g)[32], const uint32
 template <int S> struct Bars {
     static constexpr int w1Full = 0, w1Empty = w1Full + S, wdFull = w1Empty + S, wdEmpty = wdFull + S, xFull = wdEmpty + S,
                          xEmpty = xFull + 2, guFull = xEmpty + 2, guEmpty = guFull + 2, hFull = guEmpty + 2, hEmpty = hFull + 2,
-                         yFull = hEmpty + 2, yEmpty = yFull + 2, drain = yEmpty + 2, count = drain + 1;
+                         yFull = hEmpty + 2, yEmpty = yFull + 2, drain = yEmpty + 2, drainY = drain + 1, count = drainY + 1;
 };
 
 template <typename T, int KC>
@@ -159,7 +158,7 @@ __global__ void __launch_bounds__(kThreads, 1) fused_kernel(const __grid_constan
                     mbar_wait_bounded(bar(B::xFull + i), ((turn - 1 - i) / L::kXBufs) & 1, &own, &g_fused_timeouts);
         }
     } else if (warp == kWdWarp) {
-        // ---- loads of Wd, which run kLag chunks behind: a warp of their own keeps them from holding up the others ----
+        // ---- loads of Wd, which is used later than GU's weights: a warp of their own keeps them from holding those up ----
         const bool lead = elect_one();
         const uint32_t first = in_first_cta(bars);
         uint32_t q = 0;
@@ -183,44 +182,19 @@ __global__ void __launch_bounds__(kThreads, 1) fused_kernel(const __grid_constan
                     mbar_wait_bounded(bar(B::wdFull + i), ((q - 1 - i) / S) & 1, &own, &g_fused_timeouts);
         }
     } else if (warp == 1 && rank == 0) {
-        // ---- matrix instructions: the first CTA's, for both ----
+        // ---- GU's matrix instructions: the first CTA's, for both ----
         const bool lead = elect_one();
         constexpr int format = std::is_same<T, __nv_bfloat16>::value ? 1 : 0;
-        constexpr uint32_t idescGU = instr_desc<false, false>(format, 2 * kChunk), idescY = instr_desc<false, false>(format, L::kYCols);
-        // Y's product of chunk number i (over all tiles)
-        auto issue_y = [&](uint32_t i) -> bool {
-            const uint32_t turn = i / n, j = i - turn * n, st = i % S, hb = i & 1, yb = turn % L::kYBufs;
-            if (j == 0 && turn >= L::kYBufs && !wait(B::yEmpty + yb, turn / L::kYBufs - 1))
-                return false;
-            if (!wait(B::wdFull + st, i / S) || !wait(B::hFull + hb, i >> 1))
-                return false;
-            tc_fence_after();
-            if (lead) {
-                const uint64_t da = operand_desc<false>(smem + L::kH + hb * L::kHBytes), db = operand_desc<false>(smem + L::kWd + st * L::kWdBytes);
-#pragma unroll
-                for (int k = 0; k < 4; ++k)
-                    mma_f16(tmem + 256 + yb * L::kYCols, da + k * kDescStep<false>, db + k * kDescStep<false>, idescY, j > 0 || k > 0);
-                mma_commit_pair(bar(B::wdEmpty + st));
-                mma_commit_pair(bar(B::hEmpty + hb));
-                if (j == n - 1u)
-                    mma_commit_pair(bar(B::yFull + yb));
-            }
-            __syncwarp();
-            return true;
-        };
-        // Y runs kLag chunks behind GU, across tiles, so that an epilogue has the time of kLag products
-        uint32_t turn = 0, q = 0, done = 0;     // chunks of GU and of Y issued
+        constexpr uint32_t idesc = instr_desc<false, false>(format, 2 * kChunk);
+        uint32_t turn = 0, q = 0, st = 0, phase = 0;
         bool ok = true;
         for (int t = pair; ok && t < tiles; t += pairs, ++turn) {
             const uint32_t xb = turn % L::kXBufs;
-            // with one buffer X of this tile is still on its way: the last tile's products go first
-            while (L::kXBufs == 1 && ok && done < q)
-                ok = issue_y(done++);
-            if (!ok || !(ok = wait(B::xFull + xb, turn / L::kXBufs)))
+            if (!(ok = wait(B::xFull + xb, turn / L::kXBufs)))
                 break;
             for (int j = 0; j < n; ++j, ++q) {
-                const uint32_t st = q % S, gb = q & 1;
-                if ((q >= 2 && !wait(B::guEmpty + gb, (q >> 1) - 1)) || !wait(B::w1Full + st, q / S)) {
+                const uint32_t gb = q & 1;
+                if ((q >= 2 && !wait(B::guEmpty + gb, (q >> 1) - 1)) || !wait(B::w1Full + st, phase)) {
                     ok = false;
                     break;
                 }
@@ -232,25 +206,62 @@ __global__ void __launch_bounds__(kThreads, 1) fused_kernel(const __grid_constan
                                        db = operand_desc<false>(smem + L::kW1 + st * L::kW1Bytes + k * kChunk * 128);
 #pragma unroll
                         for (int i = 0; i < 4; ++i)
-                            mma_f16(tmem + gb * 128, da + i * kDescStep<false>, db + i * kDescStep<false>, idescGU, k > 0 || i > 0);
+                            mma_f16(tmem + gb * 128, da + i * kDescStep<false>, db + i * kDescStep<false>, idesc, k > 0 || i > 0);
                     }
-                    mma_commit_pair(bar(B::w1Empty + st));
                     mma_commit_pair(bar(B::guFull + gb));
+                    mma_commit_pair(bar(B::w1Empty + st));
                     if (j == n - 1)
                         mma_commit_pair(bar(B::xEmpty + xb));
                 }
                 __syncwarp();
-                if (done + kLag <= q && !(ok = issue_y(done++)))
-                    break;
+                if (++st == S)
+                    st = 0, phase ^= 1;
             }
         }
-        while (ok && done < q)
-            ok = issue_y(done++);
         if (*abort) {
             int own = 0;
             if (lead)
                 mma_commit_pair(bar(B::drain));
             mbar_wait_bounded(bar(B::drain), 0, &own, &g_fused_timeouts);
+        }
+    } else if (warp == kYWarp && rank == 0) {
+        // ---- Y's: from a warp of their own, so that neither product's waits hold up the other's instructions ----
+        const bool lead = elect_one();
+        constexpr int format = std::is_same<T, __nv_bfloat16>::value ? 1 : 0;
+        constexpr uint32_t idesc = instr_desc<false, false>(format, L::kYCols);
+        uint32_t turn = 0, q = 0, st = 0, phase = 0;
+        bool ok = true;
+        for (int t = pair; ok && t < tiles; t += pairs, ++turn) {
+            const uint32_t yb = turn % L::kYBufs, d = tmem + 256 + yb * L::kYCols;
+            if (turn >= L::kYBufs && !(ok = wait(B::yEmpty + yb, turn / L::kYBufs - 1)))
+                break;
+            for (int j = 0; j < n; ++j, ++q) {
+                const uint32_t hb = q & 1;
+                if (!wait(B::wdFull + st, phase) || !wait(B::hFull + hb, q >> 1)) {
+                    ok = false;
+                    break;
+                }
+                tc_fence_after();
+                if (lead) {
+                    const uint64_t da = operand_desc<false>(smem + L::kH + hb * L::kHBytes), db = operand_desc<false>(smem + L::kWd + st * L::kWdBytes);
+#pragma unroll
+                    for (int k = 0; k < 4; ++k)
+                        mma_f16(d, da + k * kDescStep<false>, db + k * kDescStep<false>, idesc, j > 0 || k > 0);
+                    mma_commit_pair(bar(B::hEmpty + hb));
+                    mma_commit_pair(bar(B::wdEmpty + st));
+                    if (j == n - 1)
+                        mma_commit_pair(bar(B::yFull + yb));
+                }
+                __syncwarp();
+                if (++st == S)
+                    st = 0, phase ^= 1;
+            }
+        }
+        if (*abort) {
+            int own = 0;
+            if (lead)
+                mma_commit_pair(bar(B::drainY));
+            mbar_wait_bounded(bar(B::drainY), 0, &own, &g_fused_timeouts);
         }
     } else if (warp >= 2 && warp < kWdWarp) {
         // ---- epilogue: group 0 takes the even chunks (over all tiles), group 1 the odd ones; of a chunk's 64 columns a warp
