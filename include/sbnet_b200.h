@@ -269,8 +269,6 @@ int sbnet_layer_norm_grad(const void* dy, const void* x, int dtype, int64_t rows
  *   dtype           SBNET_F16 or SBNET_BF16 (what the tensor cores multiply; SBNET_F32 is rejected), of every tensor
  *   x, y            [rows,C];  w_gate, w_up [F,C];  w_down [C,F]
  *   act             SBNET_ACT_*
- *   gate, up        [rows, F rounded up to a multiple of 8], 16-byte aligned: receive x w_gate^T and x w_up^T for the
- *                   backward pass (columns past F are not written); both NULL when they are not wanted
  *   workspace       256-byte aligned device memory of at least sbnet_gated_ffn_workspace() bytes, used by this call
  *                   only until it is done on `stream`
  * Accumulation and the element-wise steps are fp32; act(gate)*up is rounded to dtype once, as the operand of the last
@@ -286,19 +284,17 @@ int sbnet_layer_norm_grad(const void* dy, const void* x, int dtype, int64_t rows
 /* grad: workspace of the backward pass.  aligned: 0 if any input tensor's address is not a multiple of 16 bytes. */
 size_t sbnet_gated_ffn_workspace(int64_t rows, int C, int F, int grad, int aligned);
 int sbnet_gated_ffn(const void* x, int dtype, int64_t rows, int C, int F, const void* w_gate, const void* w_up,
-                    const void* w_down, int act, void* y, void* gate, void* up, void* workspace,
-                    size_t workspace_bytes, void* stream);
+                    const void* w_down, int act, void* y, void* workspace, size_t workspace_bytes, void* stream);
 int sbnet_gated_ffn_dyn(const void* x, int dtype, int64_t maxBlocks, int rowsPerBlock, const int32_t* num_blocks_dev,
                         int C, int F, const void* w_gate, const void* w_up, const void* w_down, int act, void* y,
                         void* workspace, size_t workspace_bytes, void* stream);
 /*
- * Backward pass from dy, x and the forward pass' gate and up, which are multiplied again from x where both are NULL
- * (4*C operations per hidden element instead of 4 bytes kept, written and read; quicker up to some 512 channels).  dx [rows,C], dw_gate and dw_up [F,C], dw_down [C,F]
+ * Backward pass from dy and the forward pass' inputs (the projections are multiplied again, so training keeps nothing
+ * else of the forward pass).  dx [rows,C], dw_gate and dw_up [F,C], dw_down [C,F]
  * are each skipped where NULL (dw_gate and dw_up go together); no output may overlap an input.  With rows == 0 the
  * weight gradients are set to zero.
  */
-int sbnet_gated_ffn_grad(const void* dy, const void* x, const void* gate, const void* up, int dtype, int64_t rows,
-                         int C, int F, const void* w_gate, const void* w_up, const void* w_down, int act, void* dx,
+int sbnet_gated_ffn_grad(const void* dy, const void* x, int dtype, int64_t rows, int C, int F, const void* w_gate, const void* w_up, const void* w_down, int act, void* dx,
                          void* dw_gate, void* dw_up, void* dw_down, void* workspace, size_t workspace_bytes,
                          void* stream);
 

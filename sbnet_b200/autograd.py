@@ -100,32 +100,23 @@ def layer_norm(x, weight=None, bias=None, eps=1e-5):
     return _LayerNorm.apply(x, weight, bias, eps)
 
 
-# Up to this many channels the backward pass of the gated feed-forward block multiplies the two projections again
-# instead of keeping them (4*C operations per hidden element against writing, keeping and reading 4 bytes).
-RECOMPUTE_CHANNELS = 512
-
-
 class _GatedFfn(torch.autograd.Function):
     @staticmethod
     def forward(ctx, x, w_gate, w_up, w_down, activation):
-        gate = up = None
-        if x.shape[-1] <= RECOMPUTE_CHANNELS or not any(ctx.needs_input_grad):
-            y = ops.gated_ffn(x, w_gate, w_up, w_down, activation)
-        else:
-            y, gate, up = ops.gated_ffn_train(x, w_gate, w_up, w_down, activation)
-        ctx.save_for_backward(x, w_gate, w_up, w_down, gate, up)
+        ctx.save_for_backward(x, w_gate, w_up, w_down)
         ctx.activation = activation
-        return y
+        return ops.gated_ffn(x, w_gate, w_up, w_down, activation)
 
     @staticmethod
     @once_differentiable
     def backward(ctx, grad):
-        x, w_gate, w_up, w_down, gate, up = ctx.saved_tensors
+        x, w_gate, w_up, w_down = ctx.saved_tensors
         need = ctx.needs_input_grad
-        return (*ops.gated_ffn_grad(grad.contiguous(), x, gate, up, w_gate, w_up, w_down, ctx.activation,
+        return (*ops.gated_ffn_grad(grad.contiguous(), x, w_gate, w_up, w_down, ctx.activation,
                                     need[0], need[1] or need[2], need[3]), None)
 
 
 def gated_ffn(x, w_gate, w_up, w_down, activation="silu"):
-    """Differentiable :func:`sbnet_b200.ops.gated_ffn` (gradients flow to ``x`` and the three weights)."""
+    """Differentiable :func:`sbnet_b200.ops.gated_ffn` (gradients flow to ``x`` and the three weights).  Nothing but
+    the inputs is kept for the backward pass."""
     return _GatedFfn.apply(x, w_gate, w_up, w_down, activation)

@@ -9,16 +9,17 @@
 // does with an accumulator tile:
 //
 //   kGate   both projections at once: a tile's B operand is 128 rows of Wg followed by 128 rows of Wu, so G and
-//           U of the same 128 x 128 positions come out of one instruction stream side by side in TMEM and the
-//           epilogue writes H (and, in training, G and U) without either having been to memory
-//   kGrad   dH stays in TMEM; the epilogue reads G and U and writes dG, dU and H
-//   kRegrad the same without G and U from the forward pass: a tile multiplies dH (128 columns), then G and U again
-//           (256 columns), and the epilogue takes all three from TMEM.  With few channels that costs less than
-//           writing and reading G and U: 4 C operations per hidden element against 8 bytes of HBM traffic
+//           U of the same positions come out of one instruction stream side by side in TMEM and the epilogue
+//           writes H without either having been to memory
+//   kGrad   the hidden gradients: a tile multiplies dH (128 columns) and then G and U again (256 columns), and the
+//           epilogue takes all three from TMEM and writes H, dG and dU.  The backward pass so needs nothing of the
+//           forward pass but its inputs.  Keeping G and U instead would save 4 of its 16 R F C operations, but in 16
+//           bits their rounding shows in every gradient (error against 64 bits 2.1 times that of one rounding
+//           instead of 1.4) and in 32 bits they cost 16 bytes of HBM traffic per hidden element
 //   kStore  a plain product, rounded once
 //
-// G, U, H, dG and dU are held between kernels in the type of X (they are operands of the next product, and the
-// tensor cores multiply 16-bit types); accumulators and every element-wise step are fp32.
+// H, dG and dU are held between kernels in the type of X (they are operands of the next product, and the tensor
+// cores multiply 16-bit types); accumulators and every element-wise step are fp32.
 //
 // Structure: persistent pairs of CTAs (one CTA per SM) over 256 x 256 (or 256 x 128) output tiles.  A pair
 // multiplies as one (cta_group::2): each CTA holds its own 128 rows of A and half of B, so a stage of 64
@@ -44,21 +45,21 @@ namespace {
 
 constexpr int kTileM = 256;                      // rows of a tile
 constexpr int kCtaM = 128;                       // ... in each CTA of the pair
-enum Epilogue { kStore, kGate, kGrad, kRegrad };
+enum Epilogue { kStore, kGate, kGrad };
 // Epilogue warps: the element-wise epilogues are chains of special functions, shared and global accesses, which four
 // warps per scheduler hide better than two.
 template <int EPI> constexpr int kEpiWarps = EPI == kStore ? 8 : 16;
 template <int EPI> constexpr int kGemmThreads = (2 + kEpiWarps<EPI>) * 32;
 // 32 x 32 tiles of 16-bit elements (2 KB) that a warp stages between registers and memory
-template <int EPI> constexpr int kStaged = EPI == kStore ? 1 : EPI == kGrad ? 3 : 2;
+template <int EPI> constexpr int kStaged = EPI == kStore ? 1 : 2;
 template <int EPI> constexpr int kStagingBytes = kEpiWarps<EPI> * kStaged<EPI> * 2048;
 constexpr int kGroupM = 8;
 
 __device__ unsigned int g_ffn_timeouts = 0;
 
 struct Maps {
-    CUtensorMap a[2], b[2], c;     // c: kRegrad's Wd
-    CUtensorMap out[3];            // what kGate (H, G, U) and kGrad (H, dG, dU) write by TMA
+    CUtensorMap a[2], b[2], c;     // c: kGrad's Wd
+    CUtensorMap out;               // H, which kGate writes by TMA
 };
 
 struct Plan {
@@ -75,13 +76,11 @@ struct Plan {
     int act;
     void* out[2];                  // kStore: D of product z.  kGate: H
     long long ldo;
-    void *gate, *up;               // kGate: written unless null.  kGrad: read
-    void *dgate, *dup, *hid;       // kGrad: written
-    long long ldh;                 // pitch of gate .. hid (a multiple of 8)
+    void *hid, *dgate, *dup;       // kGrad: written, pitch ldo
     float* partials;               // splits > 1: [splits][batch][mTiles * 256][nTiles * BN]
 };
 
-template <int EPI, int BN> constexpr int kStages = EPI == kGrad ? 4 : EPI != kStore ? 5 : BN == 256 ? 6 : 8;
+template <int EPI, int BN> constexpr int kStages = EPI != kStore ? 5 : BN == 256 ? 6 : 8;
 template <int BN> constexpr int kStageBytes = (kCtaM + BN / 2) * kStepK * 2;    // of one CTA
 template <int EPI, int BN> constexpr int kGemmSmem = 1024 + kStages<EPI, BN> * kStageBytes<BN> + kStagingBytes<EPI> + 256;
 
@@ -95,25 +94,9 @@ __device__ __forceinline__ void gate_chunk(const uint32_t (&g)[32], const uint32
         h[i] = pack2<T>(a0 * __uint_as_float(u[2 * i]), a1 * __uint_as_float(u[2 * i + 1]));
     }
 }
-// g and u are replaced by dG and dU
+// H, dG and dU of 16 columns
 template <typename T, int ACT>
-__device__ __forceinline__ void grad_chunk(const uint32_t (&dh)[32], uint32_t (&g)[16], uint32_t (&u)[16], uint32_t (&h)[16])
-{
-#pragma unroll
-    for (int i = 0; i < 16; ++i) {
-        const float2 gg = unpack2<T>(g[i]), uu = unpack2<T>(u[i]);
-        const float d0 = __uint_as_float(dh[2 * i]), d1 = __uint_as_float(dh[2 * i + 1]);
-        float a0, a1, s0, s1;
-        activate2<ACT, true>(gg.x, gg.y, a0, a1, s0, s1);
-        h[i] = pack2<T>(a0 * uu.x, a1 * uu.y);
-        u[i] = pack2<T>(d0 * a0, d1 * a1);
-        g[i] = pack2<T>(d0 * uu.x * s0, d1 * uu.y * s1);
-    }
-}
-
-// The same for 16 columns from fp32 G and U
-template <typename T, int ACT>
-__device__ __forceinline__ void regrad_chunk(const uint32_t (&dh)[16], const uint32_t (&g)[16], const uint32_t (&u)[16], uint32_t (&h)[8],
+__device__ __forceinline__ void grad_chunk(const uint32_t (&dh)[16], const uint32_t (&g)[16], const uint32_t (&u)[16], uint32_t (&h)[8],
                                              uint32_t (&dg)[8], uint32_t* du)
 {
 #pragma unroll
@@ -238,7 +221,7 @@ __global__ void __launch_bounds__(kGemmThreads<EPI>, 1) gemm_kernel(const __grid
                 const int kk = (k - seg * p.kIters) * kStepK;
                 const int which = p.segs > 1 ? seg : w.z;
                 const uint32_t a = smem + st * kStageBytes<BN>, b = a + kCtaM * kStepK * 2, bar = fullFirst + 8 * st;
-                if (lead && EPI == kRegrad) {    // segment 0: dY and 64 columns of Wd; segment 1: X and 128 rows of Wg or Wu
+                if (lead && EPI == kGrad) {    // segment 0: dY and 64 columns of Wd; segment 1: X and 128 rows of Wg or Wu
                     if (rank == 0)
                         mbar_expect_tx(full + 8 * st, seg == 0 ? 2 * (kCtaM + 64) * kStepK * 2 : 2 * kStageBytes<BN>);
                     tma_load_2d(a, &maps.a[seg], kk, row, bar);
@@ -282,9 +265,9 @@ __global__ void __launch_bounds__(kGemmThreads<EPI>, 1) gemm_kernel(const __grid
         for (int t = blockIdx.x >> 1; ok && t < tiles; t += gridDim.x >> 1, ++turn) {
             const Tile w = tile_at(t, p, mTiles);
             const int k0 = (int)((long long)kAll * w.s / p.splits), k1 = (int)((long long)kAll * (w.s + 1) / p.splits);
-            // kRegrad: G and U have columns 0 .. 255, dH 256 .. 383 or 384 .. 511 in turn, and one pair of barriers
-            const uint32_t acc = EPI == kRegrad ? 0 : turn & 1, d = EPI == kRegrad ? tmem + 256 + 128 * (turn & 1) : tmem + acc * BN;
-            if (EPI != kRegrad && turn > 1 && !mbar_wait_warp(accEmpty + 8 * acc, ((turn >> 1) - 1) & 1, abort, &g_ffn_timeouts))
+            // kGrad: G and U have columns 0 .. 255, dH 256 .. 383 or 384 .. 511 in turn, and one pair of barriers
+            const uint32_t acc = EPI == kGrad ? 0 : turn & 1, d = EPI == kGrad ? tmem + 256 + 128 * (turn & 1) : tmem + acc * BN;
+            if (EPI != kGrad && turn > 1 && !mbar_wait_warp(accEmpty + 8 * acc, ((turn >> 1) - 1) & 1, abort, &g_ffn_timeouts))
                 break;
             tc_fence_after();
             for (int k = k0; k < k1; ++k, ++used) {
@@ -295,7 +278,7 @@ __global__ void __launch_bounds__(kGemmThreads<EPI>, 1) gemm_kernel(const __grid
                 }
                 tc_fence_after();
                 const uint32_t a = smem + st * kStageBytes<BN>;
-                if constexpr (EPI == kRegrad) {
+                if constexpr (EPI == kGrad) {
                     // dH of the next tile is multiplied while the epilogue still reads G and U of this one
                     if (k == p.kIters) {
                         if (turn > 0 && !mbar_wait_warp(accEmpty, (turn - 1) & 1, abort, &g_ffn_timeouts)) {
@@ -346,13 +329,13 @@ __global__ void __launch_bounds__(kGemmThreads<EPI>, 1) gemm_kernel(const __grid
     } else if (warp >= 2) {
         // ---- epilogue: warp w may touch TMEM lanes 32 (w % 4) ..; W / 4 warps share each quarter and split its columns ----
         const int quarter = warp & 3, share = (warp - 2) >> 2;
-        const uint32_t buf0 = staging + (warp - 2) * (kStaged<EPI> * 2048), buf1 = buf0 + 2048, buf2 = buf0 + 4096;
+        const uint32_t buf0 = staging + (warp - 2) * (kStaged<EPI> * 2048), buf1 = buf0 + 2048;
         const uint32_t accEmptyFirst = in_first_cta(accEmpty);
         uint32_t turn = 0;
         for (int t = blockIdx.x >> 1; t < tiles; t += gridDim.x >> 1, ++turn) {
             const Tile w = tile_at(t, p, mTiles);
-            const uint32_t acc = EPI == kRegrad ? 0 : turn & 1, d = tmem + acc * BN + ((uint32_t)(quarter * 32) << 16);
-            if (!mbar_wait_warp(accFull + 8 * acc, (EPI == kRegrad ? turn : turn >> 1) & 1, abort, &g_ffn_timeouts))
+            const uint32_t acc = EPI == kGrad ? 0 : turn & 1, d = tmem + acc * BN + ((uint32_t)(quarter * 32) << 16);
+            if (!mbar_wait_warp(accFull + 8 * acc, (EPI == kGrad ? turn : turn >> 1) & 1, abort, &g_ffn_timeouts))
                 break;
             tc_fence_after();
             const long long row0 = (long long)w.m * kTileM + rank * kCtaM + quarter * 32;
@@ -394,29 +377,12 @@ __global__ void __launch_bounds__(kGemmThreads<EPI>, 1) gemm_kernel(const __grid
                     else
                         gate_chunk<T, kRelu>(g, u, h);
                     const int col = w.n * 128 + c;
-                    if (p.gate == nullptr) {    // the two buffers in turn
-                        const uint32_t buf = turn & 1 ? buf1 : buf0;
-                        wait_sent<1>(lane);
-                        stage_rows(buf, lane, h);
-                        send_tile(&maps.out[0], buf, col, (int)row0, lane);
-                        continue;
-                    }
-                    wait_sent<0>(lane);
-                    stage_rows(buf0, lane, h);
-                    send_tile(&maps.out[0], buf0, col, (int)row0, lane);
-#pragma unroll
-                    for (int i = 0; i < 16; ++i)
-                        h[i] = pack2<T>(__uint_as_float(g[2 * i]), __uint_as_float(g[2 * i + 1]));
-                    stage_rows(buf1, lane, h);
-                    send_tile(&maps.out[1], buf1, col, (int)row0, lane);
-#pragma unroll
-                    for (int i = 0; i < 16; ++i)
-                        h[i] = pack2<T>(__uint_as_float(u[2 * i]), __uint_as_float(u[2 * i + 1]));
+                    const uint32_t buf = turn & 1 ? buf1 : buf0;      // the two buffers in turn
                     wait_sent<1>(lane);
-                    stage_rows(buf0, lane, h);
-                    send_tile(&maps.out[2], buf0, col, (int)row0, lane);
+                    stage_rows(buf, lane, h);
+                    send_tile(&maps.out, buf, col, (int)row0, lane);
                 }
-            } else if (EPI == kRegrad) {     // one chunk of 32 columns a warp: TMEM is free again after three loads
+            } else if (EPI == kGrad) {     // one chunk of 32 columns a warp: TMEM is free again after three loads
                 const int c = share * 32;
                 uint32_t du[16];
 #pragma unroll
@@ -429,11 +395,11 @@ __global__ void __launch_bounds__(kGemmThreads<EPI>, 1) gemm_kernel(const __grid
                     if (i == 1)
                         release();
                     if (p.act == kSilu)
-                        regrad_chunk<T, kSilu>(dh, g, u, h, dg, du + 8 * i);
+                        grad_chunk<T, kSilu>(dh, g, u, h, dg, du + 8 * i);
                     else if (p.act == kGelu)
-                        regrad_chunk<T, kGelu>(dh, g, u, h, dg, du + 8 * i);
+                        grad_chunk<T, kGelu>(dh, g, u, h, dg, du + 8 * i);
                     else
-                        regrad_chunk<T, kRelu>(dh, g, u, h, dg, du + 8 * i);
+                        grad_chunk<T, kRelu>(dh, g, u, h, dg, du + 8 * i);
 #pragma unroll
                     for (int q = 0; q < 2; ++q) {
                         sts128(piece(buf0, lane, 2 * i + q), make_uint4(h[4 * q], h[4 * q + 1], h[4 * q + 2], h[4 * q + 3]));
@@ -441,7 +407,7 @@ __global__ void __launch_bounds__(kGemmThreads<EPI>, 1) gemm_kernel(const __grid
                     }
                 }
                 __syncwarp();
-                const Spot at = spot(p.ldh, row0, rowEnd, w.n * 128 + c, p.N, lane);
+                const Spot at = spot(p.ldo, row0, rowEnd, w.n * 128 + c, p.N, lane);
                 store_tile<T>(p.hid, at, true, buf0, lane);
                 store_tile<T>(p.dgate, at, true, buf1, lane);
                 __syncwarp();
@@ -449,36 +415,6 @@ __global__ void __launch_bounds__(kGemmThreads<EPI>, 1) gemm_kernel(const __grid
                 __syncwarp();
                 store_tile<T>(p.dup, at, true, buf0, lane);
                 __syncwarp();
-            } else if (EPI == kGrad) {
-#pragma unroll 1
-                for (int c = share * (BN * 4 / W); c < (share + 1) * (BN * 4 / W); c += 32) {
-                    const Spot at = spot(p.ldh, row0, rowEnd, w.n * BN + c, p.N, lane);
-                    const int col = w.n * BN + c;
-                    uint32_t dh[32], g[16], u[16], h[16];
-                    wait_sent<0>(lane);
-                    load_tile<T>(p.gate, at, buf0, lane);
-                    load_tile<T>(p.up, at, buf1, lane);
-                    tmem_load32(d + c, dh);
-                    tmem_wait_load();
-                    if (c + 32 == (share + 1) * (BN * 4 / W))
-                        release();
-                    __syncwarp();
-                    unstage_rows(buf0, lane, g);
-                    unstage_rows(buf1, lane, u);
-                    if (p.act == kSilu)
-                        grad_chunk<T, kSilu>(dh, g, u, h);
-                    else if (p.act == kGelu)
-                        grad_chunk<T, kGelu>(dh, g, u, h);
-                    else
-                        grad_chunk<T, kRelu>(dh, g, u, h);
-                    __syncwarp();
-                    stage_rows(buf1, lane, g);
-                    send_tile(&maps.out[1], buf1, col, (int)row0, lane);
-                    stage_rows(buf0, lane, u);
-                    send_tile(&maps.out[2], buf0, col, (int)row0, lane);
-                    stage_rows(buf2, lane, h);
-                    send_tile(&maps.out[0], buf2, col, (int)row0, lane);
-                }
             } else {
                 T* out = static_cast<T*>(p.out[w.z]);
                 const bool wide = ((p.ldo & 7) == 0) && (reinterpret_cast<uintptr_t>(out) & 15) == 0;
@@ -499,7 +435,7 @@ __global__ void __launch_bounds__(kGemmThreads<EPI>, 1) gemm_kernel(const __grid
                 }
             }
         }
-        if ((EPI == kGate || EPI == kGrad) && lane == 0)
+        if (EPI == kGate && lane == 0)
             bulk_wait_all();     // shared memory is read until then
     }
     // every role's waits are bounded, so both CTAs get here; neither frees TMEM or leaves while the other may still
@@ -557,10 +493,6 @@ template <typename T, int EPI> __global__ void __launch_bounds__(256) finish_ker
             auto gated = [&](float a, float b) { return activate_any(p.act, a) * b; };
             h.x = gated(g.x, u.x), h.y = gated(g.y, u.y), h.z = gated(g.z, u.z), h.w = gated(g.w, u.w);
             store4<T>(out + row * p.ldo + col, h, n, wide);
-            if (p.gate != nullptr) {
-                store4<T>(static_cast<T*>(p.gate) + row * p.ldh + col, g, n, true);
-                store4<T>(static_cast<T*>(p.up) + row * p.ldh + col, u, n, true);
-            }
         } else {
             const float4 v = sum_pieces(p.partials + z * plane + row * pitch + col, p.batch * plane, p.splits);
             store4<T>(out + row * p.ldo + col, v, n, wide);
@@ -644,22 +576,9 @@ cudaError_t launch_maps(const Maps& maps, Plan& p, cudaStream_t stream)
     if (p.splits == 1)
         return cudaSuccess;
     const dim3 fgrid((unsigned)ceil_div(p.N, 128), (unsigned)std::min<long long>((p.M + 7) / 8, 65535), (unsigned)p.batch);
-    if constexpr (EPI == kStore || EPI == kGate)
+    if constexpr (EPI != kGrad)
         return launch_pdl(finish_kernel<T, EPI>, fgrid, dim3(32, 8), 0, stream, p, BN);
     return cudaErrorInvalidValue;
-}
-
-// The scratch matrices that the epilogue writes by TMA (none where the reduction is split).
-template <int EPI> cudaError_t encode_outputs(const Plan& p, Maps* maps)
-{
-    if ((EPI != kGate && EPI != kGrad) || p.splits > 1)
-        return cudaSuccess;
-    const void* m[3] = {EPI == kGate ? p.out[0] : p.hid, EPI == kGate ? p.gate : p.dgate, EPI == kGate ? p.up : p.dup};
-    for (int i = 0; i < 3; ++i)
-        if (m[i] != nullptr)
-            if (cudaError_t e = encode({m[i], p.M, p.N, p.ldh}, 32, &maps->out[i], 32))
-                return e;
-    return cudaSuccess;
 }
 
 template <typename T, bool A_MN, bool B_MN, int EPI, int BN>
@@ -680,14 +599,15 @@ cudaError_t launch_gemm(const Matrix (&a)[2], const Matrix (&b)[2], Plan& p, cud
         maps.a[1] = maps.a[0];
     if (n == 1 && EPI != kGate)
         maps.b[1] = maps.b[0];
-    if (cudaError_t e = encode_outputs<EPI>(p, &maps))
-        return e;
+    if (EPI == kGate && p.splits == 1)
+        if (cudaError_t e = encode({p.out[0], p.M, p.N, p.ldo}, 32, &maps.out, 32))
+            return e;
     return launch_maps<T, A_MN, B_MN, EPI, BN>(maps, p, stream);
 }
 
-// Hidden gradients with G and U multiplied again.
+// Hidden gradients.
 template <typename T>
-cudaError_t launch_regrad(const Matrix& dy, const Matrix& x, const Matrix& wd, const Matrix& wg, const Matrix& wu, Plan& p, cudaStream_t stream)
+cudaError_t launch_grad(const Matrix& dy, const Matrix& x, const Matrix& wd, const Matrix& wg, const Matrix& wu, Plan& p, cudaStream_t stream)
 {
     Maps maps;
     if (cudaError_t e = encode(dy, kCtaM, &maps.a[0]))
@@ -700,7 +620,7 @@ cudaError_t launch_regrad(const Matrix& dy, const Matrix& x, const Matrix& wd, c
         return e;
     if (cudaError_t e = encode(wd, kStepK, &maps.c))
         return e;
-    return launch_maps<T, false, false, kRegrad, 256>(maps, p, stream);
+    return launch_maps<T, false, false, kGrad, 256>(maps, p, stream);
 }
 
 // A plain product D[m,n] of one or two products (batch) or segments.
@@ -814,7 +734,7 @@ template <typename T> cudaError_t forward(const FfnArgs& f, Layout& l, bool run,
     p.mTiles = ceil_div(R, kTileM), p.nTiles = ceil_div(F, 128), p.batch = 1, p.segs = 1, p.kIters = ceil_div(C, kStepK);
     p.splits = split_count(R, 2ll * F, (long long)p.mTiles * p.nTiles, p.kIters);
     p.N = F, p.M = R, p.num_blocks_dev = f.num_blocks_dev, p.rowsPerBlock = f.rowsPerBlock, p.act = f.act;
-    p.out[0] = const_cast<void*>(h.ptr), p.ldo = Fp /* = ldh */, p.gate = f.gate, p.up = f.up, p.ldh = Fp, p.partials = parts;
+    p.out[0] = const_cast<void*>(h.ptr), p.ldo = Fp, p.partials = parts;
     SBNET_TRY((launch_gemm<T, false, false, kGate, 256>({x, x}, {wg, wu}, p, stream)));
     note_site("gated_ffn output");
     return product<T, false, false>({h, h}, {wd, wd}, 1, 1, R, C, F, f.y, nullptr, parts, f, true, stream);
@@ -838,16 +758,10 @@ template <typename T> cudaError_t backward(const FfnArgs& f, Layout& l, bool run
     SBNET_TRY(copies.run(stream));
     note_site("gated_ffn_grad hidden gradients");
     Plan p = {};
-    p.mTiles = ceil_div(R, kTileM), p.nTiles = ceil_div(F, 256), p.batch = 1, p.segs = 1, p.kIters = ceil_div(C, kStepK);
+    p.mTiles = ceil_div(R, kTileM), p.nTiles = ceil_div(F, 128), p.batch = 1, p.segs = 2, p.kIters = ceil_div(C, kStepK);
     p.splits = 1, p.N = F, p.M = R, p.act = f.act;
-    p.gate = f.gate, p.up = f.up, p.ldh = Fp;
-    p.dgate = const_cast<void*>(dg.ptr), p.dup = const_cast<void*>(du.ptr), p.hid = const_cast<void*>(h.ptr);
-    if (f.gate != nullptr) {
-        SBNET_TRY((launch_gemm<T, false, true, kGrad, 256>({dy, dy}, {wd, wd}, p, stream)));
-    } else {
-        p.nTiles = ceil_div(F, 128), p.segs = 2;
-        SBNET_TRY(launch_regrad<T>(dy, x, wd, wg, wu, p, stream));
-    }
+    p.hid = const_cast<void*>(h.ptr), p.dgate = const_cast<void*>(dg.ptr), p.dup = const_cast<void*>(du.ptr), p.ldo = Fp;
+    SBNET_TRY(launch_grad<T>(dy, x, wd, wg, wu, p, stream));
     if (f.dx != nullptr) {
         note_site("gated_ffn_grad dx");
         SBNET_TRY((product<T, false, true>({dg, du}, {wg, wu}, 1, 2, R, C, F, f.dx, nullptr, parts, f, false, stream)));

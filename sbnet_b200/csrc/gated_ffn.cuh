@@ -107,7 +107,7 @@ __device__ __forceinline__ long long live_rows(long long rows, const int32_t* bl
 // ---- 32 x 32 tiles of 16-bit elements between registers (one row per lane) and memory -----------------------
 // Staged through 2 KB of shared memory so that global accesses are 64 contiguous bytes per row.  16-byte pieces
 // are swizzled by row as TMA's 64-byte mode does it: eight lanes touch eight different pieces of 128 bytes whichever
-// way the tile is walked, and two of the epilogues send their tiles by TMA straight from here.
+// way the tile is walked, and one of the epilogues sends its tiles by TMA straight from here.
 __device__ __forceinline__ uint32_t piece(uint32_t buf, int row, int c) { return buf + row * 64 + ((c ^ ((row >> 1) & 3)) << 4); }
 
 __device__ __forceinline__ void stage_rows(uint32_t buf, int lane, const uint32_t (&w)[16])
@@ -115,14 +115,6 @@ __device__ __forceinline__ void stage_rows(uint32_t buf, int lane, const uint32_
 #pragma unroll
     for (int c = 0; c < 4; ++c)
         sts128(piece(buf, lane, c), make_uint4(w[4 * c], w[4 * c + 1], w[4 * c + 2], w[4 * c + 3]));
-}
-__device__ __forceinline__ void unstage_rows(uint32_t buf, int lane, uint32_t (&w)[16])
-{
-#pragma unroll
-    for (int c = 0; c < 4; ++c) {
-        const uint4 v = lds128(piece(buf, lane, c));
-        w[4 * c] = v.x, w[4 * c + 1] = v.y, w[4 * c + 2] = v.z, w[4 * c + 3] = v.w;
-    }
 }
 // Where a lane's pieces of a tile lie in a matrix of pitch ld: rows r, r + 8, .. r + 24 (r = lane / 4) of row0.., of which
 // the first `rows` pieces are below rowEnd, and columns col.., of which `cols` are below N.
@@ -156,19 +148,6 @@ template <typename T> __device__ __forceinline__ void store_tile(void* out, cons
         }
     }
 }
-// memory -> tile, from a matrix whose pitch is a multiple of 8 elements and covers the piece that holds column N - 1
-template <typename T> __device__ __forceinline__ void load_tile(const void* in, const Spot& s, uint32_t buf, int lane)
-{
-    const T* src = static_cast<const T*>(in) + s.at;
-#pragma unroll
-    for (int i = 0; i < 4; ++i, src += s.step) {
-        uint4 v = make_uint4(0, 0, 0, 0);
-        if (i < s.rows && s.cols > 0)
-            v = *reinterpret_cast<const uint4*>(src);
-        sts128(piece(buf, i * 8 + (lane >> 2), lane & 3), v);
-    }
-}
-
 // ---- host side ----
 inline PFN_cuTensorMapEncodeTiled encoder()
 {

@@ -33,7 +33,6 @@ constexpr int kSmemLimit = 224 * 1024, kSmemHalf = 110 * 1024;     // of a CTA t
 struct FewArgs {
     const void *x, *w0, *w1;         // X [M, K]; the group's first and second 8 weight rows
     void* out;                       // [M, N]
-    void *gate, *up;                 // gate kernel: [M, N] each, or nullptr
     const int32_t* num_blocks_dev;
     long long M;
     int rowsPerBlock, K, N, act;
@@ -145,8 +144,6 @@ template <typename T, int MT, bool GATE> __global__ void __launch_bounds__(kThre
         if (GATE) {
             const long long at = (long long)tok * p.N + group * 8 + r;
             static_cast<T*>(p.out)[at] = T(activate_any(p.act, s0) * s1);
-            if (p.gate != nullptr)
-                static_cast<T*>(p.gate)[at] = T(s0), static_cast<T*>(p.up)[at] = T(s1);
         } else {
             const int col = group * 16 + r;
             T* y = static_cast<T*>(p.out) + (long long)tok * p.N + col;
@@ -327,7 +324,7 @@ template <typename T, int MT, bool GATE> cudaError_t run(FewArgs& a, cudaStream_
 template <typename T, int MT> cudaError_t both(const FfnArgs& f, void* h, cudaStream_t stream, bool* taken)
 {
     FewArgs gate = {}, out = {};
-    gate.x = f.x, gate.w0 = f.w_gate, gate.w1 = f.w_up, gate.out = h, gate.gate = f.gate, gate.up = f.up;
+    gate.x = f.x, gate.w0 = f.w_gate, gate.w1 = f.w_up, gate.out = h;
     gate.K = f.C, gate.N = f.F, gate.act = f.act;
     out.x = h, out.w0 = out.w1 = f.w_down, out.out = f.y, out.K = f.F, out.N = f.C;
     gate.M = out.M = f.rows;

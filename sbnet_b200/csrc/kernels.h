@@ -58,8 +58,6 @@ struct FfnArgs {
     const void* x;                             // [rows, C]
     const void *w_gate, *w_up, *w_down;        // [F, C], [F, C], [C, F]
     void* y;                                   // forward: [rows, C]
-    void *gate, *up;                           // [rows, F rounded up to 8]: forward writes them unless null, backward reads
-                                               // them, or multiplies them again where they are null
     const void* dy;                            // backward: [rows, C]
     void *dx, *dw_gate, *dw_up, *dw_down;      // backward: written unless null (dw_gate and dw_up go together)
     const int32_t* num_blocks_dev;             // forward: live blocks of rowsPerBlock rows, or nullptr (all rows)

@@ -519,7 +519,7 @@ def _workspace(rows, channels, hidden, grad, tensors, device):
     return torch.empty(need, dtype=torch.uint8, device=device), need
 
 
-def _gated_ffn_call(x, w_gate, w_up, w_down, activation, out, train, count_dev):
+def _gated_ffn_call(x, w_gate, w_up, w_down, activation, out, count_dev):
     rows, channels, hidden, act = _check_ffn(x, w_gate, w_up, w_down, activation)
     if count_dev is not None:
         _check_count_dev(count_dev, x)
@@ -529,19 +529,15 @@ def _gated_ffn_call(x, w_gate, w_up, w_down, activation, out, train, count_dev):
     _require_cuda(x, "x")
     with _on(x.device):
         y = torch.empty_like(x) if out is None else out
-        gate = up = None
-        if train:
-            both = torch.empty((2, rows, (hidden + 7) // 8 * 8), dtype=x.dtype, device=x.device)
-            gate, up = both[0], both[1]
         ws, need = _workspace(rows, channels, hidden, 0, (x, w_gate, w_up, w_down), x.device)
         head = (channels, hidden, w_gate.data_ptr(), w_up.data_ptr(), w_down.data_ptr(), act, y.data_ptr())
         tail = (ws.data_ptr(), need, _stream(x.device))
         if count_dev is None:
-            _lib.check(_lib.load().sbnet_gated_ffn(x.data_ptr(), _DTYPES[x.dtype], rows, *head, _ptr(gate), _ptr(up), *tail))
+            _lib.check(_lib.load().sbnet_gated_ffn(x.data_ptr(), _DTYPES[x.dtype], rows, *head, *tail))
         else:
             _lib.check(_lib.load().sbnet_gated_ffn_dyn(x.data_ptr(), _DTYPES[x.dtype], blocks, per, count_dev.data_ptr(),
                                                        *head, *tail))
-    return (y, gate, up) if train else y
+    return y
 
 
 def gated_ffn(x: torch.Tensor, w_gate: torch.Tensor, w_up: torch.Tensor, w_down: torch.Tensor, activation: str = "silu",
@@ -550,7 +546,7 @@ def gated_ffn(x: torch.Tensor, w_gate: torch.Tensor, w_up: torch.Tensor, w_down:
     ``(act(x @ w_gate.T) * (x @ w_up.T)) @ w_down.T`` with ``w_gate``, ``w_up`` ``[F, C]`` and ``w_down``
     ``[C, F]`` of the same type; ``activation``: "silu", "gelu" (by the error function) or "relu".  Sums are fp32,
     the gated product is rounded to the type of ``x`` once.  ``out`` must not overlap an input."""
-    return _gated_ffn_call(x, w_gate, w_up, w_down, activation, out, False, None)
+    return _gated_ffn_call(x, w_gate, w_up, w_down, activation, out, None)
 
 
 def gated_ffn_dyn(x: torch.Tensor, count_dev: torch.Tensor, w_gate, w_up, w_down, activation: str = "silu", out=None):
@@ -558,27 +554,15 @@ def gated_ffn_dyn(x: torch.Tensor, count_dev: torch.Tensor, w_gate, w_up, w_down
     the device; the rest of the result (of ``out``) is left as it was."""
     if count_dev is None:
         raise ValueError("count_dev must be an int32 tensor with at least one element")
-    return _gated_ffn_call(x, w_gate, w_up, w_down, activation, out, False, count_dev)
+    return _gated_ffn_call(x, w_gate, w_up, w_down, activation, out, count_dev)
 
 
-def gated_ffn_train(x: torch.Tensor, w_gate, w_up, w_down, activation: str = "silu"):
-    """:func:`gated_ffn` that also returns what :func:`gated_ffn_grad` needs: ``(y, gate, up)``, the two
-    projections as ``[rows, F rounded up to a multiple of 8]`` (columns past F are undefined)."""
-    return _gated_ffn_call(x, w_gate, w_up, w_down, activation, None, True, None)
-
-
-def gated_ffn_grad(grad: torch.Tensor, x: torch.Tensor, gate: torch.Tensor, up: torch.Tensor, w_gate, w_up, w_down,
-                   activation: str = "silu", need_x: bool = True, need_gate_up: bool = True, need_down: bool = True):
-    """Backward pass of :func:`gated_ffn_train` -- or of :func:`gated_ffn`, with ``gate`` and ``up`` None: they are then
-    multiplied again.  Returns ``(dx, dw_gate, dw_up, dw_down)``, None where not asked for."""
+def gated_ffn_grad(grad: torch.Tensor, x: torch.Tensor, w_gate, w_up, w_down, activation: str = "silu",
+                   need_x: bool = True, need_gate_up: bool = True, need_down: bool = True):
+    """Backward pass of :func:`gated_ffn` from its inputs and the gradient of its result (the projections are
+    multiplied again): ``(dx, dw_gate, dw_up, dw_down)``, None where not asked for."""
     rows, channels, hidden, act = _check_ffn(x, w_gate, w_up, w_down, activation)
     _check_like(grad, "grad", x)
-    if (gate is None) != (up is None):
-        raise ValueError("gate and up go together")
-    for t, name in ((gate, "gate"), (up, "up")):
-        if t is not None and (tuple(t.shape) != (rows, (hidden + 7) // 8 * 8) or t.dtype != x.dtype or
-                              t.device != x.device or not t.is_contiguous()):
-            raise ValueError(f"{name} must be what gated_ffn_train returned")
     _require_cuda(x, "x")
     with _on(x.device):
         dx = torch.empty_like(x) if need_x else None
@@ -587,7 +571,7 @@ def gated_ffn_grad(grad: torch.Tensor, x: torch.Tensor, gate: torch.Tensor, up: 
         dwd = torch.empty_like(w_down) if need_down else None
         ws, need = _workspace(rows, channels, hidden, 1, (grad, x, w_gate, w_up, w_down), x.device)
         _lib.check(_lib.load().sbnet_gated_ffn_grad(
-            grad.data_ptr(), x.data_ptr(), _ptr(gate), _ptr(up), _DTYPES[x.dtype], rows, channels, hidden,
+            grad.data_ptr(), x.data_ptr(), _DTYPES[x.dtype], rows, channels, hidden,
             w_gate.data_ptr(), w_up.data_ptr(), w_down.data_ptr(), act, _ptr(dx), _ptr(dwg), _ptr(dwu), _ptr(dwd),
             ws.data_ptr(), need, _stream(x.device)))
     return dx, dwg, dwu, dwd

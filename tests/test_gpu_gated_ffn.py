@@ -2,13 +2,13 @@
 
 Tolerances are carried through the formula.  With u half a step of the element type (relative), every element
 that is rounded to that type is off by u of itself: the output, h (the last product's operand), and in the
-backward pass g and u as they were saved, dG, dU and h.  A sum of K products on the tensor cores is off by
+backward pass dG, dU and h.  A sum of K products on the tensor cores is off by
 2^-23 for each of its K/16 instructions and a few more (16), times the sum of the products' magnitudes; the
 element-wise steps are off by 2^-19 of their magnitude (the error bound of the fast exponential at |g| <= 16).
 Each of these is multiplied with what it meets on its way to the output.  The bounds add magnitudes, so they
 are far from what random errors add up to; the second check is on the norm of the error: independent rounding
 errors of at most u (variance u^2/3) at the output and at each operand give at most sqrt(2/3) u for y and
-sqrt(6/3) u for the gradients on random data; 2u and 3u are allowed."""
+the gradients on random data; 1.5u is allowed."""
 import math
 
 import pytest
@@ -61,9 +61,7 @@ def _expected(act, x, wg, wu, wd, dy=None):
     dh = dy @ wd
     edh = chain(c) * (dy.abs() @ wd.abs())
     du, dg = dh * a, dh * up * s
-    eg, eu = eg + u * g.abs() + tiny, eu + u * up.abs() + tiny                   # as saved
     es = (g.abs() <= eg).double() if act == "relu" else 0.8 * eg + 2.0 ** -19
-    eh = u * h.abs() + 1.13 * eg * up.abs() + a.abs() * eu + ea * up.abs() + tiny
     edu = u * du.abs() + edh * a.abs() + dh.abs() * (1.13 * eg + ea) + tiny
     edg = u * dg.abs() + edh * (up * s).abs() + dh.abs() * s.abs() * eu + (dh * up).abs() * es + tiny
     dx = dg @ wg + du @ wu
@@ -84,12 +82,11 @@ def _check(got, exp, name, dtype, norm=True):
     assert (err <= tol).all(), (name, float((err - tol).max()), float(err.max()))
     if norm and ref.numel() >= 1000:
         u = torch.finfo(dtype).eps / 2
-        assert float(err.norm() / ref.norm()) <= (2 if name == "y" else 3) * u, (name, float(err.norm() / ref.norm()) / u)
+        assert float(err.norm() / ref.norm()) <= 1.5 * u, (name, float(err.norm() / ref.norm()) / u)
 
 
 def _run(act, x, wg, wu, wd, dy):
-    y, gate, up = ops.gated_ffn_train(x, wg, wu, wd, act)
-    return dict(zip(NAMES, (y, *ops.gated_ffn_grad(dy, x, gate, up, wg, wu, wd, act))))
+    return dict(zip(NAMES, (ops.gated_ffn(x, wg, wu, wd, act), *ops.gated_ffn_grad(dy, x, wg, wu, wd, act))))
 
 
 # rows x C x F: below, at and above tile borders; sizes off 8 (rows that TMA cannot address) in every position; one
@@ -114,21 +111,6 @@ def test_forward_and_backward(cuda_ops, dtype, size):
     assert lib.wait_timeouts() == 0
 
 
-@pytest.mark.parametrize("size", SIZES, ids=str)
-@pytest.mark.parametrize("dtype", [torch.float16, torch.bfloat16])
-def test_backward_that_multiplies_the_projections_again(cuda_ops, dtype, size):
-    """The same bounds hold without the saved projections' rounding."""
-    act = ("silu", "gelu", "relu")[sum(size) % 3]
-    x, wg, wu, wd, dy = _inputs(*size, dtype, seed=sum(size) + 1)
-    exp = _expected(act, x, wg, wu, wd, dy)
-    got = ops.gated_ffn_grad(dy, x, None, None, wg, wu, wd, act)
-    for n, v in zip(NAMES[1:], got):
-        _check(v, exp, n, dtype)
-    again = ops.gated_ffn_grad(dy, x, None, None, wg, wu, wd, act)
-    assert all(torch.equal(a, b) for a, b in zip(got, again))
-    assert lib.wait_timeouts() == 0
-
-
 @pytest.mark.parametrize("act", ["silu", "gelu", "relu"])
 @pytest.mark.parametrize("dtype", [torch.float16, torch.bfloat16])
 @pytest.mark.parametrize("rows", [4, 40, 260])
@@ -140,11 +122,8 @@ def test_activations_over_their_range(cuda_ops, act, dtype, rows):
     exp = _expected(act, x, wg, wu, wd, dy)
     _check(ops.gated_ffn(x, wg, wu, wd, act), exp, "y", dtype, norm=False)
     got = _run(act, x, wg, wu, wd, dy)
-    got.update(zip(("dx2", "dwg2", "dwu2", "dwd2"), ops.gated_ffn_grad(dy, x, None, None, wg, wu, wd, act)))
     for n in NAMES:
         _check(got[n], exp, n, dtype, norm=False)
-    for n, again in zip(NAMES[1:], ("dx2", "dwg2", "dwu2", "dwd2")):
-        _check(got[again], exp, n, dtype, norm=False)
 
 
 @pytest.mark.parametrize("rows", [1, 2, 3, 4, 5, 8, 9, 16, 17, 31, 32, 33, 48, 64, 65, 96, 128])
@@ -238,10 +217,9 @@ def test_rows_that_are_not_finite_stay_alone(cuda_ops):
 
 def test_asked_for_gradients_only(cuda_ops):
     x, wg, wu, wd, dy = _inputs(260, 72, 136, torch.bfloat16)
-    y, gate, up = ops.gated_ffn_train(x, wg, wu, wd)
-    full = ops.gated_ffn_grad(dy, x, gate, up, wg, wu, wd)
+    full = ops.gated_ffn_grad(dy, x, wg, wu, wd)
     for need in ((True, False, False), (False, True, False), (False, False, True), (False, False, False)):
-        part = ops.gated_ffn_grad(dy, x, gate, up, wg, wu, wd, "silu", *need)
+        part = ops.gated_ffn_grad(dy, x, wg, wu, wd, "silu", *need)
         for got, want, asked in zip(part, full, (need[0], need[1], need[1], need[2])):
             assert (got is None) == (not asked) and (got is None or torch.equal(got, want))
 

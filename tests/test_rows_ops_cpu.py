@@ -104,7 +104,7 @@ def test_gated_ffn_rules():
                      ((x, wg, wu, wd.t().contiguous()), "w_down"), ((x, wg.float(), wu, wd), "w_gate"),
                      ((x, wg, wu.bfloat16(), wd), "w_up"), ((x, wg.t().contiguous().t(), wu, wd), "w_gate"),
                      ((x.t(), wg, wu, wd), "contiguous"), ((x, wg[:0], wu[:0], wd[:, :0].contiguous()), "w_gate")]:
-        for call in (ops.gated_ffn, ops.gated_ffn_train):
+        for call in (ops.gated_ffn, lambda *a: ops.gated_ffn_grad(a[0], *a)):
             with pytest.raises(ValueError, match=why):
                 call(*bad)
     with pytest.raises(ValueError, match="out"):
@@ -113,13 +113,10 @@ def test_gated_ffn_rules():
         ops.gated_ffn_dyn(x, None, wg, wu, wd)
     with pytest.raises(ValueError, match="int32"):
         ops.gated_ffn_dyn(x, torch.zeros(1), wg, wu, wd)
-    gate = torch.zeros(4, 16, dtype=torch.float16)
     with pytest.raises(ValueError, match="grad"):
-        ops.gated_ffn_grad(x[:3], x, gate, gate, wg, wu, wd)
-    with pytest.raises(ValueError, match="gate"):
-        ops.gated_ffn_grad(x, x, gate[:, :15], gate, wg, wu, wd)
-    with pytest.raises(ValueError, match="up"):
-        ops.gated_ffn_grad(x, x, gate, gate.float(), wg, wu, wd)
+        ops.gated_ffn_grad(x[:3], x, wg, wu, wd)
+    with pytest.raises(ValueError, match="CUDA"):
+        ops.gated_ffn_grad(x, x, wg, wu, wd)
 
 
 def test_gated_ffn_c_entries_refuse(handle):
@@ -130,11 +127,10 @@ def test_gated_ffn_c_entries_refuse(handle):
     assert handle.sbnet_gated_ffn_workspace(4, 8, 16, 0, 0) > need
     assert handle.sbnet_gated_ffn_workspace(0, 8, 16, 0, 1) == 0
 
-    def call(x=x, dtype=1, rows=4, c=8, f=16, wg=w, wu=w, wd=w, act=0, y=y, gate=None, up=None, ws=ws, n=need):
-        return ffn(x, dtype, rows, c, f, wg, wu, wd, act, y, gate, up, ws, n, None)
+    def call(x=x, dtype=1, rows=4, c=8, f=16, wg=w, wu=w, wd=w, act=0, y=y, ws=ws, n=need):
+        return ffn(x, dtype, rows, c, f, wg, wu, wd, act, y, ws, n, None)
     for bad in (dict(dtype=0), dict(dtype=7), dict(rows=-1), dict(c=0), dict(f=0), dict(act=3), dict(act=-1), dict(x=None),
-                dict(y=None), dict(wd=None), dict(gate=1 << 29), dict(up=1 << 29), dict(gate=(1 << 29) + 2, up=1 << 29),
-                dict(x=x + 1), dict(y=y + 1), dict(y=x + 32), dict(y=w), dict(ws=None), dict(ws=ws + 16), dict(n=need - 1)):
+                dict(y=None), dict(wd=None), dict(x=x + 1), dict(y=y + 1), dict(y=x + 32), dict(y=w), dict(ws=None), dict(ws=ws + 16), dict(n=need - 1)):
         assert call(**bad) == BAD, bad
         assert handle.sbnet_last_error()
     assert call(rows=1 << 31) == -2 and call(c=1 << 25) == -2 and call(f=1 << 25) == -2
@@ -144,12 +140,11 @@ def test_gated_ffn_c_entries_refuse(handle):
     assert dyn(x, 1, 4, 0, ws, 8, 16, w, w, w, 0, y, ws, 1 << 20, None) == BAD
     assert dyn(x, 1, -1, 2, ws, 8, 16, w, w, w, 0, y, ws, 1 << 20, None) == BAD
 
-    g = 1 << 29
     gneed = handle.sbnet_gated_ffn_workspace(4, 8, 16, 1, 1)
 
-    def back(dy=x, x=x, gate=g, up=g, dtype=1, rows=4, wd=w, act=0, dx=y, dwg=None, dwu=None, dwd=None, ws=ws, n=gneed):
-        return grad(dy, x, gate, up, dtype, rows, 8, 16, w, w, wd, act, dx, dwg, dwu, dwd, ws, n, None)
-    for bad in (dict(dtype=0), dict(act=5), dict(dy=None), dict(gate=None), dict(up=None), dict(gate=g + 2), dict(dwg=y + 4096),
-                dict(dwu=y + 4096), dict(dx=y + 1), dict(dx=x), dict(dx=g), dict(dwd=w), dict(ws=None), dict(n=gneed - 1),
+    def back(dy=x, x=x, dtype=1, rows=4, wd=w, act=0, dx=y, dwg=None, dwu=None, dwd=None, ws=ws, n=gneed):
+        return grad(dy, x, dtype, rows, 8, 16, w, w, wd, act, dx, dwg, dwu, dwd, ws, n, None)
+    for bad in (dict(dtype=0), dict(act=5), dict(dy=None), dict(dwg=y + 4096),
+                dict(dwu=y + 4096), dict(dx=y + 1), dict(dx=x), dict(dwd=w), dict(ws=None), dict(n=gneed - 1),
                 dict(wd=None), dict(x=x + 1)):
         assert back(**bad) == BAD, bad
