@@ -12,6 +12,10 @@ Two differences from the reference, both deliberate: the scatter gradient passes
 the gather (the reference drops it, so its gradient has the wrong layout for transposed stacks), and
 the stamp-out for ``add=False`` overwrites the scattered pixels of a copy of ``grad`` with zeros
 directly instead of building a ones/zeros mask and multiplying.
+``layer_norm`` and ``gated_ffn`` (the per-position operators of ``ops``) are differentiable once.  Their backward
+passes can be captured in a CUDA graph like any other; torch's own rule applies, that no eager autograd graph of
+the same leaves is alive then (it ties their gradients to the stream it was built on).
+
 All heavy lifting happens in the CUDA library; nothing here computes on tensors itself except
 allocating the zero base.
 """
