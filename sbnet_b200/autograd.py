@@ -86,16 +86,19 @@ def sparse_scatter(x, bin_counts, active_block_indices, ybase, dynamic_bsize, dy
 class _LayerNorm(torch.autograd.Function):
     @staticmethod
     def forward(ctx, x, weight, bias, eps):
-        y, mean, rstd = ops.layer_norm(x, weight, bias, eps, stats=True)
-        ctx.save_for_backward(x, weight, bias, mean, rstd)
+        y, stats = ops.layer_norm(x, weight, bias, eps, stats=True)
+        ctx.save_for_backward(x, weight, bias, stats)
         return y
 
     @staticmethod
     @once_differentiable
     def backward(ctx, grad):
-        x, weight, bias, mean, rstd = ctx.saved_tensors
-        gx, gw, gb = ops.layer_norm_grad(grad.contiguous(), x, mean, rstd, weight, bias,
-                                         sums=ctx.needs_input_grad[1] or ctx.needs_input_grad[2])
+        x, weight, bias, stats = ctx.saved_tensors
+        need = ctx.needs_input_grad
+        param = weight if weight is not None else bias
+        wdtype = ops._DTYPES[x.dtype if param is None else param.dtype]
+        gx, gw, gb = ops._layer_norm_grad_call(grad.contiguous(), x, stats, weight, bias, stats.shape[1], x.shape[-1],
+                                               wdtype, need[1] or need[2])
         return gx, gw, gb, None
 
 
@@ -116,8 +119,10 @@ class _GatedFfn(torch.autograd.Function):
     def backward(ctx, grad):
         x, w_gate, w_up, w_down = ctx.saved_tensors
         need = ctx.needs_input_grad
-        return (*ops.gated_ffn_grad(grad.contiguous(), x, w_gate, w_up, w_down, ctx.activation,
-                                    need[0], need[1] or need[2], need[3]), None)
+        channels = x.shape[-1]
+        return (*ops._gated_ffn_grad_call(grad.contiguous(), x, w_gate, w_up, w_down, x.numel() // channels, channels,
+                                          w_gate.shape[0], ops._lib.SBNET_ACT[ctx.activation],
+                                          need[0], need[1] or need[2], need[3]), None)
 
 
 def gated_ffn(x, w_gate, w_up, w_down, activation="silu"):

@@ -432,27 +432,30 @@ def _layer_norm_call(x, weight, bias, eps, out, stats, count_dev):
     if out is not None:
         _check_like(out, "out", x)
     _require_cuda(x, "x")
-    with _on(x.device):
+    device = x.device
+    with _on(device):
         y = torch.empty_like(x) if out is None else out
-        mean = rstd = None
+        both = mean = rstd = None
         if stats:
-            both = torch.empty((2, rows), dtype=torch.float32, device=x.device)
-            mean, rstd = both[0], both[1]
-        tail = (channels, _ptr(weight), _ptr(bias), wdtype, eps, y.data_ptr(), _ptr(mean), _ptr(rstd), _stream(x.device))
+            both = torch.empty((2, rows), dtype=torch.float32, device=device)
+            mean = both.data_ptr()
+            rstd = mean + 4 * rows
+        tail = (channels, _ptr(weight), _ptr(bias), wdtype, eps, y.data_ptr(), mean, rstd, _stream(device))
         if count_dev is None:
-            _lib.check(_lib.load().sbnet_layer_norm(x.data_ptr(), _DTYPES[x.dtype], rows, *tail))
+            rc = _lib.load().sbnet_layer_norm(x.data_ptr(), _DTYPES[x.dtype], rows, *tail)
         else:
-            _lib.check(_lib.load().sbnet_layer_norm_dyn(x.data_ptr(), _DTYPES[x.dtype], blocks, per,
-                                                        count_dev.data_ptr(), *tail))
-    return (y, mean, rstd) if stats else y
+            rc = _lib.load().sbnet_layer_norm_dyn(x.data_ptr(), _DTYPES[x.dtype], blocks, per, count_dev.data_ptr(), *tail)
+        _lib.check(rc)
+    return (y, both) if stats else y
 
 
 def layer_norm(x: torch.Tensor, weight=None, bias=None, eps: float = 1e-5, out=None, stats: bool = False):
     """Layer norm over the channels of every row of ``x`` (``[..., C]``):
     ``(x - mean) / sqrt(var + eps) * weight + bias``, statistics in fp32 over the biased variance.
 
-    ``weight`` / ``bias``: ``[C]`` of ``x``'s dtype or float32, or None.  ``stats=True`` also returns the
-    rows' fp32 ``mean`` and ``1 / sqrt(var + eps)`` for :func:`layer_norm_grad`.  ``out`` must not overlap ``x``."""
+    ``weight`` / ``bias``: ``[C]`` of ``x``'s dtype or float32, or None.  ``stats=True`` returns ``(y, stats)`` with the
+    rows' ``mean`` and ``1 / sqrt(var + eps)`` as a float32 ``[2, rows]`` tensor for :func:`layer_norm_grad`.
+    ``out`` must not overlap ``x``."""
     return _layer_norm_call(x, weight, bias, eps, out, stats, None)
 
 
@@ -464,30 +467,37 @@ def layer_norm_dyn(x: torch.Tensor, count_dev: torch.Tensor, weight=None, bias=N
     return _layer_norm_call(x, weight, bias, eps, out, False, count_dev)
 
 
-def layer_norm_grad(grad: torch.Tensor, x: torch.Tensor, mean: torch.Tensor, rstd: torch.Tensor, weight=None,
-                    bias=None, sums: bool = True):
+def _layer_norm_grad_call(grad, x, stats, weight, bias, rows, channels, wdtype, sums):
+    """The checked call (autograd's tensors come from a checked forward call)."""
+    device = x.device
+    with _on(device):
+        dx = torch.empty_like(x)
+        dw = db = ws = None
+        need = 0
+        lib = _lib.load()
+        if sums:
+            dw = None if weight is None else torch.empty_like(weight)
+            db = None if bias is None else torch.empty_like(bias)
+            if weight is not None or bias is not None:
+                need = lib.sbnet_layer_norm_grad_workspace(rows, channels)
+                ws = torch.empty(need, dtype=torch.uint8, device=device)
+        mean = stats.data_ptr()
+        _lib.check(lib.sbnet_layer_norm_grad(
+            grad.data_ptr(), x.data_ptr(), _DTYPES[x.dtype], rows, channels, _ptr(weight), wdtype, mean, mean + 4 * rows,
+            dx.data_ptr(), _ptr(dw), _ptr(db), _ptr(ws), need, _stream(device)))
+    return dx, dw, db
+
+
+def layer_norm_grad(grad: torch.Tensor, x: torch.Tensor, stats: torch.Tensor, weight=None, bias=None, sums: bool = True):
     """Backward pass of :func:`layer_norm`: ``(dx, dweight, dbias)``, the last two None where that parameter is
-    None or with ``sums=False``.  ``mean``, ``rstd``: what the forward call returned with ``stats=True``."""
+    None or with ``sums=False``.  ``stats``: what the forward call returned with ``stats=True``."""
     rows, channels = _check_rows(x, "x")
     _check_like(grad, "grad", x)
     wdtype = _check_norm_params(weight, bias, channels, x)
-    for t, name in ((mean, "mean"), (rstd, "rstd")):
-        if t.dtype != torch.float32 or t.numel() != rows or not t.is_contiguous() or t.device != x.device:
-            raise ValueError(f"{name} must be contiguous float32 with one element per row")
+    if stats.dtype != torch.float32 or tuple(stats.shape) != (2, rows) or not stats.is_contiguous() or stats.device != x.device:
+        raise ValueError(f"stats must be a contiguous float32 [2, {rows}] tensor on the device of the input")
     _require_cuda(x, "x")
-    with _on(x.device):
-        dx = torch.empty_like(x)
-        dw = torch.empty_like(weight) if sums and weight is not None else None
-        db = torch.empty_like(bias) if sums and bias is not None else None
-        lib = _lib.load()
-        need, ws = 0, None
-        if dw is not None or db is not None:
-            need = lib.sbnet_layer_norm_grad_workspace(rows, channels)
-            ws = torch.empty(need, dtype=torch.uint8, device=x.device)
-        _lib.check(lib.sbnet_layer_norm_grad(
-            grad.data_ptr(), x.data_ptr(), _DTYPES[x.dtype], rows, channels, _ptr(weight), wdtype, mean.data_ptr(),
-            rstd.data_ptr(), dx.data_ptr(), _ptr(dw), _ptr(db), _ptr(ws), need, _stream(x.device)))
-    return dx, dw, db
+    return _layer_norm_grad_call(grad, x, stats, weight, bias, rows, channels, wdtype, sums)
 
 
 def _check_ffn(x, w_gate, w_up, w_down, activation):
@@ -564,16 +574,22 @@ def gated_ffn_grad(grad: torch.Tensor, x: torch.Tensor, w_gate, w_up, w_down, ac
     rows, channels, hidden, act = _check_ffn(x, w_gate, w_up, w_down, activation)
     _check_like(grad, "grad", x)
     _require_cuda(x, "x")
-    with _on(x.device):
+    return _gated_ffn_grad_call(grad, x, w_gate, w_up, w_down, rows, channels, hidden, act, need_x, need_gate_up, need_down)
+
+
+def _gated_ffn_grad_call(grad, x, w_gate, w_up, w_down, rows, channels, hidden, act, need_x, need_gate_up, need_down):
+    """The checked call (autograd's tensors come from a checked forward call)."""
+    device = x.device
+    with _on(device):
         dx = torch.empty_like(x) if need_x else None
         dwg = torch.empty_like(w_gate) if need_gate_up else None
         dwu = torch.empty_like(w_up) if need_gate_up else None
         dwd = torch.empty_like(w_down) if need_down else None
-        ws, need = _workspace(rows, channels, hidden, 1, (grad, x, w_gate, w_up, w_down), x.device)
+        ws, need = _workspace(rows, channels, hidden, 1, (grad, x, w_gate, w_up, w_down), device)
         _lib.check(_lib.load().sbnet_gated_ffn_grad(
             grad.data_ptr(), x.data_ptr(), _DTYPES[x.dtype], rows, channels, hidden,
             w_gate.data_ptr(), w_up.data_ptr(), w_down.data_ptr(), act, _ptr(dx), _ptr(dwg), _ptr(dwu), _ptr(dwd),
-            ws.data_ptr(), need, _stream(x.device)))
+            ws.data_ptr(), need, _stream(device)))
     return dx, dwg, dwu, dwd
 
 

@@ -80,14 +80,15 @@ def test_forward_and_backward(cuda_ops, dtype, c):
     e = _expected(x, w, b, 1e-5, dy)
     if c == 1:      # a single channel is its own mean: y is the bias, no gradient reaches x or w
         e["dx_mag"] = e["dx_mag"] + 1e-3
-    y, mean, rstd = ops.layer_norm(x, w, b, 1e-5, stats=True)
+    y, stats = ops.layer_norm(x, w, b, 1e-5, stats=True)
     _close(y, e, "y", dtype)
     assert torch.equal(y, ops.layer_norm(x, w, b, 1e-5))
+    mean, rstd = stats
     n = _steps(c) * U32
     assert ((mean.double() - e["mean"][:, 0]).abs() <= n * x.double().abs().mean(-1)).all()
     kappa = 1 + x.double().abs().mean(-1) * e["rstd"][:, 0]
     assert ((rstd.double() / e["rstd"][:, 0] - 1).abs() <= 2 * n * kappa).all()
-    dx, dw, db = ops.layer_norm_grad(dy, x, mean, rstd, w, b)
+    dx, dw, db = ops.layer_norm_grad(dy, x, stats, w, b)
     _close(dx, e, "dx", dtype)
     _close(dw, e, "dw", wdtype)
     _close(db, e, "db", wdtype)
@@ -98,13 +99,13 @@ def test_forward_and_backward(cuda_ops, dtype, c):
 def test_row_counts(cuda_ops, rows, c):
     x, dy, w, b = _inputs(rows, c, torch.bfloat16, torch.float32, seed=rows)
     e = _expected(x, w, b, 1e-6, dy)
-    y, mean, rstd = ops.layer_norm(x, w, b, 1e-6, stats=True)
+    y, stats = ops.layer_norm(x, w, b, 1e-6, stats=True)
     _close(y, e, "y", x.dtype)
-    dx, dw, db = ops.layer_norm_grad(dy, x, mean, rstd, w, b)
+    dx, dw, db = ops.layer_norm_grad(dy, x, stats, w, b)
     _close(dx, e, "dx", x.dtype)
     _close(dw, e, "dw", w.dtype)
     _close(db, e, "db", w.dtype)
-    again = ops.layer_norm_grad(dy, x, mean, rstd, w, b)
+    again = ops.layer_norm_grad(dy, x, stats, w, b)
     assert torch.equal(dw, again[1]) and torch.equal(db, again[2])     # a fixed order of additions
 
 
@@ -113,9 +114,9 @@ def test_parameters_are_optional(cuda_ops, which):
     x, dy, w, b = _inputs(50, 72, torch.float16, torch.float16)
     w, b = (w if which == "weight" else None), (b if which == "bias" else None)
     e = _expected(x, w, b, 1e-5, dy)
-    y, mean, rstd = ops.layer_norm(x, w, b, stats=True)
+    y, stats = ops.layer_norm(x, w, b, stats=True)
     _close(y, e, "y", x.dtype)
-    dx, dw, db = ops.layer_norm_grad(dy, x, mean, rstd, w, b)
+    dx, dw, db = ops.layer_norm_grad(dy, x, stats, w, b)
     _close(dx, e, "dx", x.dtype)
     assert (dw is None) == (w is None) and (db is None) == (b is None)
     if w is not None:
@@ -129,12 +130,12 @@ def test_constant_rows_and_rows_that_are_not_finite(cuda_ops):
     x[2] = 5.0                       # no variance: rstd = 1 / sqrt(eps), y = b
     x[4, 7] = math.inf
     x[6, 3] = math.nan
-    y, mean, rstd = ops.layer_norm(x, w, b, 1e-5, stats=True)
+    y, stats = ops.layer_norm(x, w, b, 1e-5, stats=True)
     torch.testing.assert_close(y[2], b, rtol=0, atol=16 * 5 * U32 / math.sqrt(1e-5) * 2)
     assert torch.isnan(y[4]).any() and torch.isnan(y[6]).all()
     clean = [0, 1, 3, 5, 7, 8]
     e = _expected(x[clean], w, b, 1e-5, dy[clean])
-    dx, _, _ = ops.layer_norm_grad(dy, x, mean, rstd, w, b)
+    dx, _, _ = ops.layer_norm_grad(dy, x, stats, w, b)
     _close(y[clean], e, "y", x.dtype)
     _close(dx[clean], e, "dx", x.dtype)
 
@@ -154,11 +155,11 @@ def test_tensors_off_a_16_byte_boundary(cuda_ops, off):
     buf = torch.full((rows * c + 64,), 7.0, dtype=x.dtype, device="cuda")
     out = buf[16 + off:16 + off + rows * c].view(rows, c)
     e = _expected(x, w, b, 1e-5, dy)
-    y, mean, rstd = ops.layer_norm(place(x), w, b, out=out, stats=True)
+    y, stats = ops.layer_norm(place(x), w, b, out=out, stats=True)
     assert y.data_ptr() == out.data_ptr()
     _close(out, e, "y", x.dtype)
     assert (buf[:16 + off] == 7).all() and (buf[16 + off + rows * c:] == 7).all()
-    dx, dw, db = ops.layer_norm_grad(place(dy), place(x), mean, rstd, w, b)
+    dx, dw, db = ops.layer_norm_grad(place(dy), place(x), stats, w, b)
     _close(dx, e, "dx", x.dtype)
     _close(dw, e, "dw", x.dtype)
 
@@ -220,8 +221,8 @@ def test_autograd_matches_the_formula_and_differences(cuda_ops):
 
 def test_another_stream_and_a_captured_graph(cuda_ops):
     x, dy, w, b = _inputs(500, 96, torch.bfloat16, torch.float32)
-    want, mean, rstd = ops.layer_norm(x, w, b, stats=True)
-    gwant = ops.layer_norm_grad(dy, x, mean, rstd, w, b)
+    want, stats = ops.layer_norm(x, w, b, stats=True)
+    gwant = ops.layer_norm_grad(dy, x, stats, w, b)
     s = torch.cuda.Stream()
     s.wait_stream(torch.cuda.current_stream())
     with torch.cuda.stream(s):
@@ -231,8 +232,8 @@ def test_another_stream_and_a_captured_graph(cuda_ops):
     g = torch.cuda.CUDAGraph()
     xs = torch.zeros_like(x)
     with torch.cuda.graph(g):
-        y, m, r = ops.layer_norm(xs, w, b, stats=True)
-        grads = ops.layer_norm_grad(dy, xs, m, r, w, b)
+        y, st = ops.layer_norm(xs, w, b, stats=True)
+        grads = ops.layer_norm_grad(dy, xs, st, w, b)
     for _ in range(2):
         xs.copy_(x)
         g.replay()
