@@ -269,6 +269,8 @@ int sbnet_layer_norm_grad(const void* dy, const void* x, int dtype, int64_t rows
  *   dtype           SBNET_F16 or SBNET_BF16 (what the tensor cores multiply; SBNET_F32 is rejected), of every tensor
  *   x, y            [rows,C];  w_gate, w_up [F,C];  w_down [C,F]
  *   act             SBNET_ACT_*
+ *   kept            [2, rows, F rounded up to a multiple of 8] fp32, 16-byte aligned: receives x w_gate^T and
+ *                   x w_up^T for the backward pass (columns past F are undefined), or NULL when not wanted
  *   workspace       256-byte aligned device memory of at least sbnet_gated_ffn_workspace() bytes, used by this call
  *                   only until it is done on `stream`
  * Accumulation and the element-wise steps are fp32; act(gate)*up is rounded to dtype once, as the operand of the last
@@ -284,17 +286,19 @@ int sbnet_layer_norm_grad(const void* dy, const void* x, int dtype, int64_t rows
 /* grad: workspace of the backward pass.  aligned: 0 if any input tensor's address is not a multiple of 16 bytes. */
 size_t sbnet_gated_ffn_workspace(int64_t rows, int C, int F, int grad, int aligned);
 int sbnet_gated_ffn(const void* x, int dtype, int64_t rows, int C, int F, const void* w_gate, const void* w_up,
-                    const void* w_down, int act, void* y, void* workspace, size_t workspace_bytes, void* stream);
+                    const void* w_down, int act, void* y, float* kept, void* workspace, size_t workspace_bytes,
+                    void* stream);
 int sbnet_gated_ffn_dyn(const void* x, int dtype, int64_t maxBlocks, int rowsPerBlock, const int32_t* num_blocks_dev,
                         int C, int F, const void* w_gate, const void* w_up, const void* w_down, int act, void* y,
                         void* workspace, size_t workspace_bytes, void* stream);
 /*
- * Backward pass from dy and the forward pass' inputs (the projections are multiplied again, so training keeps nothing
- * else of the forward pass).  dx [rows,C], dw_gate and dw_up [F,C], dw_down [C,F]
+ * Backward pass from dy, the forward pass' inputs and its `kept`; with kept == NULL the projections are multiplied
+ * again (4*C operations per hidden element instead of 8 bytes kept, written and read: quicker up to some 1,000
+ * channels, and training then keeps nothing but its inputs).  dx [rows,C], dw_gate and dw_up [F,C], dw_down [C,F]
  * are each skipped where NULL (dw_gate and dw_up go together); no output may overlap an input.  With rows == 0 the
  * weight gradients are set to zero.
  */
-int sbnet_gated_ffn_grad(const void* dy, const void* x, int dtype, int64_t rows, int C, int F, const void* w_gate, const void* w_up, const void* w_down, int act, void* dx,
+int sbnet_gated_ffn_grad(const void* dy, const void* x, const float* kept, int dtype, int64_t rows, int C, int F, const void* w_gate, const void* w_up, const void* w_down, int act, void* dx,
                          void* dw_gate, void* dw_up, void* dw_down, void* workspace, size_t workspace_bytes,
                          void* stream);
 

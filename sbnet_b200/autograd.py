@@ -107,25 +107,35 @@ def layer_norm(x, weight=None, bias=None, eps=1e-5):
     return _LayerNorm.apply(x, weight, bias, eps)
 
 
+# Beyond this many channels the forward pass of the gated feed-forward block keeps its two projections (8 bytes per
+# hidden element) for the backward pass; up to it, multiplying them again takes less time than writing and reading them.
+KEEP_CHANNELS = 1024
+
+
 class _GatedFfn(torch.autograd.Function):
     @staticmethod
     def forward(ctx, x, w_gate, w_up, w_down, activation):
-        ctx.save_for_backward(x, w_gate, w_up, w_down)
+        kept = None
+        if x.shape[-1] > KEEP_CHANNELS and any(ctx.needs_input_grad):
+            y, kept = ops.gated_ffn(x, w_gate, w_up, w_down, activation, keep=True)
+        else:
+            y = ops.gated_ffn(x, w_gate, w_up, w_down, activation)
+        ctx.save_for_backward(x, w_gate, w_up, w_down, kept)
         ctx.activation = activation
-        return ops.gated_ffn(x, w_gate, w_up, w_down, activation)
+        return y
 
     @staticmethod
     @once_differentiable
     def backward(ctx, grad):
-        x, w_gate, w_up, w_down = ctx.saved_tensors
+        x, w_gate, w_up, w_down, kept = ctx.saved_tensors
         need = ctx.needs_input_grad
         channels = x.shape[-1]
         return (*ops._gated_ffn_grad_call(grad.contiguous(), x, w_gate, w_up, w_down, x.numel() // channels, channels,
                                           w_gate.shape[0], ops._lib.SBNET_ACT[ctx.activation],
-                                          need[0], need[1] or need[2], need[3]), None)
+                                          need[0], need[1] or need[2], need[3], kept), None)
 
 
 def gated_ffn(x, w_gate, w_up, w_down, activation="silu"):
-    """Differentiable :func:`sbnet_b200.ops.gated_ffn` (gradients flow to ``x`` and the three weights).  Nothing but
-    the inputs is kept for the backward pass."""
+    """Differentiable :func:`sbnet_b200.ops.gated_ffn` (gradients flow to ``x`` and the three weights).  Up to
+    ``KEEP_CHANNELS`` channels nothing but the inputs is kept for the backward pass."""
     return _GatedFfn.apply(x, w_gate, w_up, w_down, activation)

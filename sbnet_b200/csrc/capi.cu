@@ -507,7 +507,7 @@ int check_workspace(const char* op, const void* workspace, size_t bytes, size_t 
 }
 
 int ffn_call(const void* x, int dtype, int64_t rows, int rowsPerBlock, const int32_t* num_blocks_dev, int C, int F,
-             const void* w_gate, const void* w_up, const void* w_down, int act, void* y, void* workspace, size_t workspace_bytes, void* stream)
+             const void* w_gate, const void* w_up, const void* w_down, int act, void* y, float* kept, void* workspace, size_t workspace_bytes, void* stream)
 {
     const char* op = "GatedFfn";
     g_site = "";
@@ -518,8 +518,8 @@ int ffn_call(const void* x, int dtype, int64_t rows, int rowsPerBlock, const int
     if (x == nullptr || y == nullptr || w_gate == nullptr || w_up == nullptr || w_down == nullptr)
         return reject(SBNET_ERR_INVALID_ARGUMENT, "%s: null tensor pointer", op);
     const uintptr_t inputs = address(x) | address(w_gate) | address(w_up) | address(w_down);
-    if (((inputs | address(y)) & 1) || (address(num_blocks_dev) & 3))
-        return reject(SBNET_ERR_INVALID_ARGUMENT, "%s: tensor pointer not aligned to its element size", op);
+    if (((inputs | address(y)) & 1) || (address(num_blocks_dev) & 3) || (address(kept) & 15))
+        return reject(SBNET_ERR_INVALID_ARGUMENT, "%s: tensor pointer not aligned to its element size (kept: 16 bytes)", op);
     const size_t bytes = (size_t)rows * C * 2, wbytes = (size_t)F * C * 2;
     if (overlaps(x, y, bytes) || (address(y) < address(w_gate) + wbytes && address(w_gate) < address(y) + bytes) ||
         (address(y) < address(w_up) + wbytes && address(w_up) < address(y) + bytes) ||
@@ -529,7 +529,7 @@ int ffn_call(const void* x, int dtype, int64_t rows, int rowsPerBlock, const int
                                  sbnet::gated_ffn_workspace(rows, C, F, false, (inputs & 15) == 0)))
         return rc;
     sbnet::FfnArgs f = {};
-    f.x = x, f.w_gate = w_gate, f.w_up = w_up, f.w_down = w_down, f.y = y;
+    f.x = x, f.w_gate = w_gate, f.w_up = w_up, f.w_down = w_down, f.y = y, f.kept = kept;
     f.num_blocks_dev = num_blocks_dev, f.workspace = workspace, f.rows = rows, f.rowsPerBlock = rowsPerBlock;
     f.C = C, f.F = F, f.act = act;
     return cuda_status(sbnet::launch_gated_ffn(f, dtype, (cudaStream_t)stream));
@@ -544,10 +544,10 @@ SBNET_EXPORT size_t sbnet_gated_ffn_workspace(int64_t rows, int C, int F, int gr
 }
 
 SBNET_EXPORT int sbnet_gated_ffn(const void* x, int dtype, int64_t rows, int C, int F, const void* w_gate,
-                                 const void* w_up, const void* w_down, int act, void* y, void* workspace,
+                                 const void* w_up, const void* w_down, int act, void* y, float* kept, void* workspace,
                                  size_t workspace_bytes, void* stream)
 {
-    return ffn_call(x, dtype, rows, 1, nullptr, C, F, w_gate, w_up, w_down, act, y, workspace, workspace_bytes, stream);
+    return ffn_call(x, dtype, rows, 1, nullptr, C, F, w_gate, w_up, w_down, act, y, kept, workspace, workspace_bytes, stream);
 }
 
 SBNET_EXPORT int sbnet_gated_ffn_dyn(const void* x, int dtype, int64_t maxBlocks, int rowsPerBlock,
@@ -561,10 +561,10 @@ SBNET_EXPORT int sbnet_gated_ffn_dyn(const void* x, int dtype, int64_t maxBlocks
         return reject(SBNET_ERR_INVALID_ARGUMENT, "GatedFfn: bad stack of %lld blocks of %d rows", (long long)maxBlocks,
                       rowsPerBlock);
     return ffn_call(x, dtype, maxBlocks * rowsPerBlock, rowsPerBlock, num_blocks_dev, C, F, w_gate, w_up, w_down, act, y,
-                    workspace, workspace_bytes, stream);
+                    nullptr, workspace, workspace_bytes, stream);
 }
 
-SBNET_EXPORT int sbnet_gated_ffn_grad(const void* dy, const void* x, int dtype, int64_t rows, int C, int F, const void* w_gate, const void* w_up,
+SBNET_EXPORT int sbnet_gated_ffn_grad(const void* dy, const void* x, const float* kept, int dtype, int64_t rows, int C, int F, const void* w_gate, const void* w_up,
                                       const void* w_down, int act, void* dx, void* dw_gate, void* dw_up, void* dw_down,
                                       void* workspace, size_t workspace_bytes, void* stream)
 {
@@ -587,20 +587,20 @@ SBNET_EXPORT int sbnet_gated_ffn_grad(const void* dy, const void* x, int dtype, 
     if (dy == nullptr || x == nullptr || w_gate == nullptr || w_up == nullptr || w_down == nullptr)
         return reject(SBNET_ERR_INVALID_ARGUMENT, "%s: null tensor pointer", op);
     const uintptr_t inputs = address(dy) | address(x) | address(w_gate) | address(w_up) | address(w_down);
-    if (inputs & 1)
-        return reject(SBNET_ERR_INVALID_ARGUMENT, "%s: tensor pointer not aligned to its element size", op);
-    const size_t bytes = (size_t)rows * C * 2, wbytes = (size_t)F * C * 2;
-    const struct { const void* p; size_t n; } in[] = {{dy, bytes}, {x, bytes}, {w_gate, wbytes}, {w_up, wbytes}, {w_down, wbytes}},
+    if ((inputs & 1) || (address(kept) & 15))
+        return reject(SBNET_ERR_INVALID_ARGUMENT, "%s: tensor pointer not aligned to its element size (kept: 16 bytes)", op);
+    const size_t bytes = (size_t)rows * C * 2, wbytes = (size_t)F * C * 2, kbytes = (size_t)rows * ((F + 7) / 8 * 8) * 8;
+    const struct { const void* p; size_t n; } in[] = {{dy, bytes}, {x, bytes}, {kept, kbytes}, {w_gate, wbytes}, {w_up, wbytes}, {w_down, wbytes}},
                                               out[] = {{dx, bytes}, {dw_gate, wbytes}, {dw_up, wbytes}, {dw_down, wbytes}};
     for (const auto& o : out)
         for (const auto& i : in)
-            if (o.p != nullptr && address(o.p) < address(i.p) + i.n && address(i.p) < address(o.p) + o.n)
+            if (o.p != nullptr && i.p != nullptr && address(o.p) < address(i.p) + i.n && address(i.p) < address(o.p) + o.n)
                 return reject(SBNET_ERR_INVALID_ARGUMENT, "%s: an output must not overlap an input", op);
     if (int rc = check_workspace(op, workspace, workspace_bytes,
                                  sbnet::gated_ffn_workspace(rows, C, F, true, (inputs & 15) == 0)))
         return rc;
     sbnet::FfnArgs f = {};
-    f.dy = dy, f.x = x;
+    f.dy = dy, f.x = x, f.kept = const_cast<float*>(kept);
     f.w_gate = w_gate, f.w_up = w_up, f.w_down = w_down;
     f.dx = dx, f.dw_gate = dw_gate, f.dw_up = dw_up, f.dw_down = dw_down;
     f.workspace = workspace, f.rows = rows, f.rowsPerBlock = 1, f.C = C, f.F = F, f.act = act;

@@ -10,12 +10,13 @@
 //
 //   kGate   both projections at once: a tile's B operand is 128 rows of Wg followed by 128 rows of Wu, so G and
 //           U of the same positions come out of one instruction stream side by side in TMEM and the epilogue
-//           writes H without either having been to memory
-//   kGrad   the hidden gradients: a tile multiplies dH (128 columns) and then G and U again (256 columns), and the
-//           epilogue takes all three from TMEM and writes H, dG and dU.  The backward pass so needs nothing of the
-//           forward pass but its inputs.  Keeping G and U instead would save 4 of its 16 R F C operations, but in 16
-//           bits their rounding shows in every gradient (error against 64 bits 2.1 times that of one rounding
-//           instead of 1.4) and in 32 bits they cost 16 bytes of HBM traffic per hidden element
+//           writes H without either having been to memory (in training of many channels it also keeps G and U, in
+//           fp32: rounded to 16 bits they would show in every gradient)
+//   kGrad   the hidden gradients with nothing but the forward pass' inputs: a tile multiplies dH (128 columns) and
+//           then G and U again (256 columns), and the epilogue takes all three from TMEM and writes H, dG and dU.
+//           Costs 4 R F C of 16 R F C operations
+//   kKept   the same from the kept G and U, which the epilogue reads: 16 bytes of HBM traffic per hidden element
+//           instead, so it wins with many channels (8192 x 2048 x 8192 bf16: 405 us against 729)
 //   kStore  a plain product, rounded once
 //
 // H, dG and dU are held between kernels in the type of X (they are operands of the next product, and the tensor
@@ -45,10 +46,10 @@ namespace {
 
 constexpr int kTileM = 256;                      // rows of a tile
 constexpr int kCtaM = 128;                       // ... in each CTA of the pair
-enum Epilogue { kStore, kGate, kGrad };
+enum Epilogue { kStore, kGate, kGrad, kKept };
 // Epilogue warps: the element-wise epilogues are chains of special functions, shared and global accesses, which four
-// warps per scheduler hide better than two.
-template <int EPI> constexpr int kEpiWarps = EPI == kStore ? 8 : 16;
+// warps per scheduler hide better than two; kKept instead loads a step ahead into registers that 16 warps do not have.
+template <int EPI> constexpr int kEpiWarps = EPI == kStore || EPI == kKept ? 8 : 16;
 template <int EPI> constexpr int kGemmThreads = (2 + kEpiWarps<EPI>) * 32;
 // 32 x 32 tiles of 16-bit elements (2 KB) that a warp stages between registers and memory
 template <int EPI> constexpr int kStaged = EPI == kStore ? 1 : 2;
@@ -59,7 +60,7 @@ __device__ unsigned int g_ffn_timeouts = 0;
 
 struct Maps {
     CUtensorMap a[2], b[2], c;     // c: kGrad's Wd
-    CUtensorMap out;               // H, which kGate writes by TMA
+    CUtensorMap out, g, u;         // H and the kept G and U, which kGate writes by TMA
 };
 
 struct Plan {
@@ -76,11 +77,12 @@ struct Plan {
     int act;
     void* out[2];                  // kStore: D of product z.  kGate: H
     long long ldo;
-    void *hid, *dgate, *dup;       // kGrad: written, pitch ldo
+    float *gate, *up;              // kGate: written unless null, kKept: read; pitch ldo
+    void *hid, *dgate, *dup;       // kGrad, kKept: written, pitch ldo
     float* partials;               // splits > 1: [splits][batch][mTiles * 256][nTiles * BN]
 };
 
-template <int EPI, int BN> constexpr int kStages = EPI != kStore ? 5 : BN == 256 ? 6 : 8;
+template <int EPI, int BN> constexpr int kStages = EPI == kGate || EPI == kGrad ? 5 : BN == 256 ? 6 : 8;
 template <int BN> constexpr int kStageBytes = (kCtaM + BN / 2) * kStepK * 2;    // of one CTA
 template <int EPI, int BN> constexpr int kGemmSmem = 1024 + kStages<EPI, BN> * kStageBytes<BN> + kStagingBytes<EPI> + 256;
 
@@ -331,7 +333,7 @@ __global__ void __launch_bounds__(kGemmThreads<EPI>, 1) gemm_kernel(const __grid
         const int quarter = warp & 3, share = (warp - 2) >> 2;
         const uint32_t buf0 = staging + (warp - 2) * (kStaged<EPI> * 2048), buf1 = buf0 + 2048;
         const uint32_t accEmptyFirst = in_first_cta(accEmpty);
-        uint32_t turn = 0;
+        uint32_t turn = 0, sent = 0;
         for (int t = blockIdx.x >> 1; t < tiles; t += gridDim.x >> 1, ++turn) {
             const Tile w = tile_at(t, p, mTiles);
             const uint32_t acc = EPI == kGrad ? 0 : turn & 1, d = tmem + acc * BN + ((uint32_t)(quarter * 32) << 16);
@@ -377,10 +379,20 @@ __global__ void __launch_bounds__(kGemmThreads<EPI>, 1) gemm_kernel(const __grid
                     else
                         gate_chunk<T, kRelu>(g, u, h);
                     const int col = w.n * 128 + c;
-                    const uint32_t buf = turn & 1 ? buf1 : buf0;      // the two buffers in turn
-                    wait_sent<1>(lane);
-                    stage_rows(buf, lane, h);
-                    send_tile(&maps.out, buf, col, (int)row0, lane);
+                    wait_sent<1>(lane);     // the two buffers in turn
+                    stage_rows(sent & 1 ? buf1 : buf0, lane, h);
+                    send_tile(&maps.out, sent++ & 1 ? buf1 : buf0, col, (int)row0, lane);
+                    if (p.gate != nullptr) {        // 16 columns of fp32 are as wide as 32 of 16 bits
+#pragma unroll
+                        for (int i = 0; i < 4; ++i) {
+                            const uint32_t* v = (i < 2 ? g : u) + 16 * (i & 1);
+                            wait_sent<1>(lane);
+#pragma unroll
+                            for (int k = 0; k < 4; ++k)
+                                sts128(piece(sent & 1 ? buf1 : buf0, lane, k), make_uint4(v[4 * k], v[4 * k + 1], v[4 * k + 2], v[4 * k + 3]));
+                            send_tile(i < 2 ? &maps.g : &maps.u, sent++ & 1 ? buf1 : buf0, col + 16 * (i & 1), (int)row0, lane);
+                        }
+                    }
                 }
             } else if (EPI == kGrad) {     // one chunk of 32 columns a warp: TMEM is free again after three loads
                 const int c = share * 32;
@@ -415,6 +427,70 @@ __global__ void __launch_bounds__(kGemmThreads<EPI>, 1) gemm_kernel(const __grid
                 __syncwarp();
                 store_tile<T>(p.dup, at, true, buf0, lane);
                 __syncwarp();
+            } else if (EPI == kKept) {      // 16 columns at a time, the next 16 of G and U loading meanwhile
+                constexpr int kCols = BN * 4 / W;
+                const int first = w.n * BN + share * kCols;
+                uint4 gn[4], un[4];
+                auto fetch = [&](int c) {
+                    const int r = lane >> 2, col = first + c + (lane & 3) * 4;
+#pragma unroll
+                    for (int i = 0; i < 4; ++i) {
+                        const long long row = row0 + r + 8 * i;
+                        gn[i] = un[i] = make_uint4(0, 0, 0, 0);
+                        if (row < rowEnd && col < p.N) {
+                            gn[i] = ld_stream(reinterpret_cast<const uint4*>(p.gate + row * p.ldo + col));
+                            un[i] = ld_stream(reinterpret_cast<const uint4*>(p.up + row * p.ldo + col));
+                        }
+                    }
+                };
+                fetch(0);
+#pragma unroll 1
+                for (int c = 0; c < kCols; c += 32) {
+                    uint32_t h[16], dg[16], du[16];
+#pragma unroll
+                    for (int i = 0; i < 2; ++i) {
+#pragma unroll
+                        for (int k = 0; k < 4; ++k) {
+                            sts128(piece(buf0, k * 8 + (lane >> 2), lane & 3), gn[k]);
+                            sts128(piece(buf1, k * 8 + (lane >> 2), lane & 3), un[k]);
+                        }
+                        __syncwarp();
+                        if (c + 16 * i + 16 < kCols)
+                            fetch(c + 16 * i + 16);
+                        uint32_t dh[16], g[16], u[16], hh[8], gg[8], uu[8];
+                        tmem_load16(d + share * kCols + c + 16 * i, dh);
+#pragma unroll
+                        for (int k = 0; k < 4; ++k) {
+                            const uint4 a = lds128(piece(buf0, lane, k)), b = lds128(piece(buf1, lane, k));
+                            g[4 * k] = a.x, g[4 * k + 1] = a.y, g[4 * k + 2] = a.z, g[4 * k + 3] = a.w;
+                            u[4 * k] = b.x, u[4 * k + 1] = b.y, u[4 * k + 2] = b.z, u[4 * k + 3] = b.w;
+                        }
+                        tmem_wait_load();
+                        if (c + 16 * i + 16 == kCols)
+                            release();
+                        __syncwarp();
+                        if (p.act == kSilu)
+                            grad_chunk<T, kSilu>(dh, g, u, hh, gg, uu);
+                        else if (p.act == kGelu)
+                            grad_chunk<T, kGelu>(dh, g, u, hh, gg, uu);
+                        else
+                            grad_chunk<T, kRelu>(dh, g, u, hh, gg, uu);
+#pragma unroll
+                        for (int k = 0; k < 8; ++k)
+                            h[8 * i + k] = hh[k], dg[8 * i + k] = gg[k], du[8 * i + k] = uu[k];
+                    }
+                    const Spot at = spot(p.ldo, row0, rowEnd, first + c, p.N, lane);
+                    stage_rows(buf0, lane, h);
+                    stage_rows(buf1, lane, dg);
+                    __syncwarp();
+                    store_tile<T>(p.hid, at, true, buf0, lane);
+                    store_tile<T>(p.dgate, at, true, buf1, lane);
+                    __syncwarp();
+                    stage_rows(buf0, lane, du);
+                    __syncwarp();
+                    store_tile<T>(p.dup, at, true, buf0, lane);
+                    __syncwarp();
+                }
             } else {
                 T* out = static_cast<T*>(p.out[w.z]);
                 const bool wide = ((p.ldo & 7) == 0) && (reinterpret_cast<uintptr_t>(out) & 15) == 0;
@@ -493,6 +569,10 @@ template <typename T, int EPI> __global__ void __launch_bounds__(256) finish_ker
             auto gated = [&](float a, float b) { return activate_any(p.act, a) * b; };
             h.x = gated(g.x, u.x), h.y = gated(g.y, u.y), h.z = gated(g.z, u.z), h.w = gated(g.w, u.w);
             store4<T>(out + row * p.ldo + col, h, n, wide);
+            if (p.gate != nullptr) {        // the pitch is a multiple of 8
+                *reinterpret_cast<float4*>(p.gate + row * p.ldo + col) = g;
+                *reinterpret_cast<float4*>(p.up + row * p.ldo + col) = u;
+            }
         } else {
             const float4 v = sum_pieces(p.partials + z * plane + row * pitch + col, p.batch * plane, p.splits);
             store4<T>(out + row * p.ldo + col, v, n, wide);
@@ -576,7 +656,7 @@ cudaError_t launch_maps(const Maps& maps, Plan& p, cudaStream_t stream)
     if (p.splits == 1)
         return cudaSuccess;
     const dim3 fgrid((unsigned)ceil_div(p.N, 128), (unsigned)std::min<long long>((p.M + 7) / 8, 65535), (unsigned)p.batch);
-    if constexpr (EPI != kGrad)
+    if constexpr (EPI == kStore || EPI == kGate)
         return launch_pdl(finish_kernel<T, EPI>, fgrid, dim3(32, 8), 0, stream, p, BN);
     return cudaErrorInvalidValue;
 }
@@ -600,8 +680,16 @@ cudaError_t launch_gemm(const Matrix (&a)[2], const Matrix (&b)[2], Plan& p, cud
     if (n == 1 && EPI != kGate)
         maps.b[1] = maps.b[0];
     if (EPI == kGate && p.splits == 1)
+    {
         if (cudaError_t e = encode({p.out[0], p.M, p.N, p.ldo}, 32, &maps.out, 32))
             return e;
+        if (p.gate != nullptr) {
+            if (cudaError_t e = encode({p.gate, p.M, p.N, p.ldo}, 32, &maps.g, 16, 4))
+                return e;
+            if (cudaError_t e = encode({p.up, p.M, p.N, p.ldo}, 32, &maps.u, 16, 4))
+                return e;
+        }
+    }
     return launch_maps<T, A_MN, B_MN, EPI, BN>(maps, p, stream);
 }
 
@@ -735,6 +823,7 @@ template <typename T> cudaError_t forward(const FfnArgs& f, Layout& l, bool run,
     p.splits = split_count(R, 2ll * F, (long long)p.mTiles * p.nTiles, p.kIters);
     p.N = F, p.M = R, p.num_blocks_dev = f.num_blocks_dev, p.rowsPerBlock = f.rowsPerBlock, p.act = f.act;
     p.out[0] = const_cast<void*>(h.ptr), p.ldo = Fp, p.partials = parts;
+    p.gate = f.kept, p.up = f.kept == nullptr ? nullptr : f.kept + (size_t)R * Fp;
     SBNET_TRY((launch_gemm<T, false, false, kGate, 256>({x, x}, {wg, wu}, p, stream)));
     note_site("gated_ffn output");
     return product<T, false, false>({h, h}, {wd, wd}, 1, 1, R, C, F, f.y, nullptr, parts, f, true, stream);
@@ -761,7 +850,13 @@ template <typename T> cudaError_t backward(const FfnArgs& f, Layout& l, bool run
     p.mTiles = ceil_div(R, kTileM), p.nTiles = ceil_div(F, 128), p.batch = 1, p.segs = 2, p.kIters = ceil_div(C, kStepK);
     p.splits = 1, p.N = F, p.M = R, p.act = f.act;
     p.hid = const_cast<void*>(h.ptr), p.dgate = const_cast<void*>(dg.ptr), p.dup = const_cast<void*>(du.ptr), p.ldo = Fp;
-    SBNET_TRY(launch_grad<T>(dy, x, wd, wg, wu, p, stream));
+    if (f.kept == nullptr) {
+        SBNET_TRY(launch_grad<T>(dy, x, wd, wg, wu, p, stream));
+    } else {
+        p.nTiles = ceil_div(F, 256), p.segs = 1;
+        p.gate = f.kept, p.up = f.kept + (size_t)R * Fp;
+        SBNET_TRY((launch_gemm<T, false, true, kKept, 256>({dy, dy}, {wd, wd}, p, stream)));
+    }
     if (f.dx != nullptr) {
         note_site("gated_ffn_grad dx");
         SBNET_TRY((product<T, false, true>({dg, du}, {wg, wu}, 1, 2, R, C, F, f.dx, nullptr, parts, f, false, stream)));
@@ -791,14 +886,28 @@ size_t gated_ffn_workspace(long long rows, int C, int F, bool grad, bool aligned
     return l.bump.used;
 }
 
+// Tensor maps are encoded by a driver call, which wants the device's context current on the calling thread; a thread
+// that has made no runtime call yet (a fresh autograd thread) has none.  cudaSetDevice binds it.
+static cudaError_t bind_context()
+{
+    int device = 0;
+    if (cudaError_t e = cudaGetDevice(&device))
+        return e;
+    return cudaSetDevice(device);
+}
+
 cudaError_t launch_gated_ffn(const FfnArgs& f, int dtype, cudaStream_t stream)
 {
+    note_site("gated_ffn context");
+    SBNET_TRY(bind_context());
     Layout l = {{static_cast<uint8_t*>(f.workspace), 0}, true};
     return dtype == 1 ? forward<__half>(f, l, true, stream) : forward<__nv_bfloat16>(f, l, true, stream);
 }
 
 cudaError_t launch_gated_ffn_grad(const FfnArgs& f, int dtype, cudaStream_t stream)
 {
+    note_site("gated_ffn_grad context");
+    SBNET_TRY(bind_context());
     Layout l = {{static_cast<uint8_t*>(f.workspace), 0}, true};
     return dtype == 1 ? backward<__half>(f, l, true, stream) : backward<__nv_bfloat16>(f, l, true, stream);
 }

@@ -163,22 +163,23 @@ inline PFN_cuTensorMapEncodeTiled encoder()
     return fn;
 }
 
-// A row-major matrix of 16-bit elements as TMA reads it, boxes of 64 columns x boxRows rows, or writes it, 32 x 32.
+// A row-major matrix as TMA reads it (16-bit elements, boxes of 64 columns x boxRows rows) or writes it (boxes of 64
+// bytes x 32 rows).
 struct Matrix {
     const void* ptr;
     long long rows;
     int cols;
     long long ld;
 };
-inline cudaError_t encode(const Matrix& m, int boxRows, CUtensorMap* out, int boxCols = kStepK)
+inline cudaError_t encode(const Matrix& m, int boxRows, CUtensorMap* out, int boxCols = kStepK, int itemsize = 2)
 {
     PFN_cuTensorMapEncodeTiled enc = encoder();
     if (enc == nullptr)
         return cudaErrorNotSupported;
-    const cuuint64_t dims[2] = {(cuuint64_t)m.cols, (cuuint64_t)m.rows}, strides[1] = {(cuuint64_t)m.ld * 2};
+    const cuuint64_t dims[2] = {(cuuint64_t)m.cols, (cuuint64_t)m.rows}, strides[1] = {(cuuint64_t)m.ld * itemsize};
     const cuuint32_t box[2] = {(cuuint32_t)boxCols, (cuuint32_t)boxRows}, estr[2] = {1, 1};
-    return enc(out, CU_TENSOR_MAP_DATA_TYPE_UINT16, 2, const_cast<void*>(m.ptr), dims, strides, box, estr,
-               CU_TENSOR_MAP_INTERLEAVE_NONE, boxCols == 32 ? CU_TENSOR_MAP_SWIZZLE_64B : CU_TENSOR_MAP_SWIZZLE_128B,
+    return enc(out, itemsize == 4 ? CU_TENSOR_MAP_DATA_TYPE_UINT32 : CU_TENSOR_MAP_DATA_TYPE_UINT16, 2, const_cast<void*>(m.ptr), dims, strides, box, estr,
+               CU_TENSOR_MAP_INTERLEAVE_NONE, boxCols * itemsize == 64 ? CU_TENSOR_MAP_SWIZZLE_64B : CU_TENSOR_MAP_SWIZZLE_128B,
                CU_TENSOR_MAP_L2_PROMOTION_L2_256B,
                CU_TENSOR_MAP_FLOAT_OOB_FILL_NONE) == CUDA_SUCCESS
                ? cudaSuccess

@@ -33,6 +33,7 @@ constexpr int kSmemLimit = 224 * 1024, kSmemHalf = 110 * 1024;     // of a CTA t
 struct FewArgs {
     const void *x, *w0, *w1;         // X [M, K]; the group's first and second 8 weight rows
     void* out;                       // [M, N]
+    float *gate, *up;                // gate kernel: G and U [M, N], or nullptr
     const int32_t* num_blocks_dev;
     long long M;
     int rowsPerBlock, K, N, act;
@@ -144,6 +145,8 @@ template <typename T, int MT, bool GATE> __global__ void __launch_bounds__(kThre
         if (GATE) {
             const long long at = (long long)tok * p.N + group * 8 + r;
             static_cast<T*>(p.out)[at] = T(activate_any(p.act, s0) * s1);
+            if (p.gate != nullptr)
+                p.gate[at] = s0, p.up[at] = s1;
         } else {
             const int col = group * 16 + r;
             T* y = static_cast<T*>(p.out) + (long long)tok * p.N + col;
@@ -325,6 +328,8 @@ template <typename T, int MT> cudaError_t both(const FfnArgs& f, void* h, cudaSt
 {
     FewArgs gate = {}, out = {};
     gate.x = f.x, gate.w0 = f.w_gate, gate.w1 = f.w_up, gate.out = h;
+    if (f.kept != nullptr)
+        gate.gate = f.kept, gate.up = f.kept + (size_t)f.rows * f.F;
     gate.K = f.C, gate.N = f.F, gate.act = f.act;
     out.x = h, out.w0 = out.w1 = f.w_down, out.out = f.y, out.K = f.F, out.N = f.C;
     gate.M = out.M = f.rows;

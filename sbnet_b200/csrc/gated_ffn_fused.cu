@@ -395,7 +395,7 @@ template <typename T>
 cudaError_t launch_ffn_fused(const FfnArgs& f, const Matrix& x, const Matrix& wg, const Matrix& wu, const Matrix& wd,
                              cudaStream_t stream, bool* taken)
 {
-    *taken = ffn_fused_suits(f.rows, f.C);
+    *taken = f.kept == nullptr && ffn_fused_suits(f.rows, f.C);
     if (!*taken)
         return cudaSuccess;
     const int kc = ceil_div(f.C, 64);

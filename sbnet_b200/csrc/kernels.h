@@ -58,6 +58,8 @@ struct FfnArgs {
     const void* x;                             // [rows, C]
     const void *w_gate, *w_up, *w_down;        // [F, C], [F, C], [C, F]
     void* y;                                   // forward: [rows, C]
+    float* kept;                               // [2, rows, F rounded up to 8] G and U: forward writes them unless null, backward
+                                               // reads them, or multiplies them again where null
     const void* dy;                            // backward: [rows, C]
     void *dx, *dw_gate, *dw_up, *dw_down;      // backward: written unless null (dw_gate and dw_up go together)
     const int32_t* num_blocks_dev;             // forward: live blocks of rowsPerBlock rows, or nullptr (all rows)

@@ -45,9 +45,9 @@ SIGNATURES = {
     "sbnet_layer_norm_dyn": (_i, [_p, _i, _l, _i, _p, _i, _p, _p, _i, _f, _p, _p, _p, _p]),
     "sbnet_layer_norm_grad_workspace": (_sz, [_l, _i]),
     "sbnet_gated_ffn_workspace": (_sz, [_l, _i, _i, _i, _i]),
-    "sbnet_gated_ffn": (_i, [_p, _i, _l, _i, _i, _p, _p, _p, _i, _p, _p, _sz, _p]),
+    "sbnet_gated_ffn": (_i, [_p, _i, _l, _i, _i, _p, _p, _p, _i, _p, _p, _p, _sz, _p]),
     "sbnet_gated_ffn_dyn": (_i, [_p, _i, _l, _i, _p, _i, _i, _p, _p, _p, _i, _p, _p, _sz, _p]),
-    "sbnet_gated_ffn_grad": (_i, [_p, _p, _i, _l, _i, _i, _p, _p, _p, _i, _p, _p, _p, _p, _p, _sz, _p]),
+    "sbnet_gated_ffn_grad": (_i, [_p, _p, _p, _i, _l, _i, _i, _p, _p, _p, _i, _p, _p, _p, _p, _p, _sz, _p]),
     "sbnet_layer_norm_grad": (_i, [_p, _p, _i, _l, _i, _p, _i, _p, _p, _p, _p, _p, _p, _sz, _p]),
 }
 

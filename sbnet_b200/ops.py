@@ -529,7 +529,7 @@ def _workspace(rows, channels, hidden, grad, tensors, device):
     return torch.empty(need, dtype=torch.uint8, device=device), need
 
 
-def _gated_ffn_call(x, w_gate, w_up, w_down, activation, out, count_dev):
+def _gated_ffn_call(x, w_gate, w_up, w_down, activation, out, count_dev, keep=False):
     rows, channels, hidden, act = _check_ffn(x, w_gate, w_up, w_down, activation)
     if count_dev is not None:
         _check_count_dev(count_dev, x)
@@ -539,24 +539,28 @@ def _gated_ffn_call(x, w_gate, w_up, w_down, activation, out, count_dev):
     _require_cuda(x, "x")
     with _on(x.device):
         y = torch.empty_like(x) if out is None else out
+        kept = torch.empty((2, rows, (hidden + 7) // 8 * 8), dtype=torch.float32, device=x.device) if keep else None
         ws, need = _workspace(rows, channels, hidden, 0, (x, w_gate, w_up, w_down), x.device)
         head = (channels, hidden, w_gate.data_ptr(), w_up.data_ptr(), w_down.data_ptr(), act, y.data_ptr())
         tail = (ws.data_ptr(), need, _stream(x.device))
         if count_dev is None:
-            _lib.check(_lib.load().sbnet_gated_ffn(x.data_ptr(), _DTYPES[x.dtype], rows, *head, *tail))
+            _lib.check(_lib.load().sbnet_gated_ffn(x.data_ptr(), _DTYPES[x.dtype], rows, *head, _ptr(kept), *tail))
         else:
             _lib.check(_lib.load().sbnet_gated_ffn_dyn(x.data_ptr(), _DTYPES[x.dtype], blocks, per, count_dev.data_ptr(),
                                                        *head, *tail))
-    return y
+    return (y, kept) if keep else y
 
 
 def gated_ffn(x: torch.Tensor, w_gate: torch.Tensor, w_up: torch.Tensor, w_down: torch.Tensor, activation: str = "silu",
-              out=None) -> torch.Tensor:
+              out=None, keep: bool = False):
     """Gated feed-forward block over the rows of ``x`` (``[..., C]``, float16 or bfloat16):
     ``(act(x @ w_gate.T) * (x @ w_up.T)) @ w_down.T`` with ``w_gate``, ``w_up`` ``[F, C]`` and ``w_down``
     ``[C, F]`` of the same type; ``activation``: "silu", "gelu" (by the error function) or "relu".  Sums are fp32,
-    the gated product is rounded to the type of ``x`` once.  ``out`` must not overlap an input."""
-    return _gated_ffn_call(x, w_gate, w_up, w_down, activation, out, None)
+    the gated product is rounded to the type of ``x`` once.  ``out`` must not overlap an input.
+
+    ``keep=True`` returns ``(y, kept)``, the two projections in float32 (``[2, rows, F rounded up to a multiple of 8]``,
+    columns past F undefined), which spare :func:`gated_ffn_grad` from multiplying them again."""
+    return _gated_ffn_call(x, w_gate, w_up, w_down, activation, out, None, keep)
 
 
 def gated_ffn_dyn(x: torch.Tensor, count_dev: torch.Tensor, w_gate, w_up, w_down, activation: str = "silu", out=None):
@@ -568,16 +572,20 @@ def gated_ffn_dyn(x: torch.Tensor, count_dev: torch.Tensor, w_gate, w_up, w_down
 
 
 def gated_ffn_grad(grad: torch.Tensor, x: torch.Tensor, w_gate, w_up, w_down, activation: str = "silu",
-                   need_x: bool = True, need_gate_up: bool = True, need_down: bool = True):
-    """Backward pass of :func:`gated_ffn` from its inputs and the gradient of its result (the projections are
-    multiplied again): ``(dx, dw_gate, dw_up, dw_down)``, None where not asked for."""
+                   need_x: bool = True, need_gate_up: bool = True, need_down: bool = True, kept=None):
+    """Backward pass of :func:`gated_ffn` from its inputs and the gradient of its result:
+    ``(dx, dw_gate, dw_up, dw_down)``, None where not asked for.  ``kept``: what the forward call returned with
+    ``keep=True``, or None to multiply the projections again."""
     rows, channels, hidden, act = _check_ffn(x, w_gate, w_up, w_down, activation)
     _check_like(grad, "grad", x)
+    if kept is not None and (kept.dtype != torch.float32 or tuple(kept.shape) != (2, rows, (hidden + 7) // 8 * 8) or
+                             not kept.is_contiguous() or kept.device != x.device):
+        raise ValueError("kept must be what gated_ffn returned with keep=True, or None")
     _require_cuda(x, "x")
-    return _gated_ffn_grad_call(grad, x, w_gate, w_up, w_down, rows, channels, hidden, act, need_x, need_gate_up, need_down)
+    return _gated_ffn_grad_call(grad, x, w_gate, w_up, w_down, rows, channels, hidden, act, need_x, need_gate_up, need_down, kept)
 
 
-def _gated_ffn_grad_call(grad, x, w_gate, w_up, w_down, rows, channels, hidden, act, need_x, need_gate_up, need_down):
+def _gated_ffn_grad_call(grad, x, w_gate, w_up, w_down, rows, channels, hidden, act, need_x, need_gate_up, need_down, kept):
     """The checked call (autograd's tensors come from a checked forward call)."""
     device = x.device
     with _on(device):
@@ -587,7 +595,7 @@ def _gated_ffn_grad_call(grad, x, w_gate, w_up, w_down, rows, channels, hidden, 
         dwd = torch.empty_like(w_down) if need_down else None
         ws, need = _workspace(rows, channels, hidden, 1, (grad, x, w_gate, w_up, w_down), device)
         _lib.check(_lib.load().sbnet_gated_ffn_grad(
-            grad.data_ptr(), x.data_ptr(), _DTYPES[x.dtype], rows, channels, hidden,
+            grad.data_ptr(), x.data_ptr(), _ptr(kept), _DTYPES[x.dtype], rows, channels, hidden,
             w_gate.data_ptr(), w_up.data_ptr(), w_down.data_ptr(), act, _ptr(dx), _ptr(dwg), _ptr(dwu), _ptr(dwd),
             ws.data_ptr(), need, _stream(device)))
     return dx, dwg, dwu, dwd

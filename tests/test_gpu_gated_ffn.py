@@ -111,6 +111,36 @@ def test_forward_and_backward(cuda_ops, dtype, size):
     assert lib.wait_timeouts() == 0
 
 
+@pytest.mark.parametrize("size", SIZES, ids=str)
+@pytest.mark.parametrize("dtype", [torch.float16, torch.bfloat16])
+def test_kept_projections(cuda_ops, dtype, size):
+    """The forward pass that keeps G and U, and the backward pass that reads them: the same bounds."""
+    act = ("silu", "gelu", "relu")[sum(size) % 3]
+    x, wg, wu, wd, dy = _inputs(*size, dtype, seed=sum(size) + 1)
+    exp = _expected(act, x, wg, wu, wd, dy)
+    y, kept = ops.gated_ffn(x, wg, wu, wd, act, keep=True)
+    _check(y, exp, "y", dtype)
+    for k, w in enumerate((wg, wu)):
+        ref = x.double() @ w.double().T
+        tol = (size[1] / 16 + 16) * 2.0 ** -23 * (x.double().abs() @ w.double().abs().T)
+        assert ((kept[k, :, :size[2]].double() - ref).abs() <= tol).all()
+    got = ops.gated_ffn_grad(dy, x, wg, wu, wd, act, kept=kept)
+    for n, v in zip(NAMES[1:], got):
+        _check(v, exp, n, dtype)
+    assert lib.wait_timeouts() == 0
+
+
+@pytest.mark.parametrize("channels", [1024, 1032])
+def test_autograd_on_both_sides_of_the_keeping_limit(cuda_ops, channels):
+    args = _inputs(200, channels, 264, torch.bfloat16, seed=channels)
+    leaves = [t.requires_grad_(True) for t in args[:4]]
+    y = sb.gated_ffn(*leaves, activation="gelu")
+    grads = torch.autograd.grad(y, leaves, args[4])
+    exp = _expected("gelu", *(t.detach() for t in args))
+    for n, v in zip(NAMES, (y.detach(), *grads)):
+        _check(v, exp, n, y.dtype)
+
+
 @pytest.mark.parametrize("act", ["silu", "gelu", "relu"])
 @pytest.mark.parametrize("dtype", [torch.float16, torch.bfloat16])
 @pytest.mark.parametrize("rows", [4, 40, 260])
@@ -297,3 +327,43 @@ def test_many_rows(cuda_ops):
     y = ops.gated_ffn(big, wg, wu, wd)
     _check(y[-256:].contiguous(), _expected("silu", x, wg, wu, wd), "y", x.dtype)
     assert not y[:1000].any()
+
+
+def test_a_thread_that_has_no_context_yet(cuda_ops):
+    """Every call from a fresh thread whose memory all comes from the allocator's cache, so that the library's call is the
+    thread's first."""
+    import threading
+    args = _inputs(700, 64, 136, torch.float16)
+    few = [args[0][:3].contiguous(), *args[1:4]]
+    many = _inputs(12_000, 64, 136, torch.float16)
+    calls = [lambda: ops.gated_ffn(*args[:4]), lambda: ops.gated_ffn_grad(args[4], *args[:4])[1], lambda: ops.gated_ffn(*few),
+             lambda: ops.gated_ffn(*many[:4]), lambda: ops.gated_ffn(*args[:4], keep=True)[0], lambda: ops.layer_norm(args[0])]
+    for call in calls:
+        want, got = call(), []
+        torch.cuda.synchronize()
+        thread = threading.Thread(target=lambda: got.append(call()))
+        thread.start()
+        thread.join()
+        torch.cuda.synchronize()
+        assert got and torch.equal(got[0], want)
+
+
+def test_two_threads_on_streams_of_their_own(cuda_ops):
+    import threading
+    jobs = [_inputs(500 + 300 * i, 128, 264, torch.bfloat16, seed=i) for i in range(2)]
+    want = [ops.gated_ffn_grad(j[4], *j[:4]) for j in jobs]
+    torch.cuda.synchronize()
+    results = [[], []]
+
+    def work(i):
+        with torch.cuda.stream(torch.cuda.Stream()):
+            for _ in range(20):
+                results[i] = ops.gated_ffn_grad(jobs[i][4], *jobs[i][:4])
+            torch.cuda.current_stream().synchronize()
+    threads = [threading.Thread(target=work, args=(i,)) for i in range(2)]
+    for t in threads:
+        t.start()
+    for t in threads:
+        t.join()
+    for got, exp in zip(results, want):
+        assert all(torch.equal(g, e) for g, e in zip(got, exp))

@@ -116,6 +116,10 @@ def test_gated_ffn_rules():
         ops.gated_ffn_grad(x[:3], x, wg, wu, wd)
     with pytest.raises(ValueError, match="CUDA"):
         ops.gated_ffn_grad(x, x, wg, wu, wd)
+    kept = torch.zeros(2, 4, 16)
+    for bad in (kept[:1], kept[:, :3].contiguous(), kept[..., :15], kept.half()):
+        with pytest.raises(ValueError, match="kept"):
+            ops.gated_ffn_grad(x, x, wg, wu, wd, kept=bad)
 
 
 def test_gated_ffn_c_entries_refuse(handle):
@@ -126,10 +130,10 @@ def test_gated_ffn_c_entries_refuse(handle):
     assert handle.sbnet_gated_ffn_workspace(4, 8, 16, 0, 0) > need
     assert handle.sbnet_gated_ffn_workspace(0, 8, 16, 0, 1) == 0
 
-    def call(x=x, dtype=1, rows=4, c=8, f=16, wg=w, wu=w, wd=w, act=0, y=y, ws=ws, n=need):
-        return ffn(x, dtype, rows, c, f, wg, wu, wd, act, y, ws, n, None)
+    def call(x=x, dtype=1, rows=4, c=8, f=16, wg=w, wu=w, wd=w, act=0, y=y, kept=None, ws=ws, n=need):
+        return ffn(x, dtype, rows, c, f, wg, wu, wd, act, y, kept, ws, n, None)
     for bad in (dict(dtype=0), dict(dtype=7), dict(rows=-1), dict(c=0), dict(f=0), dict(act=3), dict(act=-1), dict(x=None),
-                dict(y=None), dict(wd=None), dict(x=x + 1), dict(y=y + 1), dict(y=x + 32), dict(y=w), dict(ws=None), dict(ws=ws + 16), dict(n=need - 1)):
+                dict(y=None), dict(wd=None), dict(kept=(1 << 29) + 4), dict(x=x + 1), dict(y=y + 1), dict(y=x + 32), dict(y=w), dict(ws=None), dict(ws=ws + 16), dict(n=need - 1)):
         assert call(**bad) == BAD, bad
         assert handle.sbnet_last_error()
     assert call(rows=1 << 31) == -2 and call(c=1 << 25) == -2 and call(f=1 << 25) == -2
@@ -141,9 +145,9 @@ def test_gated_ffn_c_entries_refuse(handle):
 
     gneed = handle.sbnet_gated_ffn_workspace(4, 8, 16, 1, 1)
 
-    def back(dy=x, x=x, dtype=1, rows=4, wd=w, act=0, dx=y, dwg=None, dwu=None, dwd=None, ws=ws, n=gneed):
-        return grad(dy, x, dtype, rows, 8, 16, w, w, wd, act, dx, dwg, dwu, dwd, ws, n, None)
+    def back(dy=x, x=x, kept=1 << 29, dtype=1, rows=4, wd=w, act=0, dx=y, dwg=None, dwu=None, dwd=None, ws=ws, n=gneed):
+        return grad(dy, x, kept, dtype, rows, 8, 16, w, w, wd, act, dx, dwg, dwu, dwd, ws, n, None)
     for bad in (dict(dtype=0), dict(act=5), dict(dy=None), dict(dwg=y + 4096),
-                dict(dwu=y + 4096), dict(dx=y + 1), dict(dx=x), dict(dwd=w), dict(ws=None), dict(n=gneed - 1),
+                dict(dwu=y + 4096), dict(dx=y + 1), dict(dx=x), dict(dx=1 << 29), dict(kept=(1 << 29) + 4), dict(dwd=w), dict(ws=None), dict(n=gneed - 1),
                 dict(wd=None), dict(x=x + 1)):
         assert back(**bad) == BAD, bad
