@@ -255,7 +255,7 @@ int sbnet_layer_norm_dyn(const void* x, int dtype, int64_t maxBlocks, int rowsPe
 /*
  * Backward pass: dx [rows,C] of dtype from dy, x and the forward pass' mean and rstd; dweight, dbias [C] of
  * wdtype (either or both may be NULL).  workspace: 16-byte aligned device memory of at least
- * sbnet_layer_norm_grad_workspace(rows, C) bytes, used by this call only until it is done on `stream`
+ * sbnet_layer_norm_grad_workspace(rows, C) bytes (asked on the same device), used by this call only until it is done on `stream`
  * (not needed when dweight and dbias are both NULL).  The column sums are added in a fixed order: the same
  * call on the same GPU model gives the same bits.  dx must not overlap x or dy.
  */
@@ -283,8 +283,12 @@ int sbnet_layer_norm_grad(const void* dy, const void* x, int dtype, int64_t rows
 #define SBNET_ACT_SILU 0
 #define SBNET_ACT_GELU 1 /* g * Phi(g), by the error function */
 #define SBNET_ACT_RELU 2
-/* grad: workspace of the backward pass.  aligned: 0 if any input tensor's address is not a multiple of 16 bytes. */
-size_t sbnet_gated_ffn_workspace(int64_t rows, int C, int F, int grad, int aligned);
+/* Bytes of workspace a call needs on the current device.  aligned: 0 if any input tensor's address is not a multiple of
+ * 16 bytes (rows that do not start on 16-byte boundaries are copied to the workspace first). */
+#define SBNET_FFN_FORWARD 0
+#define SBNET_FFN_BACKWARD 1
+#define SBNET_FFN_FORWARD_KEEP 2 /* forward with `kept` */
+size_t sbnet_gated_ffn_workspace(int64_t rows, int C, int F, int mode, int aligned);
 int sbnet_gated_ffn(const void* x, int dtype, int64_t rows, int C, int F, const void* w_gate, const void* w_up,
                     const void* w_down, int act, void* y, float* kept, void* workspace, size_t workspace_bytes,
                     void* stream);

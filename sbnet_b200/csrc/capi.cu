@@ -526,7 +526,7 @@ int ffn_call(const void* x, int dtype, int64_t rows, int rowsPerBlock, const int
         (address(y) < address(w_down) + wbytes && address(w_down) < address(y) + bytes))
         return reject(SBNET_ERR_INVALID_ARGUMENT, "%s: the output must not overlap an input", op);
     if (int rc = check_workspace(op, workspace, workspace_bytes,
-                                 sbnet::gated_ffn_workspace(rows, C, F, false, (inputs & 15) == 0)))
+                                 sbnet::gated_ffn_workspace(rows, C, F, false, kept != nullptr, (inputs & 15) == 0)))
         return rc;
     sbnet::FfnArgs f = {};
     f.x = x, f.w_gate = w_gate, f.w_up = w_up, f.w_down = w_down, f.y = y, f.kept = kept;
@@ -536,11 +536,11 @@ int ffn_call(const void* x, int dtype, int64_t rows, int rowsPerBlock, const int
 }
 } // namespace
 
-SBNET_EXPORT size_t sbnet_gated_ffn_workspace(int64_t rows, int C, int F, int grad, int aligned)
+SBNET_EXPORT size_t sbnet_gated_ffn_workspace(int64_t rows, int C, int F, int mode, int aligned)
 {
     if (rows < 1 || C < 1 || F < 1)
         return 0;
-    return sbnet::gated_ffn_workspace(rows, C, F, grad != 0, aligned != 0);
+    return sbnet::gated_ffn_workspace(rows, C, F, mode == SBNET_FFN_BACKWARD, mode == SBNET_FFN_FORWARD_KEEP, aligned != 0);
 }
 
 SBNET_EXPORT int sbnet_gated_ffn(const void* x, int dtype, int64_t rows, int C, int F, const void* w_gate,
@@ -597,7 +597,7 @@ SBNET_EXPORT int sbnet_gated_ffn_grad(const void* dy, const void* x, const float
             if (o.p != nullptr && i.p != nullptr && address(o.p) < address(i.p) + i.n && address(i.p) < address(o.p) + o.n)
                 return reject(SBNET_ERR_INVALID_ARGUMENT, "%s: an output must not overlap an input", op);
     if (int rc = check_workspace(op, workspace, workspace_bytes,
-                                 sbnet::gated_ffn_workspace(rows, C, F, true, (inputs & 15) == 0)))
+                                 sbnet::gated_ffn_workspace(rows, C, F, true, false, (inputs & 15) == 0)))
         return rc;
     sbnet::FfnArgs f = {};
     f.dy = dy, f.x = x, f.kept = const_cast<float*>(kept);

@@ -52,7 +52,7 @@ enum Epilogue { kStore, kGate, kGrad, kKept };
 template <int EPI> constexpr int kEpiWarps = EPI == kStore || EPI == kKept ? 8 : 16;
 template <int EPI> constexpr int kGemmThreads = (2 + kEpiWarps<EPI>) * 32;
 // 32 x 32 tiles of 16-bit elements (2 KB) that a warp stages between registers and memory
-template <int EPI> constexpr int kStaged = EPI == kStore ? 1 : 2;
+template <int EPI> constexpr int kStaged = EPI == kStore ? 1 : EPI == kGrad ? 3 : 2;
 template <int EPI> constexpr int kStagingBytes = kEpiWarps<EPI> * kStaged<EPI> * 2048;
 constexpr int kGroupM = 8;
 
@@ -82,7 +82,7 @@ struct Plan {
     float* partials;               // splits > 1: [splits][batch][mTiles * 256][nTiles * BN]
 };
 
-template <int EPI, int BN> constexpr int kStages = EPI == kGate || EPI == kGrad ? 5 : BN == 256 ? 6 : 8;
+template <int EPI, int BN> constexpr int kStages = EPI == kGate ? 5 : EPI == kGrad ? 4 : BN == 256 ? 6 : 8;
 template <int BN> constexpr int kStageBytes = (kCtaM + BN / 2) * kStepK * 2;    // of one CTA
 template <int EPI, int BN> constexpr int kGemmSmem = 1024 + kStages<EPI, BN> * kStageBytes<BN> + kStagingBytes<EPI> + 256;
 
@@ -91,25 +91,24 @@ __device__ __forceinline__ void gate_chunk(const uint32_t (&g)[32], const uint32
 {
 #pragma unroll
     for (int i = 0; i < 16; ++i) {
-        float a0, a1, unused;
-        activate2<ACT, false>(__uint_as_float(g[2 * i]), __uint_as_float(g[2 * i + 1]), a0, a1, unused, unused);
-        h[i] = pack2<T>(a0 * __uint_as_float(u[2 * i]), a1 * __uint_as_float(u[2 * i + 1]));
+        F2 a, unused;
+        activate2<ACT, false>(words(g[2 * i], g[2 * i + 1]), a, unused);
+        h[i] = pack2<T>(mul2(a, words(u[2 * i], u[2 * i + 1])));
     }
 }
 // H, dG and dU of 16 columns
 template <typename T, int ACT>
 __device__ __forceinline__ void grad_chunk(const uint32_t (&dh)[16], const uint32_t (&g)[16], const uint32_t (&u)[16], uint32_t (&h)[8],
-                                             uint32_t (&dg)[8], uint32_t* du)
+                                             uint32_t (&dg)[8], uint32_t (&du)[8])
 {
 #pragma unroll
     for (int i = 0; i < 8; ++i) {
-        const float d0 = __uint_as_float(dh[2 * i]), d1 = __uint_as_float(dh[2 * i + 1]);
-        const float u0 = __uint_as_float(u[2 * i]), u1 = __uint_as_float(u[2 * i + 1]);
-        float a0, a1, s0, s1;
-        activate2<ACT, true>(__uint_as_float(g[2 * i]), __uint_as_float(g[2 * i + 1]), a0, a1, s0, s1);
-        h[i] = pack2<T>(a0 * u0, a1 * u1);
-        du[i] = pack2<T>(d0 * a0, d1 * a1);
-        dg[i] = pack2<T>(d0 * u0 * s0, d1 * u1 * s1);
+        const F2 d = words(dh[2 * i], dh[2 * i + 1]), up = words(u[2 * i], u[2 * i + 1]);
+        F2 a, slope;
+        activate2<ACT, true>(words(g[2 * i], g[2 * i + 1]), a, slope);
+        h[i] = pack2<T>(mul2(a, up));
+        du[i] = pack2<T>(mul2(d, a));
+        dg[i] = pack2<T>(mul2(mul2(d, up), slope));
     }
 }
 
@@ -331,7 +330,7 @@ __global__ void __launch_bounds__(kGemmThreads<EPI>, 1) gemm_kernel(const __grid
     } else if (warp >= 2) {
         // ---- epilogue: warp w may touch TMEM lanes 32 (w % 4) ..; W / 4 warps share each quarter and split its columns ----
         const int quarter = warp & 3, share = (warp - 2) >> 2;
-        const uint32_t buf0 = staging + (warp - 2) * (kStaged<EPI> * 2048), buf1 = buf0 + 2048;
+        const uint32_t buf0 = staging + (warp - 2) * (kStaged<EPI> * 2048), buf1 = buf0 + 2048, buf2 = buf0 + 4096;
         const uint32_t accEmptyFirst = in_first_cta(accEmpty);
         uint32_t turn = 0, sent = 0;
         for (int t = blockIdx.x >> 1; t < tiles; t += gridDim.x >> 1, ++turn) {
@@ -396,10 +395,9 @@ __global__ void __launch_bounds__(kGemmThreads<EPI>, 1) gemm_kernel(const __grid
                 }
             } else if (EPI == kGrad) {     // one chunk of 32 columns a warp: TMEM is free again after three loads
                 const int c = share * 32;
-                uint32_t du[16];
 #pragma unroll
                 for (int i = 0; i < 2; ++i) {       // 16 columns at a time: 32 of all three would not fit the registers
-                    uint32_t dh[16], g[16], u[16], h[8], dg[8];
+                    uint32_t dh[16], g[16], u[16], h[8], dg[8], du[8];
                     tmem_load16(d + c + 16 * i, g);
                     tmem_load16(d + 128 + c + 16 * i, u);
                     tmem_load16(d + 256 + 128 * (turn & 1) + c + 16 * i, dh);
@@ -407,25 +405,23 @@ __global__ void __launch_bounds__(kGemmThreads<EPI>, 1) gemm_kernel(const __grid
                     if (i == 1)
                         release();
                     if (p.act == kSilu)
-                        grad_chunk<T, kSilu>(dh, g, u, h, dg, du + 8 * i);
+                        grad_chunk<T, kSilu>(dh, g, u, h, dg, du);
                     else if (p.act == kGelu)
-                        grad_chunk<T, kGelu>(dh, g, u, h, dg, du + 8 * i);
+                        grad_chunk<T, kGelu>(dh, g, u, h, dg, du);
                     else
-                        grad_chunk<T, kRelu>(dh, g, u, h, dg, du + 8 * i);
+                        grad_chunk<T, kRelu>(dh, g, u, h, dg, du);
 #pragma unroll
                     for (int q = 0; q < 2; ++q) {
                         sts128(piece(buf0, lane, 2 * i + q), make_uint4(h[4 * q], h[4 * q + 1], h[4 * q + 2], h[4 * q + 3]));
                         sts128(piece(buf1, lane, 2 * i + q), make_uint4(dg[4 * q], dg[4 * q + 1], dg[4 * q + 2], dg[4 * q + 3]));
+                        sts128(piece(buf2, lane, 2 * i + q), make_uint4(du[4 * q], du[4 * q + 1], du[4 * q + 2], du[4 * q + 3]));
                     }
                 }
                 __syncwarp();
                 const Spot at = spot(p.ldo, row0, rowEnd, w.n * 128 + c, p.N, lane);
                 store_tile<T>(p.hid, at, true, buf0, lane);
                 store_tile<T>(p.dgate, at, true, buf1, lane);
-                __syncwarp();
-                stage_rows(buf0, lane, du);
-                __syncwarp();
-                store_tile<T>(p.dup, at, true, buf0, lane);
+                store_tile<T>(p.dup, at, true, buf2, lane);
                 __syncwarp();
             } else if (EPI == kKept) {      // 16 columns at a time, the next 16 of G and U loading meanwhile
                 constexpr int kCols = BN * 4 / W;
@@ -802,21 +798,22 @@ template <typename T> cudaError_t forward(const FfnArgs& f, Layout& l, bool run,
     const long long R = f.rows;
     const int C = f.C, F = f.F, Fp = padded(F);
     const Matrix x = l.plan(f.x, R, C), wg = l.plan(f.w_gate, F, C), wu = l.plan(f.w_up, F, C), wd = l.plan(f.w_down, C, F);
-    const Matrix h = {l.bump.take((size_t)R * Fp * 2), R, F, Fp};
-    float* parts = static_cast<float*>(l.bump.take(std::max(gate_partials(R, F, C), product_partials(1, 1, R, C, F))));
+    const bool fused = f.kept == nullptr && ffn_fused_suits(R, C);      // needs neither H nor partial sums
+    const Matrix h = {fused ? nullptr : l.bump.take((size_t)R * Fp * 2), R, F, Fp};
+    float* parts = fused ? nullptr : static_cast<float*>(l.bump.take(std::max(gate_partials(R, F, C), product_partials(1, 1, R, C, F))));
     if (!run)
         return cudaSuccess;
     bool taken = false;
-    SBNET_TRY(launch_ffn_few<T>(f, const_cast<void*>(h.ptr), stream, &taken));
+    if (!fused)
+        SBNET_TRY(launch_ffn_few<T>(f, const_cast<void*>(h.ptr), stream, &taken));
     if (taken)
         return cudaSuccess;
     note_site("gated_ffn repack");
     Repacks copies;
     copies.add(f.x, x), copies.add(f.w_gate, wg), copies.add(f.w_up, wu), copies.add(f.w_down, wd);
     SBNET_TRY(copies.run(stream));
-    SBNET_TRY(launch_ffn_fused<T>(f, x, wg, wu, wd, stream, &taken));
-    if (taken)
-        return cudaSuccess;
+    if (fused)
+        return launch_ffn_fused<T>(f, x, wg, wu, wd, stream);
     note_site("gated_ffn projections");
     Plan p = {};
     p.mTiles = ceil_div(R, kTileM), p.nTiles = ceil_div(F, 128), p.batch = 1, p.segs = 1, p.kIters = ceil_div(C, kStepK);
@@ -874,10 +871,11 @@ template <typename T> cudaError_t backward(const FfnArgs& f, Layout& l, bool run
 
 } // namespace
 
-size_t gated_ffn_workspace(long long rows, int C, int F, bool grad, bool aligned)
+size_t gated_ffn_workspace(long long rows, int C, int F, bool grad, bool keep, bool aligned)
 {
+    static float kept;      // only its being there matters
     FfnArgs f = {};
-    f.rows = rows, f.C = C, f.F = F;
+    f.rows = rows, f.C = C, f.F = F, f.kept = keep ? &kept : nullptr;
     Layout l = {{nullptr, 0}, aligned};
     if (grad)
         backward<__half>(f, l, false, nullptr);

@@ -55,47 +55,58 @@ __device__ __forceinline__ float recip_fast(float x)
 //        as 2^-60, an error of |g| 2^-60).
 //  gelu: Phi(g) by the rational approximation of Abramowitz and Stegun 7.1.26 for erfc (|error| <= 1.5e-7), whose
 //        exponential is the density that the derivative needs.
-template <int ACT, bool SLOPE> __device__ __forceinline__ void activate2(float g0, float g1, float& a0, float& a1, float& s0, float& s1)
+template <int ACT, bool SLOPE> __device__ __forceinline__ void activate2(F2 g, F2& a, F2& slope)
 {
+    const F2 one = f2(1.f, 1.f);
     if constexpr (ACT == kSilu) {
-        const F2 g = f2(g0, g1);
         const float2 x = unpair(mul2(g, f2(-1.4426950408889634f, -1.4426950408889634f)));
-        const float2 f = unpair(add2(f2(exp2_fast(fminf(x.x, 60.f)), exp2_fast(fminf(x.y, 60.f))), f2(1.f, 1.f)));
+        const float2 f = unpair(add2(f2(exp2_fast(fminf(x.x, 60.f)), exp2_fast(fminf(x.y, 60.f))), one));
         const float r = recip_fast(f.x * f.y);
-        const F2 sig = mul2(f2(r, r), f2(f.y, f.x)), a = mul2(g, sig);
-        a0 = unpair(a).x, a1 = unpair(a).y;
-        if (SLOPE) {    // sig + a (1 - sig)
-            const F2 s = fma2(a, fma2(sig, f2(-1.f, -1.f), f2(1.f, 1.f)), sig);
-            s0 = unpair(s).x, s1 = unpair(s).y;
-        }
+        const F2 sig = mul2(f2(r, r), f2(f.y, f.x));
+        a = mul2(g, sig);
+        if (SLOPE)      // sig + a (1 - sig)
+            slope = fma2(a, fma2(sig, f2(-1.f, -1.f), one), sig);
     } else if constexpr (ACT == kGelu) {
-        auto one = [](float g, float& a, float& s) {
-            const float z = fabsf(g) * 0.70710678118654752f, t = recip_fast(1.f + 0.3275911f * z);
-            const float e = exp2_fast(g * g * -0.72134752044448170f);        // exp(-g^2 / 2)
-            const float q = 0.5f * e * t *
-                            (0.254829592f + t * (-0.284496736f + t * (1.421413741f + t * (-1.453152027f + t * 1.061405429f))));
-            const float cdf = g < 0.f ? q : 1.f - q;
-            a = g * cdf;
-            if (SLOPE)
-                s = cdf + g * 0.3989422804014327f * e;
-        };
-        one(g0, a0, s0), one(g1, a1, s1);
-    } else {
-        a0 = g0 != g0 ? g0 : fmaxf(g0, 0.f), a1 = g1 != g1 ? g1 : fmaxf(g1, 0.f);
+        const float2 gs = unpair(g);
+        const float2 z = make_float2(fabsf(gs.x) * 0.70710678118654752f, fabsf(gs.y) * 0.70710678118654752f);
+        const float2 den = unpair(fma2(f2(z.x, z.y), f2(0.3275911f, 0.3275911f), one));
+        const F2 t = f2(recip_fast(den.x), recip_fast(den.y));
+        const float2 x = unpair(mul2(mul2(g, g), f2(-0.72134752044448170f, -0.72134752044448170f)));
+        const F2 e = f2(exp2_fast(x.x), exp2_fast(x.y));        // exp(-g^2 / 2)
+        F2 q = f2(1.061405429f, 1.061405429f);
+        q = fma2(q, t, f2(-1.453152027f, -1.453152027f));
+        q = fma2(q, t, f2(1.421413741f, 1.421413741f));
+        q = fma2(q, t, f2(-0.284496736f, -0.284496736f));
+        q = fma2(q, t, f2(0.254829592f, 0.254829592f));
+        const float2 tail = unpair(mul2(mul2(q, t), mul2(e, f2(0.5f, 0.5f))));
+        const F2 cdf = f2(gs.x < 0.f ? tail.x : 1.f - tail.x, gs.y < 0.f ? tail.y : 1.f - tail.y);
+        a = mul2(g, cdf);
         if (SLOPE)
-            s0 = g0 > 0.f ? 1.f : 0.f, s1 = g1 > 0.f ? 1.f : 0.f;
+            slope = fma2(mul2(g, f2(0.3989422804014327f, 0.3989422804014327f)), e, cdf);
+    } else {
+        const float2 gs = unpair(g);
+        a = f2(gs.x != gs.x ? gs.x : fmaxf(gs.x, 0.f), gs.y != gs.y ? gs.y : fmaxf(gs.y, 0.f));
+        if (SLOPE)
+            slope = f2(gs.x > 0.f ? 1.f : 0.f, gs.y > 0.f ? 1.f : 0.f);
     }
 }
 __device__ __forceinline__ float activate_any(int act, float g)
 {
-    float a, unused;
+    F2 a, unused;
     if (act == kSilu)
-        activate2<kSilu, false>(g, 0.f, a, unused, unused, unused);
+        activate2<kSilu, false>(f2(g, 0.f), a, unused);
     else if (act == kGelu)
-        activate2<kGelu, false>(g, 0.f, a, unused, unused, unused);
+        activate2<kGelu, false>(f2(g, 0.f), a, unused);
     else
-        activate2<kRelu, false>(g, 0.f, a, unused, unused, unused);
-    return a;
+        activate2<kRelu, false>(f2(g, 0.f), a, unused);
+    return unpair(a).x;
+}
+// Two neighbouring accumulator words as a pair; a pair rounded to 16 bits.
+__device__ __forceinline__ F2 words(uint32_t lo, uint32_t hi) { return f2(__uint_as_float(lo), __uint_as_float(hi)); }
+template <typename T> __device__ __forceinline__ uint32_t pack2(F2 v)
+{
+    const float2 f = unpair(v);
+    return pack2<T>(f.x, f.y);
 }
 
 // Rows to work on: all of them, or those of the live blocks of a stack whose count is on the device.
@@ -191,11 +202,10 @@ inline int ceil_div(long long a, long long b) { return (int)((a + b - 1) / b); }
 // Up to 32 rows (gated_ffn_few.cu): h [rows, F] is scratch.  *taken tells whether the sizes suit the kernels.
 template <typename T> cudaError_t launch_ffn_few(const FfnArgs& f, void* h, cudaStream_t stream, bool* taken);
 
-// Up to 256 channels and many rows, both products in one kernel (gated_ffn_fused.cu).  The matrices are what TMA can
-// read.  *taken tells whether the sizes suit it.
+// Where ffn_fused_suits(), both products in one kernel (gated_ffn_fused.cu).  The matrices are what TMA can read.
 template <typename T>
 cudaError_t launch_ffn_fused(const FfnArgs& f, const Matrix& x, const Matrix& wg, const Matrix& wu, const Matrix& wd,
-                             cudaStream_t stream, bool* taken);
+                             cudaStream_t stream);
 bool ffn_fused_suits(long long rows, int C);
 cudaError_t read_ffn_fused_wait_timeouts(unsigned int* out);
 

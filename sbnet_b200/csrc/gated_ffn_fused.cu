@@ -58,9 +58,9 @@ __device__ __forceinline__ void gate_words(const uint32_t (&g)[32], const uint32
 {
 #pragma unroll
     for (int i = 0; i < 16; ++i) {
-        float a0, a1, unused;
-        activate2<ACT, false>(__uint_as_float(g[2 * i]), __uint_as_float(g[2 * i + 1]), a0, a1, unused, unused);
-        h[i] = pack2<T>(a0 * __uint_as_float(u[2 * i]), a1 * __uint_as_float(u[2 * i + 1]));
+        F2 a, unused;
+        activate2<ACT, false>(words(g[2 * i], g[2 * i + 1]), a, unused);
+        h[i] = pack2<T>(mul2(a, words(u[2 * i], u[2 * i + 1])));
     }
 }
 
@@ -393,11 +393,8 @@ bool ffn_fused_suits(long long rows, int C) { return C <= 256 && 2 * ((rows + kR
 
 template <typename T>
 cudaError_t launch_ffn_fused(const FfnArgs& f, const Matrix& x, const Matrix& wg, const Matrix& wu, const Matrix& wd,
-                             cudaStream_t stream, bool* taken)
+                             cudaStream_t stream)
 {
-    *taken = f.kept == nullptr && ffn_fused_suits(f.rows, f.C);
-    if (!*taken)
-        return cudaSuccess;
     const int kc = ceil_div(f.C, 64);
     FusedMaps maps;
     if (cudaError_t e = encode(x, kCtaRows, &maps.x))
@@ -420,8 +417,8 @@ cudaError_t launch_ffn_fused(const FfnArgs& f, const Matrix& x, const Matrix& wg
     default: return launch<T, 4>(maps, p, tiles, stream);
     }
 }
-template cudaError_t launch_ffn_fused<__half>(const FfnArgs&, const Matrix&, const Matrix&, const Matrix&, const Matrix&, cudaStream_t, bool*);
-template cudaError_t launch_ffn_fused<__nv_bfloat16>(const FfnArgs&, const Matrix&, const Matrix&, const Matrix&, const Matrix&, cudaStream_t, bool*);
+template cudaError_t launch_ffn_fused<__half>(const FfnArgs&, const Matrix&, const Matrix&, const Matrix&, const Matrix&, cudaStream_t);
+template cudaError_t launch_ffn_fused<__nv_bfloat16>(const FfnArgs&, const Matrix&, const Matrix&, const Matrix&, const Matrix&, cudaStream_t);
 
 cudaError_t read_ffn_fused_wait_timeouts(unsigned int* out) { return cudaMemcpyFromSymbol(out, g_fused_timeouts, sizeof(*out)); }
 

@@ -67,7 +67,7 @@ struct FfnArgs {
     long long rows;
     int rowsPerBlock, C, F, act;
 };
-size_t gated_ffn_workspace(long long rows, int C, int F, bool grad, bool aligned);
+size_t gated_ffn_workspace(long long rows, int C, int F, bool grad, bool keep, bool aligned);
 cudaError_t launch_gated_ffn(const FfnArgs& f, int dtype, cudaStream_t stream);
 cudaError_t launch_gated_ffn_grad(const FfnArgs& f, int dtype, cudaStream_t stream);
 cudaError_t read_ffn_wait_timeouts(unsigned int* out);

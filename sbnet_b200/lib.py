@@ -19,6 +19,7 @@ SBNET_COUNT_YIELD = 8
 SBNET_COUNT_NOWAIT = 16
 SBNET_COUNT_PENDING = -(2 ** 31)
 SBNET_REDUCE_MASK_SCRATCH_INTS = 4
+SBNET_FFN_FORWARD, SBNET_FFN_BACKWARD, SBNET_FFN_FORWARD_KEEP = 0, 1, 2
 SBNET_ACT = {"silu": 0, "gelu": 1, "relu": 2}
 
 _i, _f, _p, _sz, _l = C.c_int, C.c_float, C.c_void_p, C.c_size_t, C.c_int64

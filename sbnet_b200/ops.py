@@ -520,12 +520,12 @@ def _check_ffn(x, w_gate, w_up, w_down, activation):
     return rows, channels, hidden, act
 
 
-def _workspace(rows, channels, hidden, grad, tensors, device):
+def _workspace(rows, channels, hidden, mode, tensors, device):
     """Device memory for one call (the caching allocator's: on the current stream, and a capturing graph's own)."""
     bits = 0
     for t in tensors:
         bits |= t.data_ptr()
-    need = _lib.load().sbnet_gated_ffn_workspace(rows, channels, hidden, grad, int(bits & 15 == 0))
+    need = _lib.load().sbnet_gated_ffn_workspace(rows, channels, hidden, mode, int(bits & 15 == 0))
     return torch.empty(need, dtype=torch.uint8, device=device), need
 
 
@@ -540,7 +540,8 @@ def _gated_ffn_call(x, w_gate, w_up, w_down, activation, out, count_dev, keep=Fa
     with _on(x.device):
         y = torch.empty_like(x) if out is None else out
         kept = torch.empty((2, rows, (hidden + 7) // 8 * 8), dtype=torch.float32, device=x.device) if keep else None
-        ws, need = _workspace(rows, channels, hidden, 0, (x, w_gate, w_up, w_down), x.device)
+        mode = _lib.SBNET_FFN_FORWARD_KEEP if keep else _lib.SBNET_FFN_FORWARD
+        ws, need = _workspace(rows, channels, hidden, mode, (x, w_gate, w_up, w_down), x.device)
         head = (channels, hidden, w_gate.data_ptr(), w_up.data_ptr(), w_down.data_ptr(), act, y.data_ptr())
         tail = (ws.data_ptr(), need, _stream(x.device))
         if count_dev is None:
@@ -593,7 +594,7 @@ def _gated_ffn_grad_call(grad, x, w_gate, w_up, w_down, rows, channels, hidden, 
         dwg = torch.empty_like(w_gate) if need_gate_up else None
         dwu = torch.empty_like(w_up) if need_gate_up else None
         dwd = torch.empty_like(w_down) if need_down else None
-        ws, need = _workspace(rows, channels, hidden, 1, (grad, x, w_gate, w_up, w_down), device)
+        ws, need = _workspace(rows, channels, hidden, _lib.SBNET_FFN_BACKWARD, (grad, x, w_gate, w_up, w_down), device)
         _lib.check(_lib.load().sbnet_gated_ffn_grad(
             grad.data_ptr(), x.data_ptr(), _ptr(kept), _DTYPES[x.dtype], rows, channels, hidden,
             w_gate.data_ptr(), w_up.data_ptr(), w_down.data_ptr(), act, _ptr(dx), _ptr(dwg), _ptr(dwu), _ptr(dwd),
