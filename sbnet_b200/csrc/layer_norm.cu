@@ -569,7 +569,7 @@ template <typename T, int MAXT> constexpr int kCtaRows = sizeof(T) == 4 && MAXT 
 
 // The whole CTA shares a row; two rows at a time share a barrier.  Their products are computed twice, before and after
 // it, from the copies in shared memory: two rows of them would not fit the registers beside w, dw and db.
-template <typename T, int VE, int NV, int MAXT> __global__ void __launch_bounds__(MAXT) layer_norm_grad_cta_kernel(NormArgs a)
+template <typename T, int VE, int NV, int MAXT> __global__ void __launch_bounds__(MAXT, MAXT == 256 ? 2 : 1) layer_norm_grad_cta_kernel(NormArgs a)
 {
     constexpr int E = NV * VE, ROWS = kCtaRows<T, MAXT>;
     extern __shared__ __align__(16) uint8_t dyn[];
@@ -876,7 +876,7 @@ int layer_norm_grad_parts(long long rows, int C)
     if (s.tpr == 0)
         return (int)std::min<long long>(rows, sm_count());
     if (s.cta)
-        return (int)std::min<long long>(rows, (long long)sm_count() * std::max(1, 1024 / s.tpr));
+        return (int)std::min<long long>(rows, (long long)sm_count() * std::max(1, 512 / s.tpr));
     return (int)std::min<long long>((rows * s.tpr + kWarpThreads - 1) / kWarpThreads, (long long)sm_count() * (s.elems == 8 ? kGradCtas : kGradCtas16));
 }
 
