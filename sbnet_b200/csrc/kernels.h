@@ -51,7 +51,7 @@ struct NormArgs {
 };
 cudaError_t launch_layer_norm(const NormArgs& a, int dtype, cudaStream_t stream);
 cudaError_t launch_layer_norm_grad(const NormArgs& a, int dtype, cudaStream_t stream);
-int layer_norm_grad_parts(long long rows, int C);
+int layer_norm_grad_parts(long long rows, int C);   // partial rows that launch_layer_norm_grad may write
 
 // The gated feed-forward block (gated_ffn.cu): 16-bit types only.  act: 0 silu, 1 gelu (erf), 2 relu.
 struct FfnArgs {
