@@ -71,7 +71,7 @@ template <typename T, int VE, int NV> __device__ __forceinline__ F2 pair_of(cons
 {
     return f2(v[2 * j / VE].get(2 * j % VE), v[(2 * j + 1) / VE].get((2 * j + 1) % VE));
 }
-template <typename T, int VE, int NV>
+template <typename T, int VE, int NV, bool FULL = false>
 __device__ __forceinline__ void store_pairs(T* row, const F2 (&o)[NV * VE / 2], int t, int tpr, int C)
 {
 #pragma unroll
@@ -85,7 +85,7 @@ __device__ __forceinline__ void store_pairs(T* row, const F2 (&o)[NV * VE / 2], 
             for (int i = 0; i < VE; i += 2)
                 p.set2(i, unpair(o[(k * VE + i) / 2]));
         }
-        if (c < C)
+        if (FULL || c < C)
             p.store(row + c);
     }
 }
@@ -165,7 +165,8 @@ constexpr int kAheadCta = 2;   // the same in the whole-CTA backward kernel, who
 template <typename T, int VE> constexpr bool kCanRunAhead = VE * sizeof(T) >= 4;
 template <typename T, int VE> constexpr int kSlotBytes = kCanRunAhead<T, VE> ? VE * (int)sizeof(T) : 0;
 
-template <typename T, int VE, int NV>
+// FULL: the row is there and every thread's vectors lie inside it.
+template <typename T, int VE, int NV, bool FULL = false>
 __device__ __forceinline__ void copy_row(uint32_t slots, const T* row, bool live, int t, int tpr, int C)
 {
     if constexpr (kCanRunAhead<T, VE>) {
@@ -173,7 +174,7 @@ __device__ __forceinline__ void copy_row(uint32_t slots, const T* row, bool live
         for (int k = 0; k < NV; ++k) {
             const int c = (k * tpr + t) * VE;
             const uint32_t dst = slots + k * blockDim.x * kSlotBytes<T, VE>;
-            if (live && c < C) {
+            if (FULL || (live && c < C)) {
                 if constexpr (VE * sizeof(T) == 16)
                     asm volatile("cp.async.cg.shared.global [%0], [%1], 16;" ::"r"(dst), "l"(row + c) : "memory");
                 else
@@ -182,15 +183,16 @@ __device__ __forceinline__ void copy_row(uint32_t slots, const T* row, bool live
         }
     }
 }
-template <typename T, int VE, int NV>
+template <typename T, int VE, int NV, bool FULL = false>
 __device__ __forceinline__ void take_row(Pack<T, VE> (&v)[NV], uint32_t slots, const T* row, bool live, int t, int tpr, int C)
 {
     if constexpr (kCanRunAhead<T, VE>) {
 #pragma unroll
         for (int k = 0; k < NV; ++k) {
             const uint32_t src = slots + k * blockDim.x * kSlotBytes<T, VE>;
-            v[k].clear();
-            if (live && (k * tpr + t) * VE < C) {
+            if (!FULL)
+                v[k].clear();
+            if (FULL || (live && (k * tpr + t) * VE < C)) {
                 if constexpr (VE * sizeof(T) == 16)
                     v[k].raw = lds128(src);
                 else
@@ -198,7 +200,7 @@ __device__ __forceinline__ void take_row(Pack<T, VE> (&v)[NV], uint32_t slots, c
             }
         }
     } else {
-        load_row<T, VE, NV>(v, row, live, t, tpr, C);
+        load_row<T, VE, NV>(v, row, FULL || live, t, tpr, C);
     }
 }
 __device__ __forceinline__ void copies_commit() { asm volatile("cp.async.commit_group;" ::: "memory"); }
@@ -219,14 +221,14 @@ __device__ __forceinline__ float row_sum(const Pack<T, VE> (&v)[NV], F2 (&f)[NV 
     return both(s);
 }
 // Replaces the row by its distances from `mean` (zero past the row's end); returns the sum of their squares.
-template <int VE, int NV>
+template <int VE, int NV, bool FULL = false>
 __device__ __forceinline__ float row_spread(F2 (&f)[NV * VE / 2], float mean, int t, int tpr, int C)
 {
     const F2 m = f2(-mean, -mean);
 #pragma unroll
     for (int j = 0; j < NV * VE / 2; ++j)
         f[j] = add2(f[j], m);
-    if (tpr * NV * VE != C) {    // some threads reach past the end
+    if (!FULL && tpr * NV * VE != C) {    // some threads reach past the end
 #pragma unroll
         for (int j = 0; j < NV * VE / 2; ++j) {
             float2 d = unpair(f[j]);
@@ -257,7 +259,7 @@ __device__ __forceinline__ void load_params(F2 (&w)[NV * VE / 2], const void* p,
 }
 
 // f: distances from the row's mean + `shift`
-template <typename T, int VE, int NV>
+template <typename T, int VE, int NV, bool FULL = false>
 __device__ __forceinline__ void store_normed(T* y, F2 (&f)[NV * VE / 2], float shift, float rstd, const F2 (&w)[NV * VE / 2],
                                              const F2 (&b)[NV * VE / 2], int t, int tpr, int C)
 {
@@ -265,7 +267,7 @@ __device__ __forceinline__ void store_normed(T* y, F2 (&f)[NV * VE / 2], float s
 #pragma unroll
     for (int j = 0; j < NV * VE / 2; ++j)
         f[j] = fma2(mul2(shift == 0.f ? f[j] : add2(f[j], m), r), w[j], b[j]);
-    store_pairs<T, VE, NV>(y, f, t, tpr, C);
+    store_pairs<T, VE, NV, FULL>(y, f, t, tpr, C);
 }
 
 // `tpr` threads (<= 32) share a row; every turn takes ROWS rows per group.
@@ -286,25 +288,28 @@ __global__ void __launch_bounds__(kWarpThreads, kFwdCtas) layer_norm_warp_kernel
     // all lanes of a warp make the same number of turns (the shuffles need every lane); a lane without a
     // row of its own works on zeros and stores nothing
     const long long turns = (rows + groups * ROWS - 1) / (groups * ROWS);
-    auto fetch = [&](long long turn, uint32_t stage) {
+    auto fetch = [&](auto full, long long turn, uint32_t stage) {
         const uint32_t at = slots + stage * ROWS * rowBytes;
 #pragma unroll
         for (int r = 0; r < ROWS; ++r) {
             const long long row = (turn * ROWS + r) * groups + first;
-            copy_row<T, VE, NV>(at + r * rowBytes, x + row * a.C, row < rows, t, tpr, a.C);
+            copy_row<T, VE, NV, decltype(full)::value>(at + r * rowBytes, x + row * a.C, row < rows, t, tpr, a.C);
         }
         copies_commit();
     };
 #pragma unroll
     for (int i = 0; i < kAhead - 1; ++i)
-        fetch(i, i);
+        fetch(std::false_type(), i, i);
     F2 w[NV * VE / 2], b[NV * VE / 2];
     load_params<VE, NV>(w, a.weight, 1.f, a.wdtype, t, tpr, a.C);
     load_params<VE, NV>(b, a.bias, 0.f, a.wdtype, t, tpr, a.C);
+    // One turn; FULL: all of its rows are there, those it fetches too, and the threads cover the channels exactly, so that
+    // nothing is checked (a fifth of the instructions of this kernel, which sits at the issue limit)
     uint32_t stage = 0;
-    for (long long turn = 0; turn < turns; ++turn, stage = stage + 1 == kAhead ? 0 : stage + 1) {
+    auto body = [&](auto full, long long turn) {
+        constexpr bool FULL = decltype(full)::value;
         const long long row0 = turn * ROWS * groups + first;
-        fetch(turn + kAhead - 1, stage == 0 ? kAhead - 1 : stage - 1);
+        fetch(full, turn + kAhead - 1, stage == 0 ? kAhead - 1 : stage - 1);
         copies_wait();
         const uint32_t at = slots + stage * ROWS * rowBytes;
         F2 f[ROWS][NV * VE / 2];
@@ -313,7 +318,7 @@ __global__ void __launch_bounds__(kWarpThreads, kFwdCtas) layer_norm_warp_kernel
         for (int r = 0; r < ROWS; ++r) {
             const long long row = row0 + r * groups;
             Pack<T, VE> v[NV];
-            take_row<T, VE, NV>(v, at + r * rowBytes, x + row * a.C, row < rows, t, tpr, a.C);
+            take_row<T, VE, NV, FULL>(v, at + r * rowBytes, x + row * a.C, row < rows, t, tpr, a.C);
             mean[r] = row_sum<T, VE, NV>(v, f[r]);
         }
         for (int m = tpr >> 1; m > 0; m >>= 1)
@@ -323,7 +328,7 @@ __global__ void __launch_bounds__(kWarpThreads, kFwdCtas) layer_norm_warp_kernel
 #pragma unroll
         for (int r = 0; r < ROWS; ++r) {
             mean[r] *= inv;
-            rstd[r] = row_spread<VE, NV>(f[r], mean[r], t, tpr, a.C);
+            rstd[r] = row_spread<VE, NV, FULL>(f[r], mean[r], t, tpr, a.C);
         }
         for (int m = tpr >> 1; m > 0; m >>= 1)
 #pragma unroll
@@ -332,14 +337,21 @@ __global__ void __launch_bounds__(kWarpThreads, kFwdCtas) layer_norm_warp_kernel
 #pragma unroll
         for (int r = 0; r < ROWS; ++r) {
             const long long row = row0 + r * groups;
-            if (row >= rows)
+            if (!FULL && row >= rows)
                 continue;
             rstd[r] = rsqrtf(rstd[r] * inv + a.eps);
-            store_normed<T, VE, NV>(static_cast<T*>(a.y) + row * a.C, f[r], 0.f, rstd[r], w, b, t, tpr, a.C);
+            store_normed<T, VE, NV, FULL>(static_cast<T*>(a.y) + row * a.C, f[r], 0.f, rstd[r], w, b, t, tpr, a.C);
             if (t == 0 && a.mean != nullptr)
                 a.mean[row] = mean[r], a.rstd[row] = rstd[r];
         }
-    }
+        stage = stage + 1 == kAhead ? 0 : stage + 1;
+    };
+    long long turn = 0;
+    if (tpr * NV * VE == a.C)
+        for (; turn + kAhead < turns; ++turn)       // the last turn may lack rows, and kAhead - 1 turns are fetched ahead
+            body(std::true_type(), turn);
+    for (; turn < turns; ++turn)
+        body(std::false_type(), turn);
 }
 
 // The whole CTA shares a row.  Each warp takes mean and spread of its own channels, and the warps' results are joined
@@ -456,7 +468,7 @@ __device__ __forceinline__ void grad_sums(const Pack<T, VE> (&xv)[NV], const Pac
     }
     s0 = both(a0), s1 = both(a1);
 }
-template <typename T, int VE, int NV>
+template <typename T, int VE, int NV, bool FULL = false>
 __device__ __forceinline__ void store_dx(T* dx, F2 (&xh)[NV * VE / 2], const F2 (&gw)[NV * VE / 2], float rstd, float m0, float m1,
                                          int t, int tpr, int C)
 {
@@ -464,7 +476,7 @@ __device__ __forceinline__ void store_dx(T* dx, F2 (&xh)[NV * VE / 2], const F2 
 #pragma unroll
     for (int j = 0; j < NV * VE / 2; ++j)
         xh[j] = mul2(r, fma2(xh[j], n1, add2(gw[j], n0)));
-    store_pairs<T, VE, NV>(dx, xh, t, tpr, C);
+    store_pairs<T, VE, NV, FULL>(dx, xh, t, tpr, C);
 }
 
 template <typename T, int VE, int NV, int ROWS>
@@ -484,13 +496,14 @@ __global__ void __launch_bounds__(kWarpThreads, NV * VE == 8 ? kGradCtas : kGrad
     const uint32_t slots = smem_u32(dyn) + threadIdx.x * kSlotBytes<T, VE>;
     const long long turns = (a.rows + groups * ROWS - 1) / (groups * ROWS);
     float meanNext[ROWS], rstdNext[ROWS];
-    auto fetch = [&](long long turn, uint32_t stage) {
+    auto fetch = [&](auto full, long long turn, uint32_t stage) {
+        constexpr bool FULL = decltype(full)::value;
         const uint32_t at = slots + stage * 2 * ROWS * rowBytes;
 #pragma unroll
         for (int r = 0; r < ROWS; ++r) {
             const long long row = (turn * ROWS + r) * groups + first;
-            copy_row<T, VE, NV>(at + 2 * r * rowBytes, x + row * a.C, row < a.rows, t, tpr, a.C);
-            copy_row<T, VE, NV>(at + (2 * r + 1) * rowBytes, g + row * a.C, row < a.rows, t, tpr, a.C);
+            copy_row<T, VE, NV, FULL>(at + 2 * r * rowBytes, x + row * a.C, row < a.rows, t, tpr, a.C);
+            copy_row<T, VE, NV, FULL>(at + (2 * r + 1) * rowBytes, g + row * a.C, row < a.rows, t, tpr, a.C);
         }
         copies_commit();
     };
@@ -503,14 +516,15 @@ __global__ void __launch_bounds__(kWarpThreads, NV * VE == 8 ? kGradCtas : kGrad
     };
 #pragma unroll
     for (int i = 0; i < kAhead - 1; ++i)
-        fetch(i, i);
+        fetch(std::false_type(), i, i);
     stats(0);
     F2 w[E / 2], dw[E / 2] = {}, db[E / 2] = {};
     load_params<VE, NV>(w, a.weight, 1.f, a.wdtype, t, tpr, a.C);
     uint32_t stage = 0;
-    for (long long turn = 0; turn < turns; ++turn, stage = stage + 1 == kAhead ? 0 : stage + 1) {
+    auto body = [&](auto full, long long turn) {
+        constexpr bool FULL = decltype(full)::value;
         const long long row0 = turn * ROWS * groups + first;
-        fetch(turn + kAhead - 1, stage == 0 ? kAhead - 1 : stage - 1);
+        fetch(full, turn + kAhead - 1, stage == 0 ? kAhead - 1 : stage - 1);
         float mean[ROWS], rstd[ROWS], s0[ROWS], s1[ROWS];
 #pragma unroll
         for (int r = 0; r < ROWS; ++r)
@@ -523,8 +537,8 @@ __global__ void __launch_bounds__(kWarpThreads, NV * VE == 8 ? kGradCtas : kGrad
         for (int r = 0; r < ROWS; ++r) {
             const long long row = row0 + r * groups;
             Pack<T, VE> xv[NV], gv[NV];
-            take_row<T, VE, NV>(xv, at + 2 * r * rowBytes, x + row * a.C, row < a.rows, t, tpr, a.C);
-            take_row<T, VE, NV>(gv, at + (2 * r + 1) * rowBytes, g + row * a.C, row < a.rows, t, tpr, a.C);
+            take_row<T, VE, NV, FULL>(xv, at + 2 * r * rowBytes, x + row * a.C, row < a.rows, t, tpr, a.C);
+            take_row<T, VE, NV, FULL>(gv, at + (2 * r + 1) * rowBytes, g + row * a.C, row < a.rows, t, tpr, a.C);
             grad_sums<T, VE, NV>(xv, gv, mean[r], rstd[r], w, dw, db, xh[r], gw[r], s0[r], s1[r]);
         }
         for (int m = tpr >> 1; m > 0; m >>= 1)
@@ -536,10 +550,17 @@ __global__ void __launch_bounds__(kWarpThreads, NV * VE == 8 ? kGradCtas : kGrad
 #pragma unroll
         for (int r = 0; r < ROWS; ++r) {
             const long long row = row0 + r * groups;
-            if (row < a.rows)
-                store_dx<T, VE, NV>(static_cast<T*>(a.y) + row * a.C, xh[r], gw[r], rstd[r], s0[r] * inv, s1[r] * inv, t, tpr, a.C);
+            if (FULL || row < a.rows)
+                store_dx<T, VE, NV, FULL>(static_cast<T*>(a.y) + row * a.C, xh[r], gw[r], rstd[r], s0[r] * inv, s1[r] * inv, t, tpr, a.C);
         }
-    }
+        stage = stage + 1 == kAhead ? 0 : stage + 1;
+    };
+    long long turn = 0;
+    if (tpr * E == a.C)
+        for (; turn + kAhead < turns; ++turn)
+            body(std::true_type(), turn);
+    for (; turn < turns; ++turn)
+        body(std::false_type(), turn);
     // no copy is in flight into the slots that the sums go over: the last ones issued had no row
     asm volatile("cp.async.wait_all;" ::: "memory");
     __syncthreads();
