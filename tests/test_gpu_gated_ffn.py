@@ -367,3 +367,67 @@ def test_two_threads_on_streams_of_their_own(cuda_ops):
         t.join()
     for got, exp in zip(results, want):
         assert all(torch.equal(g, e) for g, e in zip(got, exp))
+
+
+@pytest.mark.parametrize("which", [(0,), (1,), (2,), (3,), (0, 3), (1, 2, 3)])
+def test_some_leaves_only_and_gradients_that_are_not_contiguous(cuda_ops, which):
+    args = _inputs(150, 72, 136, torch.bfloat16, seed=8)
+    leaves = [t.clone().requires_grad_(i in which) for i, t in enumerate(args[:4])]
+    y = sb.gated_ffn(*leaves, activation="relu")
+    # the gradient of a sum over the transposed result: a broadcast scalar, no memory of its own
+    (y.t().sum() * 2).backward()
+    exp = _expected("relu", *args[:4], torch.full_like(args[0], 2))
+    for i, (leaf, name) in enumerate(zip(leaves, NAMES[1:])):
+        assert (leaf.grad is not None) == (i in which)
+        if i in which:
+            _check(leaf.grad, exp, name, leaf.dtype, norm=False)
+
+
+def test_one_matrix_for_both_projections_and_shapes_of_any_rank(cuda_ops):
+    x, wg, _, wd, dy = _inputs(2 * 3 * 35, 48, 80, torch.float16, seed=6)
+    shaped, dys = x.view(2, 3, 35, 48), dy.view(2, 3, 35, 48)
+    y = ops.gated_ffn(shaped, wg, wg, wd)
+    assert y.shape == shaped.shape
+    exp = _expected("silu", x, wg, wg, wd, dy)
+    _check(y.view(-1, 48), exp, "y", x.dtype)
+    got = ops.gated_ffn_grad(dys, shaped, wg, wg, wd)
+    for n, v in zip(NAMES[1:], got):
+        _check(v.reshape(exp[n][0].shape), exp, n, x.dtype)
+
+
+def test_second_derivatives_are_refused(cuda_ops):
+    leaves = [t.requires_grad_(True) for t in _inputs(20, 16, 24, torch.float16)[:4]]
+    y = sb.gated_ffn(*leaves)
+    (g,) = torch.autograd.grad(y.float().square().sum(), leaves[:1], create_graph=True)
+    with pytest.raises(RuntimeError, match="once_differentiable|twice"):
+        g.float().sum().backward()
+
+
+FIRST_CALL = """
+import sys
+sys.path.insert(0, %r)
+import torch
+from sbnet_b200 import ops
+x = torch.randn(%d, %d, device="cuda").half()
+w = [torch.randn(s, device="cuda").half() * 0.05 for s in ((96, %d), (96, %d), (%d, 96))]
+torch.cuda.synchronize()
+g = torch.cuda.CUDAGraph()
+with torch.cuda.graph(g):
+    y = ops.gated_ffn(ops.layer_norm(x), *w)
+    d = ops.gated_ffn_grad(x, x, *w)
+g.replay()
+torch.cuda.synchronize()
+first = y.clone(), [t.clone() for t in d]
+assert torch.equal(first[0], ops.gated_ffn(ops.layer_norm(x), *w))
+assert all(torch.equal(a, b) for a, b in zip(first[1], ops.gated_ffn_grad(x, x, *w)))
+"""
+
+
+@pytest.mark.parametrize("rows,c", [(5, 64), (300, 520), (10_000, 72)])
+def test_the_first_call_of_a_process_may_be_captured(cuda_ops, rows, c):
+    import os
+    import subprocess
+    import sys
+    root = os.path.dirname(os.path.dirname(os.path.abspath(__file__)))
+    res = subprocess.run([sys.executable, "-c", FIRST_CALL % (root, rows, c, c, c, c)], capture_output=True, text=True, timeout=300)
+    assert res.returncode == 0, res.stderr[-2000:]
