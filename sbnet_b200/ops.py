@@ -374,13 +374,14 @@ def sparse_scatter_var_dyn(x, count_dev: torch.Tensor, max_blocks: int, active_b
 
 def _check_rows(t: torch.Tensor, name: str):
     """A contiguous ``[..., C]`` tensor of a supported type; returns ``(rows, C)``."""
-    if t.dim() < 1 or t.shape[-1] < 1:
+    shape = t.shape
+    if not shape or shape[-1] < 1:
         raise ValueError(f"{name} must be [..., C] with at least one channel")
     if t.dtype not in _DTYPES:
         raise ValueError(f"unsupported dtype {t.dtype}")
     if not t.is_contiguous():
         raise ValueError(f"{name} must be contiguous")
-    channels = t.shape[-1]
+    channels = shape[-1]
     return t.numel() // channels, channels
 
 
@@ -391,20 +392,21 @@ def _check_like(t: torch.Tensor, name: str, like: torch.Tensor) -> None:
 
 def _check_norm_params(weight, bias, channels: int, x: torch.Tensor) -> int:
     """weight / bias: None or contiguous ``[C]`` of the input's type or float32, both of one type."""
-    wdtype = None
+    dtype, device, wdtype, shape = x.dtype, x.device, None, (channels,)
     for t, name in ((weight, "weight"), (bias, "bias")):
         if t is None:
             continue
-        if t.dim() != 1 or t.shape[0] != channels or not t.is_contiguous():
+        have = t.dtype
+        if t.shape != shape or not t.is_contiguous():
             raise ValueError(f"{name} must be a contiguous [{channels}] tensor")
-        if t.dtype != x.dtype and t.dtype != torch.float32:
-            raise ValueError(f"{name} must be of the input's dtype or float32, got {t.dtype}")
-        if wdtype is not None and t.dtype != wdtype:
+        if have != dtype and have != torch.float32:
+            raise ValueError(f"{name} must be of the input's dtype or float32, got {have}")
+        if wdtype is not None and have != wdtype:
             raise ValueError("weight and bias must share a dtype")
-        if t.device != x.device:
+        if t.device != device:
             raise ValueError(f"{name} must live on the device of the input")
-        wdtype = t.dtype
-    return _DTYPES[x.dtype if wdtype is None else wdtype]
+        wdtype = have
+    return _DTYPES[dtype if wdtype is None else wdtype]
 
 
 def _ptr(t):
@@ -511,11 +513,12 @@ def _check_ffn(x, w_gate, w_up, w_down, activation):
     if w_gate.dim() != 2 or w_gate.shape[1] != channels or w_gate.shape[0] < 1:
         raise ValueError(f"w_gate must be [hidden, {channels}]")
     hidden = w_gate.shape[0]
+    dtype, device = x.dtype, x.device
     for t, name, shape in ((w_gate, "w_gate", (hidden, channels)), (w_up, "w_up", (hidden, channels)),
                            (w_down, "w_down", (channels, hidden))):
-        if t.dim() != 2 or t.shape[0] != shape[0] or t.shape[1] != shape[1]:
+        if t.shape != shape:
             raise ValueError(f"{name} must be [{shape[0]}, {shape[1]}]")
-        if t.dtype != x.dtype or t.device != x.device or not t.is_contiguous():
+        if t.dtype != dtype or t.device != device or not t.is_contiguous():
             raise ValueError(f"{name} must be contiguous and of the dtype and device of the input")
     return rows, channels, hidden, act
 
