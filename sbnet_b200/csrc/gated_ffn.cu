@@ -16,7 +16,7 @@
 //           then G and U again (256 columns), and the epilogue takes all three from TMEM and writes H, dG and dU.
 //           Costs 4 R F C of 16 R F C operations
 //   kKept   the same from the kept G and U, which the epilogue reads: 16 bytes of HBM traffic per hidden element
-//           instead, so it wins with many channels (8192 x 2048 x 8192 bf16: 405 us against 729)
+//           instead, so it wins with many channels (8192 x 2048 x 8192 bf16: 352 us against 729)
 //   kStore  a plain product, rounded once
 //
 // H, dG and dU are held between kernels in the type of X (they are operands of the next product, and the tensor
@@ -48,11 +48,12 @@ constexpr int kTileM = 256;                      // rows of a tile
 constexpr int kCtaM = 128;                       // ... in each CTA of the pair
 enum Epilogue { kStore, kGate, kGrad, kKept };
 // Epilogue warps: the element-wise epilogues are chains of special functions, shared and global accesses, which four
-// warps per scheduler hide better than two; kKept instead loads a step ahead into registers that 16 warps do not have.
+// warps per scheduler hide better than two; kKept is bound by the loads of G and U, which 8 warps keep in flight in shared
+// memory (8 KB each) while they work on the 8 KB before.
 template <int EPI> constexpr int kEpiWarps = EPI == kStore || EPI == kKept ? 8 : 16;
 template <int EPI> constexpr int kGemmThreads = (2 + kEpiWarps<EPI>) * 32;
 // 32 x 32 tiles of 16-bit elements (2 KB) that a warp stages between registers and memory
-template <int EPI> constexpr int kStaged = EPI == kStore ? 1 : EPI == kGrad ? 3 : 2;
+template <int EPI> constexpr int kStaged = EPI == kStore ? 1 : EPI == kKept ? 8 : EPI == kGrad ? 3 : 2;
 template <int EPI> constexpr int kStagingBytes = kEpiWarps<EPI> * kStaged<EPI> * 2048;
 constexpr int kGroupM = 8;
 
@@ -82,7 +83,7 @@ struct Plan {
     float* partials;               // splits > 1: [splits][batch][mTiles * 256][nTiles * BN]
 };
 
-template <int EPI, int BN> constexpr int kStages = EPI == kGate ? 5 : EPI == kGrad ? 4 : BN == 256 ? 6 : 8;
+template <int EPI, int BN> constexpr int kStages = EPI == kGate ? 5 : EPI == kGrad ? 4 : EPI == kKept ? 3 : BN == 256 ? 6 : 8;
 template <int BN> constexpr int kStageBytes = (kCtaM + BN / 2) * kStepK * 2;    // of one CTA
 template <int EPI, int BN> constexpr int kGemmSmem = 1024 + kStages<EPI, BN> * kStageBytes<BN> + kStagingBytes<EPI> + 256;
 
@@ -333,6 +334,27 @@ __global__ void __launch_bounds__(kGemmThreads<EPI>, 1) gemm_kernel(const __grid
         const uint32_t buf0 = staging + (warp - 2) * (kStaged<EPI> * 2048), buf1 = buf0 + 2048, buf2 = buf0 + 4096;
         const uint32_t accEmptyFirst = in_first_cta(accEmpty);
         uint32_t turn = 0, sent = 0;
+        // kKept: copies this warp's 32 rows x 32 columns of G and U, from column c of its share of a tile.  What lies outside
+        // the matrix is not copied; it only reaches results that are not stored
+        constexpr int kKeptCols = BN * 4 / W;
+        auto keptAhead = [&](uint32_t slot, const Tile& w, int c) {
+            const long long row = (long long)w.m * kTileM + rank * kCtaM + quarter * 32 + (lane >> 2);
+            const int col = w.n * BN + share * kKeptCols + c + (lane & 3) * 4;
+            const float *g = p.gate + row * p.ldo + col, *u = p.up + row * p.ldo + col;
+#pragma unroll
+            for (int i = 0; i < 4; ++i)
+#pragma unroll
+                for (int k = 0; k < 2; ++k)
+                    if (row + 8 * i < rowEnd && col + 16 * k < p.N) {
+                        const uint32_t dst = piece(slot + k * 4096, i * 8 + (lane >> 2), lane & 3);
+                        asm volatile("cp.async.cg.shared.global [%0], [%1], 16;" ::"r"(dst), "l"(g + 8 * i * p.ldo + 16 * k) : "memory");
+                        asm volatile("cp.async.cg.shared.global [%0], [%1], 16;" ::"r"(dst + 2048), "l"(u + 8 * i * p.ldo + 16 * k) : "memory");
+                    }
+        };
+        if (EPI == kKept && (int)(blockIdx.x >> 1) < tiles) {
+            keptAhead(buf0, tile_at(blockIdx.x >> 1, p, mTiles), 0);
+            asm volatile("cp.async.commit_group;" ::: "memory");
+        }
         for (int t = blockIdx.x >> 1; t < tiles; t += gridDim.x >> 1, ++turn) {
             const Tile w = tile_at(t, p, mTiles);
             const uint32_t acc = EPI == kGrad ? 0 : turn & 1, d = tmem + acc * BN + ((uint32_t)(quarter * 32) << 16);
@@ -423,48 +445,31 @@ __global__ void __launch_bounds__(kGemmThreads<EPI>, 1) gemm_kernel(const __grid
                 store_tile<T>(p.dgate, at, true, buf1, lane);
                 store_tile<T>(p.dup, at, true, buf2, lane);
                 __syncwarp();
-            } else if (EPI == kKept) {      // 16 columns at a time, the next 16 of G and U loading meanwhile
-                constexpr int kCols = BN * 4 / W;
-                const int first = w.n * BN + share * kCols;
-                uint4 gn[4], un[4];
-                auto fetch = [&](int c) {
-                    const int r = lane >> 2, col = first + c + (lane & 3) * 4;
-#pragma unroll
-                    for (int i = 0; i < 4; ++i) {
-                        const long long row = row0 + r + 8 * i;
-                        gn[i] = un[i] = make_uint4(0, 0, 0, 0);
-                        if (row < rowEnd && col < p.N) {
-                            gn[i] = ld_stream(reinterpret_cast<const uint4*>(p.gate + row * p.ldo + col));
-                            un[i] = ld_stream(reinterpret_cast<const uint4*>(p.up + row * p.ldo + col));
-                        }
-                    }
-                };
-                fetch(0);
+            } else if (EPI == kKept) {      // 32 columns at a time from one of two slots, the next 32 copying into the other
 #pragma unroll 1
-                for (int c = 0; c < kCols; c += 32) {
+                for (int c = 0; c < kKeptCols; c += 32, ++sent) {
+                    const uint32_t slot = buf0 + (sent & 1) * 8192;       // G and U of 16 columns, then of the next 16
+                    if (c + 32 < kKeptCols)
+                        keptAhead(buf0 + (~sent & 1) * 8192, w, c + 32);
+                    else if (t + (int)(gridDim.x >> 1) < tiles)
+                        keptAhead(buf0 + (~sent & 1) * 8192, tile_at(t + (gridDim.x >> 1), p, mTiles), 0);
+                    asm volatile("cp.async.commit_group;" ::: "memory");
+                    asm volatile("cp.async.wait_group 1;" ::: "memory");
+                    __syncwarp();
                     uint32_t h[16], dg[16], du[16];
 #pragma unroll
                     for (int i = 0; i < 2; ++i) {
-#pragma unroll
-                        for (int k = 0; k < 4; ++k) {
-                            sts128(piece(buf0, k * 8 + (lane >> 2), lane & 3), gn[k]);
-                            sts128(piece(buf1, k * 8 + (lane >> 2), lane & 3), un[k]);
-                        }
-                        __syncwarp();
-                        if (c + 16 * i + 16 < kCols)
-                            fetch(c + 16 * i + 16);
                         uint32_t dh[16], g[16], u[16], hh[8], gg[8], uu[8];
-                        tmem_load16(d + share * kCols + c + 16 * i, dh);
+                        tmem_load16(d + share * kKeptCols + c + 16 * i, dh);
 #pragma unroll
                         for (int k = 0; k < 4; ++k) {
-                            const uint4 a = lds128(piece(buf0, lane, k)), b = lds128(piece(buf1, lane, k));
+                            const uint4 a = lds128(piece(slot + i * 4096, lane, k)), b = lds128(piece(slot + i * 4096 + 2048, lane, k));
                             g[4 * k] = a.x, g[4 * k + 1] = a.y, g[4 * k + 2] = a.z, g[4 * k + 3] = a.w;
                             u[4 * k] = b.x, u[4 * k + 1] = b.y, u[4 * k + 2] = b.z, u[4 * k + 3] = b.w;
                         }
                         tmem_wait_load();
-                        if (c + 16 * i + 16 == kCols)
+                        if (c + 16 * i + 16 == kKeptCols)
                             release();
-                        __syncwarp();
                         if (p.act == kSilu)
                             grad_chunk<T, kSilu>(dh, g, u, hh, gg, uu);
                         else if (p.act == kGelu)
@@ -475,17 +480,16 @@ __global__ void __launch_bounds__(kGemmThreads<EPI>, 1) gemm_kernel(const __grid
                         for (int k = 0; k < 8; ++k)
                             h[8 * i + k] = hh[k], dg[8 * i + k] = gg[k], du[8 * i + k] = uu[k];
                     }
-                    const Spot at = spot(p.ldo, row0, rowEnd, first + c, p.N, lane);
-                    stage_rows(buf0, lane, h);
-                    stage_rows(buf1, lane, dg);
+                    __syncwarp();       // the slot has been read: the results are staged in it
+                    const Spot at = spot(p.ldo, row0, rowEnd, w.n * BN + share * kKeptCols + c, p.N, lane);
+                    stage_rows(slot, lane, h);
+                    stage_rows(slot + 2048, lane, dg);
+                    stage_rows(slot + 4096, lane, du);
                     __syncwarp();
-                    store_tile<T>(p.hid, at, true, buf0, lane);
-                    store_tile<T>(p.dgate, at, true, buf1, lane);
-                    __syncwarp();
-                    stage_rows(buf0, lane, du);
-                    __syncwarp();
-                    store_tile<T>(p.dup, at, true, buf0, lane);
-                    __syncwarp();
+                    store_tile<T>(p.hid, at, true, slot, lane);
+                    store_tile<T>(p.dgate, at, true, slot + 2048, lane);
+                    store_tile<T>(p.dup, at, true, slot + 4096, lane);
+                    __syncwarp();       // before the slot is copied into again
                 }
             } else {
                 T* out = static_cast<T*>(p.out[w.z]);
@@ -507,6 +511,8 @@ __global__ void __launch_bounds__(kGemmThreads<EPI>, 1) gemm_kernel(const __grid
                 }
             }
         }
+        if (EPI == kKept)
+            asm volatile("cp.async.wait_all;" ::: "memory");     // none is left but after a wait that gave up
         if (EPI == kGate && lane == 0)
             bulk_wait_all();     // shared memory is read until then
     }
