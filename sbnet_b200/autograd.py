@@ -108,8 +108,10 @@ def layer_norm(x, weight=None, bias=None, eps=1e-5):
 
 
 # Beyond this many channels the forward pass of the gated feed-forward block keeps its two projections (8 bytes per
-# hidden element) for the backward pass; up to it, multiplying them again takes less time than writing and reading them.
-KEEP_CHANNELS = 1024
+# hidden element) for the backward pass; up to it they are multiplied again.  Forward + backward in bf16, kept against
+# multiplied again: 32,768 x 512 x 2,048 690 / 670 us, 16,384 x 768 x 2,304 573 / 588, 16,384 x 896 x 3,584 994 / 1,109,
+# 16,384 x 1,024 x 4,096 1,171 / 1,306; with 300 rows keeping costs 6 us more at 1,024 channels (115 / 109).
+KEEP_CHANNELS = 768
 
 
 class _GatedFfn(torch.autograd.Function):

