@@ -60,12 +60,14 @@ template <int ACT, bool SLOPE> __device__ __forceinline__ void activate2(F2 g, F
     const F2 one = f2(1.f, 1.f);
     if constexpr (ACT == kSilu) {
         const float2 x = unpair(mul2(g, f2(-1.4426950408889634f, -1.4426950408889634f)));
-        const float2 f = unpair(add2(f2(exp2_fast(fminf(x.x, 60.f)), exp2_fast(fminf(x.y, 60.f))), one));
+        const F2 e = f2(exp2_fast(fminf(x.x, 60.f)), exp2_fast(fminf(x.y, 60.f)));
+        const float2 f = unpair(add2(e, one));
         const float r = recip_fast(f.x * f.y);
         const F2 sig = mul2(f2(r, r), f2(f.y, f.x));
         a = mul2(g, sig);
-        if (SLOPE)      // sig + a (1 - sig)
-            slope = fma2(a, fma2(sig, f2(-1.f, -1.f), one), sig);
+        if (SLOPE)      // sig + a (1 - sig); 1 - sig as e sig, which vanishes with e: sig itself is off by its rounding, and a
+                        // large g would carry that into the slope
+            slope = fma2(a, mul2(e, sig), sig);
     } else if constexpr (ACT == kGelu) {
         const float2 gs = unpair(g);
         const float2 z = make_float2(fabsf(gs.x) * 0.70710678118654752f, fabsf(gs.y) * 0.70710678118654752f);
