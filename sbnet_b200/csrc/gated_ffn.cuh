@@ -42,6 +42,13 @@ __device__ __forceinline__ float exp2_fast(float x)
     asm("ex2.approx.ftz.f32 %0, %1;" : "=f"(r) : "f"(x));
     return r;
 }
+// The larger of two, or not a number where one is.
+__device__ __forceinline__ float max_or_nan(float x, float y)
+{
+    float r;
+    asm("max.NaN.f32 %0, %1, %2;" : "=f"(r) : "f"(x), "f"(y));
+    return r;
+}
 __device__ __forceinline__ float recip_fast(float x)
 {
     float r;
@@ -51,8 +58,8 @@ __device__ __forceinline__ float recip_fast(float x)
 
 // act of two values, and the derivatives where they are asked for.  The epilogues are bound by the special-function unit
 // (16 operations a clock and SM) and by issue slots, hence:
-//  silu: both sigmoids from one reciprocal, 1 / ((1 + e0)(1 + e1)); 2^60 bounds each factor (sigmoids below 2^-60 read
-//        as 2^-60, an error of |g| 2^-60).
+//  silu: both sigmoids from one reciprocal, 1 / ((1 + e0)(1 + e1)); 2^60 bounds each factor.  Sigmoids below 2^-60, of g
+//        below -60 ln 2, read as 2^-60, and g is bounded there too: silu is off by at most 42 * 2^-60 however far g is.
 //  gelu: Phi(g) by the rational approximation of Abramowitz and Stegun 7.1.26 for erfc (|error| <= 1.5e-7), whose
 //        exponential is the density that the derivative needs.
 template <int ACT, bool SLOPE> __device__ __forceinline__ void activate2(F2 g, F2& a, F2& slope)
@@ -64,7 +71,8 @@ template <int ACT, bool SLOPE> __device__ __forceinline__ void activate2(F2 g, F
         const float2 f = unpair(add2(e, one));
         const float r = recip_fast(f.x * f.y);
         const F2 sig = mul2(f2(r, r), f2(f.y, f.x));
-        a = mul2(g, sig);
+        const float2 gs = unpair(g);
+        a = mul2(f2(max_or_nan(gs.x, -41.588830833596717f), max_or_nan(gs.y, -41.588830833596717f)), sig);
         if (SLOPE)      // sig + a (1 - sig); 1 - sig as e sig, which vanishes with e: sig itself is off by its rounding, and a
                         // large g would carry that into the slope
             slope = fma2(a, mul2(e, sig), sig);

@@ -16,7 +16,7 @@ import math
 import pytest
 import torch
 
-from sbnet_b200 import ops
+from sbnet_b200 import lib, ops
 
 pytestmark = pytest.mark.gpu
 
@@ -67,6 +67,34 @@ def _near(got, want, tol, dtype):
     bar = tol + u * (want.abs() + tol) + info.smallest_normal * info.eps
     bad = ~(err <= bar)
     assert not bad.any(), [(float(want[i, j]), float(got[i, j]), float(bar[i, j])) for i, j in bad.nonzero()[:8].tolist()]
+
+
+# the forms for a few rows, for some and for many
+@pytest.mark.parametrize("rows", [4, 16, 32, 64, 300, 9217])
+@pytest.mark.parametrize("up", [1.0, -0.75])
+@pytest.mark.parametrize("act", ["silu", "gelu", "relu"])
+@pytest.mark.parametrize("dtype", [torch.float16, torch.bfloat16])
+def test_far_from_zero(cuda_ops, dtype, act, up, rows):
+    all_x, wg, wu, wd, all_dy = _case(dtype, max(rows, 64), up)
+    for first in range(0, all_x.shape[0] - rows + 1, rows):
+        x, dy = all_x[first:first + rows].contiguous(), all_dy[first:first + rows].contiguous()
+        h, th, dg, tg = _reference(act, x, wg, up)
+        y, kept = ops.gated_ffn(x, wg, wu, wd, act, keep=True)
+        for out in (ops.gated_ffn(x, wg, wu, wd, act), y):
+            _near(out[:, :F], h, th, dtype)
+        for k in (None, kept):
+            dx, _, _, dwd = ops.gated_ffn_grad(dy, x, wg, wu, wd, act, kept=k)
+            _near(dx[:, F:2 * F], dg, tg, dtype)
+    assert lib.wait_timeouts() == 0
+
+
+@pytest.mark.parametrize("rows", [4, 300, 9217])
+@pytest.mark.parametrize("act", ["silu", "gelu", "relu"])
+def test_a_gate_that_is_not_a_number_is_not_hidden(cuda_ops, act, rows):
+    x, wg, wu, wd, _ = _case(torch.bfloat16, rows, 1.0)
+    assert torch.isfinite(ops.gated_ffn(x, wg, wu, wd, act)).all()
+    wg[7, 0] = math.nan         # U is finite
+    assert torch.isnan(ops.gated_ffn(x, wg, wu, wd, act)).all()
 
 
 @pytest.mark.parametrize("rows", [16, 300, 9217])
