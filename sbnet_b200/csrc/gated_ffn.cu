@@ -339,7 +339,7 @@ __global__ void __launch_bounds__(kGemmThreads<EPI>, 1) gemm_kernel(const __grid
         const uint32_t accEmptyFirst = in_first_cta(accEmpty);
         uint32_t turn = 0, sent = 0;
         // kKept: copies this warp's 32 rows x 32 columns of G and U, from column c of its share of a tile.  What lies outside
-        // the matrix is not copied; it only reaches results that are not stored
+        // the matrix is copied in whole 16-byte pieces or not at all; it only reaches results that are not stored
         constexpr int kKeptCols = BN * 4 / W;
         auto keptAhead = [&](uint32_t slot, const Tile& w, int c) {
             const long long row = (long long)w.m * kTileM + rank * kCtaM + quarter * 32 + (lane >> 2);
@@ -471,6 +471,13 @@ __global__ void __launch_bounds__(kGemmThreads<EPI>, 1) gemm_kernel(const __grid
                             g[4 * k] = a.x, g[4 * k + 1] = a.y, g[4 * k + 2] = a.z, g[4 * k + 3] = a.w;
                             u[4 * k] = b.x, u[4 * k + 1] = b.y, u[4 * k + 2] = b.z, u[4 * k + 3] = b.w;
                         }
+                        // column N of an odd N is padding, whatever it holds, and silu shares a reciprocal between columns N - 1
+                        // and N: zero, as the recomputing form has it
+                        const int past = p.N - (w.n * BN + share * kKeptCols + c + 16 * i);
+                        if (p.N & 1)
+#pragma unroll
+                            for (int k = 1; k < 16; k += 2)
+                                g[k] = k == past ? 0 : g[k];
                         tmem_wait_load();
                         if (c + 16 * i + 16 == kKeptCols)
                             release();
