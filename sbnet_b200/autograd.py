@@ -107,18 +107,25 @@ def layer_norm(x, weight=None, bias=None, eps=1e-5):
     return _LayerNorm.apply(x, weight, bias, eps)
 
 
+def _will_differentiate(*inputs):
+    """Whether a backward pass can follow a call made now.  Asked before ``apply``: inside ``forward`` the grad mode is
+    always off, and ``ctx.needs_input_grad`` speaks of the leaves whatever the mode."""
+    return torch.is_grad_enabled() and any(t is not None and t.requires_grad for t in inputs)
+
+
 # Beyond this many channels the forward pass of the gated feed-forward block keeps its two projections (8 bytes per
-# hidden element) for the backward pass; up to it they are multiplied again.  Forward + backward in bf16, kept against
-# multiplied again: 32,768 x 512 x 2,048 690 / 670 us, 16,384 x 768 x 2,304 573 / 588, 16,384 x 896 x 3,584 994 / 1,109,
-# 16,384 x 1,024 x 4,096 1,171 / 1,306; with 300 rows keeping costs 6 us more at 1,024 channels (115 / 109).
+# hidden element) for the backward pass, where one can follow; up to it they are multiplied again.  Forward + backward
+# in bf16, kept against multiplied again: 32,768 x 512 x 2,048 690 / 670 us, 16,384 x 768 x 2,304 573 / 588,
+# 16,384 x 896 x 3,584 994 / 1,109, 16,384 x 1,024 x 4,096 1,171 / 1,306; with 300 rows keeping costs 6 us more at 1,024
+# channels (115 / 109).
 KEEP_CHANNELS = 768
 
 
 class _GatedFfn(torch.autograd.Function):
     @staticmethod
-    def forward(ctx, x, w_gate, w_up, w_down, activation):
+    def forward(ctx, x, w_gate, w_up, w_down, activation, keep):
         kept = None
-        if x.shape[-1] > KEEP_CHANNELS and any(ctx.needs_input_grad):
+        if keep:
             y, kept = ops.gated_ffn(x, w_gate, w_up, w_down, activation, keep=True)
         else:
             y = ops.gated_ffn(x, w_gate, w_up, w_down, activation)
@@ -134,10 +141,11 @@ class _GatedFfn(torch.autograd.Function):
         channels = x.shape[-1]
         return (*ops._gated_ffn_grad_call(grad.contiguous(), x, w_gate, w_up, w_down, x.numel() // channels, channels,
                                           w_gate.shape[0], ops._lib.SBNET_ACT[ctx.activation],
-                                          need[0], need[1] or need[2], need[3], kept), None)
+                                          need[0], need[1] or need[2], need[3], kept), None, None)
 
 
 def gated_ffn(x, w_gate, w_up, w_down, activation="silu"):
     """Differentiable :func:`sbnet_b200.ops.gated_ffn` (gradients flow to ``x`` and the three weights).  Up to
     ``KEEP_CHANNELS`` channels nothing but the inputs is kept for the backward pass."""
-    return _GatedFfn.apply(x, w_gate, w_up, w_down, activation)
+    keep = x.dim() > 0 and x.shape[-1] > KEEP_CHANNELS and _will_differentiate(x, w_gate, w_up, w_down)
+    return _GatedFfn.apply(x, w_gate, w_up, w_down, activation, keep)
