@@ -83,10 +83,20 @@ def sparse_scatter(x, bin_counts, active_block_indices, ybase, dynamic_bsize, dy
                                 dynamic_bstride, dynamic_boffset, add, atomic, transpose)
 
 
+def _will_differentiate(*inputs):
+    """Whether a backward pass can follow a call made now.  Asked before ``apply``: inside ``forward`` the grad mode is
+    always off, and ``ctx.needs_input_grad`` speaks of the leaves whatever the mode."""
+    return torch.is_grad_enabled() and any(t is not None and t.requires_grad for t in inputs)
+
+
 class _LayerNorm(torch.autograd.Function):
     @staticmethod
-    def forward(ctx, x, weight, bias, eps):
-        y, stats = ops.layer_norm(x, weight, bias, eps, stats=True)
+    def forward(ctx, x, weight, bias, eps, keep):
+        stats = None
+        if keep:
+            y, stats = ops.layer_norm(x, weight, bias, eps, stats=True)
+        else:
+            y = ops.layer_norm(x, weight, bias, eps)
         ctx.save_for_backward(x, weight, bias, stats)
         return y
 
@@ -99,18 +109,12 @@ class _LayerNorm(torch.autograd.Function):
         wdtype = ops._DTYPES[x.dtype if param is None else param.dtype]
         gx, gw, gb = ops._layer_norm_grad_call(grad.contiguous(), x, stats, weight, bias, stats.shape[1], x.shape[-1],
                                                wdtype, need[1] or need[2])
-        return gx, gw, gb, None
+        return gx, gw, gb, None, None
 
 
 def layer_norm(x, weight=None, bias=None, eps=1e-5):
     """Differentiable :func:`sbnet_b200.ops.layer_norm` (gradients flow to ``x``, ``weight`` and ``bias``)."""
-    return _LayerNorm.apply(x, weight, bias, eps)
-
-
-def _will_differentiate(*inputs):
-    """Whether a backward pass can follow a call made now.  Asked before ``apply``: inside ``forward`` the grad mode is
-    always off, and ``ctx.needs_input_grad`` speaks of the leaves whatever the mode."""
-    return torch.is_grad_enabled() and any(t is not None and t.requires_grad for t in inputs)
+    return _LayerNorm.apply(x, weight, bias, eps, _will_differentiate(x, weight, bias))
 
 
 # Beyond this many channels the forward pass of the gated feed-forward block keeps its two projections (8 bytes per

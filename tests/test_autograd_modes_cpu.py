@@ -74,3 +74,27 @@ def test_a_graph_inside_and_outside_a_block_without_one(calls):
             assert sb.gated_ffn(*args).requires_grad
         sb.gated_ffn(*args)
     assert calls == [False, True, False]
+
+
+def _norm(weight=True, grad=True):
+    x = torch.randn(5, 16, generator=torch.Generator().manual_seed(2))
+    return x, *((nn.Parameter(torch.ones(16), requires_grad=grad), nn.Parameter(torch.zeros(16), requires_grad=grad)) if weight else (None, None))
+
+
+@pytest.mark.parametrize("mode", ["no_grad", "inference_mode"])
+def test_statistics_are_not_written_without_a_graph(calls, mode):
+    with MODES[mode]():
+        y = sb.layer_norm(*_norm())
+    trained = sb.layer_norm(*_norm())
+    assert calls == [False, True] and not y.requires_grad and trained.requires_grad and torch.equal(trained.detach(), y)
+
+
+@pytest.mark.parametrize("weight", [True, False])
+def test_statistics_are_not_written_for_constants(calls, weight):
+    assert not sb.layer_norm(*_norm(weight, grad=False)).requires_grad and calls == [False]
+
+
+@pytest.mark.parametrize("which", range(3))
+def test_statistics_are_written_for_any_leaf(calls, which):
+    y = sb.layer_norm(*[t.detach().requires_grad_(i == which) for i, t in enumerate(_norm())])
+    assert y.requires_grad and calls == [True] and y.grad_fn.saved_tensors[-1] is not None
