@@ -7,6 +7,7 @@
 #include <cuda_runtime.h>
 #include <stdint.h>
 
+#include <atomic>
 #include <utility>
 
 #include "options.h"
@@ -30,6 +31,25 @@ inline cudaError_t launch_pdl(void (*kernel)(KArgs...), dim3 grid, dim3 block, s
     cfg.attrs = attr;
     cfg.numAttrs = options().pdl ? 1 : 0;
     return cudaLaunchKernelEx(&cfg, kernel, std::forward<Args>(args)...);
+}
+
+// Raises a kernel's dynamic shared-memory limit, once per device; `done` is the kernel's own.  The limit is what was set
+// last, by whichever host thread, so `bytes` is one size for every call of a kernel -- the largest that any launch of it
+// asks for -- and threads that race here set the same limit twice.
+template <typename K> inline cudaError_t allow_smem(K kernel, int bytes, std::atomic<bool> (&done)[64])
+{
+    if (bytes <= 40 * 1024)     // with the static arrays, inside the 48 KB that need no asking
+        return cudaSuccess;
+    int device = 0;
+    if (cudaError_t e = cudaGetDevice(&device))
+        return e;
+    if (device < 64 && done[device].load(std::memory_order_relaxed))
+        return cudaSuccess;
+    if (cudaError_t e = cudaFuncSetAttribute(kernel, cudaFuncAttributeMaxDynamicSharedMemorySize, bytes))
+        return e;
+    if (device < 64)
+        done[device].store(true, std::memory_order_relaxed);
+    return cudaSuccess;
 }
 
 // ---- exact unsigned division by a runtime constant ----------------------------------------------

@@ -643,16 +643,9 @@ template <typename T, bool A_MN, bool B_MN, int EPI, int BN>
 cudaError_t launch_maps(const Maps& maps, Plan& p, cudaStream_t stream)
 {
     auto kernel = gemm_kernel<T, A_MN, B_MN, EPI, BN>;
-    static bool raised[64] = {};       // per device; a race only repeats the call
-    int device = 0;
-    if (cudaError_t e = cudaGetDevice(&device))
+    static std::atomic<bool> done[64] = {};
+    if (cudaError_t e = allow_smem(kernel, kGemmSmem<EPI, BN>, done))
         return e;
-    if (device >= 64 || !raised[device]) {
-        if (cudaError_t e = cudaFuncSetAttribute(kernel, cudaFuncAttributeMaxDynamicSharedMemorySize, kGemmSmem<EPI, BN>))
-            return e;
-        if (device < 64)
-            raised[device] = true;
-    }
     const long long tiles = (long long)p.mTiles * p.nTiles * p.batch * p.splits;
     p.perGroup = FastDiv((uint32_t)(kGroupM * p.nTiles));
     cudaLaunchConfig_t cfg = {};

@@ -301,16 +301,9 @@ template <typename K> FewPlan plan_few(K kernel, int M, int mt, int K_, int grou
 template <typename T, int MT, bool GATE> cudaError_t run(FewArgs& a, cudaStream_t stream, bool dry, bool* fits)
 {
     auto kernel = few_kernel<T, MT, GATE>;
-    static bool raised[64] = {};
-    int device = 0;
-    if (cudaError_t e = cudaGetDevice(&device))
+    static std::atomic<bool> done[64] = {};
+    if (cudaError_t e = allow_smem(kernel, kSmemLimit, done))
         return e;
-    if (device >= 64 || !raised[device]) {
-        if (cudaError_t e = cudaFuncSetAttribute(kernel, cudaFuncAttributeMaxDynamicSharedMemorySize, kSmemLimit))
-            return e;
-        if (device < 64)
-            raised[device] = true;
-    }
     a.groups = GATE ? a.N / 8 : (a.N + 15) / 16;
     a.pieces = (a.K + 63) / 64;
     const FewPlan plan = plan_few(kernel, (int)a.M, MT, a.K, a.groups);

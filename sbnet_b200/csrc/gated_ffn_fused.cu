@@ -367,16 +367,9 @@ cudaError_t launch(const FusedMaps& maps, const FusedArgs& p, int tiles, cudaStr
     auto kernel = fused_kernel<T, KC>;
     constexpr int smem = Fused<KC>::kSmem;
     static_assert(smem <= 227 * 1024, "shared memory of one SM");
-    static bool raised[64] = {};       // per device; a race only repeats the call
-    int device = 0;
-    if (cudaError_t e = cudaGetDevice(&device))
+    static std::atomic<bool> done[64] = {};
+    if (cudaError_t e = allow_smem(kernel, smem, done))
         return e;
-    if (device >= 64 || !raised[device]) {
-        if (cudaError_t e = cudaFuncSetAttribute(kernel, cudaFuncAttributeMaxDynamicSharedMemorySize, smem))
-            return e;
-        if (device < 64)
-            raised[device] = true;
-    }
     cudaLaunchConfig_t cfg = {};
     cfg.gridDim = dim3(2 * (unsigned)std::min(tiles, sm_count() / 2)), cfg.blockDim = dim3(kThreads);
     cfg.dynamicSmemBytes = smem, cfg.stream = stream;

@@ -772,30 +772,13 @@ NormShape pick(int C, int itemsize, uintptr_t bits, bool grad)
     return s;
 }
 
-// Raises a kernel's shared-memory limit once per device (a race only repeats the call).
-template <typename K> cudaError_t allow_smem(K kernel, int bytes, int (&done)[64])
-{
-    if (bytes <= 40 * 1024)     // with the static arrays, inside the 48 KB that need no asking
-        return cudaSuccess;
-    int device = 0;
-    if (cudaError_t e = cudaGetDevice(&device))
-        return e;
-    if (device < 64 && done[device] >= bytes)
-        return cudaSuccess;
-    if (cudaError_t e = cudaFuncSetAttribute(kernel, cudaFuncAttributeMaxDynamicSharedMemorySize, bytes))
-        return e;
-    if (device < 64)
-        done[device] = bytes;
-    return cudaSuccess;
-}
-
 template <typename T, int VE, int NV, int MAXT> cudaError_t launch_fwd_cta(const NormArgs& a, const NormShape& s, cudaStream_t stream)
 {
     auto kernel = layer_norm_cta_kernel<T, VE, NV, MAXT>;
-    static int done[64] = {};
-    const int smem = slots_bytes<T, VE, NV>(s.tpr, 1);
-    if (cudaError_t e = allow_smem(kernel, smem, done))
+    static std::atomic<bool> done[64] = {};
+    if (cudaError_t e = allow_smem(kernel, slots_bytes<T, VE, NV>(MAXT, 1), done))
         return e;
+    const int smem = slots_bytes<T, VE, NV>(s.tpr, 1);
     const long long grid = std::min<long long>(a.rows, (long long)sm_count() * (1024 / s.tpr));
     return launch_pdl(kernel, dim3((unsigned)grid), dim3(s.tpr), smem, stream, a);
 }
@@ -815,7 +798,7 @@ template <typename T, int VE, int NV> cudaError_t launch_fwd(const NormArgs& a, 
     const long long grid = std::min<long long>(ctas, (long long)sm_count() * kFwdCtas);
     if (ctas <= (long long)sm_count() * kFwdCtas) {
         auto kernel = layer_norm_warp_kernel<T, VE, NV, 1>;
-        static int done[64] = {};
+        static std::atomic<bool> done[64] = {};
         constexpr int smem = slots_bytes<T, VE, NV>(kWarpThreads, 1);
         if (cudaError_t e = allow_smem(kernel, smem, done))
             return e;
@@ -823,7 +806,7 @@ template <typename T, int VE, int NV> cudaError_t launch_fwd(const NormArgs& a, 
     }
     constexpr int ROWS = sizeof(T) == 4 && E == 16 ? 1 : 2;     // 48 KB of slots a CTA
     auto kernel = layer_norm_warp_kernel<T, VE, NV, ROWS>;
-    static int done[64] = {};
+    static std::atomic<bool> done[64] = {};
     constexpr int smem = slots_bytes<T, VE, NV>(kWarpThreads, ROWS);
     if (cudaError_t e = allow_smem(kernel, smem, done))
         return e;
@@ -834,10 +817,11 @@ template <typename T, int VE, int NV, int MAXT>
 cudaError_t launch_bwd_cta(const NormArgs& a, const NormShape& s, int grid, cudaStream_t stream)
 {
     auto kernel = layer_norm_grad_cta_kernel<T, VE, NV, MAXT>;
-    static int done[64] = {};
-    const int smem = kAheadCta * 2 * kCtaRows<T, MAXT> * NV * s.tpr * kSlotBytes<T, VE>;
-    if (cudaError_t e = allow_smem(kernel, smem, done))
+    static std::atomic<bool> done[64] = {};
+    constexpr int perThread = kAheadCta * 2 * kCtaRows<T, MAXT> * NV * kSlotBytes<T, VE>;
+    if (cudaError_t e = allow_smem(kernel, perThread * MAXT, done))
         return e;
+    const int smem = perThread * s.tpr;
     return launch_pdl(kernel, dim3(grid), dim3(s.tpr), smem, stream, a);
 }
 
@@ -857,7 +841,7 @@ template <typename T, int VE, int NV> cudaError_t launch_bwd(const NormArgs& a, 
     }
     constexpr int ROWS = E == 8 && sizeof(T) == 2 ? 2 : 1;
     auto kernel = layer_norm_grad_warp_kernel<T, VE, NV, ROWS>;
-    static int done[64] = {};
+    static std::atomic<bool> done[64] = {};
     constexpr int smem = std::max(slots_bytes<T, VE, NV>(kWarpThreads, 2 * ROWS), (int)sizeof(float) * 2 * kWarpThreads * E);
     if (cudaError_t e = allow_smem(kernel, smem, done))
         return e;
