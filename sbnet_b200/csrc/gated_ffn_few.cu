@@ -251,32 +251,37 @@ struct FewPlan {
 };
 
 // Clusters of `splits` CTAs that the device holds at once, with `smem` bytes of shared memory each or, for `perSm` == 2,
-// half of an SM's.  Asked once per device and size: it depends on how the SMs are grouped, not on the call.
-template <typename K> int resident_clusters(K kernel, int splits, int perSm)
+// half of an SM's.  Asked once per kernel, device and size: it depends on how the SMs are grouped, not on the call.  A
+// question that fails is asked again by the next call.
+struct Residency {      // one kernel's answers, 0 where there is none yet; shared by the host threads
+    std::atomic<int> known[64][2][4];
+};
+template <typename K> int resident_clusters(K kernel, Residency& residency, int splits, int perSm)
 {
-    static int known[64][2][4] = {};
     if (splits == 1)
         return sm_count() * perSm;
-    int device = 0, slot = splits == 2 ? 1 : splits == 4 ? 2 : 3, n = 0;
+    int device = 0, slot = splits == 2 ? 1 : splits == 4 ? 2 : 3;
     if (cudaGetDevice(&device) != cudaSuccess || device >= 64)
         return 0;
-    int& hit = known[device][perSm - 1][slot];
-    if (hit == 0) {
+    std::atomic<int>& known = residency.known[device][perSm - 1][slot];
+    int n = known.load(std::memory_order_relaxed);
+    if (n == 0) {
         cudaLaunchAttribute attr[2];
         cudaLaunchConfig_t cfg = config(sm_count() * perSm / splits * splits, perSm == 2 ? kSmemHalf : kSmemLimit, splits, nullptr, attr);
         cfg.numAttrs = 1;
         if (cudaOccupancyMaxActiveClusters(&n, kernel, &cfg) != cudaSuccess) {
             (void)cudaGetLastError();
-            n = 0;
+            return 0;
         }
-        hit = n > 0 ? n : -1;
+        n = n > 0 ? n : -1;
+        known.store(n, std::memory_order_relaxed);
     }
-    return std::max(hit, 0);
+    return std::max(n, 0);
 }
 
 // The split of the reduction under which the SMs stay busiest (the share of the last round of groups that is in use),
 // more CTAs to a cluster only where that gains 4 % a step; none where X and the sums do not fit shared memory.
-template <typename K> FewPlan plan_few(K kernel, int M, int mt, int K_, int groups)
+template <typename K> FewPlan plan_few(K kernel, Residency& residency, int M, int mt, int K_, int groups)
 {
     FewPlan best = {0, 0, 0};
     double score = 0;
@@ -285,7 +290,7 @@ template <typename K> FewPlan plan_few(K kernel, int M, int mt, int K_, int grou
         for (int s = 1, step = 0; s <= 8; s *= 2, ++step) {
             if (s > pieces)
                 break;
-            const int clusters = std::min(groups, resident_clusters(kernel, s, perSm));
+            const int clusters = std::min(groups, resident_clusters(kernel, residency, s, perSm));
             if (clusters < 1)
                 continue;
             const int per = (groups + clusters - 1) / clusters, smem = few_smem(M, mt, (pieces + s - 1) / s, s, per);
@@ -302,11 +307,12 @@ template <typename T, int MT, bool GATE> cudaError_t run(FewArgs& a, cudaStream_
 {
     auto kernel = few_kernel<T, MT, GATE>;
     static std::atomic<bool> done[64] = {};
+    static Residency residency = {};
     if (cudaError_t e = allow_smem(kernel, kSmemLimit, done))
         return e;
     a.groups = GATE ? a.N / 8 : (a.N + 15) / 16;
     a.pieces = (a.K + 63) / 64;
-    const FewPlan plan = plan_few(kernel, (int)a.M, MT, a.K, a.groups);
+    const FewPlan plan = plan_few(kernel, residency, (int)a.M, MT, a.K, a.groups);
     *fits = plan.splits > 0;
     if (!*fits || dry)
         return cudaSuccess;

@@ -34,3 +34,7 @@ def _program(tmp_path, name, source):
 
 def test_layer_norm_calls_of_two_widths_from_two_threads(tmp_path):
     assert "PASS" in _run([_program(tmp_path, "norm_threads", "layer_norm")])
+
+
+def test_few_row_kernels_ask_for_clusters_one_by_one(tmp_path):
+    assert "PASS" in _run([_program(tmp_path, "few_clusters", "gated_ffn_few")])
