@@ -244,7 +244,7 @@ int sbnet_reduce_mask_static(const float* mask, int N, int H, int W, float tol, 
  *   dtype         element type of x and y (SBNET_F32, SBNET_F16, SBNET_BF16)
  *   weight, bias  [C] of wdtype, which is dtype or SBNET_F32; either may be NULL (1 and 0)
  *   mean, rstd    [rows] fp32 for the backward pass, both NULL when they are not wanted
- *   y must not overlap x.  rows == 0 is a successful no-op.
+ *   y, mean and rstd must not overlap an input or one another.  rows == 0 is a successful no-op.
  * The _dyn form works on the first min(*num_blocks_dev, maxBlocks) blocks of rowsPerBlock rows each and
  * leaves the rest of y (and of mean, rstd) as it was.
  */
@@ -258,7 +258,7 @@ int sbnet_layer_norm_dyn(const void* x, int dtype, int64_t maxBlocks, int rowsPe
  * wdtype (either or both may be NULL).  workspace: 16-byte aligned device memory of at least
  * sbnet_layer_norm_grad_workspace(rows, C) bytes (asked on the same device), used by this call only until it is done on `stream`
  * (not needed when dweight and dbias are both NULL).  The column sums are added in a fixed order: the same
- * call on the same GPU model gives the same bits.  dx must not overlap x or dy.
+ * call on the same GPU model gives the same bits.  dx must not overlap an input, nor an output another.
  */
 size_t sbnet_layer_norm_grad_workspace(int64_t rows, int C);
 int sbnet_layer_norm_grad(const void* dy, const void* x, int dtype, int64_t rows, int C, const void* weight,
@@ -276,7 +276,8 @@ int sbnet_layer_norm_grad(const void* dy, const void* x, int dtype, int64_t rows
  *                   only until it is done on `stream`
  * Accumulation and the element-wise steps are fp32; act(gate)*up is rounded to dtype once, as the operand of the last
  * product (in fp16 it overflows beyond 65504, as it would in a network built from separate products).  Sums are
- * taken in a fixed order.  y must not overlap an input.  rows == 0 is a successful no-op.
+ * taken in a fixed order.  y and kept must not overlap an input or each other.  rows == 0 is a
+ * successful no-op.
  * The _dyn form works on the first min(*num_blocks_dev, maxBlocks) blocks of rowsPerBlock rows each and leaves the
  * rest of y as it was; its workspace is sized for maxBlocks * rowsPerBlock rows.
  * Limits: C, F <= 2^24; rows < 2^31 - 256; (rows/128 + 1) * (max(C,F)/128 + 1) < 2^31 / 256.
@@ -300,8 +301,8 @@ int sbnet_gated_ffn_dyn(const void* x, int dtype, int64_t maxBlocks, int rowsPer
  * Backward pass from dy, the forward pass' inputs and its `kept`; with kept == NULL the projections are multiplied
  * again (4*C operations per hidden element instead of 8 bytes kept, written and read: quicker up to some 1,000
  * channels, and training then keeps nothing but its inputs).  dx [rows,C], dw_gate and dw_up [F,C], dw_down [C,F]
- * are each skipped where NULL (dw_gate and dw_up go together); no output may overlap an input.  With rows == 0 the
- * weight gradients are set to zero.
+ * are each skipped where NULL (dw_gate and dw_up go together); no output may overlap an input or another output.
+ * With rows == 0 the weight gradients are set to zero.
  */
 int sbnet_gated_ffn_grad(const void* dy, const void* x, const float* kept, int dtype, int64_t rows, int C, int F, const void* w_gate, const void* w_up, const void* w_down, int act, void* dx,
                          void* dw_gate, void* dw_up, void* dw_down, void* workspace, size_t workspace_bytes,

@@ -378,9 +378,27 @@ bool known_dtype(int dtype) { return dtype == SBNET_F32 || dtype == SBNET_F16 ||
 uintptr_t address(const void* p) { return reinterpret_cast<uintptr_t>(p); }
 uintptr_t elem_mask(int dtype) { return dtype == SBNET_F32 ? 3 : 1; }
 
-bool overlaps(const void* a, const void* b, size_t bytes)
+// Memory of a call: nothing where p is null.
+struct Span {
+    const void* p;
+    size_t n;
+    bool meets(const Span& o) const
+    {
+        return p != nullptr && o.p != nullptr && address(p) < address(o.p) + o.n && address(o.p) < address(p) + n;
+    }
+};
+// Whether one of `out` overlaps one of `in` or another of `out`: what one block writes another reads or writes too.
+template <size_t O, size_t I> bool overlap(const Span (&out)[O], const Span (&in)[I])
 {
-    return address(a) < address(b) + bytes && address(b) < address(a) + bytes;
+    for (size_t o = 0; o < O; ++o) {
+        for (const Span& i : in)
+            if (out[o].meets(i))
+                return true;
+        for (size_t q = 0; q < o; ++q)
+            if (out[o].meets(out[q]))
+                return true;
+    }
+    return false;
 }
 
 // Rules shared by the row operators: types, sizes (row counts and element counts are 64-bit).
@@ -416,8 +434,11 @@ int norm_call(const void* x, int dtype, int64_t rows, int rowsPerBlock, const in
     if (((address(x) | address(y)) & elem_mask(dtype)) || ((address(weight) | address(bias)) & elem_mask(wdtype)) ||
         ((address(mean) | address(rstd) | address(num_blocks_dev)) & 3))
         return reject(SBNET_ERR_INVALID_ARGUMENT, "%s: tensor pointer not aligned to its element size", op);
-    if (overlaps(x, y, (size_t)rows * C * (elem_mask(dtype) + 1)))
-        return reject(SBNET_ERR_INVALID_ARGUMENT, "%s: the output must not overlap the input", op);
+    const size_t bytes = (size_t)rows * C * (elem_mask(dtype) + 1), pbytes = (size_t)C * (elem_mask(wdtype) + 1), sbytes = (size_t)rows * 4;
+    const Span in[] = {{x, bytes}, {weight, pbytes}, {bias, pbytes}, {num_blocks_dev, 4}},
+               out[] = {{y, bytes}, {mean, sbytes}, {rstd, sbytes}};
+    if (overlap(out, in))
+        return reject(SBNET_ERR_INVALID_ARGUMENT, "%s: an output must not overlap another tensor", op);
     sbnet::NormArgs a = {};
     a.x = x, a.y = y, a.weight = weight, a.bias = bias, a.mean = mean, a.rstd = rstd;
     a.num_blocks_dev = num_blocks_dev, a.rows = rows, a.rowsPerBlock = rowsPerBlock, a.C = C, a.wdtype = wdtype, a.eps = eps;
@@ -469,9 +490,12 @@ SBNET_EXPORT int sbnet_layer_norm_grad(const void* dy, const void* x, int dtype,
     if (((address(x) | address(dy) | address(dx)) & elem_mask(dtype)) ||
         ((address(weight) | address(dweight) | address(dbias)) & elem_mask(wdtype)) || ((address(mean) | address(rstd)) & 3))
         return reject(SBNET_ERR_INVALID_ARGUMENT, "%s: tensor pointer not aligned to its element size", op);
-    const size_t bytes = (size_t)rows * C * (elem_mask(dtype) + 1);
-    if (rows > 0 && (overlaps(dx, x, bytes) || overlaps(dx, dy, bytes)))
-        return reject(SBNET_ERR_INVALID_ARGUMENT, "%s: the output must not overlap an input", op);
+    // dweight and dbias are written when all of the inputs have been read
+    const size_t bytes = (size_t)rows * C * (elem_mask(dtype) + 1), pbytes = (size_t)C * (elem_mask(wdtype) + 1), sbytes = (size_t)rows * 4;
+    const Span in[] = {{x, bytes}, {dy, bytes}, {weight, pbytes}, {mean, sbytes}, {rstd, sbytes}}, dxs[] = {{dx, bytes}};
+    const Span none[] = {{nullptr, 0}}, out[] = {{dx, bytes}, {dweight, pbytes}, {dbias, pbytes}};
+    if (rows > 0 && (overlap(dxs, in) || overlap(out, none)))
+        return reject(SBNET_ERR_INVALID_ARGUMENT, "%s: dx must not overlap an input, nor an output another", op);
     if (sums && rows > 0 && (workspace == nullptr || (address(workspace) & 15) ||
                  workspace_bytes < sbnet_layer_norm_grad_workspace(rows, C)))
         return reject(SBNET_ERR_INVALID_ARGUMENT, "%s: needs %zu bytes of 16-byte aligned workspace", op,
@@ -520,11 +544,10 @@ int ffn_call(const void* x, int dtype, int64_t rows, int rowsPerBlock, const int
     const uintptr_t inputs = address(x) | address(w_gate) | address(w_up) | address(w_down);
     if (((inputs | address(y)) & 1) || (address(num_blocks_dev) & 3) || (address(kept) & 15))
         return reject(SBNET_ERR_INVALID_ARGUMENT, "%s: tensor pointer not aligned to its element size (kept: 16 bytes)", op);
-    const size_t bytes = (size_t)rows * C * 2, wbytes = (size_t)F * C * 2;
-    if (overlaps(x, y, bytes) || (address(y) < address(w_gate) + wbytes && address(w_gate) < address(y) + bytes) ||
-        (address(y) < address(w_up) + wbytes && address(w_up) < address(y) + bytes) ||
-        (address(y) < address(w_down) + wbytes && address(w_down) < address(y) + bytes))
-        return reject(SBNET_ERR_INVALID_ARGUMENT, "%s: the output must not overlap an input", op);
+    const size_t bytes = (size_t)rows * C * 2, wbytes = (size_t)F * C * 2, kbytes = (size_t)rows * ((F + 7) / 8 * 8) * 8;
+    const Span in[] = {{x, bytes}, {w_gate, wbytes}, {w_up, wbytes}, {w_down, wbytes}, {num_blocks_dev, 4}}, out[] = {{y, bytes}, {kept, kbytes}};
+    if (overlap(out, in))
+        return reject(SBNET_ERR_INVALID_ARGUMENT, "%s: an output must not overlap another tensor", op);
     if (int rc = check_workspace(op, workspace, workspace_bytes,
                                  sbnet::gated_ffn_workspace(rows, C, F, false, kept != nullptr, (inputs & 15) == 0)))
         return rc;
@@ -590,12 +613,10 @@ SBNET_EXPORT int sbnet_gated_ffn_grad(const void* dy, const void* x, const float
     if ((inputs & 1) || (address(kept) & 15))
         return reject(SBNET_ERR_INVALID_ARGUMENT, "%s: tensor pointer not aligned to its element size (kept: 16 bytes)", op);
     const size_t bytes = (size_t)rows * C * 2, wbytes = (size_t)F * C * 2, kbytes = (size_t)rows * ((F + 7) / 8 * 8) * 8;
-    const struct { const void* p; size_t n; } in[] = {{dy, bytes}, {x, bytes}, {kept, kbytes}, {w_gate, wbytes}, {w_up, wbytes}, {w_down, wbytes}},
-                                              out[] = {{dx, bytes}, {dw_gate, wbytes}, {dw_up, wbytes}, {dw_down, wbytes}};
-    for (const auto& o : out)
-        for (const auto& i : in)
-            if (o.p != nullptr && i.p != nullptr && address(o.p) < address(i.p) + i.n && address(i.p) < address(o.p) + o.n)
-                return reject(SBNET_ERR_INVALID_ARGUMENT, "%s: an output must not overlap an input", op);
+    const Span in[] = {{dy, bytes}, {x, bytes}, {kept, kbytes}, {w_gate, wbytes}, {w_up, wbytes}, {w_down, wbytes}},
+               out[] = {{dx, bytes}, {dw_gate, wbytes}, {dw_up, wbytes}, {dw_down, wbytes}};
+    if (overlap(out, in))
+        return reject(SBNET_ERR_INVALID_ARGUMENT, "%s: an output must not overlap another tensor", op);
     if (int rc = check_workspace(op, workspace, workspace_bytes,
                                  sbnet::gated_ffn_workspace(rows, C, F, true, false, (inputs & 15) == 0)))
         return rc;

@@ -457,7 +457,7 @@ def layer_norm(x: torch.Tensor, weight=None, bias=None, eps: float = 1e-5, out=N
 
     ``weight`` / ``bias``: ``[C]`` of ``x``'s dtype or float32, or None.  ``stats=True`` returns ``(y, stats)`` with the
     rows' ``mean`` and ``1 / sqrt(var + eps)`` as a float32 ``[2, rows]`` tensor for :func:`layer_norm_grad`.
-    ``out`` must not overlap ``x``."""
+    ``out`` must not overlap an input."""
     return _layer_norm_call(x, weight, bias, eps, out, stats, None)
 
 
