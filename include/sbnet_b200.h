@@ -299,7 +299,7 @@ int sbnet_gated_ffn_dyn(const void* x, int dtype, int64_t maxBlocks, int rowsPer
                         void* workspace, size_t workspace_bytes, void* stream);
 /*
  * Backward pass from dy, the forward pass' inputs and its `kept`; with kept == NULL the projections are multiplied
- * again (4*C operations per hidden element instead of 8 bytes kept, written and read: quicker up to some 1,000
+ * again (4*C operations per hidden element instead of 8 bytes kept, written and read: quicker up to some 700
  * channels, and training then keeps nothing but its inputs).  dx [rows,C], dw_gate and dw_up [F,C], dw_down [C,F]
  * are each skipped where NULL (dw_gate and dw_up go together); no output may overlap an input or another output.
  * With rows == 0 the weight gradients are set to zero.

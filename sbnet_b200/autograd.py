@@ -121,7 +121,8 @@ def layer_norm(x, weight=None, bias=None, eps=1e-5):
 # hidden element) for the backward pass, where one can follow; up to it they are multiplied again.  Forward + backward
 # in bf16, kept against multiplied again: 32,768 x 512 x 2,048 690 / 670 us, 16,384 x 768 x 2,304 573 / 588,
 # 16,384 x 896 x 3,584 994 / 1,109, 16,384 x 1,024 x 4,096 1,171 / 1,306; with 300 rows keeping costs 6 us more at 1,024
-# channels (115 / 109).
+# channels (115 / 109).  The limit is on the channels alone: at 768 many rows would be 3 % quicker kept, which does not
+# pay for the memory.
 KEEP_CHANNELS = 768
 
 

@@ -14,8 +14,9 @@
 // cores, the special-function units (two exponentials and a reciprocal for two values of H) and the loads overlap.
 // Waits are bounded as in the other matrix kernels.
 //
-// Measured (one call with a cold L2, launch included): 419,328 rows x 128 channels x 512 hidden, fp16, silu 178 us, the
-// tensor pipe 0.52 and the issue slots 0.59 busy; 102,400 x 256 x 1,024 bf16 138 us.
+// Measured (one call with a cold L2, launch included): 419,328 rows x 128 channels x 512 hidden, fp16, silu 179 us, the
+// tensor pipe 0.50 and the issue slots 0.63 busy; 102,400 x 256 x 1,024 bf16 136 us.  Beyond 64 channels
+// a thread reloads 36 bytes from spills.
 #include <algorithm>
 
 #include "gated_ffn.cuh"
